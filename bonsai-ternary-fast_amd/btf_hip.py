@@ -86,6 +86,46 @@ class _DeviceInfo(C.Structure):
                 ("total_mem_bytes", C.c_int64), ("name", C.c_char * 256), ("gcn_arch", C.c_char * 64)]
 
 
+class _KvCache(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("type", C.c_int), ("page", C.c_int), ("heads", C.c_int),
+                ("dim", C.c_int), ("pages", C.c_int64), ("page_stride", C.c_int64), ("head_stride", C.c_int64),
+                ("tok_stride", C.c_int64)]
+
+
+class _PagePlan(C.Structure):
+    _fields_ = [("S", C.c_int), ("T", C.c_int), ("page", C.c_int), ("ldt", C.c_int), ("pages", C.c_int64),
+                ("ctx", C.c_void_p), ("n_new", C.c_void_p), ("held", C.c_void_p), ("parent", C.c_void_p),
+                ("free_list", C.c_void_p), ("n_free", C.c_void_p), ("table", C.c_void_p), ("held_out", C.c_void_p),
+                ("n_free_out", C.c_void_p), ("row0", C.c_void_p), ("kv_len", C.c_void_p), ("pos", C.c_void_p),
+                ("slot", C.c_void_p), ("tree", C.c_void_p)]
+
+
+class _RopeScale(C.Structure):
+    _fields_ = [("kind", C.c_int), ("factor", C.c_double), ("trained", C.c_double), ("beta_fast", C.c_double),
+                ("beta_slow", C.c_double)]
+
+
+class _RopeCache(C.Structure):
+    _fields_ = [("T", C.c_int), ("heads", C.c_int), ("q", C.c_void_p), ("ldq", C.c_int), ("k", C.c_void_p),
+                ("ldk", C.c_int), ("v", C.c_void_p), ("ldv", C.c_int), ("q_norm", C.c_void_p),
+                ("k_norm", C.c_void_p), ("eps", C.c_float), ("n_rot", C.c_int), ("layout", C.c_int),
+                ("turns", C.c_void_p), ("mscale", C.c_float), ("pos", C.c_void_p), ("slot", C.c_void_p),
+                ("rows", C.c_void_p), ("q_out", C.c_void_p), ("ldqo", C.c_int)]
+
+
+class _PagedAttention(C.Structure):
+    _fields_ = [("S", C.c_int), ("T", C.c_int), ("heads", C.c_int), ("q", C.c_void_p), ("ldq", C.c_int),
+                ("table", C.c_void_p), ("ldt", C.c_int), ("row0", C.c_void_p), ("kv_len", C.c_void_p),
+                ("tree", C.c_void_p), ("scale", C.c_float), ("out", C.c_void_p), ("ldo", C.c_int),
+                ("ws", C.c_void_p)]
+
+
+class _Sampling(C.Structure):
+    _fields_ = [("M", C.c_int), ("V", C.c_int), ("logits", C.c_void_p), ("ldl", C.c_int),
+                ("temperature", C.c_void_p), ("top_k", C.c_void_p), ("top_p", C.c_void_p), ("min_p", C.c_void_p),
+                ("u", C.c_void_p), ("token", C.c_void_p), ("logprob", C.c_void_p), ("ws", C.c_void_p)]
+
+
 class _GgufHeader(C.Structure):
     _fields_ = [("version", C.c_uint32), ("alignment", C.c_uint64), ("data_offset", C.c_uint64),
                 ("file_bytes", C.c_uint64), ("n_tensors", C.c_int64), ("n_kv", C.c_int64)]
@@ -126,6 +166,14 @@ _argmax_part_bytes = _decl("btf_hip_argmax_part_bytes", [_i], _i64)
 _launch_argmax = _decl("btf_hip_launch_argmax", [_vp, _i, _vp, _vp, _vp])
 _launch_argmax_noalloc = _decl("btf_hip_launch_argmax_noalloc", [_vp, _i, _vp, _vp])
 _launch_pos_add = _decl("btf_hip_launch_pos_add", [_vp, _i, _vp])
+_launch_page_plan = _decl("btf_hip_launch_page_plan", [C.POINTER(_PagePlan), _vp])
+_rope_table = _decl("btf_hip_rope_table", [_i, C.c_double, C.POINTER(_RopeScale), _vp, C.POINTER(C.c_float)])
+_launch_rope_cache = _decl("btf_hip_launch_rope_cache", [C.POINTER(_RopeCache), C.POINTER(_KvCache), _vp])
+_paged_attention_ws_bytes = _decl("btf_hip_paged_attention_ws_bytes", [_i, _i, _i, C.POINTER(_KvCache)], _i64)
+_launch_paged_attention = _decl("btf_hip_launch_paged_attention",
+                                [C.POINTER(_PagedAttention), C.POINTER(_KvCache), _vp])
+_sample_ws_bytes = _decl("btf_hip_sample_ws_bytes", [_i, _i], _i64)
+_launch_sample = _decl("btf_hip_launch_sample", [C.POINTER(_Sampling), _vp])
 _launch_gemv_ex = _decl("btf_hip_launch_gemv_ex", [C.POINTER(_GemvSeg), _i, _i, _i, C.POINTER(_Q8Act), _vp, _i, _i,
                                                     C.POINTER(_Q8Act), _vp])
 _launch_gemv_ptq1_0 = _decl("btf_hip_launch_gemv_ptq1_0",
@@ -193,6 +241,9 @@ ABI_SYMBOLS = (
     "btf_hip_gguf_find_kv", "btf_hip_gguf_kv_num", "btf_hip_gguf_kv_str", "btf_hip_ggml_row_bytes",
     "btf_hip_gguf_plan", "btf_hip_loader_create", "btf_hip_loader_upload_ptq1_0", "btf_hip_loader_finish",
     "btf_hip_loader_destroy",
+    "btf_hip_launch_page_plan", "btf_hip_rope_table", "btf_hip_launch_rope_cache",
+    "btf_hip_paged_attention_ws_bytes", "btf_hip_launch_paged_attention", "btf_hip_sample_ws_bytes",
+    "btf_hip_launch_sample",
 )
 
 
@@ -271,6 +322,163 @@ class GemvSeg:
 
     def _c(self):
         return _GemvSeg(_addr(self.codes), _addr(self.scales), self.N, _addr(self.y), self.ldy)
+
+
+class CacheType(enum.IntEnum):
+    """Type of the KV cache's values and of the turned queries."""
+    f16 = 0
+    bf16 = 1
+
+
+class RopeLayout(enum.IntEnum):
+    """Pairs that the rotary positions turn: (i, i + n_rot / 2) or (2i, 2i + 1)."""
+    half = 0
+    pairs = 1
+
+
+class RopeScaling(enum.IntEnum):
+    none = 0
+    linear = 1
+    ntk = 2
+    yarn = 3
+
+
+#: Nodes of a drafted tree at most (a request with more new tokens is a prompt).
+TREE_NODES = 64
+
+
+def _struct(obj, c):
+    """The ctypes struct `c` of a dataclass with the same fields in the same order."""
+    return c(*[v if (t is not C.c_void_p) else _addr(v)
+               for (_, t), v in zip(c._fields_, (getattr(obj, f) for f in obj.__dataclass_fields__))])
+
+
+@dataclass
+class KvCache:
+    """K and V of one layer in pages (btf_kv_cache; strides in values)."""
+    k: object = None
+    v: object = None
+    type: int = CacheType.f16
+    page: int = 64
+    heads: int = 0
+    dim: int = 0
+    pages: int = 0
+    page_stride: int = 0
+    head_stride: int = 0
+    tok_stride: int = 0
+
+    def _c(self):
+        return _struct(self, _KvCache)
+
+
+@dataclass
+class PagePlan:
+    """Arguments of launch_page_plan (btf_page_plan)."""
+    S: int = 0
+    T: int = 0
+    page: int = 64
+    ldt: int = 0
+    pages: int = 0
+    ctx: object = None         # i32 [S]
+    n_new: object = None       # i32 [S]
+    held: object = None        # i32 [S]
+    parent: object = None      # i32 [T] or None
+    free: object = None        # i32, at least *n_free
+    n_free: object = None      # i32 [1]
+    table: object = None       # i32 [S][ldt]
+    held_out: object = None    # i32 [S], may be held
+    n_free_out: object = None  # i32 [1], may be n_free
+    row0: object = None        # i32 [S + 1]
+    kv_len: object = None      # i32 [S]
+    pos: object = None         # i32 [T]
+    slot: object = None        # i32 [T]
+    tree: object = None        # i64 [T] or None
+
+    def _c(self):
+        return _struct(self, _PagePlan)
+
+
+@dataclass
+class RopeScale:
+    """Stretching of the rotary frequencies for contexts beyond the trained one (btf_rope_scale)."""
+    kind: int = RopeScaling.none
+    factor: float = 1.0
+    trained: float = 0.0
+    beta_fast: float = 32.0
+    beta_slow: float = 1.0
+
+    def _c(self):
+        return _struct(self, _RopeScale)
+
+
+@dataclass
+class RopeCache:
+    """Arguments of launch_rope_cache (btf_rope_cache)."""
+    T: int = 0
+    heads: int = 0
+    q: object = None        # f32 [T][ldq]
+    ldq: int = 0
+    k: object = None        # f32 [T][ldk]
+    ldk: int = 0
+    v: object = None        # f32 [T][ldv]
+    ldv: int = 0
+    q_norm: object = None   # f32 [dim] or None
+    k_norm: object = None   # f32 [dim] or None
+    eps: float = 0.0
+    n_rot: int = 0
+    layout: int = RopeLayout.half
+    turns: object = None    # f64 [n_rot / 2]
+    mscale: float = 1.0
+    pos: object = None      # i32 [T]
+    slot: object = None     # i32 [T]
+    rows: object = None     # i32 [1] or None
+    q_out: object = None    # 16 bits [T][ldqo]
+    ldqo: int = 0
+
+    def _c(self):
+        return _struct(self, _RopeCache)
+
+
+@dataclass
+class PagedAttention:
+    """Arguments of launch_paged_attention (btf_paged_attention)."""
+    S: int = 0
+    T: int = 0
+    heads: int = 0
+    q: object = None       # 16 bits [T][ldq]
+    ldq: int = 0
+    table: object = None   # i32 [S][ldt]
+    ldt: int = 0
+    row0: object = None    # i32 [S + 1]
+    kv_len: object = None  # i32 [S]
+    tree: object = None    # i64 [T] or None
+    scale: float = 1.0
+    out: object = None     # f32 [T][ldo]
+    ldo: int = 0
+    ws: object = None      # paged_attention_ws_bytes
+
+    def _c(self):
+        return _struct(self, _PagedAttention)
+
+
+@dataclass
+class Sampling:
+    """Arguments of launch_sample (btf_sampling)."""
+    M: int = 0
+    V: int = 0
+    logits: object = None       # f32 [M][ldl]
+    ldl: int = 0
+    temperature: object = None  # f32 [M] or None
+    top_k: object = None        # i32 [M] or None
+    top_p: object = None        # f32 [M] or None
+    min_p: object = None        # f32 [M] or None
+    u: object = None            # f32 [M]
+    token: object = None        # i32 [M]
+    logprob: object = None      # f32 [M] or None
+    ws: object = None           # sample_ws_bytes
+
+    def _c(self):
+        return _struct(self, _Sampling)
 
 
 # The launchers below go through the native calls of _btf_call; arguments that
@@ -358,6 +566,59 @@ def launch_argmax_noalloc_raw(logits, V, d_tok_out, stream=None) -> int:
 def launch_pos_add(d_pos, M: int, stream=None) -> None:
     """src/cuda/kernels.cuh:92."""
     _check(_launch_pos_add(_addr(d_pos), M, _stream(stream)))
+
+
+def launch_page_plan(a: PagePlan, stream=None) -> None:
+    """Rows, positions, cache slots and pages of a step (btf_hip_launch_page_plan)."""
+    _check(launch_page_plan_raw(a, stream))
+
+
+def launch_page_plan_raw(a: PagePlan, stream=None) -> int:
+    return _launch_page_plan(C.byref(a._c()) if a is not None else None, _stream(stream))
+
+
+def rope_table(n_rot: int, base: float, scale: RopeScale = None):
+    """(turns per position of the n_rot / 2 pairs as float64, mscale): btf_hip_rope_table, host only."""
+    turns, m = (C.c_double * max(1, n_rot // 2))(), C.c_float()
+    _check(_rope_table(n_rot, base, C.byref(scale._c()) if scale is not None else None, turns, C.byref(m)))
+    return list(turns), m.value
+
+
+def launch_rope_cache(a: RopeCache, kv: KvCache, stream=None) -> None:
+    """Head norms, rotary positions and the cache write (btf_hip_launch_rope_cache)."""
+    _check(launch_rope_cache_raw(a, kv, stream))
+
+
+def launch_rope_cache_raw(a: RopeCache, kv: KvCache, stream=None) -> int:
+    return _launch_rope_cache(C.byref(a._c()) if a is not None else None, C.byref(kv._c()) if kv is not None else None,
+                              _stream(stream))
+
+
+def paged_attention_ws_bytes(S: int, T: int, heads: int, kv: KvCache) -> int:
+    return int(_paged_attention_ws_bytes(S, T, heads, C.byref(kv._c())))
+
+
+def launch_paged_attention(a: PagedAttention, kv: KvCache, stream=None) -> None:
+    """Attention of a step's rows over the paged cache (btf_hip_launch_paged_attention)."""
+    _check(launch_paged_attention_raw(a, kv, stream))
+
+
+def launch_paged_attention_raw(a: PagedAttention, kv: KvCache, stream=None) -> int:
+    return _launch_paged_attention(C.byref(a._c()) if a is not None else None,
+                                   C.byref(kv._c()) if kv is not None else None, _stream(stream))
+
+
+def sample_ws_bytes(M: int, V: int) -> int:
+    return int(_sample_ws_bytes(M, V))
+
+
+def launch_sample(a: Sampling, stream=None) -> None:
+    """One token per row with temperature, top-k, top-p and min-p (btf_hip_launch_sample)."""
+    _check(launch_sample_raw(a, stream))
+
+
+def launch_sample_raw(a: Sampling, stream=None) -> int:
+    return _launch_sample(C.byref(a._c()) if a is not None else None, _stream(stream))
 
 
 def launch_gemv_ex(segs, K: int, M: int, a: Q8Act = None, x=None, ldx: int = 0,

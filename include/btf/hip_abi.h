@@ -401,6 +401,190 @@ int btf_hip_loader_upload_ptq1_0(btf_loader_t L, const uint8_t* src, int64_t N, 
 int btf_hip_loader_finish(btf_loader_t L, uint64_t* source_bytes); /* total PTQ1_0 bytes uploaded */
 int btf_hip_loader_destroy(btf_loader_t L);
 
+/* ---- a serving step of several requests ----------------------------------
+ * The operators of a step between its matrix products, for a batch of
+ * requests over a paged cache: lay the step's rows and cache pages out, norm
+ * and turn Q and K and write K and V into the cache, let the new rows attend
+ * to the cache, draw the next tokens. The reference's decoder serves one
+ * request from one dense cache (launch_attn_prep, launch_attention,
+ * launch_attn_combine and launch_argmax, src/cuda/kernels.cuh:72-90).
+ *
+ * A step's rows are its requests' new tokens in order: rows row0[s] ..
+ * row0[s+1]-1 belong to request s, which then has kv_len[s] tokens in the
+ * cache, these rows included (the last ones). The lengths are device data, so
+ * a captured step serves steps of other lengths; T is the rows that the row
+ * arrays hold, and rows from row0[S] on are left as they were.
+ *
+ * A request with at most BTF_TREE_NODES new tokens may hold a tree of drafted
+ * tokens: tree[row] has bit j set if the request's new row j is the row itself
+ * or one of its ancestors, all that the row sees of the new tokens. More new
+ * tokens, or tree == NULL: row i sees the new rows 0 .. i. */
+#define BTF_TREE_NODES 64
+enum { BTF_F16 = 0, BTF_BF16 = 1 };
+
+/* K and V of one layer in pages of `page` tokens. Token t of a page, KV head
+ * h: `dim` values of 16 bits at page * page_stride + h * head_stride +
+ * t * tok_stride (counted in values), the same in k and v. */
+typedef struct btf_kv_cache {
+  void* k;
+  void* v;          /* both 16-byte aligned */
+  int type;         /* BTF_F16 or BTF_BF16 */
+  int page;         /* 16, 32, 64, 128 or 256 */
+  int heads;        /* KV heads */
+  int dim;          /* 64, 128 or 256 */
+  int64_t pages;    /* pages * page < 2^31 */
+  int64_t page_stride, head_stride, tok_stride; /* multiples of 8, tok_stride >= dim */
+} btf_kv_cache;
+
+/* Rows, positions, cache slots and pages of a step from the requests' lengths.
+ * Request s has ctx[s] tokens in the cache, adds n_new[s] (0: none) and holds
+ * held[s] pages, the ids in table[s][0 .. held[s]).
+ *  - row0[s]: the new tokens of the requests before s, at most T.
+ *  - Pages for the new tokens come off the end of the free list: the request
+ *    order's first page is free_list[*n_free - 1]. A request is refused if a
+ *    length is negative or passes 2^31, ctx[s] > held[s] * page, its rows pass
+ *    T, its pages pass ldt, or the free pages do not reach for it and those before it (then every
+ *    later request that needs a page is refused too). A refused request gets no
+ *    page, kv_len 0, and its rows position 0, slot -1 and tree 0, with which
+ *    the launches below neither write the cache for it nor read it.
+ *  - kv_len[s] = ctx[s] + n_new[s]; held_out, n_free_out: held and *n_free
+ *    less what was handed out (each may be the input itself).
+ *  - row i of request s: pos = ctx[s] + i, slot = its place in the cache
+ *    (page id * page + token in the page; -1 if the page id is not in
+ *    [0, pages)).
+ *  - with trees (parent and tree set): parent[row] < i is the new row (counted
+ *    in the request) that row i follows, -1 (or anything else) the cache's last
+ *    token. Then pos = ctx[s] + depth and tree[row] = the bits of the row and
+ *    its ancestors; a request of more than BTF_TREE_NODES rows is a prompt
+ *    (pos = ctx[s] + i, tree 0). */
+typedef struct btf_page_plan {
+  int S, T;              /* requests, rows */
+  int page;              /* tokens of a page: a power of two */
+  int ldt;               /* page ids that a row of table holds */
+  int64_t pages;         /* pages of the cache */
+  const int* ctx;        /* [S] */
+  const int* n_new;      /* [S] */
+  const int* held;       /* [S] */
+  const int* parent;     /* [T] or NULL */
+  const int* free_list;  /* page ids, at least *n_free */
+  const int* n_free;     /* [1] */
+  int* table;            /* [S][ldt] */
+  int* held_out;         /* [S] */
+  int* n_free_out;       /* [1] */
+  int* row0;             /* [S + 1] */
+  int* kv_len;           /* [S] */
+  int* pos;              /* [T] */
+  int* slot;             /* [T] */
+  uint64_t* tree;        /* [T] or NULL (with parent) */
+} btf_page_plan;
+int btf_hip_launch_page_plan(const btf_page_plan* a, btf_stream_t stream);
+
+/* Turns per position of the n_rot / 2 pairs, base^(-2i/n_rot) / (2 pi), stretched
+ * for contexts beyond the trained one (host only; the caller copies the table
+ * to the device once):
+ *  BTF_ROPE_LINEAR: every frequency / factor;
+ *  BTF_ROPE_NTK: the base times factor^(n_rot / (n_rot - 2));
+ *  BTF_ROPE_YARN: pairs that turn more than beta_fast times over `trained`
+ *   positions stay, those that turn less than beta_slow times are divided by
+ *   factor, a linear ramp over the pairs between; *mscale = 0.1 ln(factor) + 1.
+ * *mscale (1 for the others) multiplies the turned values. scale NULL: none. */
+enum { BTF_ROPE_NONE = 0, BTF_ROPE_LINEAR = 1, BTF_ROPE_NTK = 2, BTF_ROPE_YARN = 3 };
+typedef struct btf_rope_scale {
+  int kind;
+  double factor;               /* >= 1 */
+  double trained;              /* yarn: trained context */
+  double beta_fast, beta_slow; /* yarn: 32 and 1 by custom */
+} btf_rope_scale;
+int btf_hip_rope_table(int n_rot, double base, const btf_rope_scale* scale, double* turns, float* mscale);
+
+/* Rows of Q, K and V as the QKV product leaves them (fp32; head h of a row at
+ * h * dim) -> per head RMSNorm (x / sqrt(mean x^2 + eps) * norm; NULL: none),
+ * the first n_rot values of a head turned by the row's position, rounded to
+ * kv->type: Q to q_out rows, K and V (V as it is) to the row's cache slot.
+ * BTF_ROPE_HALF turns the pairs (i, i + n_rot / 2), BTF_ROPE_PAIRS (2i, 2i + 1):
+ * (a cos - b sin, a sin + b cos) * mscale, the angle pos * turns[i] turns.
+ * q (with q_out) or k and v may be NULL: left out. A slot outside the cache
+ * is not written. rows (optional): the rows to do are min(*rows, T), as
+ * row0 + S gives them. */
+enum { BTF_ROPE_HALF = 0, BTF_ROPE_PAIRS = 1 };
+typedef struct btf_rope_cache {
+  int T, heads;         /* rows, Q heads */
+  const float* q;       /* [T][ldq] */
+  int ldq;
+  const float* k;       /* [T][ldk] */
+  int ldk;
+  const float* v;       /* [T][ldv] */
+  int ldv;
+  const float* q_norm;  /* [dim] or NULL */
+  const float* k_norm;  /* [dim] or NULL */
+  float eps;
+  int n_rot;            /* even, 0 .. dim */
+  int layout;
+  const double* turns;  /* [n_rot / 2] */
+  float mscale;
+  const int* pos;       /* [T] */
+  const int* slot;      /* [T] */
+  const int* rows;      /* [1] or NULL */
+  void* q_out;          /* [T][ldqo], 16 bits */
+  int ldqo;
+} btf_rope_cache;
+int btf_hip_launch_rope_cache(const btf_rope_cache* a, const btf_kv_cache* kv, btf_stream_t stream);
+
+/* out = softmax(scale * Q K^T) V of every new row over what it sees: the
+ * cache's tokens before the request's rows, and of these what the tree's bits
+ * or the order gives. Q head h reads KV head h / (heads / kv->heads). Pages
+ * whose id in table is not in [0, pages) are not seen. A row that sees nothing,
+ * or nothing but scores of -infinity, gives zeros. What a row does not see has
+ * no effect on it, infinities and NaN included. out is fp32, as launch_prep
+ * takes it; products are of 16-bit values, everything else is in 32 bits.
+ * ws: paged_attention_ws_bytes of device scratch, 16-byte aligned, one for
+ * each stream that launches; 0 bytes needed: ws may be NULL. */
+typedef struct btf_paged_attention {
+  int S, T, heads;       /* requests, rows, Q heads */
+  const void* q;         /* [T][ldq], 16 bits of kv->type, 16-byte aligned, ldq % 8 == 0 */
+  int ldq;
+  const int* table;      /* [S][ldt] */
+  int ldt;
+  const int* row0;       /* [S + 1] */
+  const int* kv_len;     /* [S], at most ldt * page is read */
+  const uint64_t* tree;  /* [T] or NULL */
+  float scale;
+  float* out;            /* [T][ldo], 16-byte aligned, ldo % 4 == 0 */
+  int ldo;
+  void* ws;
+} btf_paged_attention;
+int64_t btf_hip_paged_attention_ws_bytes(int S, int T, int heads, const btf_kv_cache* kv);
+int btf_hip_launch_paged_attention(const btf_paged_attention* a, const btf_kv_cache* kv, btf_stream_t stream);
+
+/* One token per row of logits, drawn with the row's settings and a given
+ * uniform number u in [0, 1). With the weights w_i = exp((x_i - max x) / T):
+ * kept are, in order of falling x (the smaller index first on ties), the first
+ * top_k, of these those before which less than top_p of their sum lies, and of
+ * these the ones with w >= min_p. The token is the first index, in index order,
+ * at which the sum of the kept weights passes u times their sum; its logprob is
+ * ln(w / that sum). temperature <= 0 (or NaN): the greedy pick, as
+ * launch_argmax, logprob 0. top_k <= 0, top_p >= 1, min_p <= 0 (or NaN) and NULL
+ * arrays: not applied (temperature NULL: 1). At least the largest is kept. A NaN
+ * logit is never drawn; logits equal to the row's largest have the weight 1,
+ * infinities too. Sums are of 64-bit integers (w in units of 2^-43): the result
+ * does not depend on any order. V <= 2^20. ws: sample_ws_bytes of device scratch,
+ * 8-byte aligned, one for each stream that launches. */
+typedef struct btf_sampling {
+  int M, V;
+  const float* logits;       /* [M][ldl] */
+  int ldl;
+  const float* temperature;  /* [M] or NULL */
+  const int* top_k;          /* [M] or NULL */
+  const float* top_p;        /* [M] or NULL */
+  const float* min_p;        /* [M] or NULL */
+  const float* u;            /* [M] */
+  int* token;                /* [M] */
+  float* logprob;            /* [M] or NULL */
+  void* ws;
+} btf_sampling;
+int64_t btf_hip_sample_ws_bytes(int M, int V);
+int btf_hip_launch_sample(const btf_sampling* a, btf_stream_t stream);
+
 /* Device description for reports. name must hold name_len bytes. */
 typedef struct btf_device_info {
   int cu_count;

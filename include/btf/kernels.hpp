@@ -105,6 +105,37 @@ inline void launch_pos_add(int* d_pos, int M, btf_stream_t st) {
   detail::check(btf_hip_launch_pos_add(d_pos, M, st), "launch_pos_add");
 }
 
+// ---- a serving step of several requests over a paged cache (hip_abi.h has the
+// structs; the reference's decoder serves one request, kernels.cuh:72-90)
+using KvCache = btf_kv_cache;
+using PagePlan = btf_page_plan;
+using RopeScale = btf_rope_scale;
+using RopeCache = btf_rope_cache;
+using PagedAttention = btf_paged_attention;
+using Sampling = btf_sampling;
+inline void launch_page_plan(const PagePlan& a, btf_stream_t st) {
+  detail::check(btf_hip_launch_page_plan(&a, st), "launch_page_plan");
+}
+// turns: host [n_rot / 2]; returns mscale
+inline float rope_table(int n_rot, double base, const RopeScale* scale, double* turns) {
+  float m = 1.0f;
+  detail::check(btf_hip_rope_table(n_rot, base, scale, turns, &m), "rope_table");
+  return m;
+}
+inline void launch_rope_cache(const RopeCache& a, const KvCache& kv, btf_stream_t st) {
+  detail::check(btf_hip_launch_rope_cache(&a, &kv, st), "launch_rope_cache");
+}
+inline size_t paged_attention_ws_bytes(int S, int T, int heads, const KvCache& kv) {
+  return (size_t)btf_hip_paged_attention_ws_bytes(S, T, heads, &kv);
+}
+inline void launch_paged_attention(const PagedAttention& a, const KvCache& kv, btf_stream_t st) {
+  detail::check(btf_hip_launch_paged_attention(&a, &kv, st), "launch_paged_attention");
+}
+inline size_t sample_ws_bytes(int M, int V) { return (size_t)btf_hip_sample_ws_bytes(M, V); }
+inline void launch_sample(const Sampling& a, btf_stream_t st) {
+  detail::check(btf_hip_launch_sample(&a, st), "launch_sample");
+}
+
 // launch_gemv with the chain's quantizes fused in (no counterpart in
 // kernels.cuh: the decoder's launch_prep + launch_gemv pairs without norm or
 // transform, src/cuda/gpu_decoder.cu:411-418): input from Q8 rows `a` or fp32

@@ -1,0 +1,166 @@
+"""CPU tests of a serving step's operators: what the launches refuse before any
+HIP call (no device exists in this process, so reaching one gives another
+code), the layout of the argument structs, and the table of rotary frequencies.
+"""
+import dataclasses
+import math
+import os
+import subprocess
+
+import numpy as np
+import pytest
+
+import btf_hip as h
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+A = 0x100000  # an aligned address; nothing reads it
+ARGS, NOT_INIT = h.BTF_ERR_ARGS, h.BTF_ERR_NOT_INIT
+
+KV = h.KvCache(A, A, h.CacheType.f16, 64, 4, 256, 100, 4 * 64 * 256, 64 * 256, 256)
+PLAN = h.PagePlan(S=2, T=8, page=64, ldt=4, pages=100, ctx=A, n_new=A, held=A, parent=A, free=A, n_free=A, table=A,
+                  held_out=A, n_free_out=A, row0=A, kv_len=A, pos=A, slot=A, tree=A)
+ROPE = h.RopeCache(T=3, heads=20, q=A, ldq=7168, k=A, ldk=7168, v=A, ldv=7168, q_norm=A, k_norm=A, eps=1e-6, n_rot=64,
+                   layout=0, turns=A, mscale=1.0, pos=A, slot=A, rows=A, q_out=A, ldqo=5120)
+ATTN = h.PagedAttention(S=2, T=8, heads=20, q=A, ldq=5120, table=A, ldt=4, row0=A, kv_len=A, tree=A, scale=0.0625,
+                        out=A, ldo=5120, ws=A)
+SAMPLE = h.Sampling(M=2, V=1000, logits=A, ldl=1000, temperature=A, top_k=A, top_p=A, min_p=A, u=A, token=A, logprob=A,
+                    ws=A)
+
+
+def launch(op, a, kv=KV):
+    return {"plan": lambda: h.launch_page_plan_raw(a), "rope": lambda: h.launch_rope_cache_raw(a, kv),
+            "attn": lambda: h.launch_paged_attention_raw(a, kv), "sample": lambda: h.launch_sample_raw(a)}[op]()
+
+
+VALID = {"plan": PLAN, "rope": ROPE, "attn": ATTN, "sample": SAMPLE}
+REFUSED = [
+    ("plan", dict(T=-1)), ("plan", dict(page=48)), ("plan", dict(page=0)), ("plan", dict(ldt=0)),
+    ("plan", dict(pages=0)), ("plan", dict(pages=1 << 25, page=64)), ("plan", dict(parent=None)),
+    ("plan", dict(tree=None)), ("plan", dict(tree=A + 4)),
+    *[("plan", {n: None}) for n in ("ctx", "n_new", "held", "free", "n_free", "table", "held_out", "n_free_out", "row0",
+                                    "kv_len", "pos", "slot")],
+    ("rope", dict(q=None, k=None, v=None)), ("rope", dict(v=None)), ("rope", dict(k=None)), ("rope", dict(heads=0)),
+    ("rope", dict(q_out=None)), ("rope", dict(ldq=5119)), ("rope", dict(ldqo=5119)), ("rope", dict(ldk=1023)),
+    ("rope", dict(ldv=1023)), ("rope", dict(slot=None)), ("rope", dict(n_rot=63)), ("rope", dict(n_rot=258)),
+    ("rope", dict(n_rot=-2)), ("rope", dict(layout=2)), ("rope", dict(turns=None)), ("rope", dict(pos=None)),
+    ("rope", dict(q=A + 2)), ("rope", dict(turns=A + 4)),
+    ("attn", dict(heads=0)), ("attn", dict(heads=18)), ("attn", dict(q=A + 8)), ("attn", dict(ldq=5124)),
+    ("attn", dict(ldq=5112)), ("attn", dict(out=A + 4)), ("attn", dict(ldo=5122)), ("attn", dict(ldo=5116)),
+    ("attn", dict(ldt=0)), ("attn", dict(tree=A + 4)), ("attn", dict(scale=math.nan)),
+    *[("attn", {n: None}) for n in ("q", "table", "row0", "kv_len", "out")],
+    ("sample", dict(V=0)), ("sample", dict(V=(1 << 20) + 1, ldl=1 << 21)), ("sample", dict(ldl=999)),
+    *[("sample", {n: None}) for n in ("logits", "u", "token")],
+]
+
+
+@pytest.mark.parametrize("op,change", REFUSED, ids=lambda v: str(v))
+def test_refused_before_any_hip_call(op, change):
+    assert launch(op, dataclasses.replace(VALID[op], **change)) == ARGS
+    assert h.last_error()
+
+
+@pytest.mark.parametrize("op", ["rope", "attn"])
+@pytest.mark.parametrize("change", [
+    dict(type=2), dict(page=8), dict(page=512), dict(page=24), dict(dim=96), dict(heads=0), dict(k=None), dict(v=None),
+    dict(k=A + 8), dict(v=A + 8), dict(pages=0), dict(pages=1 << 25), dict(tok_stride=248), dict(tok_stride=260),
+    dict(head_stride=-8), dict(head_stride=4), dict(page_stride=12)], ids=str)
+def test_caches_refused(op, change):
+    assert launch(op, VALID[op], dataclasses.replace(KV, **change)) == ARGS
+
+
+@pytest.mark.parametrize("op", list(VALID))
+def test_null_arguments(op):
+    assert launch(op, None) == ARGS
+    if op in ("rope", "attn"):
+        assert launch(op, VALID[op], None) == ARGS
+
+
+@pytest.mark.parametrize("op,change", [("plan", {}), ("plan", dict(parent=None, tree=None)), ("plan", dict(T=0, pos=None, slot=None)),
+                                       ("rope", {}), ("rope", dict(q=None)), ("rope", dict(k=None, v=None, slot=None)),
+                                       ("rope", dict(n_rot=0, turns=None, pos=None)), ("rope", dict(n_rot=62)),
+                                       ("attn", {}), ("attn", dict(tree=None)), ("sample", {}),
+                                       ("sample", dict(temperature=None, top_k=None, top_p=None, min_p=None, logprob=None)),
+                                       ("sample", dict(M=1, ldl=0))], ids=lambda v: str(v))
+def test_valid_arguments_need_a_device(op, change):
+    assert launch(op, dataclasses.replace(VALID[op], **change)) == NOT_INIT
+
+
+@pytest.mark.parametrize("op,change", [("plan", dict(S=0)), ("plan", dict(S=-1)), ("rope", dict(T=0)), ("attn", dict(T=0)),
+                                       ("attn", dict(S=0)), ("sample", dict(M=0)), ("sample", dict(M=-3))], ids=lambda v: str(v))
+def test_nothing_to_do(op, change):
+    assert launch(op, dataclasses.replace(VALID[op], **change)) == h.BTF_OK
+
+
+def test_missing_workspace():
+    if h.paged_attention_ws_bytes(2, 8, 20, KV) > 0:
+        assert launch("attn", dataclasses.replace(ATTN, ws=None)) == ARGS
+        assert launch("attn", dataclasses.replace(ATTN, ws=A + 8)) == ARGS
+    if h.sample_ws_bytes(2, 1000) > 0:
+        assert launch("sample", dataclasses.replace(SAMPLE, ws=None)) == ARGS
+        assert launch("sample", dataclasses.replace(SAMPLE, ws=A + 4)) == ARGS
+
+
+def test_workspace_of_nothing():
+    assert h.paged_attention_ws_bytes(0, 8, 20, KV) == 0
+    assert h.paged_attention_ws_bytes(2, 8, 18, KV) == 0
+    assert h.paged_attention_ws_bytes(2, 8, 20, dataclasses.replace(KV, dim=96)) == 0
+    assert h.sample_ws_bytes(0, 1000) == 0 and h.sample_ws_bytes(2, 0) == 0
+
+
+def test_struct_layouts(tmp_path):
+    """The ctypes structs have the header's sizes and field offsets."""
+    structs = {"btf_kv_cache": h._KvCache, "btf_page_plan": h._PagePlan, "btf_rope_scale": h._RopeScale,
+               "btf_rope_cache": h._RopeCache, "btf_paged_attention": h._PagedAttention, "btf_sampling": h._Sampling}
+    src = ["#include <stdio.h>", "#include <stddef.h>", '#include "btf/hip_abi.h"', "int main(void) {"]
+    want = []
+    for name, c in structs.items():
+        src.append(f'printf("%zu\\n", sizeof({name}));')
+        want.append(str(__import__("ctypes").sizeof(c)))
+        for f, _ in c._fields_:
+            src.append(f'printf("%zu\\n", offsetof({name}, {f}));')
+            want.append(str(getattr(c, f).offset))
+    (tmp_path / "s.c").write_text("\n".join(src + ["return 0; }"]))
+    subprocess.run(["cc", "-I", os.path.join(ROOT, "include"), str(tmp_path / "s.c"), "-o", str(tmp_path / "s")], check=True)
+    assert subprocess.run([str(tmp_path / "s")], capture_output=True, text=True, check=True).stdout.split() == want
+
+
+# ---- the table of frequencies (host) ----
+@pytest.mark.parametrize("n_rot", [2, 6, 64, 128, 246, 256])
+@pytest.mark.parametrize("base", [1e4, 1e7])
+def test_rope_table_plain_linear_ntk(n_rot, base):
+    i = np.arange(n_rot // 2)
+    plain = base ** (-2.0 * i / n_rot) / (2 * math.pi)
+    turns, m = h.rope_table(n_rot, base)
+    np.testing.assert_allclose(turns, plain, rtol=1e-13)
+    assert m == 1.0
+    turns, m = h.rope_table(n_rot, base, h.RopeScale(h.RopeScaling.linear, 8.0))
+    np.testing.assert_allclose(turns, plain / 8, rtol=1e-13)
+    assert m == 1.0
+    if n_rot > 2:
+        turns, m = h.rope_table(n_rot, base, h.RopeScale(h.RopeScaling.ntk, 4.0))
+        np.testing.assert_allclose(turns, (base * 4.0 ** (n_rot / (n_rot - 2))) ** (-2.0 * i / n_rot) / (2 * math.pi), rtol=1e-12)
+        # the slowest pair is stretched by the whole factor, the fastest not at all
+        np.testing.assert_allclose([turns[0], turns[-1]], [plain[0], plain[-1] / 4.0], rtol=1e-12)
+
+
+@pytest.mark.parametrize("n_rot,trained,factor", [(64, 32768, 4.0), (128, 4096, 16.0), (256, 8192, 2.0)])
+def test_rope_table_yarn(n_rot, trained, factor):
+    base = 1e6
+    plain = np.array(h.rope_table(n_rot, base)[0])
+    turns, m = h.rope_table(n_rot, base, h.RopeScale(h.RopeScaling.yarn, factor, trained, 32.0, 1.0))
+    assert m == pytest.approx(0.1 * math.log(factor) + 1, rel=1e-7)
+    ratio = plain / np.array(turns)
+    # pairs that turn often over the trained context keep their frequency, slow ones are stretched, between them a ramp
+    assert np.all(np.diff(ratio) >= -1e-9)
+    np.testing.assert_allclose(ratio[plain * trained > 32.0 * base ** (2.0 / n_rot)], 1.0, rtol=1e-12)
+    np.testing.assert_allclose(ratio[plain * trained < 1.0 / base ** (2.0 / n_rot)], factor, rtol=1e-12)
+    assert ratio[0] == pytest.approx(1.0) and ratio[-1] == pytest.approx(factor)
+
+
+@pytest.mark.parametrize("n_rot,base,scale", [
+    (0, 1e4, None), (3, 1e4, None), (64, 1.0, None), (64, math.nan, None), (64, 1e4, h.RopeScale(4, 2.0)),
+    (64, 1e4, h.RopeScale(1, 0.5)), (2, 1e4, h.RopeScale(2, 2.0)), (64, 1e4, h.RopeScale(3, 2.0, 0.0)),
+    (64, 1e4, h.RopeScale(3, 2.0, 4096.0, 1.0, 32.0)), (64, 1e4, h.RopeScale(1, math.nan))], ids=str)
+def test_rope_table_refused(n_rot, base, scale):
+    with pytest.raises(RuntimeError, match="rope_table"):
+        h.rope_table(n_rot, base, scale)
