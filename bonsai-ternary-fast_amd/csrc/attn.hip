@@ -1,8 +1,35 @@
 // attn.hip -- attention of a step's rows over the paged KV cache
 // (btf_hip_launch_paged_attention; gfx950).
 //
-// One wave per row and head: the keys one after the other with the running
-// maximum and sum of the softmax, the head's values spread over the lanes.
+// Work. A request's rows are its new tokens times the G = heads / kv->heads
+// query heads of one KV head, in tiles of R; its keys are cut into pieces of C.
+// An item, the work of one workgroup, is one (request, KV head, row tile,
+// piece). C follows from all requests' lengths (read on the device), so that
+// about kTarget items of like size come out whatever the lengths: one long
+// request among short ones is cut, the short ones are not. An item of a request
+// that is not cut writes out; the others leave (maximum, sum, values) in the
+// workspace and attn_join_kernel puts the pieces of a row together.
+//
+// Inside an item each of 4 waves takes every fourth block of 32 keys, with its
+// own running maximum m and sum l of the softmax, and the waves join in LDS at
+// the end. Scores come transposed, S^T = K Q^T, from 16x16x32 MFMA: a lane then
+// has one row (column of the result) and, of two key tiles, eight keys. Which
+// eight is free, as any order of the keys will do if V has the same: tile t row
+// m is key 8 (m / 4) + 4 t + m % 4, so lane group g (lanes 16 g ..) holds keys
+// 8 g .. 8 g + 7, which is also what the second product wants from it, O^T = V^T
+// P^T: no probability changes its lane. V^T's operand, eight keys of one dim, is
+// put together from eight 16-byte loads (eight dims of one key) by one byte
+// permute per register: lane c of a group reads dims 8 c .. 8 c + 7 and serves
+// MFMA e with dim 8 c + e. K and V go from HBM to registers, with no LDS between.
+//
+// Probabilities are 32-bit; as MFMA takes 16-bit factors they are carried in
+// parts, p = hi + lo (+ lo2 for bf16), each the rounding of what the parts
+// before leave: 22 and 24 bits. One part would put 2^-12 or 2^-9 on fp32 output.
+//
+// What a row does not see takes no part, whatever it holds: masked scores become
+// -infinity, V of keys behind the end is cleared. Where V or a score is not
+// finite all the same (0 * infinity in a product), the item's result shows it,
+// and the item is done again one row at a time by the plain loop.
 #include <string>
 
 #include "../../include/btf/hip_abi.h"
@@ -11,74 +38,474 @@
 namespace btfhip {
 namespace {
 
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef __bf16 b8 __attribute__((ext_vector_type(8)));
+
+constexpr int kWaves = 4;
+constexpr int kKeys = 32;      // keys of a block
+constexpr int kStep = kWaves * kKeys;
+constexpr int kTarget = 512;   // items that a launch is cut into: two for each CU
+
 template <bool BF>
 __device__ __forceinline__ float from16(uint16_t h) {
   if (BF) return __uint_as_float((uint32_t)h << 16);
   return h2f(h);
 }
 
-template <int D, bool BF>
-__global__ void __launch_bounds__(64) attn_row_kernel(btf_paged_attention a, btf_kv_cache kv) {
-  constexpr int E = D / 64;
-  const int lane = threadIdx.x, t = blockIdx.x, h = blockIdx.y;
-  if (t >= a.row0[a.S]) return;
-  int lo = 0, hi = a.S - 1;  // the last request with row0 <= t that has rows
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (a.row0[mid] <= t) lo = mid;
-    else hi = mid - 1;
+template <bool BF>
+__device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
+  if (BF) return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8, a), __builtin_bit_cast(b8, b), c, 0, 0, 0);
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
+}
+
+// Two values rounded to 16 bits, and what the rounding left.
+template <bool BF>
+__device__ __forceinline__ uint32_t round2(float& x, float& y) {
+  if (BF) {
+    typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+    const b2 r = {(__bf16)x, (__bf16)y};
+    x -= (float)r[0];
+    y -= (float)r[1];
+    return __builtin_bit_cast(uint32_t, r);
   }
-  const int s = lo, i = t - a.row0[s], n = a.row0[s + 1] - a.row0[s];
-  const int kvh = h / (a.heads / kv.heads);
-  const long long cap = (long long)a.ldt * kv.page;
-  const int len = (int)min((long long)a.kv_len[s], cap), ctx = a.kv_len[s] - n;
-  const bool tree = a.tree && n <= BTF_TREE_NODES;
-  const unsigned long long bits = tree ? a.tree[t] : 0;
-  const uint16_t* q = static_cast<const uint16_t*>(a.q) + (size_t)t * a.ldq + h * D + lane * E;
-  float qf[E], o[E] = {};
+  typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+  const h2 r = {(_Float16)x, (_Float16)y};
+  x -= (float)r[0];
+  y -= (float)r[1];
+  return __builtin_bit_cast(uint32_t, r);
+}
+
+// Max / sum over the four lane groups (lanes l, l ^ 16, l ^ 32, l ^ 48).
+__device__ __forceinline__ float groups_max(float v) {
+  auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+}
+__device__ __forceinline__ float groups_sum(float v) {
+  auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+  a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(a[0]) + __uint_as_float(a[1]);
+}
+
+// A request as an item sees it.
+struct Req {
+  int s, row0, n;         // request, its first row, its rows
+  int len, ctx;           // keys; keys before its rows (negative: its first rows see nothing)
+  int tiles, pieces;      // row tiles, pieces of its keys
+  int local;              // the item's (or row's) number in the request's items
+  int slot;               // workspace slot of the request's first item (pieces > 1)
+  int C;                  // keys of a piece
+};
+
+__device__ __forceinline__ int wave_sum_i(int v) {
 #pragma unroll
-  for (int e = 0; e < E; ++e) qf[e] = from16<BF>(q[e]);
-  float m = -INFINITY, l = 0.f;
-  for (int j = 0; j < len; ++j) {
-    const int nj = j - ctx;
-    if (nj >= 0 && (tree ? !(bits >> nj & 1) : nj > i)) continue;
-    const int pg = a.table[(size_t)s * a.ldt + j / kv.page];
+  for (int o = 1; o < 64; o <<= 1) v += __shfl_xor(v, o, 64);
+  return v;
+}
+__device__ __forceinline__ float wave_sum_f(float v) {
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) v += __shfl_xor(v, o, 64);
+  return v;
+}
+
+// The request of item `id` (BY_ROW: of row `id`), found by every wave for itself:
+// the lanes take 64 requests at a time. False: there is no such item.
+template <int R, bool BY_ROW>
+__device__ bool find(const btf_paged_attention& a, const btf_kv_cache& kv, int id, Req& q) {
+  const int lane = threadIdx.x & 63, G = a.heads / kv.heads;
+  const long long cap = (long long)a.ldt * kv.page;
+  auto read = [&](int s, int& r0, int& n, int& len, int& full) {
+    r0 = n = len = full = 0;
+    if (s < a.S) {
+      r0 = a.row0[s];
+      n = min(a.row0[s + 1], a.T) - r0;
+      full = a.kv_len[s];
+      len = (int)max(0ll, min((long long)full, cap));
+    }
+  };
+  float work = 0.f;  // (a whole number below 2^24 times its size: the split need not be exact)
+  int r0, n, len, full;
+  for (int s0 = 0; s0 < a.S; s0 += 64) {
+    read(s0 + lane, r0, n, len, full);
+    if (n > 0) work += (float)((n * G + R - 1) / R) * (float)len;
+  }
+  work = wave_sum_f(work) * (float)kv.heads;
+  const int C = max(kStep, (int)(work / (float)(kTarget * kStep) + 1.f) * kStep);
+  int items = 0, slots = 0;  // before the chunk
+  for (int s0 = 0; s0 < a.S; s0 += 64) {
+    read(s0 + lane, r0, n, len, full);
+    const int tiles = n > 0 ? (n * G + R - 1) / R : 0, pieces = max(1, (len + C - 1) / C);
+    const int mine = kv.heads * tiles * pieces, cut = pieces > 1 ? mine : 0;
+    int upto = mine, cuts = cut;  // inclusive sums
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int u = __shfl_up(upto, o, 64), w = __shfl_up(cuts, o, 64);
+      if (lane >= o) upto += u, cuts += w;
+    }
+    const bool here = BY_ROW ? n > 0 && id >= r0 && id < r0 + n : mine > 0 && id >= items + upto - mine && id < items + upto;
+    const unsigned long long who = __ballot(here);
+    if (who) {
+      const int l = __builtin_ctzll(who);
+      q.s = s0 + l;
+      q.row0 = __shfl(r0, l, 64);
+      q.n = __shfl(n, l, 64);
+      q.len = __shfl(len, l, 64);
+      q.ctx = __shfl(full, l, 64) - q.n;
+      q.tiles = __shfl(tiles, l, 64);
+      q.pieces = __shfl(pieces, l, 64);
+      q.local = id - (BY_ROW ? q.row0 : items + __shfl(upto - mine, l, 64));
+      q.slot = slots + __shfl(cuts - cut, l, 64);
+      q.C = C;
+      return true;
+    }
+    items += __shfl(upto, 63, 64);
+    slots += __shfl(cuts, 63, 64);
+  }
+  return false;
+}
+
+// A workspace slot: R rows of D values, then R maxima, then R sums.
+template <int D, int R>
+constexpr size_t kSlot = (size_t)R * (D + 2);
+
+// Row r of the item by the plain loop over keys [k0, k1), by one wave: lane's
+// D / 64 values, the row's maximum and sum. Any input.
+template <int D, bool BF>
+__device__ void plain_row(const btf_paged_attention& a, const btf_kv_cache& kv, const Req& q, int kvh, int row, int k0, int k1,
+                          float c2, float* o, float& m, float& l) {
+  constexpr int E = D / 64;
+  const int lane = threadIdx.x & 63, G = a.heads / kv.heads, i = row / G, t = q.row0 + i, h = kvh * G + row % G;
+  const bool tree = a.tree && q.n <= BTF_TREE_NODES;
+  const unsigned long long bits = tree ? a.tree[t] : 0;
+  const uint16_t* x = static_cast<const uint16_t*>(a.q) + (size_t)t * a.ldq + h * D + lane * E;
+  float qf[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) qf[e] = from16<BF>(x[e]), o[e] = 0.f;
+  m = -INFINITY, l = 0.f;
+  for (int j = k0; j < k1; ++j) {
+    const int nj = j - q.ctx;
+    if (nj >= 0 && (tree ? nj >= 64 || !(bits >> nj & 1) : nj > i)) continue;
+    const int pg = a.table[(size_t)q.s * a.ldt + j / kv.page];
     if (pg < 0 || pg >= kv.pages) continue;
     const size_t at = (size_t)pg * kv.page_stride + (size_t)kvh * kv.head_stride + (size_t)(j % kv.page) * kv.tok_stride +
                       lane * E;
-    float x = 0.f;
+    float d = 0.f;
 #pragma unroll
-    for (int e = 0; e < E; ++e) x += qf[e] * from16<BF>(static_cast<const uint16_t*>(kv.k)[at + e]);
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) x += __shfl_xor(x, d, 64);
-    x *= a.scale;
-    if (x == -INFINITY) continue;
-    const float mn = fmaxf(m, x), c = __expf(m - mn), p = __expf(x - mn);
+    for (int e = 0; e < E; ++e) d += qf[e] * from16<BF>(static_cast<const uint16_t*>(kv.k)[at + e]);
+    d = wave_sum_f(d) * c2;
+    if (d == -INFINITY) continue;
+    const float mn = fmaxf(m, d), c = exp2f(m - mn), p = exp2f(d - mn);
     l = l * c + p;
 #pragma unroll
     for (int e = 0; e < E; ++e) o[e] = o[e] * c + p * from16<BF>(static_cast<const uint16_t*>(kv.v)[at + e]);
     m = mn;
   }
-  float* y = a.out + (size_t)t * a.ldo + h * D + lane * E;
+}
+
+template <int D, bool BF, int RT>
+__global__ void __launch_bounds__(64 * kWaves) attn_stream_kernel(btf_paged_attention a, btf_kv_cache kv) {
+  constexpr int R = 16 * RT;             // rows of a tile
+  constexpr int KS = D / 32;             // steps over the dims in Q K^T
+  constexpr int VD = D < 128 ? D / 16 : 8;  // dims that a lane reads of a key of V
+  constexpr int VG = D / (16 * VD);      // ... in so many groups of 16 lanes
+  constexpr int PARTS = BF ? 3 : 2;      // 16-bit parts of a probability
+  constexpr int LD = D + 4;              // row of a wave's values in LDS, in floats
+  __shared__ float sh_o[kWaves * R * LD];
+  __shared__ float sh_m[kWaves][R], sh_l[kWaves][R];
+  __shared__ int sh_odd;
+
+  Req q;
+  if (!find<R, false>(a, kv, blockIdx.x, q)) return;  // the whole workgroup
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int c16 = lane & 15, g = lane >> 4;
+  const int G = a.heads / kv.heads;
+  const int tile = q.local % q.tiles, rest = q.local / q.tiles;
+  const int piece = rest % q.pieces, kvh = rest / q.pieces;
+  const int nrows = min(R, q.n * G - tile * R);  // of this tile
+  const bool tree = a.tree && q.n <= BTF_TREE_NODES;
+  const float c2 = a.scale * 1.4426950408889634f;  // scores in powers of two
+  // keys: [k0, k1) is the piece, cut behind the last key that any row of the tile sees; all rows see those before `all`
+  const int i0 = tile * R / G, i1 = (tile * R + nrows - 1) / G;
+  const int kend = tree ? q.len : max(0, min(q.len, q.ctx + i1 + 1));
+  const int k0 = piece * q.C, k1 = min(kend, k0 + q.C);
+  const int all = min(kend, tree ? q.ctx : q.ctx + i0 + 1);
+
+  // Q^T: row c16 of row tile rt, dims 32 ks + 8 g ..
+  u32x4 qf[RT][KS];
+  int tok[RT];                     // the lane's row: its token
+  unsigned long long bits[RT];
 #pragma unroll
-  for (int e = 0; e < E; ++e) y[e] = l == 0.f ? 0.f : o[e] / l;
+  for (int rt = 0; rt < RT; ++rt) {
+    const int row = tile * R + rt * 16 + c16;
+    const bool live = rt * 16 + c16 < nrows;
+    tok[rt] = live ? row / G : -1;
+    bits[rt] = tree && live ? a.tree[q.row0 + row / G] : 0;
+    const uint16_t* x = static_cast<const uint16_t*>(a.q) + (size_t)(q.row0 + row / G) * a.ldq + (kvh * G + row % G) * D + 8 * g;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) qf[rt][ks] = live ? *reinterpret_cast<const u32x4*>(x + 32 * ks) : u32x4{0, 0, 0, 0};
+  }
+  f32x4 o[RT][VG][VD];
+  float m[RT], l[RT];
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    m[rt] = -INFINITY, l[rt] = 0.f;
+#pragma unroll
+    for (int i = 0; i < VG; ++i)
+#pragma unroll
+      for (int e = 0; e < VD; ++e) o[rt][i][e] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+
+  const uint16_t* kp = static_cast<const uint16_t*>(kv.k) + (size_t)kvh * kv.head_stride;
+  const uint16_t* vp = static_cast<const uint16_t*>(kv.v) + (size_t)kvh * kv.head_stride;
+  const int* tab = a.table + (size_t)q.s * a.ldt;
+  const int sh = __builtin_ctz(kv.page), last = (q.len - 1) >> sh;
+  // the lane's key of K in a block (tile 0; tile 1: 4 on) and first key of V
+  const int kk = 8 * (c16 >> 2) + (c16 & 3), kv0 = 8 * g;
+  auto page_of = [&](int key) {  // page id of a key, -1: none
+    const int p = key < q.len ? tab[min(key >> sh, last)] : -1;
+    return p >= 0 && p < kv.pages ? p : -1;
+  };
+  u32x4 kf[2][KS];
+  auto load_k = [&](int kb, int pg) {
+    const uint16_t* x = kp + (size_t)max(pg, 0) * kv.page_stride + (size_t)((kb + kk) & (kv.page - 1)) * kv.tok_stride + 8 * g;
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) kf[t][ks] = *reinterpret_cast<const u32x4*>(x + (size_t)(4 * t) * kv.tok_stride + 32 * ks);
+  };
+  typedef uint32_t vdw __attribute__((ext_vector_type(VD / 2)));
+  vdw vf[VG][8];
+  auto load_v = [&](int kb, int pg) {
+    const uint16_t* x = vp + (size_t)max(pg, 0) * kv.page_stride + (size_t)((kb + kv0) & (kv.page - 1)) * kv.tok_stride + VD * c16;
+#pragma unroll
+    for (int i = 0; i < VG; ++i)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) vf[i][j] = *reinterpret_cast<const vdw*>(x + (size_t)j * kv.tok_stride + 16 * VD * i);
+  };
+
+  int kb = k0 + w * kKeys;
+  int pk = kb < k1 ? page_of(kb + kk) : -1, pv = kb < k1 ? page_of(kb + kv0) : -1;
+  if (kb < k1) {
+    load_k(kb, pk);
+    load_v(kb, pv);
+  }
+  for (; kb < k1; kb += kStep) {
+    const int nb = kb + kStep;
+    const bool more = nb < k1;
+    int npk = -1, npv = -1;
+    if (more) npk = page_of(nb + kk), npv = page_of(nb + kv0);
+    f32x4 s[RT][2];
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        s[rt][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) s[rt][t] = mfma<BF>(kf[t][ks], qf[rt][ks], s[rt][t]);
+      }
+    // a block that some row does not see all of
+    const bool edge = kb + kKeys > all || __any(pk < 0 || pv < 0);
+    if (edge) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int key = kb + kv0 + j, nj = key - q.ctx;
+        if (pv < 0 || key >= k1)
+#pragma unroll
+          for (int i = 0; i < VG; ++i) vf[i][j] = vdw(0);
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+          const bool see = pv >= 0 && key < k1 && (nj < 0 || (tree ? nj < 64 && (bits[rt] >> (nj & 63) & 1) : nj <= tok[rt]));
+          if (!see) s[rt][j >> 2][j & 3] = -INFINITY;
+          else s[rt][j >> 2][j & 3] *= c2;
+        }
+      }
+    } else {
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+        for (int t = 0; t < 2; ++t) s[rt][t] *= c2;
+    }
+    if (more) load_k(nb, npk);
+    // the running maximum and sum; probabilities in 16-bit parts, keys 8 g .. 8 g + 7
+    u32x4 p[RT][PARTS];
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      float mx = fmaxf(fmaxf(fmaxf(s[rt][0][0], s[rt][0][1]), fmaxf(s[rt][0][2], s[rt][0][3])),
+                       fmaxf(fmaxf(s[rt][1][0], s[rt][1][1]), fmaxf(s[rt][1][2], s[rt][1][3])));
+      const float mn = fmaxf(m[rt], groups_max(mx));
+      if (__any(mn > m[rt])) {
+        const float c = mn == -INFINITY ? 1.f : exp2f(m[rt] - mn);
+        l[rt] *= c;
+#pragma unroll
+        for (int i = 0; i < VG; ++i)
+#pragma unroll
+          for (int e = 0; e < VD; ++e) o[rt][i][e] *= c;
+        m[rt] = mn;
+      }
+      const float base = m[rt] == -INFINITY ? 0.f : m[rt];
+      float x[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        x[j] = exp2f(s[rt][j >> 2][j & 3] - base);
+        l[rt] += x[j];
+      }
+#pragma unroll
+      for (int n = 0; n < PARTS; ++n)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) p[rt][n][j] = round2<BF>(x[2 * j], x[2 * j + 1]);
+    }
+    // O^T += V^T P^T: dim VD c16 + e of each lane group's eight keys
+#pragma unroll
+    for (int i = 0; i < VG; ++i)
+#pragma unroll
+      for (int e = 0; e < VD; ++e) {
+        u32x4 vt;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          vt[j] = __builtin_amdgcn_perm(vf[i][2 * j + 1][e >> 1], vf[i][2 * j][e >> 1], (e & 1) ? 0x07060302u : 0x05040100u);
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+          for (int n = 0; n < PARTS; ++n) o[rt][i][e] = mfma<BF>(vt, p[rt][n], o[rt][i][e]);
+      }
+    if (more) load_v(nb, npv);
+    pk = npk, pv = npv;
+  }
+
+  // join the waves
+  if (threadIdx.x == 0) sh_odd = 0;
+  __syncthreads();
+  bool odd = false;
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    l[rt] = groups_sum(l[rt]);
+    float chk = l[rt];
+    if (g == 0) sh_m[w][rt * 16 + c16] = m[rt], sh_l[w][rt * 16 + c16] = l[rt];
+    float* y = sh_o + (size_t)(w * R + rt * 16 + c16) * LD;
+#pragma unroll
+    for (int i = 0; i < VG; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {  // row r of the MFMA tiles: dim VD (4 g + r) + e
+#pragma unroll
+        for (int e = 0; e < VD; e += 4) {
+          const f32x4 v = {o[rt][i][e][r], o[rt][i][e + 1][r], o[rt][i][e + 2][r], o[rt][i][e + 3][r]};
+          chk += (v[0] - v[0]) + (v[1] - v[1]) + (v[2] - v[2]) + (v[3] - v[3]);
+          *reinterpret_cast<f32x4*>(y + 16 * VD * i + VD * (4 * g + r) + e) = v;
+        }
+      }
+    odd |= !(fabsf(chk) < INFINITY);  // (x - x is NaN for an infinity and for NaN)
+  }
+  if (__any(odd) && lane == 0) sh_odd = 1;
+  __syncthreads();
+
+  const bool cut = q.pieces > 1;
+  float* slot = nullptr;
+  if (cut) slot = static_cast<float*>(a.ws) + (size_t)(q.slot + q.local) * kSlot<D, R>;
+  if (sh_odd) {
+    for (int r = w; r < nrows; r += kWaves) {
+      constexpr int E = D / 64;
+      float po[E], pm, pl;
+      const int row = tile * R + r;
+      plain_row<D, BF>(a, kv, q, kvh, row, k0, max(k0, k1), c2, po, pm, pl);
+      float* y = cut ? slot + (size_t)r * D : a.out + (size_t)(q.row0 + row / G) * a.ldo + (kvh * G + row % G) * D;
+#pragma unroll
+      for (int e = 0; e < E; ++e) y[lane * E + e] = cut ? po[e] : pl == 0.f ? 0.f : po[e] / pl;
+      if (cut && lane == 0) slot[R * D + r] = pm, slot[R * D + R + r] = pl;
+    }
+    return;
+  }
+  constexpr int TPR = D / 4, RPP = 64 * kWaves / TPR;  // threads per row (4 values each), rows at a time
+  const int d4 = (threadIdx.x % TPR) * 4;
+  for (int r = threadIdx.x / TPR; r < nrows; r += RPP) {
+    float top = sh_m[0][r];
+#pragma unroll
+    for (int i = 1; i < kWaves; ++i) top = fmaxf(top, sh_m[i][r]);
+    const float base = top == -INFINITY ? 0.f : top;
+    float sum = 0.f;
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < kWaves; ++i) {
+      const float c = exp2f(sh_m[i][r] - base);
+      sum += c * sh_l[i][r];
+      v += c * *reinterpret_cast<const f32x4*>(sh_o + (size_t)(i * R + r) * LD + d4);
+    }
+    const int row = tile * R + r;
+    if (cut) {
+      *reinterpret_cast<f32x4*>(slot + (size_t)r * D + d4) = v;
+      if (d4 == 0) slot[R * D + r] = top, slot[R * D + R + r] = sum;
+    } else {
+      const float inv = sum == 0.f ? 0.f : 1.f / sum;
+      *reinterpret_cast<f32x4*>(a.out + (size_t)(q.row0 + row / G) * a.ldo + (kvh * G + row % G) * D + d4) = v * inv;
+    }
+  }
+}
+
+// The pieces of one row of one head put together: D / 4 threads, four values each.
+template <int D, int R>
+__global__ void __launch_bounds__(D / 4 < 64 ? 64 : D / 4) attn_join_kernel(btf_paged_attention a, btf_kv_cache kv) {
+  Req q;
+  if (!find<R, true>(a, kv, blockIdx.x, q) || q.pieces == 1) return;
+  if (threadIdx.x >= D / 4) return;
+  const int G = a.heads / kv.heads, h = blockIdx.y, kvh = h / G;
+  const int row = q.local * G + h % G, tile = row / R, r = row % R, d4 = threadIdx.x * 4;
+  const float* slot = static_cast<const float*>(a.ws) +
+                      (size_t)(q.slot + (kvh * q.pieces) * q.tiles + tile) * kSlot<D, R>;
+  const size_t step = (size_t)q.tiles * kSlot<D, R>;
+  float top = -INFINITY;
+  for (int i = 0; i < q.pieces; ++i) top = fmaxf(top, slot[i * step + R * D + r]);
+  const float base = top == -INFINITY ? 0.f : top;
+  float sum = 0.f;
+  f32x4 v = {0.f, 0.f, 0.f, 0.f};
+  for (int i = 0; i < q.pieces; ++i) {
+    const float* x = slot + i * step;
+    const float c = exp2f(x[R * D + r] - base);
+    sum += c * x[R * D + R + r];
+    v += c * *reinterpret_cast<const f32x4*>(x + (size_t)r * D + d4);
+  }
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  *reinterpret_cast<f32x4*>(a.out + (size_t)(q.row0 + q.local) * a.ldo + h * D + d4) = v * inv;
+}
+
+// Row tiles: one or two of 16, by the rows that a request has on average.
+int row_tiles(int S, int T, int heads, const btf_kv_cache& kv) {
+  return (int64_t)T * (heads / kv.heads) > 16 * (int64_t)S ? 2 : 1;
+}
+
+template <int D, bool BF, int RT>
+int attn_go(const btf_paged_attention& a, const btf_kv_cache& kv, hipStream_t st) {
+  constexpr int R = 16 * RT;
+  const int64_t tiles = (int64_t)a.T * (a.heads / kv.heads) / R + a.S;  // at most
+  hipLaunchKernelGGL((attn_stream_kernel<D, BF, RT>), dim3((unsigned)(kTarget + tiles * kv.heads)), dim3(64 * kWaves), 0, st, a, kv);
+  const int rc = launch_status("attn_stream_kernel");
+  if (rc != BTF_OK) return rc;
+  hipLaunchKernelGGL((attn_join_kernel<D, R>), dim3(a.T, a.heads), dim3(D / 4 < 64 ? 64 : D / 4), 0, st, a, kv);
+  return launch_status("attn_join_kernel");
 }
 
 template <int D, bool BF>
-void attn_go(const btf_paged_attention& a, const btf_kv_cache& kv, hipStream_t st) {
-  hipLaunchKernelGGL((attn_row_kernel<D, BF>), dim3(a.T, a.heads), dim3(64), 0, st, a, kv);
+int attn_pick(const btf_paged_attention& a, const btf_kv_cache& kv, hipStream_t st) {
+  return row_tiles(a.S, a.T, a.heads, kv) == 1 ? attn_go<D, BF, 1>(a, kv, st) : attn_go<D, BF, 2>(a, kv, st);
 }
 
 }  // namespace
 
-int64_t paged_attention_ws_bytes(int S, int T, int heads, const btf_kv_cache& kv) { return 0; }
+// Cut requests have at most 2 kTarget items: a piece of them holds C keys, or at least half of it on average, and C is
+// at least all the work over kTarget.
+int64_t paged_attention_ws_bytes(int S, int T, int heads, const btf_kv_cache& kv) {
+  const int R = 16 * row_tiles(S, T, heads, kv);
+  return (int64_t)2 * kTarget * R * (kv.dim + 2) * 4;
+}
 
 int paged_attention(const btf_paged_attention& a, const btf_kv_cache& kv, hipStream_t st, const DevState& ds) {
   const bool bf = kv.type == BTF_BF16;
-  if (kv.dim == 64) bf ? attn_go<64, true>(a, kv, st) : attn_go<64, false>(a, kv, st);
-  else if (kv.dim == 128) bf ? attn_go<128, true>(a, kv, st) : attn_go<128, false>(a, kv, st);
-  else bf ? attn_go<256, true>(a, kv, st) : attn_go<256, false>(a, kv, st);
-  return launch_status("attn_row_kernel");
+  if (kv.dim == 64) return bf ? attn_pick<64, true>(a, kv, st) : attn_pick<64, false>(a, kv, st);
+  if (kv.dim == 128) return bf ? attn_pick<128, true>(a, kv, st) : attn_pick<128, false>(a, kv, st);
+  return bf ? attn_pick<256, true>(a, kv, st) : attn_pick<256, false>(a, kv, st);
 }
 
 }  // namespace btfhip
