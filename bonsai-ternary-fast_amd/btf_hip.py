@@ -40,7 +40,8 @@ else:
     class _call:
         """No native calls: every launch takes the ctypes path."""
         prep = gemv = gemv_ptq1_0 = gemv_ex = staticmethod(lambda *args: NotImplemented)
-        bind = staticmethod(lambda *args: None)
+        launch = staticmethod(lambda *args: NotImplemented)
+        bind = layout = staticmethod(lambda *args: None)
 
 BTF_OK, BTF_ERR_ARGS, BTF_ERR_DEVICE, BTF_ERR_LAUNCH, BTF_ERR_NOT_INIT = 0, 1, 2, 3, 4
 
@@ -485,6 +486,14 @@ class Sampling:
 # those do not read (NotImplemented) take the ctypes path.
 _call.bind(*[C.cast(f, C.c_void_p).value for f in (_launch_prep, _launch_gemv, _launch_gemv_ptq1_0, _launch_gemv_ex)],
            Q8Act, Hx, GemvSeg)
+_kv_layout, _plan_layout, _rope_layout, _attn_layout, _sample_layout = (
+    _call.layout(_cls, tuple((_f, {C.c_int: "i", C.c_int64: "q", C.c_float: "f", C.c_void_p: "p"}[_t],
+                              getattr(_c_struct, _n).offset)
+                             for _f, (_n, _t) in zip(_cls.__dataclass_fields__, _c_struct._fields_)), C.sizeof(_c_struct))
+    for _cls, _c_struct in ((KvCache, _KvCache), (PagePlan, _PagePlan), (RopeCache, _RopeCache),
+                            (PagedAttention, _PagedAttention), (Sampling, _Sampling)))
+_addr_page_plan, _addr_rope_cache, _addr_paged_attention, _addr_sample = (
+    C.cast(f, C.c_void_p).value for f in (_launch_page_plan, _launch_rope_cache, _launch_paged_attention, _launch_sample))
 
 
 def kernels_init(device: int = 0) -> None:
@@ -570,6 +579,11 @@ def launch_pos_add(d_pos, M: int, stream=None) -> None:
 
 def launch_page_plan(a: PagePlan, stream=None) -> None:
     """Rows, positions, cache slots and pages of a step (btf_hip_launch_page_plan)."""
+    rc = _call.launch(_addr_page_plan, _plan_layout, a, -1, None, stream)
+    if rc is not NotImplemented:
+        if rc:
+            _check(rc)
+        return
     _check(launch_page_plan_raw(a, stream))
 
 
@@ -586,6 +600,11 @@ def rope_table(n_rot: int, base: float, scale: RopeScale = None):
 
 def launch_rope_cache(a: RopeCache, kv: KvCache, stream=None) -> None:
     """Head norms, rotary positions and the cache write (btf_hip_launch_rope_cache)."""
+    rc = _call.launch(_addr_rope_cache, _rope_layout, a, _kv_layout, kv, stream)
+    if rc is not NotImplemented:
+        if rc:
+            _check(rc)
+        return
     _check(launch_rope_cache_raw(a, kv, stream))
 
 
@@ -600,6 +619,11 @@ def paged_attention_ws_bytes(S: int, T: int, heads: int, kv: KvCache) -> int:
 
 def launch_paged_attention(a: PagedAttention, kv: KvCache, stream=None) -> None:
     """Attention of a step's rows over the paged cache (btf_hip_launch_paged_attention)."""
+    rc = _call.launch(_addr_paged_attention, _attn_layout, a, _kv_layout, kv, stream)
+    if rc is not NotImplemented:
+        if rc:
+            _check(rc)
+        return
     _check(launch_paged_attention_raw(a, kv, stream))
 
 
@@ -614,6 +638,11 @@ def sample_ws_bytes(M: int, V: int) -> int:
 
 def launch_sample(a: Sampling, stream=None) -> None:
     """One token per row with temperature, top-k, top-p and min-p (btf_hip_launch_sample)."""
+    rc = _call.launch(_addr_sample, _sample_layout, a, -1, None, stream)
+    if rc is not NotImplemented:
+        if rc:
+            _check(rc)
+        return
     _check(launch_sample_raw(a, stream))
 
 

@@ -200,12 +200,108 @@ static int do_gemv_ex(PyObject* const* v, int* status) {
   return OK;
 }
 
+/* ---- launches that take one argument struct, or two (a serving step's operators) ----
+ * layout(cls, fields, size) describes the C struct of a class of btf_hip.py:
+ * fields = ((name, kind, offset), ...), kind i int, q int64, f float, p pointer. */
+#define MAX_LAYOUTS 8
+#define MAX_FIELDS 24
+#define MAX_STRUCT 256
+typedef struct {
+  PyObject* cls;
+  Py_ssize_t n;
+  struct {
+    PyObject* name;
+    char kind;
+    Py_ssize_t offset;
+  } f[MAX_FIELDS];
+} layout_t;
+static layout_t layouts[MAX_LAYOUTS];
+static int n_layouts;
+
+static PyObject* py_layout(PyObject* self, PyObject* const* v, Py_ssize_t n) {
+  if (n != 3 || !PyTuple_CheckExact(v[1]) || PyTuple_GET_SIZE(v[1]) > MAX_FIELDS || PyLong_AsSsize_t(v[2]) > MAX_STRUCT ||
+      n_layouts == MAX_LAYOUTS) {
+    if (!PyErr_Occurred()) PyErr_SetString(PyExc_ValueError, "layout(cls, fields, size)");
+    return NULL;
+  }
+  layout_t* L = &layouts[n_layouts];
+  for (L->n = 0; L->n < PyTuple_GET_SIZE(v[1]); ++L->n) {
+    const char *name, *kind;
+    Py_ssize_t off;
+    if (!PyArg_ParseTuple(PyTuple_GET_ITEM(v[1], L->n), "ssn", &name, &kind, &off)) return NULL;
+    if (off < 0 || off + 8 > MAX_STRUCT) {
+      PyErr_SetString(PyExc_ValueError, "layout: offset");
+      return NULL;
+    }
+    L->f[L->n].name = PyUnicode_InternFromString(name);
+    if (!L->f[L->n].name) return NULL;
+    L->f[L->n].kind = kind[0];
+    L->f[L->n].offset = off;
+  }
+  Py_INCREF(v[0]);
+  L->cls = v[0];
+  return PyLong_FromLong(n_layouts++);
+}
+
+static int read_struct(PyObject* o, int which, char* to) {
+  const layout_t* L = &layouts[which];
+  if ((PyObject*)Py_TYPE(o) != L->cls) return OTHER;
+  for (Py_ssize_t i = 0; i < L->n; ++i) {
+    PyObject* v = PyObject_GetAttr(o, L->f[i].name);
+    if (!v) return RAISED;
+    char* at = to + L->f[i].offset;
+    int rc = OK;
+    switch (L->f[i].kind) {
+      case 'i': rc = read_int(v, (int*)at); break;
+      case 'q':
+        if (PyLong_Check(v)) *(int64_t*)at = (int64_t)PyLong_AsUnsignedLongLongMask(v);
+        else rc = OTHER;
+        break;
+      case 'f':
+        if (PyFloat_CheckExact(v)) *(float*)at = (float)PyFloat_AS_DOUBLE(v);
+        else rc = OTHER;
+        break;
+      default: rc = read_ptr(v, (void**)at);
+    }
+    Py_DECREF(v);
+    if (rc != OK) return rc;
+  }
+  return OK;
+}
+
+/* launch(function address, layout of a, a, layout of b or -1 for a launch without b, b, stream) */
+static int do_launch(PyObject* const* v, int* status) {
+  _Alignas(8) char a[MAX_STRUCT] = {0}, b[MAX_STRUCT] = {0};
+  btf_stream_t st;
+  int la, lb;
+  if (!PyLong_CheckExact(v[0])) return OTHER;
+  void* f = PyLong_AsVoidPtr(v[0]);
+  if (!f) return PyErr_Occurred() ? RAISED : OTHER;
+  TRY(read_int(v[1], &la));
+  TRY(read_int(v[3], &lb));
+  if (la < 0 || la >= n_layouts || lb < -1 || lb >= n_layouts) return OTHER;
+  TRY(read_struct(v[2], la, a));
+  if (lb >= 0) TRY(read_struct(v[4], lb, b));
+  TRY(read_stream(v[5], &st));
+  Py_BEGIN_ALLOW_THREADS
+  *status = lb >= 0 ? ((int (*)(const void*, const void*, btf_stream_t))f)(a, b, st)
+                    : ((int (*)(const void*, btf_stream_t))f)(a, st);
+  Py_END_ALLOW_THREADS
+  return OK;
+}
+
 static int args(Py_ssize_t got, Py_ssize_t want) {
   if (got == want) return 1;
   PyErr_Format(PyExc_TypeError, "%zd arguments, got %zd", want, got);
   return 0;
 }
 
+static PyObject* py_launch(PyObject* self, PyObject* const* v, Py_ssize_t n) {
+  int status = 0;
+  if (!args(n, 6)) return NULL;
+  const int rc = do_launch(v, &status);
+  return answer(rc, status);
+}
 static PyObject* py_prep(PyObject* self, PyObject* const* v, Py_ssize_t n) {
   int status = 0;
   if (!args(n, 11)) return NULL;
@@ -260,6 +356,8 @@ static PyMethodDef methods[] = {
     {"gemv", (PyCFunction)(void (*)(void))py_gemv, METH_FASTCALL, NULL},
     {"gemv_ptq1_0", (PyCFunction)(void (*)(void))py_gemv_ptq1_0, METH_FASTCALL, NULL},
     {"gemv_ex", (PyCFunction)(void (*)(void))py_gemv_ex, METH_FASTCALL, NULL},
+    {"layout", (PyCFunction)(void (*)(void))py_layout, METH_FASTCALL, NULL},
+    {"launch", (PyCFunction)(void (*)(void))py_launch, METH_FASTCALL, NULL},
     {NULL, NULL, 0, NULL}};
 
 static struct PyModuleDef module = {PyModuleDef_HEAD_INIT, "_btf_call", NULL, -1, methods, NULL, NULL, NULL, NULL};

@@ -164,3 +164,63 @@ def test_rope_table_yarn(n_rot, trained, factor):
 def test_rope_table_refused(n_rot, base, scale):
     with pytest.raises(RuntimeError, match="rope_table"):
         h.rope_table(n_rot, base, scale)
+
+
+# ---- the native launch calls ----
+@pytest.mark.skipif(not os.path.exists(h.CALL_PATH), reason="native launch calls not built")
+@pytest.mark.parametrize("op", list(VALID))
+@pytest.mark.parametrize("stream", [None, 0, 1 << 45])
+def test_native_calls_hand_over_the_same_structs(op, stream):
+    """Recorders in place of the launchers: the struct bytes of the native call are those of the ctypes path."""
+    import ctypes as C
+    import torch
+    t = torch.zeros(64)
+    two = op in ("rope", "attn")
+    c_types = {"plan": h._PagePlan, "rope": h._RopeCache, "attn": h._PagedAttention, "sample": h._Sampling}
+    seen = []
+    ptr = [C.POINTER(c_types[op])] + ([C.POINTER(h._KvCache)] if two else []) + [C.c_void_p]
+
+    def record(*v):
+        seen.append(([tuple(getattr(x[0], f) for f, _ in x[0]._fields_) for x in v[:-1]], v[-1]))
+        return 5
+    f = C.CFUNCTYPE(C.c_int, *ptr)(record)
+    a = VALID[op]
+    for name in a.__dataclass_fields__:  # tensors and None among the addresses
+        if getattr(a, name) is A:
+            a = dataclasses.replace(a, **{name: t})
+            break
+    a = dataclasses.replace(a, **{[n for n in a.__dataclass_fields__ if getattr(a, n) is A][-1]: None})
+    kv = dataclasses.replace(KV, v=t) if two else None
+    layout = {"plan": h._plan_layout, "rope": h._rope_layout, "attn": h._attn_layout, "sample": h._sample_layout}[op]
+    rc = h._call.launch(C.cast(f, C.c_void_p).value, layout, a, h._kv_layout if two else -1, kv, stream)
+    assert rc == 5
+    want = [tuple(getattr(x._c(), n) for n, _ in x._c()._fields_) for x in ([a, kv] if two else [a])]
+    assert seen == [(want, stream or None)]
+
+
+@pytest.mark.skipif(not os.path.exists(h.CALL_PATH), reason="native launch calls not built")
+def test_native_calls_leave_other_forms_to_ctypes():
+    class Sub(h.Sampling):
+        pass
+    sample = lambda a: h._call.launch(h._addr_sample, h._sample_layout, a, -1, None, None)  # noqa: E731
+    rope = lambda a, kv: h._call.launch(h._addr_rope_cache, h._rope_layout, a, h._kv_layout, kv, None)  # noqa: E731
+    assert sample(Sub()) is NotImplemented
+    assert sample(None) is NotImplemented
+    assert sample(PLAN) is NotImplemented  # (a struct of another launch)
+    assert sample(dataclasses.replace(SAMPLE, V=3.5)) is NotImplemented
+    assert rope(dataclasses.replace(ROPE, eps=1), KV) is NotImplemented
+    assert rope(ROPE, None) is NotImplemented
+    assert rope(ROPE, SAMPLE) is NotImplemented
+    with pytest.raises(AttributeError):
+        sample(dataclasses.replace(SAMPLE, u=object()))
+    with pytest.raises(TypeError):
+        h._call.launch(h._addr_sample, SAMPLE)
+    with pytest.raises(RuntimeError, match="sample"):
+        h.launch_sample(dataclasses.replace(SAMPLE, V=0))
+    with pytest.raises(RuntimeError, match="null arguments"):
+        h.launch_sample(None)
+    with pytest.raises(RuntimeError, match="null cache"):
+        h.launch_rope_cache(ROPE, None)
+    import ctypes
+    with pytest.raises(ctypes.ArgumentError):
+        h.launch_sample(PLAN)
