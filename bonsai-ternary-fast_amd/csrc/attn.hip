@@ -207,6 +207,36 @@ __device__ void plain_row(const btf_paged_attention& a, const btf_kv_cache& kv, 
   }
 }
 
+// A block's scores s of the lane's row (tiles 0 and 1: keys 8 g .. 8 g + 7, in powers
+// of two): the running maximum, the lane's share of the sum, the values so far scaled
+// to the new maximum, and the probabilities in 16-bit parts.
+template <bool BF, int PARTS, int VG, int VD>
+__device__ __forceinline__ void softmax_block(const f32x4 (&s)[2], float& m, float& l, f32x4 (&o)[VG][VD], u32x4 (&p)[PARTS]) {
+  const float mx = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
+                         fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
+  const float mn = fmaxf(m, groups_max(mx));
+  if (__any(mn > m)) {
+    const float c = mn == -INFINITY ? 1.f : exp2f(m - mn);
+    l *= c;
+#pragma unroll
+    for (int i = 0; i < VG; ++i)
+#pragma unroll
+      for (int e = 0; e < VD; ++e) o[i][e] *= c;
+    m = mn;
+  }
+  const float base = m == -INFINITY ? 0.f : m;
+  float x[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    x[j] = exp2f(s[j >> 2][j & 3] - base);
+    l += x[j];
+  }
+#pragma unroll
+  for (int n = 0; n < PARTS; ++n)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) p[n][j] = round2<BF>(x[2 * j], x[2 * j + 1]);
+}
+
 template <int D, bool BF, int RT>
 __global__ void __launch_bounds__(64 * kWaves) attn_stream_kernel(btf_paged_attention a, btf_kv_cache kv) {
   constexpr int R = 16 * RT;             // rows of a tile
@@ -224,8 +254,8 @@ __global__ void __launch_bounds__(64 * kWaves) attn_stream_kernel(btf_paged_atte
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int c16 = lane & 15, g = lane >> 4;
   const int G = a.heads / kv.heads;
-  const int tile = q.local % q.tiles, rest = q.local / q.tiles;
-  const int piece = rest % q.pieces, kvh = rest / q.pieces;
+  const int kvh = q.local % kv.heads, rest = q.local / kv.heads;
+  const int tile = q.tiles - 1 - rest % q.tiles, piece = rest / q.tiles;
   const int nrows = min(R, q.n * G - tile * R);  // of this tile
   const bool tree = a.tree && q.n <= BTF_TREE_NODES;
   const float c2 = a.scale * 1.4426950408889634f;  // scores in powers of two
@@ -334,31 +364,7 @@ __global__ void __launch_bounds__(64 * kWaves) attn_stream_kernel(btf_paged_atte
     // the running maximum and sum; probabilities in 16-bit parts, keys 8 g .. 8 g + 7
     u32x4 p[RT][PARTS];
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-      float mx = fmaxf(fmaxf(fmaxf(s[rt][0][0], s[rt][0][1]), fmaxf(s[rt][0][2], s[rt][0][3])),
-                       fmaxf(fmaxf(s[rt][1][0], s[rt][1][1]), fmaxf(s[rt][1][2], s[rt][1][3])));
-      const float mn = fmaxf(m[rt], groups_max(mx));
-      if (__any(mn > m[rt])) {
-        const float c = mn == -INFINITY ? 1.f : exp2f(m[rt] - mn);
-        l[rt] *= c;
-#pragma unroll
-        for (int i = 0; i < VG; ++i)
-#pragma unroll
-          for (int e = 0; e < VD; ++e) o[rt][i][e] *= c;
-        m[rt] = mn;
-      }
-      const float base = m[rt] == -INFINITY ? 0.f : m[rt];
-      float x[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        x[j] = exp2f(s[rt][j >> 2][j & 3] - base);
-        l[rt] += x[j];
-      }
-#pragma unroll
-      for (int n = 0; n < PARTS; ++n)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) p[rt][n][j] = round2<BF>(x[2 * j], x[2 * j + 1]);
-    }
+    for (int rt = 0; rt < RT; ++rt) softmax_block<BF, PARTS, VG, VD>(s[rt], m[rt], l[rt], o[rt], p[rt]);
     // O^T += V^T P^T: dim VD c16 + e of each lane group's eight keys
 #pragma unroll
     for (int i = 0; i < VG; ++i)
@@ -445,67 +451,289 @@ __global__ void __launch_bounds__(64 * kWaves) attn_stream_kernel(btf_paged_atte
   }
 }
 
-// The pieces of one row of one head put together: D / 4 threads, four values each.
-template <int D, int R>
-__global__ void __launch_bounds__(D / 4 < 64 ? 64 : D / 4) attn_join_kernel(btf_paged_attention a, btf_kv_cache kv) {
+// ---- many rows: K and V through LDS ----
+// A workgroup's 4 waves have 32 rows each (two MFMA tiles, which share every operand
+// of K and V) and walk the same keys, 32 at a time, from two buffers in LDS: the
+// next block is on its way to registers while this one is worked on, and is written
+// to the other buffer after it. K's rows are stored in the order of the score tiles'
+// rows, 16-byte chunks turned by the row, so that the 16 rows that a lane group reads
+// at once lie in different banks; V's rows are read 256 bytes at a time.
+template <int D, bool BF>
+__global__ void __launch_bounds__(64 * kWaves) attn_tile_kernel(btf_paged_attention a, btf_kv_cache kv) {
+  constexpr int RT = 2, RW = 16 * RT, R = kWaves * RW;
+  constexpr int KS = D / 32;
+  constexpr int VD = D < 128 ? D / 16 : 8, VG = D / (16 * VD);
+  constexpr int PARTS = BF ? 3 : 2;
+  constexpr int CH = D / 8;             // 16-byte chunks of a row
+  constexpr int NC = kKeys * CH / (64 * kWaves);  // of a block, for each thread
+  typedef uint32_t vdw __attribute__((ext_vector_type(VD / 2)));
+  __shared__ u32x4 sh_k[2][kKeys * CH], sh_v[2][kKeys * CH];
+
   Req q;
-  if (!find<R, true>(a, kv, blockIdx.x, q) || q.pieces == 1) return;
-  if (threadIdx.x >= D / 4) return;
-  const int G = a.heads / kv.heads, h = blockIdx.y, kvh = h / G;
-  const int row = q.local * G + h % G, tile = row / R, r = row % R, d4 = threadIdx.x * 4;
-  const float* slot = static_cast<const float*>(a.ws) +
-                      (size_t)(q.slot + (kvh * q.pieces) * q.tiles + tile) * kSlot<D, R>;
-  const size_t step = (size_t)q.tiles * kSlot<D, R>;
-  float top = -INFINITY;
-  for (int i = 0; i < q.pieces; ++i) top = fmaxf(top, slot[i * step + R * D + r]);
-  const float base = top == -INFINITY ? 0.f : top;
-  float sum = 0.f;
-  f32x4 v = {0.f, 0.f, 0.f, 0.f};
-  for (int i = 0; i < q.pieces; ++i) {
-    const float* x = slot + i * step;
-    const float c = exp2f(x[R * D + r] - base);
-    sum += c * x[R * D + R + r];
-    v += c * *reinterpret_cast<const f32x4*>(x + (size_t)r * D + d4);
+  if (!find<R, false>(a, kv, blockIdx.x, q)) return;  // the whole workgroup
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int c16 = lane & 15, g = lane >> 4;
+  const int G = a.heads / kv.heads;
+  const int kvh = q.local % kv.heads, rest = q.local / kv.heads;
+  const int tile = q.tiles - 1 - rest % q.tiles, piece = rest / q.tiles;
+  const int nrows = min(R, q.n * G - tile * R);
+  const bool tree = a.tree && q.n <= BTF_TREE_NODES;
+  const float c2 = a.scale * 1.4426950408889634f;
+  const int i0 = tile * R / G, i1 = (tile * R + nrows - 1) / G;
+  const int kend = tree ? q.len : max(0, min(q.len, q.ctx + i1 + 1));
+  const int k0 = piece * q.C, k1 = min(kend, k0 + q.C);
+  const int all = min(kend, tree ? q.ctx : q.ctx + i0 + 1);
+
+  u32x4 qf[RT][KS];
+  int tok[RT];
+  unsigned long long bits[RT];
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    const int r = w * RW + rt * 16 + c16, row = tile * R + r;
+    const bool live = r < nrows;
+    tok[rt] = live ? row / G : -1;
+    bits[rt] = tree && live ? a.tree[q.row0 + row / G] : 0;
+    const uint16_t* x = static_cast<const uint16_t*>(a.q) + (size_t)(q.row0 + row / G) * a.ldq + (kvh * G + row % G) * D + 8 * g;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) qf[rt][ks] = live ? *reinterpret_cast<const u32x4*>(x + 32 * ks) : u32x4{0, 0, 0, 0};
   }
+  f32x4 o[RT][VG][VD];
+  float m[RT], l[RT];
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    m[rt] = -INFINITY, l[rt] = 0.f;
+#pragma unroll
+    for (int i = 0; i < VG; ++i)
+#pragma unroll
+      for (int e = 0; e < VD; ++e) o[rt][i][e] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+
+  const uint16_t* kp = static_cast<const uint16_t*>(kv.k) + (size_t)kvh * kv.head_stride;
+  const uint16_t* vp = static_cast<const uint16_t*>(kv.v) + (size_t)kvh * kv.head_stride;
+  const int* tab = a.table + (size_t)q.s * a.ldt;
+  const int sh = __builtin_ctz(kv.page), last = (q.len - 1) >> sh;
+  auto page_of = [&](int key) {
+    const int p = key < q.len ? tab[min(key >> sh, last)] : -1;
+    return p >= 0 && p < kv.pages ? p : -1;
+  };
+  u32x4 rk[NC], rv[NC];
+  int p0, p1;  // pages of a block's two halves
+  auto load = [&](int kb) {  // a block to registers: cleared where no row sees it
+#pragma unroll
+    for (int n = 0; n < NC; ++n) {
+      const int c = threadIdx.x + 64 * kWaves * n, j = c / CH, ch = c % CH;
+      const int pg = j < 16 ? p0 : p1;
+      const size_t at = (size_t)max(pg, 0) * kv.page_stride + (size_t)((kb + j) & (kv.page - 1)) * kv.tok_stride + 8 * ch;
+      rk[n] = *reinterpret_cast<const u32x4*>(kp + at);
+      rv[n] = *reinterpret_cast<const u32x4*>(vp + at);
+    }
+  };
+  auto store = [&](int kb, int buf) {
+#pragma unroll
+    for (int n = 0; n < NC; ++n) {
+      const int c = threadIdx.x + 64 * kWaves * n, j = c / CH, ch = c % CH;
+      if ((j < 16 ? p0 : p1) < 0 || kb + j >= k1) rk[n] = rv[n] = u32x4{0, 0, 0, 0};
+      const int row = 16 * (j >> 2 & 1) + 4 * (j >> 3) + (j & 3);
+      const int turn = D == 64 ? row >> 1 & 7 : row & 15;
+      sh_k[buf][row * CH + (ch ^ turn)] = rk[n];
+      sh_v[buf][c] = rv[n];
+    }
+  };
+  if (k0 < k1) {
+    p0 = page_of(k0), p1 = page_of(k0 + 16);
+    load(k0);
+    store(k0, 0);
+  }
+  int buf = 0;
+  for (int kb = k0; kb < k1; kb += kKeys, buf ^= 1) {
+    const bool hole = p0 < 0 || (p1 < 0 && kb + 16 < k1);  // of this block
+    const int h0 = p0, h1 = p1, nb = kb + kKeys;
+    const bool more = nb < k1;
+    __syncthreads();  // this block is in LDS; the other buffer's readers are done
+    if (more) {
+      p0 = page_of(nb), p1 = page_of(nb + 16);
+      load(nb);
+    }
+    f32x4 s[RT][2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) s[rt][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+      const int row = 16 * t + c16, turn = D == 64 ? row >> 1 & 7 : row & 15;
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        const u32x4 kf = sh_k[buf][row * CH + ((4 * ks + g) ^ turn)];
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) s[rt][t] = mfma<BF>(kf, qf[rt][ks], s[rt][t]);
+      }
+    }
+    if (kb + kKeys > all || hole) {
+      const bool have = (g < 2 ? h0 : h1) >= 0;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int key = kb + 8 * g + j, nj = key - q.ctx;
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+          const bool see = have && key < k1 && (nj < 0 || (tree ? nj < 64 && (bits[rt] >> (nj & 63) & 1) : nj <= tok[rt]));
+          s[rt][j >> 2][j & 3] = see ? s[rt][j >> 2][j & 3] * c2 : -INFINITY;
+        }
+      }
+    } else {
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+        for (int t = 0; t < 2; ++t) s[rt][t] *= c2;
+    }
+    u32x4 p[RT][PARTS];
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) softmax_block<BF, PARTS, VG, VD>(s[rt], m[rt], l[rt], o[rt], p[rt]);
+#pragma unroll
+    for (int i = 0; i < VG; ++i) {
+      vdw vf[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        vf[j] = reinterpret_cast<const vdw*>(&sh_v[buf][(8 * g + j) * CH])[16 * i + c16];
+#pragma unroll
+      for (int e = 0; e < VD; ++e) {
+        u32x4 vt;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          vt[j] = __builtin_amdgcn_perm(vf[2 * j + 1][e >> 1], vf[2 * j][e >> 1], (e & 1) ? 0x07060302u : 0x05040100u);
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+          for (int n = 0; n < PARTS; ++n) o[rt][i][e] = mfma<BF>(vt, p[rt][n], o[rt][i][e]);
+      }
+    }
+    if (more) store(nb, buf ^ 1);
+  }
+
+  const bool cut = q.pieces > 1;
+  float* slot = nullptr;
+  if (cut) slot = static_cast<float*>(a.ws) + (size_t)(q.slot + q.local) * kSlot<D, R>;
+  bool odd = false;
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    const int r = w * RW + rt * 16 + c16, row = tile * R + r;
+    l[rt] = groups_sum(l[rt]);
+    float chk = l[rt] - l[rt];
+    const float f = cut ? 1.f : l[rt] == 0.f ? 0.f : 1.f / l[rt];
+    float* y = cut ? slot + (size_t)r * D : a.out + (size_t)(q.row0 + row / G) * a.ldo + (kvh * G + row % G) * D;
+    const bool live = r < nrows;
+#pragma unroll
+    for (int i = 0; i < VG; ++i)
+#pragma unroll
+      for (int d = 0; d < 4; ++d)
+#pragma unroll
+        for (int e = 0; e < VD; e += 4) {
+          f32x4 v = {o[rt][i][e][d], o[rt][i][e + 1][d], o[rt][i][e + 2][d], o[rt][i][e + 3][d]};
+          chk += (v[0] - v[0]) + (v[1] - v[1]) + (v[2] - v[2]) + (v[3] - v[3]);
+          if (live) *reinterpret_cast<f32x4*>(y + 16 * VD * i + VD * (4 * g + d) + e) = v * f;
+        }
+    if (cut && live && g == 0) slot[R * D + r] = m[rt], slot[R * D + R + r] = l[rt];
+    odd |= chk != 0.f;
+  }
+  if (!__any(odd)) return;
+  __threadfence_block();  // (the rows below are written again by other lanes of this wave)
+  for (int r = w * RW; r < min(nrows, (w + 1) * RW); ++r) {
+    constexpr int E = D / 64;
+    float po[E], pm, pl;
+    const int row = tile * R + r;
+    plain_row<D, BF>(a, kv, q, kvh, row, k0, max(k0, k1), c2, po, pm, pl);
+    float* y = cut ? slot + (size_t)r * D : a.out + (size_t)(q.row0 + row / G) * a.ldo + (kvh * G + row % G) * D;
+#pragma unroll
+    for (int e = 0; e < E; ++e) y[lane * E + e] = cut ? po[e] : pl == 0.f ? 0.f : po[e] / pl;
+    if (cut && lane == 0) slot[R * D + r] = pm, slot[R * D + R + r] = pl;
+  }
+}
+
+// The pieces of one row of one head put together: a wave takes the pieces' maxima
+// and sums 64 at a time, then every wave its share of the pieces' values (so that
+// many loads are in flight), and the waves join in LDS.
+constexpr int kJoinWaves = 4;
+template <int D, int R>
+__global__ void __launch_bounds__(64 * kJoinWaves) attn_join_kernel(btf_paged_attention a, btf_kv_cache kv) {
+  constexpr int E = D / 64;  // values of a lane
+  typedef float vE __attribute__((ext_vector_type(E)));
+  __shared__ float sh[kJoinWaves][D];
+  Req q;
+  if (!find<R, true>(a, kv, blockIdx.x, q) || q.pieces == 1) return;  // the whole workgroup
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int G = a.heads / kv.heads, h = blockIdx.y, kvh = h / G;
+  const int row = q.local * G + h % G, tile = row / R, r = row % R;
+  const float* slot = static_cast<const float*>(a.ws) + (size_t)(q.slot + (q.tiles - 1 - tile) * kv.heads + kvh) * kSlot<D, R>;
+  const size_t step = (size_t)q.tiles * kv.heads * kSlot<D, R>;
+  float top = -INFINITY, sum = 0.f;
+  for (int i = lane; i < q.pieces; i += 64) top = fmaxf(top, slot[i * step + R * D + r]);
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
+  const float base = top == -INFINITY ? 0.f : top;
+  vE v = vE(0.f);
+  for (int i0 = 0; i0 < q.pieces; i0 += 64) {
+    float c = 0.f;
+    if (i0 + lane < q.pieces) {
+      const float* x = slot + (i0 + lane) * step + R * D + r;
+      c = exp2f(x[0] - base);
+      sum += c * x[R];
+    }
+    const int n = min(64, q.pieces - i0);
+    for (int i = w; i < n; i += 4 * kJoinWaves)
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int j = min(i + u * kJoinWaves, n - 1);
+        const float f = i + u * kJoinWaves < n ? __shfl(c, j, 64) : 0.f;
+        const vE x = *reinterpret_cast<const vE*>(slot + (i0 + j) * step + (size_t)r * D + lane * E);
+        if (i + u * kJoinWaves < n) v += f * x;
+      }
+  }
+  sum = wave_sum_f(sum);
+  *reinterpret_cast<vE*>(&sh[w][lane * E]) = v;
+  __syncthreads();
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
-  *reinterpret_cast<f32x4*>(a.out + (size_t)(q.row0 + q.local) * a.ldo + h * D + d4) = v * inv;
+  for (int d = threadIdx.x; d < D; d += 64 * kJoinWaves) {
+    float y = sh[0][d];
+#pragma unroll
+    for (int i = 1; i < kJoinWaves; ++i) y += sh[i][d];
+    a.out[(size_t)(q.row0 + q.local) * a.ldo + h * D + d] = y * inv;
+  }
 }
 
-// Row tiles: one or two of 16, by the rows that a request has on average.
-int row_tiles(int S, int T, int heads, const btf_kv_cache& kv) {
-  return (int64_t)T * (heads / kv.heads) > 16 * (int64_t)S ? 2 : 1;
-}
-
-template <int D, bool BF, int RT>
-int attn_go(const btf_paged_attention& a, const btf_kv_cache& kv, hipStream_t st) {
-  constexpr int R = 16 * RT;
-  const int64_t tiles = (int64_t)a.T * (a.heads / kv.heads) / R + a.S;  // at most
-  hipLaunchKernelGGL((attn_stream_kernel<D, BF, RT>), dim3((unsigned)(kTarget + tiles * kv.heads)), dim3(64 * kWaves), 0, st, a, kv);
-  const int rc = launch_status("attn_stream_kernel");
-  if (rc != BTF_OK) return rc;
-  hipLaunchKernelGGL((attn_join_kernel<D, R>), dim3(a.T, a.heads), dim3(D / 4 < 64 ? 64 : D / 4), 0, st, a, kv);
-  return launch_status("attn_join_kernel");
+// Rows of an item's tile, by the rows that a request has on average for a KV head.
+int tile_rows(int S, int T, int heads, const btf_kv_cache& kv) {
+  const int64_t rows = (int64_t)T * (heads / kv.heads);
+  return rows <= 16 * (int64_t)S ? 16 : rows <= 32 * (int64_t)S ? 32 : 128;
 }
 
 template <int D, bool BF>
-int attn_pick(const btf_paged_attention& a, const btf_kv_cache& kv, hipStream_t st) {
-  return row_tiles(a.S, a.T, a.heads, kv) == 1 ? attn_go<D, BF, 1>(a, kv, st) : attn_go<D, BF, 2>(a, kv, st);
+int attn_go(const btf_paged_attention& a, const btf_kv_cache& kv, hipStream_t st) {
+  const int R = tile_rows(a.S, a.T, a.heads, kv);
+  const int64_t tiles = (int64_t)a.T * (a.heads / kv.heads) / R + a.S;  // at most
+  const dim3 grid((unsigned)(kTarget + tiles * kv.heads)), join(a.T, a.heads), blk(64 * kWaves);
+  if (R == 16) hipLaunchKernelGGL((attn_stream_kernel<D, BF, 1>), grid, blk, 0, st, a, kv);
+  else if (R == 32) hipLaunchKernelGGL((attn_stream_kernel<D, BF, 2>), grid, blk, 0, st, a, kv);
+  else hipLaunchKernelGGL((attn_tile_kernel<D, BF>), grid, blk, 0, st, a, kv);
+  const int rc = launch_status("attn kernel");
+  if (rc != BTF_OK) return rc;
+  const dim3 jblk(64 * kJoinWaves);
+  if (R == 16) hipLaunchKernelGGL((attn_join_kernel<D, 16>), join, jblk, 0, st, a, kv);
+  else if (R == 32) hipLaunchKernelGGL((attn_join_kernel<D, 32>), join, jblk, 0, st, a, kv);
+  else hipLaunchKernelGGL((attn_join_kernel<D, 128>), join, jblk, 0, st, a, kv);
+  return launch_status("attn_join_kernel");
 }
 
 }  // namespace
 
-// Cut requests have at most 2 kTarget items: a piece of them holds C keys, or at least half of it on average, and C is
-// at least all the work over kTarget.
+// Cut requests have at most 2 kTarget items: a piece of them holds at least C / 2 keys on average, and C is at least
+// all the work over kTarget.
 int64_t paged_attention_ws_bytes(int S, int T, int heads, const btf_kv_cache& kv) {
-  const int R = 16 * row_tiles(S, T, heads, kv);
-  return (int64_t)2 * kTarget * R * (kv.dim + 2) * 4;
+  return (int64_t)2 * kTarget * tile_rows(S, T, heads, kv) * (kv.dim + 2) * 4;
 }
 
 int paged_attention(const btf_paged_attention& a, const btf_kv_cache& kv, hipStream_t st, const DevState& ds) {
   const bool bf = kv.type == BTF_BF16;
-  if (kv.dim == 64) return bf ? attn_pick<64, true>(a, kv, st) : attn_pick<64, false>(a, kv, st);
-  if (kv.dim == 128) return bf ? attn_pick<128, true>(a, kv, st) : attn_pick<128, false>(a, kv, st);
-  return bf ? attn_pick<256, true>(a, kv, st) : attn_pick<256, false>(a, kv, st);
+  if (kv.dim == 64) return bf ? attn_go<64, true>(a, kv, st) : attn_go<64, false>(a, kv, st);
+  if (kv.dim == 128) return bf ? attn_go<128, true>(a, kv, st) : attn_go<128, false>(a, kv, st);
+  return bf ? attn_go<256, true>(a, kv, st) : attn_go<256, false>(a, kv, st);
 }
 
 }  // namespace btfhip
