@@ -61,22 +61,30 @@ __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
 }
 
-// Two values rounded to 16 bits, and what the rounding left.
+// Two values rounded to 16 bits, and what the rounding left. (The empty asm keeps the
+// compiler from rounding a second time for the difference.)
 template <bool BF>
 __device__ __forceinline__ uint32_t round2(float& x, float& y) {
+  uint32_t u;
   if (BF) {
     typedef __bf16 b2 __attribute__((ext_vector_type(2)));
-    const b2 r = {(__bf16)x, (__bf16)y};
-    x -= (float)r[0];
-    y -= (float)r[1];
-    return __builtin_bit_cast(uint32_t, r);
+    u = __builtin_bit_cast(uint32_t, b2{(__bf16)x, (__bf16)y});
+    asm("" : "+v"(u));
+    x -= __uint_as_float(u << 16);
+    y -= __uint_as_float(u & 0xffff0000u);
+    return u;
   }
   typedef _Float16 h2 __attribute__((ext_vector_type(2)));
-  const h2 r = {(_Float16)x, (_Float16)y};
-  x -= (float)r[0];
-  y -= (float)r[1];
-  return __builtin_bit_cast(uint32_t, r);
+  u = __builtin_bit_cast(uint32_t, h2{(_Float16)x, (_Float16)y});
+  asm("" : "+v"(u));
+  const h2 r = __builtin_bit_cast(h2, u);
+  x = __builtin_fmaf((float)r[0], -1.f, x);  // (one instruction, with the conversion)
+  y = __builtin_fmaf((float)r[1], -1.f, y);
+  return u;
 }
+
+// 2^x in one instruction (1 ulp; below 2^-126 it gives 0, which is no weight here).
+__device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // Max / sum over the four lane groups (lanes l, l ^ 16, l ^ 32, l ^ 48).
 __device__ __forceinline__ float groups_max(float v) {
@@ -115,7 +123,8 @@ __device__ __forceinline__ float wave_sum_f(float v) {
 
 // The request of item `id` (BY_ROW: of row `id`), found by every wave for itself:
 // the lanes take 64 requests at a time. False: there is no such item.
-template <int R, bool BY_ROW>
+// SCALAR: the answer in scalar registers (the stream kernel has none to spare).
+template <int R, bool BY_ROW, bool SCALAR>
 __device__ bool find(const btf_paged_attention& a, const btf_kv_cache& kv, int id, Req& q) {
   const int lane = threadIdx.x & 63, G = a.heads / kv.heads;
   const long long cap = (long long)a.ldt * kv.page;
@@ -135,7 +144,7 @@ __device__ bool find(const btf_paged_attention& a, const btf_kv_cache& kv, int i
     if (n > 0) work += (float)((n * G + R - 1) / R) * (float)len;
   }
   work = wave_sum_f(work) * (float)kv.heads;
-  const int C = max(kStep, (int)(work / (float)(kTarget * kStep) + 1.f) * kStep);
+  const int C = max(kStep, __builtin_amdgcn_readfirstlane((int)(work / (float)(kTarget * kStep) + 1.f)) * kStep);
   int items = 0, slots = 0;  // before the chunk
   for (int s0 = 0; s0 < a.S; s0 += 64) {
     read(s0 + lane, r0, n, len, full);
@@ -151,20 +160,21 @@ __device__ bool find(const btf_paged_attention& a, const btf_kv_cache& kv, int i
     const unsigned long long who = __ballot(here);
     if (who) {
       const int l = __builtin_ctzll(who);
+      auto of = [&](int v) { return SCALAR ? __builtin_amdgcn_readlane(v, l) : __shfl(v, l, 64); };
       q.s = s0 + l;
-      q.row0 = __shfl(r0, l, 64);
-      q.n = __shfl(n, l, 64);
-      q.len = __shfl(len, l, 64);
-      q.ctx = __shfl(full, l, 64) - q.n;
-      q.tiles = __shfl(tiles, l, 64);
-      q.pieces = __shfl(pieces, l, 64);
-      q.local = id - (BY_ROW ? q.row0 : items + __shfl(upto - mine, l, 64));
-      q.slot = slots + __shfl(cuts - cut, l, 64);
+      q.row0 = of(r0);
+      q.n = of(n);
+      q.len = of(len);
+      q.ctx = of(full) - q.n;
+      q.tiles = of(tiles);
+      q.pieces = of(pieces);
+      q.local = id - (BY_ROW ? q.row0 : items + of(upto - mine));
+      q.slot = slots + of(cuts - cut);
       q.C = C;
       return true;
     }
-    items += __shfl(upto, 63, 64);
-    slots += __shfl(cuts, 63, 64);
+    items += __builtin_amdgcn_readlane(upto, 63);
+    slots += __builtin_amdgcn_readlane(cuts, 63);
   }
   return false;
 }
@@ -177,7 +187,7 @@ constexpr size_t kSlot = (size_t)R * (D + 2);
 // D / 64 values, the row's maximum and sum. Any input.
 template <int D, bool BF>
 __device__ void plain_row(const btf_paged_attention& a, const btf_kv_cache& kv, const Req& q, int kvh, int row, int k0, int k1,
-                          float c2, float* o, float& m, float& l) {
+                          float* o, float& m, float& l) {
   constexpr int E = D / 64;
   const int lane = threadIdx.x & 63, G = a.heads / kv.heads, i = row / G, t = q.row0 + i, h = kvh * G + row % G;
   const bool tree = a.tree && q.n <= BTF_TREE_NODES;
@@ -197,9 +207,9 @@ __device__ void plain_row(const btf_paged_attention& a, const btf_kv_cache& kv, 
     float d = 0.f;
 #pragma unroll
     for (int e = 0; e < E; ++e) d += qf[e] * from16<BF>(static_cast<const uint16_t*>(kv.k)[at + e]);
-    d = wave_sum_f(d) * c2;
+    d = wave_sum_f(d) * (a.scale * 1.4426950408889634f);
     if (d == -INFINITY) continue;
-    const float mn = fmaxf(m, d), c = exp2f(m - mn), p = exp2f(d - mn);
+    const float mn = fmaxf(m, d), c = fast_exp2(m - mn), p = fast_exp2(d - mn);
     l = l * c + p;
 #pragma unroll
     for (int e = 0; e < E; ++e) o[e] = o[e] * c + p * from16<BF>(static_cast<const uint16_t*>(kv.v)[at + e]);
@@ -207,28 +217,32 @@ __device__ void plain_row(const btf_paged_attention& a, const btf_kv_cache& kv, 
   }
 }
 
-// A block's scores s of the lane's row (tiles 0 and 1: keys 8 g .. 8 g + 7, in powers
-// of two): the running maximum, the lane's share of the sum, the values so far scaled
-// to the new maximum, and the probabilities in 16-bit parts.
-template <bool BF, int PARTS, int VG, int VD>
-__device__ __forceinline__ void softmax_block(const f32x4 (&s)[2], float& m, float& l, f32x4 (&o)[VG][VD], u32x4 (&p)[PARTS]) {
+// A block's scores s of the lane's row before their scale (tiles 0 and 1: keys 8 g ..
+// 8 g + 7): the running maximum m (in powers of two, as the scores times c2 > 0 are),
+// the lane's share of the sum, the values so far scaled to the new maximum, and the
+// probabilities in 16-bit parts. m follows the maximum only when that is more than
+// kLag above it, so that the values are rarely scaled: probabilities reach 2^kLag,
+// which changes nothing in their relative rounding.
+constexpr float kLag = 8.f;
+template <bool BF, int PARTS, int N>
+__device__ __forceinline__ void softmax_block(const f32x4 (&s)[2], float c2, float& m, float& l, f32x4 (&o)[N],
+                                              u32x4 (&p)[PARTS]) {
   const float mx = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
                          fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
-  const float mn = fmaxf(m, groups_max(mx));
-  if (__any(mn > m)) {
-    const float c = mn == -INFINITY ? 1.f : exp2f(m - mn);
+  const float mn = groups_max(mx) * c2;
+  if (__any(mn > m + kLag)) {
+    const float to = fmaxf(m, mn);
+    const float c = to == -INFINITY ? 1.f : fast_exp2(m - to);
     l *= c;
 #pragma unroll
-    for (int i = 0; i < VG; ++i)
-#pragma unroll
-      for (int e = 0; e < VD; ++e) o[i][e] *= c;
-    m = mn;
+    for (int i = 0; i < N; ++i) o[i] *= c;
+    m = to;
   }
   const float base = m == -INFINITY ? 0.f : m;
   float x[8];
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
-    x[j] = exp2f(s[j >> 2][j & 3] - base);
+    x[j] = fast_exp2(__builtin_fmaf(s[j >> 2][j & 3], c2, -base));
     l += x[j];
   }
 #pragma unroll
@@ -237,8 +251,32 @@ __device__ __forceinline__ void softmax_block(const f32x4 (&s)[2], float& m, flo
     for (int j = 0; j < 4; ++j) p[n][j] = round2<BF>(x[2 * j], x[2 * j + 1]);
 }
 
+// Scores of keys key0 .. key0 + 7 that the row (new token tok, -1: none) does not see become -infinity; there are keys
+// up to end. A tree's row sees its bits of the new tokens, another's those up to its own. (By selects: every score is
+// read before it is written, so no write can come before the product's own.)
+__device__ __forceinline__ void mask_block(f32x4 (&s)[2], int key0, int end, int ctx, bool tree, int tok,
+                                           unsigned long long bits) {
+  const int upto = tree ? ctx - 1 : ctx + tok, nj = key0 - ctx;
+  const uint32_t own = !tree || nj >= 64 || nj <= -8 ? 0 : nj >= 0 ? (uint32_t)(bits >> nj) : (uint32_t)(bits << -nj);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const bool see = (key0 + j < end) & ((key0 + j <= upto) | ((own >> j & 1) != 0));
+    s[j >> 2][j & 3] = see ? s[j >> 2][j & 3] : -INFINITY;
+  }
+}
+
+// The scale of the scores in powers of two, as a positive number (the sign goes to Q;
+// a scale of zero becomes one that leaves every finite score at zero).
+__device__ __forceinline__ float scale2(float scale) {
+  return fmaxf(fabsf(scale) * 1.4426950408889634f, 1.17549435e-38f);
+}
+__device__ __forceinline__ u32x4 signed_q(u32x4 q, float scale) {
+  const uint32_t f = scale < 0.f ? 0x80008000u : 0u;
+  return q ^ u32x4{f, f, f, f};
+}
+
 template <int D, bool BF, int RT>
-__global__ void __launch_bounds__(64 * kWaves) attn_stream_kernel(btf_paged_attention a, btf_kv_cache kv) {
+__global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(D < 256 ? 2 : 1))) attn_stream_kernel(btf_paged_attention a, btf_kv_cache kv) {
   constexpr int R = 16 * RT;             // rows of a tile
   constexpr int KS = D / 32;             // steps over the dims in Q K^T
   constexpr int VD = D < 128 ? D / 16 : 8;  // dims that a lane reads of a key of V
@@ -250,7 +288,7 @@ __global__ void __launch_bounds__(64 * kWaves) attn_stream_kernel(btf_paged_atte
   __shared__ int sh_odd;
 
   Req q;
-  if (!find<R, false>(a, kv, blockIdx.x, q)) return;  // the whole workgroup
+  if (!find<R, false, false>(a, kv, blockIdx.x, q)) return;  // the whole workgroup
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int c16 = lane & 15, g = lane >> 4;
   const int G = a.heads / kv.heads;
@@ -258,7 +296,7 @@ __global__ void __launch_bounds__(64 * kWaves) attn_stream_kernel(btf_paged_atte
   const int tile = q.tiles - 1 - rest % q.tiles, piece = rest / q.tiles;
   const int nrows = min(R, q.n * G - tile * R);  // of this tile
   const bool tree = a.tree && q.n <= BTF_TREE_NODES;
-  const float c2 = a.scale * 1.4426950408889634f;  // scores in powers of two
+  const float c2 = scale2(a.scale);
   // keys: [k0, k1) is the piece, cut behind the last key that any row of the tile sees; all rows see those before `all`
   const int i0 = tile * R / G, i1 = (tile * R + nrows - 1) / G;
   const int kend = tree ? q.len : max(0, min(q.len, q.ctx + i1 + 1));
@@ -277,17 +315,15 @@ __global__ void __launch_bounds__(64 * kWaves) attn_stream_kernel(btf_paged_atte
     bits[rt] = tree && live ? a.tree[q.row0 + row / G] : 0;
     const uint16_t* x = static_cast<const uint16_t*>(a.q) + (size_t)(q.row0 + row / G) * a.ldq + (kvh * G + row % G) * D + 8 * g;
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) qf[rt][ks] = live ? *reinterpret_cast<const u32x4*>(x + 32 * ks) : u32x4{0, 0, 0, 0};
+    for (int ks = 0; ks < KS; ++ks) qf[rt][ks] = live ? signed_q(*reinterpret_cast<const u32x4*>(x + 32 * ks), a.scale) : u32x4{0, 0, 0, 0};
   }
-  f32x4 o[RT][VG][VD];
+  f32x4 o[RT][VG * VD];
   float m[RT], l[RT];
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
     m[rt] = -INFINITY, l[rt] = 0.f;
 #pragma unroll
-    for (int i = 0; i < VG; ++i)
-#pragma unroll
-      for (int e = 0; e < VD; ++e) o[rt][i][e] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int i = 0; i < VG * VD; ++i) o[rt][i] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
 
   const uint16_t* kp = static_cast<const uint16_t*>(kv.k) + (size_t)kvh * kv.head_stride;
@@ -341,30 +377,19 @@ __global__ void __launch_bounds__(64 * kWaves) attn_stream_kernel(btf_paged_atte
     // a block that some row does not see all of
     const bool edge = kb + kKeys > all || __any(pk < 0 || pv < 0);
     if (edge) {
+      const int end = pv >= 0 ? k1 : 0, key0 = kb + kv0;  // keys that there are
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int key = kb + kv0 + j, nj = key - q.ctx;
-        if (pv < 0 || key >= k1)
+      for (int j = 0; j < 8; ++j)
 #pragma unroll
-          for (int i = 0; i < VG; ++i) vf[i][j] = vdw(0);
+        for (int i = 0; i < VG; ++i) vf[i][j] = key0 + j < end ? vf[i][j] : vdw(0);
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
-          const bool see = pv >= 0 && key < k1 && (nj < 0 || (tree ? nj < 64 && (bits[rt] >> (nj & 63) & 1) : nj <= tok[rt]));
-          if (!see) s[rt][j >> 2][j & 3] = -INFINITY;
-          else s[rt][j >> 2][j & 3] *= c2;
-        }
-      }
-    } else {
-#pragma unroll
-      for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-        for (int t = 0; t < 2; ++t) s[rt][t] *= c2;
+      for (int rt = 0; rt < RT; ++rt) mask_block(s[rt], key0, end, q.ctx, tree, tok[rt], bits[rt]);
     }
     if (more) load_k(nb, npk);
     // the running maximum and sum; probabilities in 16-bit parts, keys 8 g .. 8 g + 7
     u32x4 p[RT][PARTS];
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt) softmax_block<BF, PARTS, VG, VD>(s[rt], m[rt], l[rt], o[rt], p[rt]);
+    for (int rt = 0; rt < RT; ++rt) softmax_block<BF, PARTS>(s[rt], c2, m[rt], l[rt], o[rt], p[rt]);
     // O^T += V^T P^T: dim VD c16 + e of each lane group's eight keys
 #pragma unroll
     for (int i = 0; i < VG; ++i)
@@ -377,7 +402,7 @@ __global__ void __launch_bounds__(64 * kWaves) attn_stream_kernel(btf_paged_atte
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
-          for (int n = 0; n < PARTS; ++n) o[rt][i][e] = mfma<BF>(vt, p[rt][n], o[rt][i][e]);
+          for (int n = 0; n < PARTS; ++n) o[rt][i * VD + e] = mfma<BF>(vt, p[rt][n], o[rt][i * VD + e]);
       }
     if (more) load_v(nb, npv);
     pk = npk, pv = npv;
@@ -399,7 +424,8 @@ __global__ void __launch_bounds__(64 * kWaves) attn_stream_kernel(btf_paged_atte
       for (int r = 0; r < 4; ++r) {  // row r of the MFMA tiles: dim VD (4 g + r) + e
 #pragma unroll
         for (int e = 0; e < VD; e += 4) {
-          const f32x4 v = {o[rt][i][e][r], o[rt][i][e + 1][r], o[rt][i][e + 2][r], o[rt][i][e + 3][r]};
+          const f32x4* t = o[rt] + i * VD + e;
+          const f32x4 v = {t[0][r], t[1][r], t[2][r], t[3][r]};
           chk += (v[0] - v[0]) + (v[1] - v[1]) + (v[2] - v[2]) + (v[3] - v[3]);
           *reinterpret_cast<f32x4*>(y + 16 * VD * i + VD * (4 * g + r) + e) = v;
         }
@@ -417,7 +443,7 @@ __global__ void __launch_bounds__(64 * kWaves) attn_stream_kernel(btf_paged_atte
       constexpr int E = D / 64;
       float po[E], pm, pl;
       const int row = tile * R + r;
-      plain_row<D, BF>(a, kv, q, kvh, row, k0, max(k0, k1), c2, po, pm, pl);
+      plain_row<D, BF>(a, kv, q, kvh, row, k0, max(k0, k1), po, pm, pl);
       float* y = cut ? slot + (size_t)r * D : a.out + (size_t)(q.row0 + row / G) * a.ldo + (kvh * G + row % G) * D;
 #pragma unroll
       for (int e = 0; e < E; ++e) y[lane * E + e] = cut ? po[e] : pl == 0.f ? 0.f : po[e] / pl;
@@ -436,7 +462,7 @@ __global__ void __launch_bounds__(64 * kWaves) attn_stream_kernel(btf_paged_atte
     f32x4 v = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < kWaves; ++i) {
-      const float c = exp2f(sh_m[i][r] - base);
+      const float c = fast_exp2(sh_m[i][r] - base);
       sum += c * sh_l[i][r];
       v += c * *reinterpret_cast<const f32x4*>(sh_o + (size_t)(i * R + r) * LD + d4);
     }
@@ -456,21 +482,38 @@ __global__ void __launch_bounds__(64 * kWaves) attn_stream_kernel(btf_paged_atte
 // of K and V) and walk the same keys, 32 at a time, from two buffers in LDS: the
 // next block is on its way to registers while this one is worked on, and is written
 // to the other buffer after it. K's rows are stored in the order of the score tiles'
-// rows, 16-byte chunks turned by the row, so that the 16 rows that a lane group reads
-// at once lie in different banks; V's rows are read 256 bytes at a time.
+// rows, their 16-byte chunks turned by the row, so that the 16 rows that a lane group
+// reads at once lie in different banks. V is read by the transposing LDS read: 16
+// lanes read 4 keys of 16 dims and get one dim's 4 keys each; its rows are turned by
+// 32 bytes for the same reason.
+__device__ __forceinline__ u32x2 read_tr(const void* p) {
+  typedef short s4 __attribute__((ext_vector_type(4)));
+  typedef __attribute__((address_space(3))) s4 lds_s4;
+  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)p));
+}
+
+// The thread's number, of which the compiler does not know that it had it before: what
+// follows from it is worked out anew and takes no registers in the loop.
+__device__ __forceinline__ int fresh_tid() {
+  int t = threadIdx.x;
+  asm volatile("" : "+v"(t));
+  return t;
+}
+
 template <int D, bool BF>
-__global__ void __launch_bounds__(64 * kWaves) attn_tile_kernel(btf_paged_attention a, btf_kv_cache kv) {
+__global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(D < 256 ? 2 : 1)))
+    attn_tile_kernel(btf_paged_attention a, btf_kv_cache kv) {
   constexpr int RT = 2, RW = 16 * RT, R = kWaves * RW;
   constexpr int KS = D / 32;
-  constexpr int VD = D < 128 ? D / 16 : 8, VG = D / (16 * VD);
+  constexpr int DT = D / 16;            // dim tiles of the values
+  constexpr int DB = 4, KB = 2;         // ... read at a time, and steps of K
   constexpr int PARTS = BF ? 3 : 2;
   constexpr int CH = D / 8;             // 16-byte chunks of a row
   constexpr int NC = kKeys * CH / (64 * kWaves);  // of a block, for each thread
-  typedef uint32_t vdw __attribute__((ext_vector_type(VD / 2)));
   __shared__ u32x4 sh_k[2][kKeys * CH], sh_v[2][kKeys * CH];
 
   Req q;
-  if (!find<R, false>(a, kv, blockIdx.x, q)) return;  // the whole workgroup
+  if (!find<R, false, true>(a, kv, blockIdx.x, q)) return;  // the whole workgroup
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int c16 = lane & 15, g = lane >> 4;
   const int G = a.heads / kv.heads;
@@ -478,34 +521,29 @@ __global__ void __launch_bounds__(64 * kWaves) attn_tile_kernel(btf_paged_attent
   const int tile = q.tiles - 1 - rest % q.tiles, piece = rest / q.tiles;
   const int nrows = min(R, q.n * G - tile * R);
   const bool tree = a.tree && q.n <= BTF_TREE_NODES;
-  const float c2 = a.scale * 1.4426950408889634f;
+  const float c2 = scale2(a.scale);
   const int i0 = tile * R / G, i1 = (tile * R + nrows - 1) / G;
   const int kend = tree ? q.len : max(0, min(q.len, q.ctx + i1 + 1));
   const int k0 = piece * q.C, k1 = min(kend, k0 + q.C);
   const int all = min(kend, tree ? q.ctx : q.ctx + i0 + 1);
 
   u32x4 qf[RT][KS];
-  int tok[RT];
-  unsigned long long bits[RT];
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
     const int r = w * RW + rt * 16 + c16, row = tile * R + r;
     const bool live = r < nrows;
-    tok[rt] = live ? row / G : -1;
-    bits[rt] = tree && live ? a.tree[q.row0 + row / G] : 0;
     const uint16_t* x = static_cast<const uint16_t*>(a.q) + (size_t)(q.row0 + row / G) * a.ldq + (kvh * G + row % G) * D + 8 * g;
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) qf[rt][ks] = live ? *reinterpret_cast<const u32x4*>(x + 32 * ks) : u32x4{0, 0, 0, 0};
+    for (int ks = 0; ks < KS; ++ks)
+      qf[rt][ks] = live ? signed_q(*reinterpret_cast<const u32x4*>(x + 32 * ks), a.scale) : u32x4{0, 0, 0, 0};
   }
-  f32x4 o[RT][VG][VD];
+  f32x4 o[RT][DT];
   float m[RT], l[RT];
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
     m[rt] = -INFINITY, l[rt] = 0.f;
 #pragma unroll
-    for (int i = 0; i < VG; ++i)
-#pragma unroll
-      for (int e = 0; e < VD; ++e) o[rt][i][e] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int i = 0; i < DT; ++i) o[rt][i] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
 
   const uint16_t* kp = static_cast<const uint16_t*>(kv.k) + (size_t)kvh * kv.head_stride;
@@ -517,8 +555,8 @@ __global__ void __launch_bounds__(64 * kWaves) attn_tile_kernel(btf_paged_attent
     return p >= 0 && p < kv.pages ? p : -1;
   };
   u32x4 rk[NC], rv[NC];
-  int p0, p1;  // pages of a block's two halves
-  auto load = [&](int kb) {  // a block to registers: cleared where no row sees it
+  int p0 = -1, p1 = -1;  // pages of a block's two halves
+  auto load = [&](int kb) {  // a block to registers
 #pragma unroll
     for (int n = 0; n < NC; ++n) {
       const int c = threadIdx.x + 64 * kWaves * n, j = c / CH, ch = c % CH;
@@ -528,17 +566,25 @@ __global__ void __launch_bounds__(64 * kWaves) attn_tile_kernel(btf_paged_attent
       rv[n] = *reinterpret_cast<const u32x4*>(vp + at);
     }
   };
-  auto store = [&](int kb, int buf) {
+  auto store = [&](int kb, int buf) {  // ... and on to LDS, cleared where no row sees it
+    const int tid = D == 256 ? fresh_tid() : threadIdx.x;
+    if (p0 < 0 || p1 < 0 || kb + kKeys > k1)
+#pragma unroll
+      for (int n = 0; n < NC; ++n) {
+        const int j = (tid + 64 * kWaves * n) / CH;
+        if ((j < 16 ? p0 : p1) < 0 || kb + j >= k1) rk[n] = rv[n] = u32x4{0, 0, 0, 0};
+      }
 #pragma unroll
     for (int n = 0; n < NC; ++n) {
-      const int c = threadIdx.x + 64 * kWaves * n, j = c / CH, ch = c % CH;
-      if ((j < 16 ? p0 : p1) < 0 || kb + j >= k1) rk[n] = rv[n] = u32x4{0, 0, 0, 0};
+      const int c = tid + 64 * kWaves * n, j = c / CH, ch = c % CH;
       const int row = 16 * (j >> 2 & 1) + 4 * (j >> 3) + (j & 3);
-      const int turn = D == 64 ? row >> 1 & 7 : row & 15;
-      sh_k[buf][row * CH + (ch ^ turn)] = rk[n];
-      sh_v[buf][c] = rv[n];
+      sh_k[buf][row * CH + (ch ^ (D == 64 ? row >> 1 & 7 : row & 15))] = rk[n];
+      sh_v[buf][j * CH + (ch ^ 2 * ((4 * (j >> 3) + (j & 3)) & (DT - 1)))] = rv[n];
     }
   };
+  // the lane's places in a buffer: K chunk g of its row in score tile 0, V's key 8 g + c16 / 4 and dims 4 (c16 % 4) ..
+  const uint32_t at_k = c16 * CH * 16 + ((g ^ (D == 64 ? c16 >> 1 & 7 : c16)) << 4);
+  const uint32_t at_v = (8 * g + (c16 >> 2)) * CH * 16 + (((4 * g + (c16 >> 2)) & (DT - 1)) << 5) + 8 * (c16 & 3);
   if (k0 < k1) {
     p0 = page_of(k0), p1 = page_of(k0 + 16);
     load(k0);
@@ -554,56 +600,68 @@ __global__ void __launch_bounds__(64 * kWaves) attn_tile_kernel(btf_paged_attent
       p0 = page_of(nb), p1 = page_of(nb + 16);
       load(nb);
     }
+    const char* bk = reinterpret_cast<const char*>(sh_k[buf]);
+    const char* bv = reinterpret_cast<const char*>(sh_v[buf]);
+    u32x4 kf[2][2][KB];
+    auto read_k = [&](int k) {
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int i = 0; i < KB; ++i)
+          kf[k / KB & 1][t][i] = *reinterpret_cast<const u32x4*>(bk + (at_k ^ (k + i) << 6) + t * 16 * CH * 16);
+    };
+    read_k(0);
     f32x4 s[RT][2];
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
+    for (int t = 0; t < 2; ++t)
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt) s[rt][t] = f32x4{0.f, 0.f, 0.f, 0.f};
-      const int row = 16 * t + c16, turn = D == 64 ? row >> 1 & 7 : row & 15;
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks) {
-        const u32x4 kf = sh_k[buf][row * CH + ((4 * ks + g) ^ turn)];
+    for (int k = 0; k < KS; k += KB) {
+      if (k + KB < KS) read_k(k + KB);
+      __builtin_amdgcn_sched_barrier(0);  // the next reads are on their way before these products
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) s[rt][t] = mfma<BF>(kf, qf[rt][ks], s[rt][t]);
-      }
+      for (int i = 0; i < KB; ++i)
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int rt = 0; rt < RT; ++rt) s[rt][t] = mfma<BF>(kf[k / KB & 1][t][i], qf[rt][k + i], s[rt][t]);
+      __builtin_amdgcn_sched_barrier(0);
     }
-    if (kb + kKeys > all || hole) {
-      const bool have = (g < 2 ? h0 : h1) >= 0;
+    u32x4 vf[2][DB];
+    auto read_v = [&](int d0) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int key = kb + 8 * g + j, nj = key - q.ctx;
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
-          const bool see = have && key < k1 && (nj < 0 || (tree ? nj < 64 && (bits[rt] >> (nj & 63) & 1) : nj <= tok[rt]));
-          s[rt][j >> 2][j & 3] = see ? s[rt][j >> 2][j & 3] * c2 : -INFINITY;
-        }
+      for (int d = 0; d < DB; ++d) {
+        const char* x = bv + (at_v ^ (d0 + d) << 5);
+        const u32x2 lo = read_tr(x), hi = read_tr(x + 4 * CH * 16);
+        vf[d0 / DB & 1][d] = u32x4{lo[0], lo[1], hi[0], hi[1]};
       }
-    } else {
+    };
+    read_v(0);  // runs under the softmax
+    __builtin_amdgcn_sched_barrier(0);
+    if (kb + kKeys > all || hole) {
+      // (what the rows see is looked up here, not kept in registers over the loop)
+      const int tid = fresh_tid(), key0 = kb + 8 * (tid >> 4 & 3);
+      const int end = ((tid >> 4 & 3) < 2 ? h0 : h1) >= 0 ? k1 : 0;  // keys that there are
 #pragma unroll
-      for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-        for (int t = 0; t < 2; ++t) s[rt][t] *= c2;
+      for (int rt = 0; rt < RT; ++rt) {
+        const int r = (tid >> 6) * RW + rt * 16 + (tid & 15), tok = r < nrows ? (tile * R + r) / G : -1;
+        mask_block(s[rt], key0, end, q.ctx, tree, tok, tree && tok >= 0 ? a.tree[q.row0 + tok] : 0);
+      }
     }
     u32x4 p[RT][PARTS];
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt) softmax_block<BF, PARTS, VG, VD>(s[rt], m[rt], l[rt], o[rt], p[rt]);
+    for (int rt = 0; rt < RT; ++rt) softmax_block<BF, PARTS>(s[rt], c2, m[rt], l[rt], o[rt], p[rt]);
 #pragma unroll
-    for (int i = 0; i < VG; ++i) {
-      vdw vf[8];
+    for (int d0 = 0; d0 < DT; d0 += DB) {
+      if (d0 + DB < DT) read_v(d0 + DB);
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-        vf[j] = reinterpret_cast<const vdw*>(&sh_v[buf][(8 * g + j) * CH])[16 * i + c16];
+      for (int d = 0; d < DB; ++d)
 #pragma unroll
-      for (int e = 0; e < VD; ++e) {
-        u32x4 vt;
+        for (int n = 0; n < PARTS; ++n)
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          vt[j] = __builtin_amdgcn_perm(vf[2 * j + 1][e >> 1], vf[2 * j][e >> 1], (e & 1) ? 0x07060302u : 0x05040100u);
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-          for (int n = 0; n < PARTS; ++n) o[rt][i][e] = mfma<BF>(vt, p[rt][n], o[rt][i][e]);
-      }
+          for (int rt = 0; rt < RT; ++rt) o[rt][d0 + d] = mfma<BF>(vf[d0 / DB & 1][d], p[rt][n], o[rt][d0 + d]);
     }
     if (more) store(nb, buf ^ 1);
   }
@@ -612,54 +670,53 @@ __global__ void __launch_bounds__(64 * kWaves) attn_tile_kernel(btf_paged_attent
   float* slot = nullptr;
   if (cut) slot = static_cast<float*>(a.ws) + (size_t)(q.slot + q.local) * kSlot<D, R>;
   bool odd = false;
+  const int tid = fresh_tid();
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
-    const int r = w * RW + rt * 16 + c16, row = tile * R + r;
+    const int r = (tid >> 6) * RW + rt * 16 + (tid & 15), row = tile * R + r, g = tid >> 4 & 3;
     l[rt] = groups_sum(l[rt]);
     float chk = l[rt] - l[rt];
     const float f = cut ? 1.f : l[rt] == 0.f ? 0.f : 1.f / l[rt];
     float* y = cut ? slot + (size_t)r * D : a.out + (size_t)(q.row0 + row / G) * a.ldo + (kvh * G + row % G) * D;
     const bool live = r < nrows;
 #pragma unroll
-    for (int i = 0; i < VG; ++i)
-#pragma unroll
-      for (int d = 0; d < 4; ++d)
-#pragma unroll
-        for (int e = 0; e < VD; e += 4) {
-          f32x4 v = {o[rt][i][e][d], o[rt][i][e + 1][d], o[rt][i][e + 2][d], o[rt][i][e + 3][d]};
-          chk += (v[0] - v[0]) + (v[1] - v[1]) + (v[2] - v[2]) + (v[3] - v[3]);
-          if (live) *reinterpret_cast<f32x4*>(y + 16 * VD * i + VD * (4 * g + d) + e) = v * f;
-        }
+    for (int i = 0; i < DT; ++i) {
+      const f32x4 v = o[rt][i];  // dims 16 i + 4 g ..
+      chk += (v[0] - v[0]) + (v[1] - v[1]) + (v[2] - v[2]) + (v[3] - v[3]);
+      if (live) *reinterpret_cast<f32x4*>(y + 16 * i + 4 * g) = v * f;
+    }
     if (cut && live && g == 0) slot[R * D + r] = m[rt], slot[R * D + R + r] = l[rt];
-    odd |= chk != 0.f;
+    odd |= !(chk == 0.f);
   }
   if (!__any(odd)) return;
   __threadfence_block();  // (the rows below are written again by other lanes of this wave)
-  for (int r = w * RW; r < min(nrows, (w + 1) * RW); ++r) {
+  const int lane2 = tid & 63, r0 = __builtin_amdgcn_readfirstlane(tid >> 6) * RW;
+  for (int r = r0; r < min(nrows, r0 + RW); ++r) {
     constexpr int E = D / 64;
     float po[E], pm, pl;
     const int row = tile * R + r;
-    plain_row<D, BF>(a, kv, q, kvh, row, k0, max(k0, k1), c2, po, pm, pl);
+    plain_row<D, BF>(a, kv, q, kvh, row, k0, max(k0, k1), po, pm, pl);
     float* y = cut ? slot + (size_t)r * D : a.out + (size_t)(q.row0 + row / G) * a.ldo + (kvh * G + row % G) * D;
 #pragma unroll
-    for (int e = 0; e < E; ++e) y[lane * E + e] = cut ? po[e] : pl == 0.f ? 0.f : po[e] / pl;
-    if (cut && lane == 0) slot[R * D + r] = pm, slot[R * D + R + r] = pl;
+    for (int e = 0; e < E; ++e) y[lane2 * E + e] = cut ? po[e] : pl == 0.f ? 0.f : po[e] / pl;
+    if (cut && lane2 == 0) slot[R * D + r] = pm, slot[R * D + R + r] = pl;
   }
 }
 
-// The pieces of one row of one head put together: a wave takes the pieces' maxima
-// and sums 64 at a time, then every wave its share of the pieces' values (so that
-// many loads are in flight), and the waves join in LDS.
+// The pieces of one row of one head put together. Few rows: by the four waves of a
+// workgroup, each its share of the pieces (so that many loads are in flight), joined
+// in LDS. Many rows (ONE): by one wave.
 constexpr int kJoinWaves = 4;
-template <int D, int R>
+template <int D, int R, bool ONE>
 __global__ void __launch_bounds__(64 * kJoinWaves) attn_join_kernel(btf_paged_attention a, btf_kv_cache kv) {
   constexpr int E = D / 64;  // values of a lane
+  constexpr int BY = ONE ? 1 : kJoinWaves;  // waves of a row
   typedef float vE __attribute__((ext_vector_type(E)));
-  __shared__ float sh[kJoinWaves][D];
   Req q;
-  if (!find<R, true>(a, kv, blockIdx.x, q) || q.pieces == 1) return;  // the whole workgroup
+  if (!find<R, true, true>(a, kv, blockIdx.x, q) || q.pieces == 1) return;  // the whole workgroup
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int G = a.heads / kv.heads, h = blockIdx.y, kvh = h / G;
+  const int G = a.heads / kv.heads, h = ONE ? blockIdx.y * kJoinWaves + w : blockIdx.y, kvh = h / G;
+  if (h >= a.heads) return;
   const int row = q.local * G + h % G, tile = row / R, r = row % R;
   const float* slot = static_cast<const float*>(a.ws) + (size_t)(q.slot + (q.tiles - 1 - tile) * kv.heads + kvh) * kSlot<D, R>;
   const size_t step = (size_t)q.tiles * kv.heads * kSlot<D, R>;
@@ -673,51 +730,66 @@ __global__ void __launch_bounds__(64 * kJoinWaves) attn_join_kernel(btf_paged_at
     float c = 0.f;
     if (i0 + lane < q.pieces) {
       const float* x = slot + (i0 + lane) * step + R * D + r;
-      c = exp2f(x[0] - base);
+      c = fast_exp2(x[0] - base);
       sum += c * x[R];
     }
     const int n = min(64, q.pieces - i0);
-    for (int i = w; i < n; i += 4 * kJoinWaves)
+    for (int i = ONE ? 0 : w; i < n; i += 4 * BY)
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
-        const int j = min(i + u * kJoinWaves, n - 1);
-        const float f = i + u * kJoinWaves < n ? __shfl(c, j, 64) : 0.f;
+        const int j = min(i + u * BY, n - 1);
+        const float f = __shfl(c, j, 64);
         const vE x = *reinterpret_cast<const vE*>(slot + (i0 + j) * step + (size_t)r * D + lane * E);
-        if (i + u * kJoinWaves < n) v += f * x;
+        if (i + u * BY < n) v += f * x;
       }
   }
   sum = wave_sum_f(sum);
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  float* y = a.out + (size_t)(q.row0 + q.local) * a.ldo + h * D;
+  if (ONE) {
+    *reinterpret_cast<vE*>(y + lane * E) = v * inv;
+    return;
+  }
+  __shared__ float sh[kJoinWaves][D];
   *reinterpret_cast<vE*>(&sh[w][lane * E]) = v;
   __syncthreads();
-  const float inv = sum == 0.f ? 0.f : 1.f / sum;
   for (int d = threadIdx.x; d < D; d += 64 * kJoinWaves) {
-    float y = sh[0][d];
+    float x = sh[0][d];
 #pragma unroll
-    for (int i = 1; i < kJoinWaves; ++i) y += sh[i][d];
-    a.out[(size_t)(q.row0 + q.local) * a.ldo + h * D + d] = y * inv;
+    for (int i = 1; i < kJoinWaves; ++i) x += sh[i][d];
+    y[d] = x * inv;
   }
 }
 
-// Rows of an item's tile, by the rows that a request has on average for a KV head.
+// Rows of an item's tile, by the rows that a request has on average for a KV head. (32 rows of heads of 256 do not
+// fit a wave's registers with K and V there too.)
 int tile_rows(int S, int T, int heads, const btf_kv_cache& kv) {
   const int64_t rows = (int64_t)T * (heads / kv.heads);
-  return rows <= 16 * (int64_t)S ? 16 : rows <= 32 * (int64_t)S ? 32 : 128;
+  return rows <= 16 * (int64_t)S ? 16 : rows <= 32 * (int64_t)S && kv.dim < 256 ? 32 : 128;
 }
 
 template <int D, bool BF>
 int attn_go(const btf_paged_attention& a, const btf_kv_cache& kv, hipStream_t st) {
   const int R = tile_rows(a.S, a.T, a.heads, kv);
   const int64_t tiles = (int64_t)a.T * (a.heads / kv.heads) / R + a.S;  // at most
-  const dim3 grid((unsigned)(kTarget + tiles * kv.heads)), join(a.T, a.heads), blk(64 * kWaves);
+  const dim3 grid((unsigned)(kTarget + tiles * kv.heads)), blk(64 * kWaves);
   if (R == 16) hipLaunchKernelGGL((attn_stream_kernel<D, BF, 1>), grid, blk, 0, st, a, kv);
-  else if (R == 32) hipLaunchKernelGGL((attn_stream_kernel<D, BF, 2>), grid, blk, 0, st, a, kv);
-  else hipLaunchKernelGGL((attn_tile_kernel<D, BF>), grid, blk, 0, st, a, kv);
+  else if constexpr (D < 256) {
+    if (R == 32) hipLaunchKernelGGL((attn_stream_kernel<D, BF, 2>), grid, blk, 0, st, a, kv);
+  }
+  if (R == 128) hipLaunchKernelGGL((attn_tile_kernel<D, BF>), grid, blk, 0, st, a, kv);
   const int rc = launch_status("attn kernel");
   if (rc != BTF_OK) return rc;
-  const dim3 jblk(64 * kJoinWaves);
-  if (R == 16) hipLaunchKernelGGL((attn_join_kernel<D, 16>), join, jblk, 0, st, a, kv);
-  else if (R == 32) hipLaunchKernelGGL((attn_join_kernel<D, 32>), join, jblk, 0, st, a, kv);
-  else hipLaunchKernelGGL((attn_join_kernel<D, 128>), join, jblk, 0, st, a, kv);
+  // one wave a row from 2048 rows of heads on
+  const bool one = (int64_t)a.T * a.heads >= 2048;
+  const dim3 join(a.T, one ? (a.heads + kJoinWaves - 1) / kJoinWaves : a.heads), jblk(64 * kJoinWaves);
+  auto go = [&](auto few, auto many) {
+    if (one) hipLaunchKernelGGL(many, join, jblk, 0, st, a, kv);
+    else hipLaunchKernelGGL(few, join, jblk, 0, st, a, kv);
+  };
+  if (R == 16) go(attn_join_kernel<D, 16, false>, attn_join_kernel<D, 16, true>);
+  else if (R == 32) go(attn_join_kernel<D, 32, false>, attn_join_kernel<D, 32, true>);
+  else go(attn_join_kernel<D, 128, false>, attn_join_kernel<D, 128, true>);
   return launch_status("attn_join_kernel");
 }
 
