@@ -5,7 +5,7 @@
 // query heads of one KV head, in tiles of R; its keys are cut into pieces of C.
 // An item, the work of one workgroup, is one (request, KV head, row tile,
 // piece). C follows from all requests' lengths (read on the device), so that
-// about kTarget items of like size come out whatever the lengths: one long
+// about target(R) items of like size come out whatever the lengths: one long
 // request among short ones is cut, the short ones are not. An item of a request
 // that is not cut writes out; the others leave (maximum, sum, values) in the
 // workspace and attn_join_kernel puts the pieces of a row together.
@@ -47,7 +47,8 @@ typedef __bf16 b8 __attribute__((ext_vector_type(8)));
 constexpr int kWaves = 4;
 constexpr int kKeys = 32;      // keys of a block
 constexpr int kStep = kWaves * kKeys;
-constexpr int kTarget = 512;   // items that a launch is cut into: two for each CU
+// Items that a launch is cut into, for tiles of R rows.
+constexpr int target(int R) { return R <= 32 ? 1536 : 1024; }
 
 template <bool BF>
 __device__ __forceinline__ float from16(uint16_t h) {
@@ -123,7 +124,7 @@ __device__ __forceinline__ float wave_sum_f(float v) {
 
 // The request of item `id` (BY_ROW: of row `id`), found by every wave for itself:
 // the lanes take 64 requests at a time. False: there is no such item.
-// SCALAR: the answer in scalar registers (the stream kernel has none to spare).
+// SCALAR: most of the answer in scalar registers (the stream kernel has none to spare).
 template <int R, bool BY_ROW, bool SCALAR>
 __device__ bool find(const btf_paged_attention& a, const btf_kv_cache& kv, int id, Req& q) {
   const int lane = threadIdx.x & 63, G = a.heads / kv.heads;
@@ -144,7 +145,7 @@ __device__ bool find(const btf_paged_attention& a, const btf_kv_cache& kv, int i
     if (n > 0) work += (float)((n * G + R - 1) / R) * (float)len;
   }
   work = wave_sum_f(work) * (float)kv.heads;
-  const int C = max(kStep, __builtin_amdgcn_readfirstlane((int)(work / (float)(kTarget * kStep) + 1.f)) * kStep);
+  const int C = max(kStep, __builtin_amdgcn_readfirstlane((int)(work / (float)(target(R) * kStep) + 1.f)) * kStep);
   int items = 0, slots = 0;  // before the chunk
   for (int s0 = 0; s0 < a.S; s0 += 64) {
     read(s0 + lane, r0, n, len, full);
@@ -162,14 +163,14 @@ __device__ bool find(const btf_paged_attention& a, const btf_kv_cache& kv, int i
       const int l = __builtin_ctzll(who);
       auto of = [&](int v) { return SCALAR ? __builtin_amdgcn_readlane(v, l) : __shfl(v, l, 64); };
       q.s = s0 + l;
-      q.row0 = of(r0);
+      q.row0 = __shfl(r0, l, 64);
       q.n = of(n);
       q.len = of(len);
       q.ctx = of(full) - q.n;
       q.tiles = of(tiles);
       q.pieces = of(pieces);
       q.local = id - (BY_ROW ? q.row0 : items + of(upto - mine));
-      q.slot = slots + of(cuts - cut);
+      q.slot = slots + __shfl(cuts - cut, l, 64);
       q.C = C;
       return true;
     }
@@ -479,9 +480,9 @@ __global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_e
 
 // ---- many rows: K and V through LDS ----
 // A workgroup's 4 waves have 32 rows each (two MFMA tiles, which share every operand
-// of K and V) and walk the same keys, 32 at a time, from two buffers in LDS: the
-// next block is on its way to registers while this one is worked on, and is written
-// to the other buffer after it. K's rows are stored in the order of the score tiles'
+// of K and V; one for heads of 256, whose sums take twice the registers) and walk the
+// same keys, 32 at a time, from two buffers in LDS: the next block is on its way to
+// one while the other is worked on. K's rows lie in the order of the score tiles'
 // rows, their 16-byte chunks turned by the row, so that the 16 rows that a lane group
 // reads at once lie in different banks. V is read by the transposing LDS read: 16
 // lanes read 4 keys of 16 dims and get one dim's 4 keys each; its rows are turned by
@@ -492,6 +493,19 @@ __device__ __forceinline__ u32x2 read_tr(const void* p) {
   return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)p));
 }
 
+// 16 bytes a lane from base + off to LDS, 64 lanes in a row from `to` (the same in all lanes). As asm, which has no
+// output and whose end `landed` waits for: the compiler would wait for the builtin's end before the next read of any of
+// LDS, the other buffer's too (2048 rows over 6143 keys 602 us).
+__device__ __forceinline__ void to_lds(const void* base, uint32_t off, const void* to) {
+  const uint32_t lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char*)to;
+  asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(off), "s"(base), "{m0}"(__builtin_amdgcn_readfirstlane(lds)));
+}
+__device__ __forceinline__ void to_lds(const void* from, const void* to) {
+  const uint32_t lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char*)to;
+  asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(from), "{m0}"(__builtin_amdgcn_readfirstlane(lds)));
+}
+__device__ __forceinline__ void landed() { asm volatile("s_waitcnt vmcnt(0)" : : : "memory"); }
+
 // The thread's number, of which the compiler does not know that it had it before: what
 // follows from it is worked out anew and takes no registers in the loop.
 __device__ __forceinline__ int fresh_tid() {
@@ -500,21 +514,38 @@ __device__ __forceinline__ int fresh_tid() {
   return t;
 }
 
+constexpr int tile_R(int D) { return D == 256 ? 64 : 128; }
+// The launch's arguments, read again: what only the end needs is not kept in scalar registers over the loop.
+struct Args {
+  btf_paged_attention a;
+  btf_kv_cache kv;
+};
+typedef __attribute__((address_space(4))) const Args* args_p;
+__device__ __forceinline__ Args fresh_args() {
+  args_p p = (args_p)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(p));
+  Args g;
+  __builtin_memcpy(&g, (const Args*)p, sizeof g);
+  return g;
+}
+
 template <int D, bool BF>
-__global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(D < 256 ? 2 : 1)))
-    attn_tile_kernel(btf_paged_attention a, btf_kv_cache kv) {
-  constexpr int RT = 2, RW = 16 * RT, R = kWaves * RW;
+__global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2)))
+    attn_tile_kernel(Args args) {
+  const btf_paged_attention& a = args.a;
+  const btf_kv_cache& kv = args.kv;
+  constexpr int NW = kWaves, R = tile_R(D), RW = R / NW, RT = RW / 16;
   constexpr int KS = D / 32;
   constexpr int DT = D / 16;            // dim tiles of the values
   constexpr int DB = 4, KB = 2;         // ... read at a time, and steps of K
   constexpr int PARTS = BF ? 3 : 2;
   constexpr int CH = D / 8;             // 16-byte chunks of a row
-  constexpr int NC = kKeys * CH / (64 * kWaves);  // of a block, for each thread
+  constexpr int NC = kKeys * CH / (64 * NW);  // of a block, for each thread
   __shared__ u32x4 sh_k[2][kKeys * CH], sh_v[2][kKeys * CH];
 
   Req q;
   if (!find<R, false, true>(a, kv, blockIdx.x, q)) return;  // the whole workgroup
-  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) & (NW - 1);
   const int c16 = lane & 15, g = lane >> 4;
   const int G = a.heads / kv.heads;
   const int kvh = q.local % kv.heads, rest = q.local / kv.heads;
@@ -550,58 +581,71 @@ __global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_e
   const uint16_t* vp = static_cast<const uint16_t*>(kv.v) + (size_t)kvh * kv.head_stride;
   const int* tab = a.table + (size_t)q.s * a.ldt;
   const int sh = __builtin_ctz(kv.page), last = (q.len - 1) >> sh;
-  auto page_of = [&](int key) {
-    const int p = key < q.len ? tab[min(key >> sh, last)] : -1;
-    return p >= 0 && p < kv.pages ? p : -1;
+  // Pages of a block's two halves. They are looked up two blocks ahead (lanes 0 and 1, by a vector load that comes
+  // before the block's own: waiting for those waits for it).
+  int p0 = -1, p1 = -1, ahead = -1;
+  auto look = [&](int kb) {
+    const int key = kb + 16 * (lane & 1);
+    ahead = -1;
+    if (key < q.len) ahead = tab[min(key >> sh, last)];
   };
-  u32x4 rk[NC], rv[NC];
-  int p0 = -1, p1 = -1;  // pages of a block's two halves
-  auto load = [&](int kb) {  // a block to registers
+  auto take = [&] {
+    p0 = __builtin_amdgcn_readlane(ahead, 0), p1 = __builtin_amdgcn_readlane(ahead, 1);
+    if (p0 >= kv.pages) p0 = -1;
+    if (p1 >= kv.pages) p1 = -1;
+  };
+  // A block goes from memory to LDS with no register between: a wave's load fills 64 chunks in a row, each lane says
+  // where its chunk comes from. A half's start is in scalar registers, the lane's place in it the same for every block.
+  auto key_of = [](int row) { return 8 * (row >> 2 & 3) + 4 * (row >> 4) + (row & 3); };  // of a row of K in LDS
+  uint32_t off_k[NC], off_v[NC];
+#pragma unroll
+  for (int n = 0; n < NC; ++n) {
+    const int c = threadIdx.x + 64 * NW * n, row = c / CH, ch = c % CH;
+    const int turn_k = D == 64 ? row >> 1 & 7 : row & 15, turn_v = 2 * ((4 * (row >> 3) + (row & 3)) & (DT - 1));
+    off_k[n] = 2 * ((uint32_t)(key_of(row) & 15) * (uint32_t)kv.tok_stride + 8 * (ch ^ turn_k));
+    off_v[n] = 2 * ((uint32_t)(row & 15) * (uint32_t)kv.tok_stride + 8 * (ch ^ turn_v));
+  }
+  auto load = [&](int kb, int buf) {
+    const uint32_t tok = (uint32_t)kv.tok_stride;  // (at most 2^24, and 256 tokens a page)
+    const size_t b0 = (size_t)max(p0, 0) * kv.page_stride + (uint32_t)(kb & (kv.page - 1)) * tok;
+    const size_t b1 = (size_t)max(p1, 0) * kv.page_stride + (uint32_t)((kb + 16) & (kv.page - 1)) * tok;
 #pragma unroll
     for (int n = 0; n < NC; ++n) {
-      const int c = threadIdx.x + 64 * kWaves * n, j = c / CH, ch = c % CH;
-      const int pg = j < 16 ? p0 : p1;
-      const size_t at = (size_t)max(pg, 0) * kv.page_stride + (size_t)((kb + j) & (kv.page - 1)) * kv.tok_stride + 8 * ch;
-      rk[n] = *reinterpret_cast<const u32x4*>(kp + at);
-      rv[n] = *reinterpret_cast<const u32x4*>(vp + at);
+      const int c0 = 64 * (w + NW * n), row = (D == 64 ? c0 + lane : c0) / CH;  // (a wave's rows share a half from 128 dims on)
+      const uint16_t *k = kp + (key_of(row) < 16 ? b0 : b1), *v = vp + (row < 16 ? b0 : b1);
+      if constexpr (D == 64) {
+        to_lds(reinterpret_cast<const char*>(k) + off_k[n], &sh_k[buf][c0]);
+        to_lds(reinterpret_cast<const char*>(v) + off_v[n], &sh_v[buf][c0]);
+      } else {
+        to_lds(k, off_k[n], &sh_k[buf][c0]);
+        to_lds(v, off_v[n], &sh_v[buf][c0]);
+      }
     }
   };
-  auto store = [&](int kb, int buf) {  // ... and on to LDS, cleared where no row sees it
-    const int tid = D == 256 ? fresh_tid() : threadIdx.x;
+  auto finish = [&](int kb, int buf) {  // the block has landed; what no row sees of it is cleared by who loaded it
+    landed();
     if (p0 < 0 || p1 < 0 || kb + kKeys > k1)
 #pragma unroll
       for (int n = 0; n < NC; ++n) {
-        const int j = (tid + 64 * kWaves * n) / CH;
-        if ((j < 16 ? p0 : p1) < 0 || kb + j >= k1) rk[n] = rv[n] = u32x4{0, 0, 0, 0};
+        const int c = threadIdx.x + 64 * NW * n, j = c / CH, key = key_of(j);
+        if ((key < 16 ? p0 : p1) < 0 || kb + key >= k1) sh_k[buf][c] = u32x4{0, 0, 0, 0};
+        if ((j < 16 ? p0 : p1) < 0 || kb + j >= k1) sh_v[buf][c] = u32x4{0, 0, 0, 0};
       }
-#pragma unroll
-    for (int n = 0; n < NC; ++n) {
-      const int c = tid + 64 * kWaves * n, j = c / CH, ch = c % CH;
-      const int row = 16 * (j >> 2 & 1) + 4 * (j >> 3) + (j & 3);
-      sh_k[buf][row * CH + (ch ^ (D == 64 ? row >> 1 & 7 : row & 15))] = rk[n];
-      sh_v[buf][j * CH + (ch ^ 2 * ((4 * (j >> 3) + (j & 3)) & (DT - 1)))] = rv[n];
-    }
   };
   // the lane's places in a buffer: K chunk g of its row in score tile 0, V's key 8 g + c16 / 4 and dims 4 (c16 % 4) ..
   const uint32_t at_k = c16 * CH * 16 + ((g ^ (D == 64 ? c16 >> 1 & 7 : c16)) << 4);
   const uint32_t at_v = (8 * g + (c16 >> 2)) * CH * 16 + (((4 * g + (c16 >> 2)) & (DT - 1)) << 5) + 8 * (c16 & 3);
   if (k0 < k1) {
-    p0 = page_of(k0), p1 = page_of(k0 + 16);
-    load(k0);
-    store(k0, 0);
+    look(k0);
+    take();
+    look(k0 + kKeys);
+    load(k0, 0);
+    finish(k0, 0);
   }
-  int buf = 0;
-  for (int kb = k0; kb < k1; kb += kKeys, buf ^= 1) {
-    const bool hole = p0 < 0 || (p1 < 0 && kb + 16 < k1);  // of this block
-    const int h0 = p0, h1 = p1, nb = kb + kKeys;
-    const bool more = nb < k1;
-    __syncthreads();  // this block is in LDS; the other buffer's readers are done
-    if (more) {
-      p0 = page_of(nb), p1 = page_of(nb + 16);
-      load(nb);
-    }
+  u32x4 p[RT][PARTS];
+  // scores, softmax and probabilities of the block at kb, in buffer buf; its pages
+  auto scores = [&](int kb, int buf, int h0, int h1) {
     const char* bk = reinterpret_cast<const char*>(sh_k[buf]);
-    const char* bv = reinterpret_cast<const char*>(sh_v[buf]);
     u32x4 kf[2][2][KB];
     auto read_k = [&](int k) {
 #pragma unroll
@@ -628,6 +672,21 @@ __global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_e
           for (int rt = 0; rt < RT; ++rt) s[rt][t] = mfma<BF>(kf[k / KB & 1][t][i], qf[rt][k + i], s[rt][t]);
       __builtin_amdgcn_sched_barrier(0);
     }
+    if (kb + kKeys > all || h0 < 0 || (h1 < 0 && kb + 16 < k1)) {
+      // (what the rows see is looked up here, not kept in registers over the loop)
+      const int tid = fresh_tid(), key0 = kb + 8 * (tid >> 4 & 3);
+      const int end = ((tid >> 4 & 3) < 2 ? h0 : h1) >= 0 ? k1 : 0;  // keys that there are
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) {
+        const int r = (tid >> 6) * RW + rt * 16 + (tid & 15), tok = r < nrows ? (tile * R + r) / G : -1;
+        mask_block(s[rt], key0, end, q.ctx, tree, tok, tree && tok >= 0 ? fresh_args().a.tree[q.row0 + tok] : 0);
+      }
+    }
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) softmax_block<BF, PARTS>(s[rt], c2, m[rt], l[rt], o[rt], p[rt]);
+  };
+  auto values = [&](int buf) {  // O^T += V^T P^T
+    const char* bv = reinterpret_cast<const char*>(sh_v[buf]);
     u32x4 vf[2][DB];
     auto read_v = [&](int d0) {
 #pragma unroll
@@ -637,47 +696,47 @@ __global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_e
         vf[d0 / DB & 1][d] = u32x4{lo[0], lo[1], hi[0], hi[1]};
       }
     };
-    read_v(0);  // runs under the softmax
-    __builtin_amdgcn_sched_barrier(0);
-    if (kb + kKeys > all || hole) {
-      // (what the rows see is looked up here, not kept in registers over the loop)
-      const int tid = fresh_tid(), key0 = kb + 8 * (tid >> 4 & 3);
-      const int end = ((tid >> 4 & 3) < 2 ? h0 : h1) >= 0 ? k1 : 0;  // keys that there are
-#pragma unroll
-      for (int rt = 0; rt < RT; ++rt) {
-        const int r = (tid >> 6) * RW + rt * 16 + (tid & 15), tok = r < nrows ? (tile * R + r) / G : -1;
-        mask_block(s[rt], key0, end, q.ctx, tree, tok, tree && tok >= 0 ? a.tree[q.row0 + tok] : 0);
-      }
-    }
-    u32x4 p[RT][PARTS];
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt) softmax_block<BF, PARTS>(s[rt], c2, m[rt], l[rt], o[rt], p[rt]);
+    read_v(0);
 #pragma unroll
     for (int d0 = 0; d0 < DT; d0 += DB) {
       if (d0 + DB < DT) read_v(d0 + DB);
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int d = 0; d < DB; ++d)
+      for (int n = 0; n < PARTS; ++n)  // (a sum's next product comes after all the others')
 #pragma unroll
-        for (int n = 0; n < PARTS; ++n)
+        for (int d = 0; d < DB; ++d)
 #pragma unroll
           for (int rt = 0; rt < RT; ++rt) o[rt][d0 + d] = mfma<BF>(vf[d0 / DB & 1][d], p[rt][n], o[rt][d0 + d]);
     }
-    if (more) store(nb, buf ^ 1);
+  };
+  int buf = 0;
+  for (int kb = k0; kb < k1; kb += kKeys, buf ^= 1) {
+    const int h0 = p0, h1 = p1, nb = kb + kKeys;  // (p0 and p1 are this block's until take())
+    const bool more = nb < k1;
+    __syncthreads();  // this block is in LDS; the other buffer's readers are done
+    if (more) {
+      take();
+      look(nb + kKeys);
+      load(nb, buf ^ 1);
+    }
+    scores(kb, buf, h0, h1);
+    values(buf);
+    if (more) finish(nb, buf ^ 1);
   }
 
   const bool cut = q.pieces > 1;
   float* slot = nullptr;
-  if (cut) slot = static_cast<float*>(a.ws) + (size_t)(q.slot + q.local) * kSlot<D, R>;
   bool odd = false;
   const int tid = fresh_tid();
+  const Args end = fresh_args();
+  if (cut) slot = static_cast<float*>(end.a.ws) + (size_t)(q.slot + q.local) * kSlot<D, R>;
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
     const int r = (tid >> 6) * RW + rt * 16 + (tid & 15), row = tile * R + r, g = tid >> 4 & 3;
     l[rt] = groups_sum(l[rt]);
     float chk = l[rt] - l[rt];
     const float f = cut ? 1.f : l[rt] == 0.f ? 0.f : 1.f / l[rt];
-    float* y = cut ? slot + (size_t)r * D : a.out + (size_t)(q.row0 + row / G) * a.ldo + (kvh * G + row % G) * D;
+    float* y = cut ? slot + (size_t)r * D : end.a.out + (size_t)(q.row0 + row / G) * end.a.ldo + (kvh * G + row % G) * D;
     const bool live = r < nrows;
 #pragma unroll
     for (int i = 0; i < DT; ++i) {
@@ -695,8 +754,8 @@ __global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_e
     constexpr int E = D / 64;
     float po[E], pm, pl;
     const int row = tile * R + r;
-    plain_row<D, BF>(a, kv, q, kvh, row, k0, max(k0, k1), po, pm, pl);
-    float* y = cut ? slot + (size_t)r * D : a.out + (size_t)(q.row0 + row / G) * a.ldo + (kvh * G + row % G) * D;
+    plain_row<D, BF>(end.a, end.kv, q, kvh, row, k0, max(k0, k1), po, pm, pl);
+    float* y = cut ? slot + (size_t)r * D : end.a.out + (size_t)(q.row0 + row / G) * end.a.ldo + (kvh * G + row % G) * D;
 #pragma unroll
     for (int e = 0; e < E; ++e) y[lane2 * E + e] = cut ? po[e] : pl == 0.f ? 0.f : po[e] / pl;
     if (cut && lane2 == 0) slot[R * D + r] = pm, slot[R * D + R + r] = pl;
@@ -765,19 +824,21 @@ __global__ void __launch_bounds__(64 * kJoinWaves) attn_join_kernel(btf_paged_at
 // fit a wave's registers with K and V there too.)
 int tile_rows(int S, int T, int heads, const btf_kv_cache& kv) {
   const int64_t rows = (int64_t)T * (heads / kv.heads);
-  return rows <= 16 * (int64_t)S ? 16 : rows <= 32 * (int64_t)S && kv.dim < 256 ? 32 : 128;
+  return rows <= 16 * (int64_t)S ? 16 : rows <= 32 * (int64_t)S && kv.dim < 256 ? 32 : tile_R(kv.dim);
 }
 
 template <int D, bool BF>
 int attn_go(const btf_paged_attention& a, const btf_kv_cache& kv, hipStream_t st) {
   const int R = tile_rows(a.S, a.T, a.heads, kv);
   const int64_t tiles = (int64_t)a.T * (a.heads / kv.heads) / R + a.S;  // at most
-  const dim3 grid((unsigned)(kTarget + tiles * kv.heads)), blk(64 * kWaves);
+  // items: one for each tile and target(R) more, or all the pieces that the table has room for
+  const int64_t room = ((int64_t)a.ldt * kv.page + kStep - 1) / kStep, most = tiles * kv.heads;
+  const dim3 grid((unsigned)(most * room < most + target(R) ? most * room : most + target(R))), blk(64 * kWaves);
   if (R == 16) hipLaunchKernelGGL((attn_stream_kernel<D, BF, 1>), grid, blk, 0, st, a, kv);
   else if constexpr (D < 256) {
     if (R == 32) hipLaunchKernelGGL((attn_stream_kernel<D, BF, 2>), grid, blk, 0, st, a, kv);
   }
-  if (R == 128) hipLaunchKernelGGL((attn_tile_kernel<D, BF>), grid, blk, 0, st, a, kv);
+  if (R == tile_R(D)) hipLaunchKernelGGL((attn_tile_kernel<D, BF>), grid, dim3(64 * kWaves), 0, st, Args{a, kv});
   const int rc = launch_status("attn kernel");
   if (rc != BTF_OK) return rc;
   // one wave a row from 2048 rows of heads on
@@ -788,17 +849,20 @@ int attn_go(const btf_paged_attention& a, const btf_kv_cache& kv, hipStream_t st
     else hipLaunchKernelGGL(few, join, jblk, 0, st, a, kv);
   };
   if (R == 16) go(attn_join_kernel<D, 16, false>, attn_join_kernel<D, 16, true>);
-  else if (R == 32) go(attn_join_kernel<D, 32, false>, attn_join_kernel<D, 32, true>);
-  else go(attn_join_kernel<D, 128, false>, attn_join_kernel<D, 128, true>);
+  else if constexpr (D < 256) {
+    if (R == 32) go(attn_join_kernel<D, 32, false>, attn_join_kernel<D, 32, true>);
+  }
+  if (R == tile_R(D)) go(attn_join_kernel<D, tile_R(D), false>, attn_join_kernel<D, tile_R(D), true>);
   return launch_status("attn_join_kernel");
 }
 
 }  // namespace
 
-// Cut requests have at most 2 kTarget items: a piece of them holds at least C / 2 keys on average, and C is at least
-// all the work over kTarget.
+// Cut requests have at most 2 target(R) items: a piece of them holds at least C / 2 keys on average, and C is at least
+// all the work over target(R).
 int64_t paged_attention_ws_bytes(int S, int T, int heads, const btf_kv_cache& kv) {
-  return (int64_t)2 * kTarget * tile_rows(S, T, heads, kv) * (kv.dim + 2) * 4;
+  const int R = tile_rows(S, T, heads, kv);
+  return (int64_t)2 * target(R) * R * (kv.dim + 2) * 4;
 }
 
 int paged_attention(const btf_paged_attention& a, const btf_kv_cache& kv, hipStream_t st, const DevState& ds) {

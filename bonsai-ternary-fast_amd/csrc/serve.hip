@@ -28,6 +28,7 @@ int check_kv(const btf_kv_cache* kv, const char* who, bool need_data) {
   if (kv->page_stride < 0 || kv->head_stride < 0 || kv->tok_stride < kv->dim || kv->page_stride % 8 ||
       kv->head_stride % 8 || kv->tok_stride % 8)
     return bad(who, "cache strides must be multiples of 8 values, a token's at least the head dim");
+  if (kv->tok_stride > 1 << 24) return bad(who, "a token's stride must be at most 2^24 values");
   return BTF_OK;
 }
 

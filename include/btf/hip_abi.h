@@ -433,7 +433,7 @@ typedef struct btf_kv_cache {
   int heads;        /* KV heads */
   int dim;          /* 64, 128 or 256 */
   int64_t pages;    /* pages * page < 2^31 */
-  int64_t page_stride, head_stride, tok_stride; /* multiples of 8, tok_stride >= dim */
+  int64_t page_stride, head_stride, tok_stride; /* multiples of 8, tok_stride in [dim, 2^24] */
 } btf_kv_cache;
 
 /* Rows, positions, cache slots and pages of a step from the requests' lengths.

@@ -63,7 +63,8 @@ def test_refused_before_any_hip_call(op, change):
 @pytest.mark.parametrize("change", [
     dict(type=2), dict(page=8), dict(page=512), dict(page=24), dict(dim=96), dict(heads=0), dict(k=None), dict(v=None),
     dict(k=A + 8), dict(v=A + 8), dict(pages=0), dict(pages=1 << 25), dict(tok_stride=248), dict(tok_stride=260),
-    dict(head_stride=-8), dict(head_stride=4), dict(page_stride=12)], ids=str)
+    dict(head_stride=-8), dict(head_stride=4), dict(page_stride=12),
+    dict(tok_stride=(1 << 24) + 8)], ids=str)
 def test_caches_refused(op, change):
     assert launch(op, VALID[op], dataclasses.replace(KV, **change)) == ARGS
 
