@@ -69,6 +69,43 @@ __device__ __forceinline__ float quad_max_f(float v) {
   return v;
 }
 
+// Inclusive prefix sum over the wave's lanes: shifts within 16-lane rows (a shift
+// from outside the row adds 0), then the sums of the rows before.
+__device__ __forceinline__ uint64_t wave_scan_u64(uint64_t v) {
+  auto add = [&](int lo, int hi) { v += (uint64_t)(uint32_t)hi << 32 | (uint32_t)lo; };
+  add(dpp_i<0x111>((int)v), dpp_i<0x111>((int)(v >> 32)));  // row_shr:1
+  add(dpp_i<0x112>((int)v), dpp_i<0x112>((int)(v >> 32)));
+  add(dpp_i<0x114>((int)v), dpp_i<0x114>((int)(v >> 32)));
+  add(dpp_i<0x118>((int)v), dpp_i<0x118>((int)(v >> 32)));
+  auto of = [&](int lane) {
+    return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), lane) << 32 |
+           (uint32_t)__builtin_amdgcn_readlane((int)v, lane);
+  };
+  const uint64_t t0 = of(15), t1 = of(31), t2 = of(47);
+  const int row = (threadIdx.x & 63) >> 4;
+  return v + (row > 0 ? t0 : 0) + (row > 1 ? t1 : 0) + (row > 2 ? t2 : 0);
+}
+// Inclusive prefix sum over the N <= 1024 threads of the workgroup; *total gets the
+// whole sum. part: N / 64 words in LDS.
+template <int N>
+__device__ __forceinline__ uint64_t block_scan(uint64_t v, uint64_t* part, uint64_t* total) {
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  v = wave_scan_u64(v);
+  __syncthreads();  // (part may still be read from the scan before)
+  if (lane == 63) part[w] = v;
+  __syncthreads();
+  uint64_t sums = lane < N / 64 ? part[lane] : 0;
+  sums = wave_scan_u64(sums);
+  auto of = [&](int l) {
+    return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(sums >> 32), l) << 32 |
+           (uint32_t)__builtin_amdgcn_readlane((int)sums, l);
+  };
+  const int u = __builtin_amdgcn_readfirstlane(w);
+  const uint64_t before = u ? of(u - 1) : 0;
+  *total = of(N / 64 - 1);
+  return v + before;
+}
+
 // fp16 bits -> f32 (exact) and f32 -> fp16 (round to nearest even) -> f32.
 __device__ __forceinline__ float h2f(uint16_t h) {
   _Float16 x;

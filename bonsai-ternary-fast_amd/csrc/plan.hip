@@ -24,36 +24,8 @@ namespace {
 constexpr int kPlanThreads = 1024;
 constexpr int kRowsPerWave = 1024;
 
-__device__ __forceinline__ long long wave_scan(long long v, int lane) {  // inclusive
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const long long u = __shfl_up(v, o, 64);
-    if (lane >= o) v += u;
-  }
-  return v;
-}
-
-// Inclusive prefix sum over the workgroup's threads; *total gets the whole sum.
-__device__ __forceinline__ long long block_scan(long long v, long long* part, long long* total) {
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  constexpr int nw = kPlanThreads / 64;
-  v = wave_scan(v, lane);
-  __syncthreads();  // (part may still be read from the scan before)
-  if (lane == 63) part[w] = v;
-  __syncthreads();
-  long long sums = lane < nw ? part[lane] : 0;
-#pragma unroll
-  for (int o = 1; o < nw; o <<= 1) {
-    const long long u = __shfl_up(sums, o, 64);
-    if (lane >= o) sums += u;
-  }
-  const long long before = w ? __shfl(sums, w - 1, 64) : 0;
-  *total = __shfl(sums, nw - 1, 64);
-  return v + before;
-}
-
 __device__ void plan_requests(const btf_page_plan& a) {
-  __shared__ long long part[kPlanThreads / 64];
+  __shared__ uint64_t part[kPlanThreads / 64];
   __shared__ long long got[kPlanThreads];  // pages handed out up to and including each request of the chunk
   __shared__ int first[kPlanThreads];      // its pages before the step
   const long long free0 = max(*a.n_free, 0);
@@ -63,21 +35,22 @@ __device__ void plan_requests(const btf_page_plan& a) {
     const bool live = s < a.S;
     const long long c = live ? a.ctx[s] : 0, nn = live ? a.n_new[s] : 0, h = live ? a.held[s] : 0;
     const long long n = max(nn, 0ll);
-    long long all;
-    const long long end = rows + block_scan(n, part, &all);
+    uint64_t all;
+    const long long end = rows + (long long)block_scan<kPlanThreads>(n, part, &all);
     if (live) a.row0[s] = (int)min(end - n, (long long)a.T);
     rows += all;
     const long long total = (c + nn + a.page - 1) / a.page;
     const bool sound = live && c >= 0 && nn >= 0 && h >= 0 && h <= a.ldt && c <= h * a.page && end <= a.T &&
                        total <= a.ldt && c + nn <= 0x7fffffffll;
     const long long want = sound ? max(total - h, 0ll) : 0;
-    const long long upto = pages + block_scan(want, part, &all);
+    const long long upto = pages + (long long)block_scan<kPlanThreads>(want, part, &all);
     pages += all;
     const bool served = sound && (want == 0 || upto <= free0);
     // the served needs are the first ones: their sums are those of all needs
     const long long need = served ? want : 0;
-    long long chunk;
-    got[threadIdx.x] = block_scan(need, part, &chunk);
+    uint64_t chunk_u;
+    got[threadIdx.x] = (long long)block_scan<kPlanThreads>(need, part, &chunk_u);
+    const long long chunk = (long long)chunk_u;
     first[threadIdx.x] = (int)h;
     if (live) {
       a.kv_len[s] = served ? (int)(c + nn) : 0;

@@ -7,17 +7,20 @@
 // (units of 2^-43, in 64 bits), so no sum depends on its order.
 //
 // Four launches over the row, cut into parts of 4096 to 16384 logits:
-//  * top: the parts' largest key and smallest logit;
-//  * hist (rows with top-k or top-p): counts and weights by 1024 bins of the
-//    distance to the maximum, in LDS, then added to the row's;
-//  * border: from the bins, those in which a border can lie. top-k's is the bin
-//    in which the count passes k; top-p's lies between the bins in which the sum
-//    passes p times the least and the most that the top-k may weigh. Below them
-//    everything stays: its weights are summed part by part. What lies in them is
-//    written out, logit and index, as candidates;
+//  * top: the parts' largest key and smallest logit; with top-k also the largest key
+//    of every 128 logits;
+//  * hist (rows with top-k or top-p): weights (top-p) and counts (top-k) by 1024 bins
+//    of the distance to the maximum, in LDS, then added to the row's. With top-k only
+//    the bins down to the one in which the k-th largest of the 128-logit maxima lies:
+//    k logits are at least as large;
+//  * border: from the bins, those in which a border can lie. top-k's is the bin in
+//    which the count passes k; top-p's lies between the bins in which the sum passes p
+//    times the least and the most that the top-k may weigh. Below them everything
+//    stays: its weights are summed for every 256 logits. What lies in them is written
+//    out, logit and index, as candidates;
 //  * pick: one workgroup per row sorts the candidates (a bin of a row of 248320
 //    normal logits holds 1500 of them at most), finds the borders exactly, adds
-//    what stays to its parts, and walks the one part in which the sum passes u.
+//    what stays to its 256 logits, and walks those in which the sum passes u.
 // A row whose border bins hold more than kCand logits (many equal ones) is done by
 // that workgroup alone, eight key bits at a time.
 #include <cmath>
@@ -30,13 +33,17 @@
 namespace btfhip {
 namespace {
 
-typedef unsigned long long u64;
+typedef uint64_t u64;
 typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
 constexpr int kPartThreads = 256;
-constexpr int kPickThreads = 1024;
+constexpr int kPickThreads = 512;
 constexpr int kBins = 1024;
 constexpr int kCand = 4096;
+constexpr int kFine = 512;                        // pieces of a border bin
 constexpr int kMinPart = 4096, kMaxPart = 16384;  // logits of a part
+constexpr int kRound = 4 * kPartThreads;          // logits of a part's round, four a thread
+constexpr int kSum = 256, kTop = 128;             // logits of a partial sum (a wave's of a round), of a maximum (half of it)
+constexpr int kMaxV = 1 << 20;
 constexpr double kOne = 8796093022208.0;          // 2^43: the weight of the largest
 constexpr double kFar = 31.0;                     // exp(-31) is below half a unit
 
@@ -44,27 +51,24 @@ __device__ __forceinline__ uint32_t key_of(float x) { return (uint32_t)(argmax_k
 __device__ __forceinline__ float of_key(uint32_t k) { return __uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k); }
 
 // exp(-d) in units of 2^-43, for 0 <= d < kFar: with n the nearest whole number to
-// -d / ln 2 and r = -d - n ln 2 (ln 2 in two parts), the series of exp(r) up to r^12
-// (|r| <= 0.347: 2e-16 off), scaled by its exponent; rounded to a whole number by
-// adding 2^52.
+// -d / ln 2 and r = -d - n ln 2 (ln 2 in two parts), the polynomial of degree 9 that
+// agrees with exp at the Chebyshev points of |r| <= ln 2 / 2 (2e-14 off, a third of
+// the unit's half), scaled by its exponent; rounded to a whole number by adding 2^52.
 __device__ __forceinline__ u64 weight_at(double d) {
   const double n = rint(d * -1.4426950408889634);
   const double r = fma(n, -2.3190468138462996e-17, fma(n, -0.6931471805599453, -d));
-  double p = 1.0 / 479001600;
-  p = fma(p, r, 1.0 / 39916800);
-  p = fma(p, r, 1.0 / 3628800);
-  p = fma(p, r, 1.0 / 362880);
-  p = fma(p, r, 1.0 / 40320);
-  p = fma(p, r, 1.0 / 5040);
-  p = fma(p, r, 1.0 / 720);
-  p = fma(p, r, 1.0 / 120);
-  p = fma(p, r, 1.0 / 24);
-  p = fma(p, r, 1.0 / 6);
-  p = fma(p, r, 0.5);
-  p = fma(p, r, 1.0);
-  p = fma(p, r, 1.0);
+  double p = 2.7632640690513381e-06;
+  p = fma(p, r, 2.4884459768350122e-05);
+  p = fma(p, r, 0.00019841190647512536);
+  p = fma(p, r, 0.0013888801749621653);
+  p = fma(p, r, 0.0083333333673116239);
+  p = fma(p, r, 0.041666667040552129);
+  p = fma(p, r, 0.16666666666615648);
+  p = fma(p, r, 0.49999999999438588);
+  p = fma(p, r, 1.0000000000000013);
+  p = fma(p, r, 1.0000000000000135);
   const double v = ldexp(p, (int)n + 43) + 4503599627370496.0;
-  return (u64)(__double_as_longlong(v) & 0xfffffffffffffll);
+  return (u64)__double_as_longlong(v) & 0xfffffffffffffull;
 }
 
 // Distance of a logit to the row's largest in units of the temperature; kFar or more (or NaN): no weight.
@@ -77,33 +81,52 @@ __device__ __forceinline__ u64 weight(float x, float top, double inv_t) {
 }
 
 // ---- what the launches share: scratch, the row's settings ----
-struct Scratch {
-  u64 sum[kBins];
-  uint32_t cnt[kBins];
-  uint32_t cand[kCand][2];  // logit's bits, index
-  u64 pmax[256];            // (2^20 / kMinPart parts at most)
-  u64 psum[256];
-  float pmin[256];
-  uint32_t ncand;
-  uint32_t pad;
-};
-
 struct Row {
   bool greedy;
   float top;
-  double inv_t, scale, floor_w;  // scale: bins for a unit of distance
+  double inv_t, scale;           // scale: bins for a unit of distance
+  u64 floor_w;                   // the least weight that min-p keeps
   int k;                         // 0: no top-k
   float p;                       // 1: no top-p
 };
 
+// Where the borders lie, by bins: [0, lo) stays whole; candidates are in [lo, hi] and kb.
+struct Borders {
+  int lo, hi, kb;         // kBins: none
+  uint32_t k_left;        // top-k: how many of bin kb stay
+  u64 below_lo, below_kb; // weights of the bins before lo, before kb
+};
+
+struct Scratch {
+  u64 sum[kBins];
+  uint32_t cnt[kBins];
+  uint32_t cand[kCand][2];  // logit's bits, index
+  u64 pmax[kMaxV / kMinPart];
+  float pmin[kMaxV / kMinPart];
+  uint32_t ncand;
+  uint32_t done;            // workgroups of the row that have added their bins
+  Row row;
+  u64 best;                 // the row's largest key
+  Borders borders;
+  // then u64 psum[V / kSum], uint32_t tops[V / kTop] (rounded up)
+  __device__ u64* psum() { return reinterpret_cast<u64*>(this + 1); }
+  __device__ uint32_t* tops(int V) { return reinterpret_cast<uint32_t*>(psum() + (V + kSum - 1) / kSum); }
+};
+__host__ __device__ inline int64_t scratch_bytes(int V) {
+  return (int64_t)sizeof(Scratch) + 8 * (int64_t)((V + kSum - 1) / kSum) + 8 * (int64_t)((V + 2 * kTop - 1) / (2 * kTop));
+}
+__device__ __forceinline__ Scratch& scratch_of(const btf_sampling& a, int m) {
+  return *reinterpret_cast<Scratch*>(static_cast<char*>(a.ws) + (size_t)m * scratch_bytes(a.V));
+}
+
 struct Parts {
-  int n, size;  // size a multiple of 4
+  int n, size;  // size a multiple of kRound
 };
 __host__ __device__ inline Parts parts_of(int M, int V) {
   // about 1024 workgroups over the rows
   int want = (1024 + M - 1) / M;
   int size = (V + want - 1) / want;
-  size = size < kMinPart ? kMinPart : size > kMaxPart ? kMaxPart : (size + 3) / 4 * 4;
+  size = size < kMinPart ? kMinPart : size > kMaxPart ? kMaxPart : (size + kRound - 1) / kRound * kRound;
   return {(V + size - 1) / size, size};
 }
 
@@ -128,7 +151,7 @@ __device__ Row settings(const btf_sampling& a, const Scratch& s, int m, int part
   const float p = a.top_p ? a.top_p[m] : 1.f;
   r.p = p < 1.f ? p : 1.f;
   const float mp = a.min_p ? a.min_p[m] : 0.f;
-  r.floor_w = mp > 0.f ? (double)fminf(mp, 1.f) * kOne : 0.0;
+  r.floor_w = mp > 0.f ? (u64)ceil((double)fminf(mp, 1.f) * kOne) : 1;
   *best = b;
   return r;
 }
@@ -138,42 +161,59 @@ __device__ __forceinline__ int bin_of(double d, const Row& r) {
   return b < kBins ? b : kBins - 1;
 }
 
-// fn(logit, index) over a part, four at a time.
+// A logit below which every bin is deeper than `bin`: what a row's bulk is skipped by, without the 64-bit distance.
+// (Less by more than the roundings of the distance and its bin.)
+__device__ __forceinline__ float cut_below(int bin, const Row& r) {
+  const double c = (double)r.top - (double)(bin + 1) / r.scale / r.inv_t * (1.0 + 1e-9);
+  return __double2float_rd(c - fabs(c) * 1e-12);  // (NaN, nothing skipped, where the maximum is infinite)
+}
+
+// fn(the thread's four logits, their indices, how many there are) for every round of a part, by all threads.
 template <class F>
 __device__ __forceinline__ void over_part(const float* x, int i0, int i1, F fn) {
-  for (int i = i0 + 4 * (int)threadIdx.x; i < i1; i += 4 * kPartThreads) {
-    if (i + 4 <= i1) {
-      const f32x4u v = *reinterpret_cast<const f32x4u*>(x + i);
+  constexpr int AHEAD = 4;  // rounds whose loads are on their way together
+  for (int r = i0; r < i1; r += AHEAD * kRound) {
+    f32x4u v[AHEAD] = {};
+    int n[AHEAD];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) fn(v[j], i + j);
-    } else {
-      for (int j = i; j < i1; ++j) fn(x[j], j);
+    for (int k = 0; k < AHEAD; ++k) {
+      const int i = r + k * kRound + 4 * (int)threadIdx.x;
+      n[k] = min(4, i1 - i);
+      if (n[k] == 4) v[k] = *reinterpret_cast<const f32x4u*>(x + i);
+      else
+        for (int j = 0; j < 3; ++j)
+          if (j < n[k]) v[k][j] = x[i + j];
     }
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k)
+      if (r + k * kRound < i1) fn(v[k], r + k * kRound + 4 * (int)threadIdx.x, n[k]);
   }
 }
 
-// Inclusive prefix sum over the N threads of the workgroup; *total: the whole sum.
-template <int N>
-__device__ u64 block_scan(u64 v, u64* part, u64* total) {
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  constexpr int nw = N / 64;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const u64 u = __shfl_up(v, o, 64);
-    if (lane >= o) v += u;
+// Sum over the wave, in every lane. (Halves by DPP within 16 lanes, then the row swaps.)
+__device__ __forceinline__ u64 wave_sum_u64(u64 v) {
+  auto add = [&](uint32_t lo, uint32_t hi) { v += (u64)hi << 32 | lo; };
+  add(dpp_i<0xB1>((int)v), dpp_i<0xB1>((int)(v >> 32)));
+  add(dpp_i<0x4E>((int)v), dpp_i<0x4E>((int)(v >> 32)));
+  add(dpp_i<0x141>((int)v), dpp_i<0x141>((int)(v >> 32)));
+  add(dpp_i<0x140>((int)v), dpp_i<0x140>((int)(v >> 32)));
+  {
+    const auto a = __builtin_amdgcn_permlane16_swap((uint32_t)v, (uint32_t)v, false, false);
+    const auto b = __builtin_amdgcn_permlane16_swap((uint32_t)(v >> 32), (uint32_t)(v >> 32), false, false);
+    v = ((u64)b[0] << 32 | a[0]) + ((u64)b[1] << 32 | a[1]);
   }
-  __syncthreads();
-  if (lane == 63) part[w] = v;
-  __syncthreads();
-  u64 sums = lane < nw ? part[lane] : 0;
-#pragma unroll
-  for (int o = 1; o < nw; o <<= 1) {
-    const u64 u = __shfl_up(sums, o, 64);
-    if (lane >= o) sums += u;
-  }
-  const u64 before = w ? __shfl(sums, w - 1, 64) : 0;
-  *total = __shfl(sums, nw - 1, 64);
-  return v + before;
+  const auto a = __builtin_amdgcn_permlane32_swap((uint32_t)v, (uint32_t)v, false, false);
+  const auto b = __builtin_amdgcn_permlane32_swap((uint32_t)(v >> 32), (uint32_t)(v >> 32), false, false);
+  return ((u64)b[0] << 32 | a[0]) + ((u64)b[1] << 32 | a[1]);
+}
+// Largest of each half of the wave, in its lanes.
+__device__ __forceinline__ uint32_t half_max(uint32_t v) {
+  v = max(v, (uint32_t)dpp_i<0xB1>((int)v));
+  v = max(v, (uint32_t)dpp_i<0x4E>((int)v));
+  v = max(v, (uint32_t)dpp_i<0x141>((int)v));
+  v = max(v, (uint32_t)dpp_i<0x140>((int)v));
+  const auto a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+  return max(a[0], a[1]);
 }
 
 // ---- launches 1 to 3 ----
@@ -181,14 +221,27 @@ __global__ void __launch_bounds__(kPartThreads) sample_top_kernel(btf_sampling a
   __shared__ u64 wk[kPartThreads / 64];
   __shared__ float wm[kPartThreads / 64];
   const int m = blockIdx.y, i0 = blockIdx.x * size, i1 = min(a.V, i0 + size);
-  Scratch& s = static_cast<Scratch*>(a.ws)[m];
+  Scratch& s = scratch_of(a, m);
   for (int i = blockIdx.x * kPartThreads + threadIdx.x; i < kBins; i += gridDim.x * kPartThreads) s.sum[i] = 0, s.cnt[i] = 0;
-  if (blockIdx.x == 0 && threadIdx.x == 0) s.ncand = 0;
+  if (blockIdx.x == 0 && threadIdx.x == 0) s.ncand = 0, s.done = 0;
+  const bool tops = a.top_k && a.top_k[m] > 0;
+  uint32_t* top = s.tops(a.V);
   u64 best = 0;
   float lo = INFINITY;
-  over_part(a.logits + (size_t)m * a.ldl, i0, i1, [&](float x, int i) {
-    best = key_max(best, argmax_key(x, i));
-    if (x > -INFINITY) lo = fminf(lo, x);
+  over_part(a.logits + (size_t)m * a.ldl, i0, i1, [&](f32x4u x, int i, int n) {
+    uint32_t most = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (j < n) {
+        const u64 k = argmax_key(x[j], i + j);
+        best = key_max(best, k);
+        most = max(most, (uint32_t)(k >> 32));
+        if (x[j] > -INFINITY) lo = fminf(lo, x[j]);
+      }
+    if (tops) {
+      most = half_max(most);
+      if ((threadIdx.x & 31) == 0 && n > 0) top[i / kTop] = most;
+    }
   });
   best = wave_max_key(best);
 #pragma unroll
@@ -202,54 +255,25 @@ __global__ void __launch_bounds__(kPartThreads) sample_top_kernel(btf_sampling a
   }
 }
 
-__global__ void __launch_bounds__(kPartThreads) sample_hist_kernel(btf_sampling a, int size) {
-  __shared__ u64 sum[kBins];
-  __shared__ uint32_t cnt[kBins];
-  const int m = blockIdx.y, i0 = blockIdx.x * size, i1 = min(a.V, i0 + size);
-  Scratch& s = static_cast<Scratch*>(a.ws)[m];
-  u64 best;
-  const Row r = settings(a, s, m, gridDim.x, &best);
-  if (r.greedy || (r.k == 0 && r.p == 1.f)) return;
-  for (int i = threadIdx.x; i < kBins; i += kPartThreads) sum[i] = 0, cnt[i] = 0;
-  __syncthreads();
-  over_part(a.logits + (size_t)m * a.ldl, i0, i1, [&](float x, int) {
-    const double d = distance(x, r.top, r.inv_t);
-    if (!(d < kFar)) return;
-    const u64 w = weight_at(d);
-    if (w == 0) return;
-    const int b = bin_of(d, r);
-    atomicAdd(&sum[b], w);
-    atomicAdd(&cnt[b], 1u);
-  });
-  __syncthreads();
-  for (int i = threadIdx.x; i < kBins; i += kPartThreads)
-    if (cnt[i]) {
-      atomicAdd(&s.sum[i], sum[i]);
-      atomicAdd(&s.cnt[i], cnt[i]);
-    }
-}
-
-// Where the borders lie, by bins: [0, lo) stays whole; candidates are in [lo, hi] and kb.
-struct Borders {
-  int lo, hi, kb;         // kBins: none
-  uint32_t k_left;        // top-k: how many of bin kb stay
-  u64 below_lo, below_kb; // weights of the bins before lo, before kb
-};
-
+// The borders of a row whose bins are complete, by the whole workgroup. (The bins come from other workgroups of this
+// launch: they are read past the caches that those may not share.)
 template <int N>
-__device__ Borders borders(const Scratch& s, const Row& r, u64* part, u64* sh) {
+__device__ Borders borders(Scratch& s, const Row& r, u64* part, u64* sh) {
   Borders b = {kBins, -1, kBins, 0, 0, 0};
   if (r.k == 0 && r.p == 1.f) return b;
   constexpr int PER = kBins / N > 0 ? kBins / N : 1;
   const int b0 = threadIdx.x * PER;
   u64 c[PER], w[PER], cs = 0, ws = 0, total;
 #pragma unroll
-  for (int i = 0; i < PER; ++i) cs += c[i] = s.cnt[b0 + i], ws += w[i] = s.sum[b0 + i];
+  for (int i = 0; i < PER; ++i) cs += c[i] = __hip_atomic_load(&s.cnt[b0 + i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT),
+                                    ws += w[i] = __hip_atomic_load(&s.sum[b0 + i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   u64 c0 = block_scan<N>(cs, part, &total) - cs;
   if (threadIdx.x < 8) sh[threadIdx.x] = threadIdx.x < 3 ? kBins : 0;
   u64 all;
   const u64 w0 = block_scan<N>(ws, part, &all) - ws;  // (waits: sh is set)
-  if (r.k && total > (u64)r.k) {  // at most k with a weight: top-k takes nothing away
+  // (Without top-k there are no counts, without top-p no weights; with top-k both stop at a bin that it does reach. Less
+  // than k in all: fewer than k have a weight, and top-k takes nothing away.)
+  if (r.k && total >= (u64)r.k) {
     u64 at = c0, wat = w0;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
@@ -283,38 +307,165 @@ __device__ Borders borders(const Scratch& s, const Row& r, u64* part, u64* sh) {
   return b;
 }
 
-__global__ void __launch_bounds__(kPartThreads) sample_border_kernel(btf_sampling a, int size) {
-  __shared__ u64 part[kPartThreads / 64], sh[8];
+__global__ void __launch_bounds__(kPartThreads) sample_hist_kernel(btf_sampling a, int size) {
+  __shared__ u64 sum[kBins];
+  __shared__ uint32_t cnt[kBins];
+  __shared__ u64 part[kPartThreads / 64];
+  __shared__ u64 sh[8];
+  __shared__ int deepest;
+  __shared__ bool last;
   const int m = blockIdx.y, i0 = blockIdx.x * size, i1 = min(a.V, i0 + size);
-  Scratch& s = static_cast<Scratch*>(a.ws)[m];
+  Scratch& s = scratch_of(a, m);
   u64 best;
   const Row r = settings(a, s, m, gridDim.x, &best);
-  if (r.greedy) return;
-  const Borders b = borders<kPartThreads>(s, r, part, sh);
-  u64 mine = 0;
-  over_part(a.logits + (size_t)m * a.ldl, i0, i1, [&](float x, int i) {
-    const double d = distance(x, r.top, r.inv_t);
-    if (!(d < kFar)) return;
-    const int bin = bin_of(d, r);
-    if (bin < b.lo) {
-      const u64 w = weight_at(d);
-      if ((double)w >= r.floor_w) mine += w;
-    } else if (bin <= b.hi || bin == b.kb) {
-      const uint32_t n = atomicAdd(&s.ncand, 1u);
-      if (n < kCand) s.cand[n][0] = __float_as_uint(x), s.cand[n][1] = (uint32_t)i;
+  if (r.greedy || (r.k == 0 && r.p == 1.f)) {
+    if (blockIdx.x == 0 && threadIdx.x == 0) s.row = r, s.best = best, s.borders = Borders{kBins, -1, kBins, 0, 0, 0};
+    return;
+  }
+  for (int i = threadIdx.x; i < kBins; i += kPartThreads) sum[i] = 0, cnt[i] = 0;
+  if (threadIdx.x == 0) deepest = kBins - 1;
+  __syncthreads();
+  const bool weigh = r.p < 1.f;
+  int deep = kBins - 1;
+  if (r.k) {  // the deepest bin that top-k reaches, by the maxima of 128
+    const uint32_t* top = s.tops(a.V);
+    const int nt = (a.V + kTop - 1) / kTop;
+    if (r.k < nt) {
+      for (int i = threadIdx.x; i < nt; i += kPartThreads) {
+        const double d = distance(of_key(top[i]), r.top, r.inv_t);
+        if (top[i] && d < kFar) atomicAdd(&cnt[bin_of(d, r)], 1u);
+      }
+      __syncthreads();
+      constexpr int PER = kBins / kPartThreads;
+      u64 c[PER], mine = 0, total;
+#pragma unroll
+      for (int i = 0; i < PER; ++i) mine += c[i] = cnt[threadIdx.x * PER + i];
+      u64 at = block_scan<kPartThreads>(mine, part, &total) - mine;
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        if (at < (u64)r.k && at + c[i] >= (u64)r.k) deepest = threadIdx.x * PER + i;
+        at += c[i];
+        cnt[threadIdx.x * PER + i] = 0;
+      }
+      __syncthreads();
+      deep = deepest;
+    }
+  }
+  const float cut = cut_below(deep, r);
+  over_part(a.logits + (size_t)m * a.ldl, i0, i1, [&](f32x4u x, int, int n) {
+    bool in[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) in[j] = j < n && !(x[j] < cut);
+    if (!__any(in[0] | in[1] | in[2] | in[3])) return;
+    u64 w[4];
+    int bin[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {  // (without branches, so that the four go through the arithmetic together)
+      const double d = distance(x[j], r.top, r.inv_t);
+      in[j] = in[j] & (d < kFar);
+      w[j] = weight_at(in[j] ? d : 0.0);
+      bin[j] = bin_of(in[j] ? d : 0.0, r);
+      in[j] = in[j] & (bin[j] <= deep) & (w[j] != 0);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (!in[j]) continue;
+      if (weigh) atomicAdd(reinterpret_cast<unsigned long long*>(&sum[bin[j]]), (unsigned long long)w[j]);
+      if (r.k) atomicAdd(&cnt[bin[j]], 1u);
     }
   });
-  u64 total;
-  block_scan<kPartThreads>(mine, part, &total);
-  if (threadIdx.x == 0) s.psum[blockIdx.x] = total;
+  __syncthreads();
+  for (int i = threadIdx.x; i < kBins; i += kPartThreads) {
+    if (sum[i]) atomicAdd(reinterpret_cast<unsigned long long*>(&s.sum[i]), (unsigned long long)sum[i]);
+    if (cnt[i]) atomicAdd(&s.cnt[i], cnt[i]);
+  }
+  // The row's last workgroup finds the borders for the launches that follow. What it reads of the others is the bins
+  // alone, and those only ever change by atomics, which are done in memory when the wait below ends: no cache has to be
+  // written back (with a fence in every workgroup this launch took 70 us instead of 20 on 48 rows of 248320).
+  asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
+  __syncthreads();
+  if (threadIdx.x == 0) last = __hip_atomic_fetch_add(&s.done, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == gridDim.x - 1;
+  __syncthreads();
+  if (!last) return;
+  const Borders b = borders<kPartThreads>(s, r, part, sh);
+  if (threadIdx.x == 0) s.row = r, s.best = best, s.borders = b;
+}
+
+__global__ void __launch_bounds__(kPartThreads) sample_border_kernel(btf_sampling a, int size) {
+  constexpr int kHere = 1024;  // candidates of a part collected in LDS
+  __shared__ uint32_t cand[kHere][2];
+  __shared__ uint32_t n_cand, at;
+  const int m = blockIdx.y, i0 = blockIdx.x * size, i1 = min(a.V, i0 + size);
+  Scratch& s = scratch_of(a, m);
+  u64 best;
+  Row r;
+  Borders b = {kBins, -1, kBins, 0, 0, 0};
+  if (a.top_k || a.top_p) {
+    r = s.row, b = s.borders;
+  } else {  // no launch before this one has found them
+    r = settings(a, s, m, gridDim.x, &best);
+    if (blockIdx.x == 0 && threadIdx.x == 0) s.row = r, s.best = best, s.borders = b;
+  }
+  if (r.greedy) return;
+  if (threadIdx.x == 0) n_cand = 0;
+  __syncthreads();
+  u64* psum = s.psum();
+  const float cut = cut_below(b.lo < kBins ? max(b.hi, b.kb < kBins ? b.kb : 0) : kBins - 1, r);
+  over_part(a.logits + (size_t)m * a.ldl, i0, i1, [&](f32x4u x, int i, int n) {
+    bool in[4], stays[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) in[j] = j < n && !(x[j] < cut);
+    u64 mine = 0;
+    if (__any(in[0] | in[1] | in[2] | in[3])) {
+      double d[4];
+      bool any = false;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        d[j] = distance(x[j], r.top, r.inv_t);
+        in[j] = in[j] & (d[j] < kFar);
+        d[j] = in[j] ? d[j] : 0.0;
+        const int bin = bin_of(d[j], r);
+        stays[j] = in[j] & (bin < b.lo);
+        in[j] = in[j] & (bin >= b.lo) & ((bin <= b.hi) | (bin == b.kb));
+        any |= stays[j];
+      }
+      if (__any(any))
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const u64 w = weight_at(d[j]);
+          mine += (stays[j] & (w >= r.floor_w)) ? w : 0;
+        }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (!in[j]) continue;
+        const uint32_t k = atomicAdd(&n_cand, 1u);
+        if (k < kHere) {
+          cand[k][0] = __float_as_uint(x[j]), cand[k][1] = (uint32_t)(i + j);
+        } else {  // (more than a part's share)
+          const uint32_t g = atomicAdd(&s.ncand, 1u);
+          if (g < kCand) s.cand[g][0] = __float_as_uint(x[j]), s.cand[g][1] = (uint32_t)(i + j);
+        }
+      }
+    }
+    if (__any(mine != 0)) mine = wave_sum_u64(mine);
+    if ((threadIdx.x & 63) == 0 && n > 0) psum[i / kSum] = mine;
+  });
+  __syncthreads();
+  const uint32_t here = min(n_cand, (uint32_t)kHere);
+  if (here == 0) return;
+  if (threadIdx.x == 0) at = atomicAdd(&s.ncand, here);
+  __syncthreads();
+  for (uint32_t k = threadIdx.x; k < here; k += kPartThreads)
+    if (at + k < kCand) s.cand[at + k][0] = cand[k][0], s.cand[at + k][1] = cand[k][1];
 }
 
 // ---- launch 4 ----
 struct Pick {
   union {
     struct {
-      u64 key[kCand];  // candidates, sorted
-      u64 sum[256];    // weights that stay, by parts
+      u64 key[kCand];           // candidates, sorted
+      u64 sum[kMaxV / kSum];    // weights that stay, of every kSum logits
+      u64 fine[kFine];          // counts or weights of a border bin's pieces
     } c;
     struct {
       u64 sum[256];
@@ -326,6 +477,7 @@ struct Pick {
   u64 part[kPickThreads / 64];
   u64 sh[8];
   u64 kth;
+  uint32_t n;
 };
 
 // The smallest key at which the count (by_count) or the weight of the logits from
@@ -344,7 +496,8 @@ __device__ bool find_key(const float* x, int V, const Row& r, bool by_count, dou
       const uint32_t k = key_of(x[i]);
       if (k <= floor || (shift < 24 && (k >> (shift + 8)) != prefix)) continue;
       if (by_count) atomicAdd(&sh.f.cnt[k >> shift & 255], 1u);
-      else atomicAdd(&sh.f.sum[k >> shift & 255], weight(x[i], r.top, r.inv_t));
+      else atomicAdd(reinterpret_cast<unsigned long long*>(&sh.f.sum[k >> shift & 255]),
+                     (unsigned long long)weight(x[i], r.top, r.inv_t));
     }
     __syncthreads();
     if (threadIdx.x == 0) {
@@ -372,13 +525,11 @@ __device__ bool find_key(const float* x, int V, const Row& r, bool by_count, dou
   return found;
 }
 
-// The index at which the sum of the kept weights in [i0, i1) passes `at`, by the whole workgroup; the kept are those
-// with keys > key and the first `ties` at it.
-__device__ void walk(const btf_sampling& a, const float* x, int m, int i0, int i1, const Row& r, uint32_t key, u64 ties,
-                     u64 at, bool relative, Pick& sh, u64 total) {
-  const int per = (i1 - i0 + kPickThreads - 1) / kPickThreads;
-  const int j0 = min(i1, i0 + (int)threadIdx.x * per), j1 = min(i1, j0 + per);
-  u64 eq = 0, n;
+// Draws from a row whose kept logits are those with keys > key and the first `ties` at it, a piece of it a thread.
+__device__ void walk(const btf_sampling& a, const float* x, int m, const Row& r, uint32_t key, u64 ties, Pick& sh) {
+  const int per = (a.V + kPickThreads - 1) / kPickThreads;
+  const int j0 = min(a.V, (int)threadIdx.x * per), j1 = min(a.V, j0 + per);
+  u64 eq = 0, n, total;
   for (int i = j0; i < j1; ++i) eq += key_of(x[i]) == key;
   const u64 eq0 = block_scan<kPickThreads>(eq, sh.part, &n) - eq;
   auto kept = [&](int i, u64& rank) -> u64 {
@@ -386,17 +537,14 @@ __device__ void walk(const btf_sampling& a, const float* x, int m, int i0, int i
     if (kk < key || kk == 0) return 0;
     if (kk == key && rank++ >= ties) return 0;
     const u64 w = weight(x[i], r.top, r.inv_t);
-    return (double)w >= r.floor_w ? w : 0;
+    return w >= r.floor_w ? w : 0;
   };
   u64 mine = 0, rank = eq0;
   for (int i = j0; i < j1; ++i) mine += kept(i, rank);
-  const u64 end = block_scan<kPickThreads>(mine, sh.part, &n);
-  if (!relative) {  // the whole row: its sum is the total
-    total = n;
-    const double u = a.u[m];
-    at = u > 0.0 ? (u64)fmin(u * (double)total, 9.0e18) : 0;
-    if (at >= total) at = total - 1;
-  }
+  const u64 end = block_scan<kPickThreads>(mine, sh.part, &total);
+  const double u = a.u[m];
+  u64 at = u > 0.0 ? (u64)fmin(u * (double)total, 9.0e18) : 0;
+  if (at >= total) at = total - 1;
   if (end > at && end - mine <= at) {
     u64 s = end - mine;
     rank = eq0;
@@ -435,48 +583,106 @@ __device__ void pick_alone(const btf_sampling& a, const float* x, int m, const R
       ties = (uint32_t)fmin((double)ties, fmax(more, 1.0));
     }
   }
-  walk(a, x, m, 0, a.V, r, key, ties, 0, false, sh, 0);
+  walk(a, x, m, r, key, ties, sh);
 }
 
-__global__ void __launch_bounds__(kPickThreads) sample_pick_kernel(btf_sampling a, int parts, int size) {
+__global__ void __launch_bounds__(kPickThreads) sample_pick_kernel(btf_sampling a) {
   __shared__ Pick sh;
   const int m = blockIdx.x, tid = threadIdx.x;
   const float* x = a.logits + (size_t)m * a.ldl;
-  const Scratch& s = static_cast<const Scratch*>(a.ws)[m];
-  u64 best;
-  const Row r = settings(a, s, m, parts, &best);
+  Scratch& s = scratch_of(a, m);
+  const Row r = s.row;
   if (r.greedy) {
     if (tid == 0) {
-      a.token[m] = argmax_key_index(best);
+      a.token[m] = argmax_key_index(s.best);
       if (a.logprob) a.logprob[m] = 0.f;
     }
     return;
   }
-  const uint32_t n = s.ncand;
+  uint32_t n = s.ncand;
   if (n > kCand) {
     pick_alone(a, x, m, r, sh);
     return;
   }
-  const Borders b = borders<kPickThreads>(s, r, sh.part, sh.sh);
+  Borders b = s.borders;
+  const int nsum = (a.V + kSum - 1) / kSum;
+  const u64* psum = s.psum();
+  for (int i = tid; i < nsum; i += kPickThreads) sh.c.sum[i] = psum[i];
+  if (tid == 0) sh.kth = 0, sh.n = 0;
+  constexpr int PER = kCand / kPickThreads;
+  const bool by_k = b.kb < kBins;
+  if (n > 64 && b.lo == b.hi && (by_k ? b.lo == b.kb && r.p == 1.f : true)) {
+    // One border in one bin: the bin again in kFine pieces. What lies in the pieces before the border's stays, only what
+    // lies in that is sorted.
+    for (int i = tid; i < kFine; i += kPickThreads) sh.c.fine[i] = 0;
+    __syncthreads();
+    u64 key[PER], w[PER];
+    int f[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      f[i] = -1;
+      const uint32_t at = tid + i * kPickThreads;
+      if (at >= n) continue;
+      const float v = __uint_as_float(s.cand[at][0]);
+      key[i] = argmax_key(v, (int)s.cand[at][1]);
+      const double d = distance(of_key((uint32_t)(key[i] >> 32)), r.top, r.inv_t);
+      w[i] = weight_at(d);
+      f[i] = max(0, min(kFine - 1, (int)((d * r.scale - (double)b.lo) * kFine)));
+      atomicAdd(reinterpret_cast<unsigned long long*>(&sh.c.fine[f[i]]), by_k ? 1ull : (unsigned long long)w[i]);
+    }
+    __syncthreads();
+    constexpr int FPER = kFine / kPickThreads;
+    u64 c[FPER], mine = 0, total;
+#pragma unroll
+    for (int i = 0; i < FPER; ++i) mine += c[i] = sh.c.fine[tid * FPER + i];
+    u64 at = block_scan<kPickThreads>(mine, sh.part, &total) - mine;
+    const double want = by_k ? (double)b.k_left : (double)r.p * (double)b.below_kb;
+    const u64 from = by_k ? 0 : b.below_lo;  // (below_kb: all of the row)
+#pragma unroll
+    for (int i = 0; i < FPER; ++i) {
+      const double before = (double)(from + at), after = (double)(from + at + c[i]);
+      const bool first = from + at == 0 && c[i] > 0;
+      if ((first || before < want) && after >= want && c[i] > 0) sh.sh[0] = tid * FPER + i, sh.sh[1] = at;
+      at += c[i];
+    }
+    __syncthreads();
+    const int piece = (int)sh.sh[0];
+    if (by_k) b.k_left -= (uint32_t)sh.sh[1];
+    else b.below_lo += sh.sh[1];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      if (f[i] < 0) continue;
+      if (f[i] < piece && w[i] >= r.floor_w)
+        atomicAdd(reinterpret_cast<unsigned long long*>(&sh.c.sum[argmax_key_index(key[i]) / kSum]), (unsigned long long)w[i]);
+      if (f[i] == piece) sh.c.key[atomicAdd(&sh.n, 1u)] = key[i];
+    }
+    __syncthreads();
+    n = sh.n;
+  } else {
+    for (int i = tid; i < (int)n; i += kPickThreads) sh.c.key[i] = argmax_key(__uint_as_float(s.cand[i][0]), (int)s.cand[i][1]);
+  }
   // candidates in order, by a bitonic sort of the next power of two of them
   int size2 = 1;
   while (size2 < (int)n) size2 *= 2;
-  for (int i = tid; i < size2; i += kPickThreads)
-    sh.c.key[i] = i < (int)n ? argmax_key(__uint_as_float(s.cand[i][0]), (int)s.cand[i][1]) : 0;
-  if (tid < parts) sh.c.sum[tid] = s.psum[tid];
-  if (tid == 0) sh.kth = 0;
+  for (int i = n + tid; i < size2; i += kPickThreads) sh.c.key[i] = 0;
   __syncthreads();
+  // (a wave's pairs of a pass with j <= 64 lie in 128 keys that no other wave touches in such a pass: its LDS accesses
+  // are in order, so only passes over longer distances need the workgroup to wait)
+  bool far = false;
   for (int k = 2; k <= size2; k *= 2)
     for (int j = k / 2; j > 0; j /= 2) {
+      if (far || j > 64) __syncthreads();
+      far = j > 64;
       for (int i = tid; i < size2 / 2; i += kPickThreads) {
         const int lo = 2 * i - (i & (j - 1)), hi = lo + j;  // falling order in the end
         const u64 x0 = sh.c.key[lo], x1 = sh.c.key[hi];
         if ((x0 < x1) == ((lo & k) == 0)) sh.c.key[lo] = x1, sh.c.key[hi] = x0;
       }
-      __syncthreads();
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
     }
-  // prefix sums of their weights, four consecutive ones a thread
-  constexpr int PER = kCand / kPickThreads;
+  __syncthreads();
+  // prefix sums of their weights, consecutive ones a thread
   u64 w[PER], ws = 0, w_all;
   int bin[PER];
 #pragma unroll
@@ -527,46 +733,63 @@ __global__ void __launch_bounds__(kPickThreads) sample_pick_kernel(btf_sampling 
     const uint32_t at = tid * PER + i;
     if (at >= n_stay) break;
     const int idx = argmax_key_index(sh.c.key[at]);
-    if ((double)w[i] >= r.floor_w) atomicAdd(&sh.c.sum[idx / size], w[i]);
+    if (w[i] >= r.floor_w) atomicAdd(reinterpret_cast<unsigned long long*>(&sh.c.sum[idx / kSum]), (unsigned long long)w[i]);
     if (at == n_stay - 1) sh.kth = sh.c.key[at];
   }
   __syncthreads();
-  // the part in which the sum passes u times the total
-  const u64 ps = tid < parts ? sh.c.sum[tid] : 0;
-  u64 total;
-  const u64 end = block_scan<kPickThreads>(ps, sh.part, &total);
+  // the kSum logits in which the sum passes u times the total
+  constexpr int SPER = kMaxV / kSum / kPickThreads;
+  const int per = (nsum + kPickThreads - 1) / kPickThreads;  // at most SPER
+  u64 ps = 0, total;
+#pragma unroll
+  for (int i = 0; i < SPER; ++i)
+    if (i < per && tid * per + i < nsum) ps += sh.c.sum[tid * per + i];
+  u64 end = block_scan<kPickThreads>(ps, sh.part, &total);
   const double u = a.u[m];
   u64 at = u > 0.0 ? (u64)fmin(u * (double)total, 9.0e18) : 0;
   if (at >= total) at = total - 1;
-  if (end > at && end - ps <= at) sh.sh[0] = tid, sh.sh[1] = at - (end - ps);
+  if (end > at && end - ps <= at) {
+    u64 before = end - ps;
+    for (int i = tid * per; i < nsum; ++i) {
+      if (before + sh.c.sum[i] > at) {
+        sh.sh[0] = i, sh.sh[1] = at - before;
+        break;
+      }
+      before += sh.c.sum[i];
+    }
+  }
   __syncthreads();
-  const int part = (int)sh.sh[0];
+  if (tid >= 64) return;
+  // one wave walks them, four a lane
+  const int i0 = (int)sh.sh[0] * kSum + 4 * tid;
   at = sh.sh[1];
   const u64 kth = sh.kth;  // the last that stays; 0: all of the bins before lo, and nothing else
-  // walk the part: 16 logits a thread at most
-  const int i0 = part * size, i1 = min(a.V, i0 + size);
-  const int per = (i1 - i0 + kPickThreads - 1) / kPickThreads;
-  const int j0 = min(i1, i0 + tid * per), j1 = min(i1, j0 + per);
-  auto kept = [&](int i) -> u64 {
-    const float v = x[i];
+  u64 wt[4], mine = 0;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    wt[j] = 0;
+    if (i0 + j >= a.V) continue;
+    const float v = x[i0 + j];
     const double d = distance(v, r.top, r.inv_t);
-    if (!(d < kFar)) return 0;
-    if (bin_of(d, r) >= b.lo && !(kth && argmax_key(v, i) >= kth)) return 0;
-    const u64 wt = weight_at(d);
-    return (double)wt >= r.floor_w ? wt : 0;
-  };
-  u64 mine = 0, all;
-  for (int i = j0; i < j1; ++i) mine += kept(i);
-  const u64 upto = block_scan<kPickThreads>(mine, sh.part, &all);
+    if (!(d < kFar)) continue;
+    if (bin_of(d, r) >= b.lo && !(kth && argmax_key(v, i0 + j) >= kth)) continue;
+    const u64 y = weight_at(d);
+    if (y >= r.floor_w) wt[j] = y, mine += y;
+  }
+  u64 upto = mine;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const u64 y = __shfl_up(upto, o, 64);
+    if (tid >= o) upto += y;
+  }
   if (upto > at && upto - mine <= at) {
     u64 sum = upto - mine;
-    for (int i = j0; i < j1; ++i) {
-      const u64 wt = kept(i);
-      sum += wt;
-      if (sum > at) {
-        a.token[m] = i;
-        if (a.logprob) a.logprob[m] = (float)log((double)wt / (double)total);
-        break;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      sum += wt[j];
+      if (sum > at && sum - wt[j] <= at) {
+        a.token[m] = i0 + j;
+        if (a.logprob) a.logprob[m] = (float)log((double)wt[j] / (double)total);
       }
     }
   }
@@ -574,7 +797,7 @@ __global__ void __launch_bounds__(kPickThreads) sample_pick_kernel(btf_sampling 
 
 }  // namespace
 
-int64_t sample_ws_bytes(int M, int V) { return (int64_t)M * (int64_t)sizeof(Scratch); }
+int64_t sample_ws_bytes(int M, int V) { return (int64_t)M * scratch_bytes(V); }
 
 int sample(const btf_sampling& a, hipStream_t st, const DevState& ds) {
   const Parts p = parts_of(a.M, a.V);
@@ -589,7 +812,7 @@ int sample(const btf_sampling& a, hipStream_t st, const DevState& ds) {
     b.u += m0;
     b.token += m0;
     if (a.logprob) b.logprob += m0;
-    b.ws = static_cast<Scratch*>(a.ws) + m0;
+    b.ws = static_cast<char*>(a.ws) + (size_t)m0 * scratch_bytes(a.V);
     const dim3 grid(p.n, M), blk(kPartThreads);
     hipLaunchKernelGGL(sample_top_kernel, grid, blk, 0, st, b, p.size);
     int rc = launch_status("sample_top_kernel");
@@ -600,7 +823,7 @@ int sample(const btf_sampling& a, hipStream_t st, const DevState& ds) {
     }
     hipLaunchKernelGGL(sample_border_kernel, grid, blk, 0, st, b, p.size);
     if ((rc = launch_status("sample_border_kernel")) != BTF_OK) return rc;
-    hipLaunchKernelGGL(sample_pick_kernel, dim3(M), dim3(kPickThreads), 0, st, b, p.n, p.size);
+    hipLaunchKernelGGL(sample_pick_kernel, dim3(M), dim3(kPickThreads), 0, st, b);
     if ((rc = launch_status("sample_pick_kernel")) != BTF_OK) return rc;
   }
   return BTF_OK;
