@@ -13,6 +13,7 @@
 // (position 10^6 turns 1.6e5 times; in 32 bits the angle would be off by
 // 2^-24 of that, 0.06 rad). A lane keeps its cosines and sines for all the heads
 // that its wave does.
+#include <algorithm>
 #include <cmath>
 #include <string>
 
@@ -142,7 +143,9 @@ template <int D, bool BF>
 void rope_go(const btf_rope_cache& a, const btf_kv_cache& kv, bool vec, hipStream_t st) {
   const int nh = (a.q ? a.heads : 0) + (a.k ? 2 * kv.heads : 0);
   const int slots = (nh + 64 / (D / 4) - 1) / (64 / (D / 4));  // a wave's passes over the heads, all of them
-  const int per = 1;
+  // Passes of a wave: one, but for rows that leave 8192 waves with more, up to 8: a wave works its angles out once
+  // (2048 rows of 56 heads of 128: 25.8 us with one pass, 19.7 with two, 18.0 with seven).
+  const int per = (int)std::min<int64_t>(8, std::max<int64_t>(1, (int64_t)a.T * slots / 8192));
   const dim3 grid(a.T, (slots + kRopeWaves * per - 1) / (kRopeWaves * per));
   if (vec) hipLaunchKernelGGL((rope_cache_kernel<D, BF, true>), grid, dim3(64 * kRopeWaves), 0, st, a, kv, per);
   else hipLaunchKernelGGL((rope_cache_kernel<D, BF, false>), grid, dim3(64 * kRopeWaves), 0, st, a, kv, per);
