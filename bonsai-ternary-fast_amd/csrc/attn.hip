@@ -111,15 +111,16 @@ struct Req {
   int C;                  // keys of a piece
 };
 
-__device__ __forceinline__ int wave_sum_i(int v) {
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) v += __shfl_xor(v, o, 64);
-  return v;
-}
-__device__ __forceinline__ float wave_sum_f(float v) {
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) v += __shfl_xor(v, o, 64);
-  return v;
+__device__ __forceinline__ float wave_sum_f(float v) { return groups_sum(row16_sum(v)); }
+// Inclusive sum over the lanes (within 16-lane rows by shifts, then the rows before).
+__device__ __forceinline__ int wave_scan_i(int v) {
+  v += dpp_i<0x111>(v);
+  v += dpp_i<0x112>(v);
+  v += dpp_i<0x114>(v);
+  v += dpp_i<0x118>(v);
+  const int t0 = __builtin_amdgcn_readlane(v, 15), t1 = __builtin_amdgcn_readlane(v, 31), t2 = __builtin_amdgcn_readlane(v, 47);
+  const int row = (threadIdx.x & 63) >> 4;
+  return v + (row > 0 ? t0 : 0) + (row > 1 ? t1 : 0) + (row > 2 ? t2 : 0);
 }
 
 // The request of item `id` (BY_ROW: of row `id`), found by every wave for itself:
@@ -151,12 +152,7 @@ __device__ bool find(const btf_paged_attention& a, const btf_kv_cache& kv, int i
     read(s0 + lane, r0, n, len, full);
     const int tiles = n > 0 ? (n * G + R - 1) / R : 0, pieces = max(1, (len + C - 1) / C);
     const int mine = kv.heads * tiles * pieces, cut = pieces > 1 ? mine : 0;
-    int upto = mine, cuts = cut;  // inclusive sums
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int u = __shfl_up(upto, o, 64), w = __shfl_up(cuts, o, 64);
-      if (lane >= o) upto += u, cuts += w;
-    }
+    const int upto = wave_scan_i(mine), cuts = wave_scan_i(cut);
     const bool here = BY_ROW ? n > 0 && id >= r0 && id < r0 + n : mine > 0 && id >= items + upto - mine && id < items + upto;
     const unsigned long long who = __ballot(here);
     if (who) {
@@ -779,8 +775,20 @@ __global__ void __launch_bounds__(64 * kJoinWaves) attn_join_kernel(btf_paged_at
   const int row = q.local * G + h % G, tile = row / R, r = row % R;
   const float* slot = static_cast<const float*>(a.ws) + (size_t)(q.slot + (q.tiles - 1 - tile) * kv.heads + kvh) * kSlot<D, R>;
   const size_t step = (size_t)q.tiles * kv.heads * kSlot<D, R>;
-  float top = -INFINITY, sum = 0.f;
-  for (int i = lane; i < q.pieces; i += 64) top = fmaxf(top, slot[i * step + R * D + r]);
+  // the first pieces' maxima, sums and values are all on their way before the first is needed
+  constexpr int AT = ONE ? 4 : 8;
+  float top = -INFINITY, sum = 0.f, l0 = 0.f;
+  if (lane < q.pieces) top = slot[lane * step + R * D + r], l0 = slot[lane * step + R * D + R + r];
+  vE x[AT];
+  auto read = [&](int i0, int i, int n) {
+#pragma unroll
+    for (int u = 0; u < AT; ++u)
+      x[u] = *reinterpret_cast<const vE*>(slot + (i0 + min(i + u * BY, n - 1)) * step + (size_t)r * D + lane * E);
+  };
+  const int first = ONE ? 0 : w;
+  read(0, first, min(64, q.pieces));
+  const float m0 = top;
+  for (int i = 64 + lane; i < q.pieces; i += 64) top = fmaxf(top, slot[i * step + R * D + r]);
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
   const float base = top == -INFINITY ? 0.f : top;
@@ -788,19 +796,20 @@ __global__ void __launch_bounds__(64 * kJoinWaves) attn_join_kernel(btf_paged_at
   for (int i0 = 0; i0 < q.pieces; i0 += 64) {
     float c = 0.f;
     if (i0 + lane < q.pieces) {
-      const float* x = slot + (i0 + lane) * step + R * D + r;
-      c = fast_exp2(x[0] - base);
-      sum += c * x[R];
+      const float* y = slot + (i0 + lane) * step + R * D + r;
+      c = fast_exp2((i0 ? y[0] : m0) - base);
+      sum += c * (i0 ? y[R] : l0);
     }
     const int n = min(64, q.pieces - i0);
-    for (int i = ONE ? 0 : w; i < n; i += 4 * BY)
+    for (int i = first; i < n; i += AT * BY) {
+      if (i0 + i != first) read(i0, i, n);
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
+      for (int u = 0; u < AT; ++u) {
         const int j = min(i + u * BY, n - 1);
-        const float f = __shfl(c, j, 64);
-        const vE x = *reinterpret_cast<const vE*>(slot + (i0 + j) * step + (size_t)r * D + lane * E);
-        if (i + u * BY < n) v += f * x;
+        const float f = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(c), j));
+        if (i + u * BY < n) v += f * x[u];
       }
+    }
   }
   sum = wave_sum_f(sum);
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
