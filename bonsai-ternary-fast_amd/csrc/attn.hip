@@ -249,12 +249,13 @@ __device__ __forceinline__ void softmax_block(const f32x4 (&s)[2], float c2, flo
 }
 
 // Scores of keys key0 .. key0 + 7 that the row (new token tok, -1: none) does not see become -infinity; there are keys
-// up to end. A tree's row sees its bits of the new tokens, another's those up to its own. (By selects: every score is
-// read before it is written, so no write can come before the product's own.)
+// up to end. A tree's row sees its bits of the new tokens, another's those up to its own. (All by selects: the lanes
+// differ in everything here, and a branch for each of 16 scores costs more than the arithmetic.)
 __device__ __forceinline__ void mask_block(f32x4 (&s)[2], int key0, int end, int ctx, bool tree, int tok,
                                            unsigned long long bits) {
   const int upto = tree ? ctx - 1 : ctx + tok, nj = key0 - ctx;
-  const uint32_t own = !tree || nj >= 64 || nj <= -8 ? 0 : nj >= 0 ? (uint32_t)(bits >> nj) : (uint32_t)(bits << -nj);
+  const uint32_t later = (uint32_t)(bits >> (nj & 63)), sooner = (uint32_t)(bits << (-nj & 63));
+  const uint32_t own = (tree & (nj > -8) & (nj < 64)) ? (nj >= 0 ? later : sooner) : 0u;
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
     const bool see = (key0 + j < end) & ((key0 + j <= upto) | ((own >> j & 1) != 0));
@@ -693,6 +694,9 @@ __global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_e
       }
     };
     read_v(0);
+    // (these products before another wave's softmax, which then runs in their shadow: trees of 8 requests 186 -> 177 us;
+    // with one row tile a wave, heads of 256, it costs: a prompt 481 -> 500)
+    if (RT == 2) __builtin_amdgcn_s_setprio(1);
 #pragma unroll
     for (int d0 = 0; d0 < DT; d0 += DB) {
       if (d0 + DB < DT) read_v(d0 + DB);
@@ -704,6 +708,7 @@ __global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_e
 #pragma unroll
           for (int rt = 0; rt < RT; ++rt) o[rt][d0 + d] = mfma<BF>(vf[d0 / DB & 1][d], p[rt][n], o[rt][d0 + d]);
     }
+    if (RT == 2) __builtin_amdgcn_s_setprio(0);
   };
   int buf = 0;
   for (int kb = k0; kb < k1; kb += kKeys, buf ^= 1) {

@@ -114,6 +114,8 @@ int btf_hip_launch_paged_attention(const btf_paged_attention* a, const btf_kv_ca
     return bad("paged_attention", "q must be 16-byte aligned with ldq % 8 == 0 and ldq >= heads * dim");
   if (!aligned(a->out, 16) || a->ldo % 4 || (int64_t)a->ldo < (int64_t)a->heads * kv->dim)
     return bad("paged_attention", "out must be 16-byte aligned with ldo % 4 == 0 and ldo >= heads * dim");
+  if (a->heads > 65535 || (int64_t)a->T * a->heads > 0x7fffffff)
+    return bad("paged_attention", "heads above 65535, or rows times heads above 2^31");
   if (a->ldt < 1) return bad("paged_attention", "ldt must be at least 1");
   if (!aligned(a->tree, 8)) return bad("paged_attention", "tree must be 8-byte aligned");
   if (!(a->scale == a->scale)) return bad("paged_attention", "scale is not a number");

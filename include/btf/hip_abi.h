@@ -537,8 +537,9 @@ int btf_hip_launch_rope_cache(const btf_rope_cache* a, const btf_kv_cache* kv, b
  * or nothing but scores of -infinity, gives zeros. What a row does not see has
  * no effect on it, infinities and NaN included. out is fp32, as launch_prep
  * takes it; products are of 16-bit values, everything else is in 32 bits.
- * ws: paged_attention_ws_bytes of device scratch, 16-byte aligned, one for
- * each stream that launches; 0 bytes needed: ws may be NULL. */
+ * ws: paged_attention_ws_bytes of device scratch for the launch's S, T and
+ * heads, 16-byte aligned, one for each stream that launches. It need not be
+ * cleared. The bytes for S = 1 and the largest T serve every launch. */
 typedef struct btf_paged_attention {
   int S, T, heads;       /* requests, rows, Q heads */
   const void* q;         /* [T][ldq], 16 bits of kv->type, 16-byte aligned, ldq % 8 == 0 */

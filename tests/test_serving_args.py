@@ -46,7 +46,7 @@ REFUSED = [
     ("rope", dict(q=A + 2)), ("rope", dict(turns=A + 4)),
     ("attn", dict(heads=0)), ("attn", dict(heads=18)), ("attn", dict(q=A + 8)), ("attn", dict(ldq=5124)),
     ("attn", dict(ldq=5112)), ("attn", dict(out=A + 4)), ("attn", dict(ldo=5122)), ("attn", dict(ldo=5116)),
-    ("attn", dict(ldt=0)), ("attn", dict(tree=A + 4)), ("attn", dict(scale=math.nan)),
+    ("attn", dict(T=1 << 28, heads=20)), ("attn", dict(ldt=0)), ("attn", dict(tree=A + 4)), ("attn", dict(scale=math.nan)),
     *[("attn", {n: None}) for n in ("q", "table", "row0", "kv_len", "out")],
     ("sample", dict(V=0)), ("sample", dict(V=(1 << 20) + 1, ldl=1 << 21)), ("sample", dict(ldl=999)),
     *[("sample", {n: None}) for n in ("logits", "u", "token")],
@@ -99,6 +99,16 @@ def test_missing_workspace():
     if h.sample_ws_bytes(2, 1000) > 0:
         assert launch("sample", dataclasses.replace(SAMPLE, ws=None)) == ARGS
         assert launch("sample", dataclasses.replace(SAMPLE, ws=A + 4)) == ARGS
+
+
+def test_workspace_for_the_largest_launch_serves_smaller_ones():
+    for dim in (64, 128, 256):
+        kv = dataclasses.replace(KV, dim=dim)
+        sizes = [h.paged_attention_ws_bytes(1, T, 20, kv) for T in (1, 3, 4, 5, 6, 7, 50, 512, 4096)]
+        assert sizes == sorted(sizes)
+        for S in (2, 16, 400):
+            assert all(h.paged_attention_ws_bytes(S, T, 20, kv) <= sizes[-1] for T in (1, 16, 400, 4096))
+    assert h.sample_ws_bytes(3, 1000) == 3 * h.sample_ws_bytes(1, 1000) < h.sample_ws_bytes(3, 200000)
 
 
 def test_workspace_of_nothing():
