@@ -227,7 +227,8 @@ ROPE_CASES = [(T, heads, n_rot, layout, kind, norm) for T, heads, n_rot, layout,
     (2, (20, 4, 256), 246, "half", "f16", True), (2, (20, 4, 256), 246, "pairs", "bf16", True),
     (5, (7, 7, 64), 2, "half", "f16", False), (5, (7, 7, 64), 54, "half", "bf16", True),
     (33, (3, 3, 128), 0, "half", "f16", True), (4, (2, 1, 256), 256, "pairs", "f16", False),
-    (70, (4, 2, 64), 32, "half", "bf16", False), (9, (9, 3, 128), 126, "half", "f16", False)]]
+    (70, (4, 2, 64), 32, "half", "bf16", False), (700, (20, 4, 256), 64, "half", "f16", True),
+    (1200, (17, 1, 128), 32, "pairs", "bf16", True), (9, (9, 3, 128), 126, "half", "f16", False)]]
 
 
 @pytest.mark.parametrize("T,heads,n_rot,layout,kind,norm", ROPE_CASES, ids=str)
@@ -508,6 +509,101 @@ def test_attention_strides(hip):
     check_attn(out, qw, k, v, table, row0, kv_len, None, heads, kind, page)
 
 
+def against_gpu64(out, q, k, v, table, row0, kv_len, heads, page):
+    """Causal attention of f16 values in 64 bits on the GPU; the tolerance is the worst case of the 32-bit sums."""
+    torch = _torch()
+    H, HK, D = heads
+    out = out[:, :H * D].double()
+    for s in range(len(kv_len)):
+        L, a, b = kv_len[s], int(row0[s]), int(row0[s + 1])
+        if b == a:
+            continue
+        ids = torch.from_numpy(table[s, :-(-L // page)]).cuda().long()
+        kk, vv = (c[ids].double().transpose(0, 1).reshape(HK, -1, D)[:, :L] for c in (k, v))
+        seen = torch.ones((b - a, L), dtype=torch.bool, device="cuda").tril(L - (b - a))
+        for h in range(H):
+            qq = q[a:b, h * D:(h + 1) * D].double()
+            p = torch.softmax((qq @ kk[h // (H // HK)].T * D ** -0.5).masked_fill(~seen, -math.inf), -1)
+            want, size = p @ vv[h // (H // HK)], p @ vv[h // (H // HK)].abs()
+            d = (out[a:b, h * D:(h + 1) * D] - want).abs()
+            assert bool((d <= ((L + 2 * D + 200) * 2.0 ** -24 + 2.0 ** -20) * size).all()), (s, h, float(d.max()))
+
+
+def gpu_cache(g, kv_len, heads, page):
+    torch = _torch()
+    H, HK, D = heads
+    held = [-(-n // page) for n in kv_len]
+    pages = sum(held) + 1
+    perm = torch.randperm(pages, generator=g, device="cuda").cpu().numpy()
+    table, at = np.full((len(kv_len), max(held)), -1), 0
+    for s, n in enumerate(held):
+        table[s, :n] = perm[at:at + n]
+        at += n
+    k, v = (torch.randn((pages, HK, page, D), generator=g, device="cuda").to(torch.float16) for _ in range(2))
+    return k, v, table
+
+
+@pytest.mark.parametrize("heads,page", [((20, 4, 256), 32), ((16, 2, 128), 16), ((8, 8, 64), 64)], ids=str)
+@pytest.mark.parametrize("new_hi", [1, 6, 40])
+def test_attention_many_requests(hip, heads, page, new_hi):
+    """More requests than a wave has lanes, lengths from 1 to 9000 in one batch, some without rows: cut and whole
+    requests side by side, found over several chunks."""
+    torch = _torch()
+    rng = np.random.default_rng(new_hi)
+    g = torch.Generator(device="cuda").manual_seed(new_hi)
+    S = 150
+    new = [int(n) for n in rng.integers(0 if new_hi > 1 else 1, new_hi + 1, S)]
+    kv_len = [n + int(c) for n, c in zip(new, np.exp(rng.uniform(0, 6, S)).astype(int))]
+    kv_len[7], kv_len[77], kv_len[149] = 9001, 5003, 3001
+    kv_len = [max(1, n) for n in kv_len]
+    k, v, table = gpu_cache(g, kv_len, heads, page)
+    q = torch.randn((sum(new), heads[0] * heads[2]), generator=g, device="cuda").to(torch.float16)
+    row0 = np.cumsum([0] + new)
+    out = run_attn(hip, q, k, v, table, row0, kv_len, None, heads, "f16", page)
+    against_gpu64(out, q, k, v, table, row0, kv_len, heads, page)
+
+
+@pytest.mark.parametrize("heads", [(128, 1, 64), (64, 1, 128), (48, 1, 256)], ids=str)
+def test_attention_many_heads_of_one_kv_head(hip, heads):
+    rng = np.random.default_rng(30)
+    kv_len, new = [200, 31], [1, 3]
+    x = attn_inputs(rng, kv_len, new, heads, "bf16", 16)
+    check_attn(run_attn(hip, *x, kv_len, None, heads, "bf16", 16), *x, kv_len, None, heads, "bf16", 16)
+
+
+def test_attention_shared_pages(hip):
+    """Requests with a common beginning hold the same pages."""
+    rng = np.random.default_rng(31)
+    heads, page, kv_len, new = (10, 2, 128), 16, [60, 60, 40], [1, 2, 1]
+    q, k, v, table, row0 = attn_inputs(rng, kv_len, new, heads, "f16", page)
+    table[1, :3], table[2, :2] = table[0, :3], table[0, :2]
+    x = (q, k, v, table, row0)
+    check_attn(run_attn(hip, *x, kv_len, None, heads, "f16", page), *x, kv_len, None, heads, "f16", page)
+
+
+@pytest.mark.parametrize("new", [1, 40])
+def test_attention_infinities_in_a_long_cache(hip, new):
+    """An infinity in V that the rows of one request see: infinities there (the formula's), nothing in the other's."""
+    torch = _torch()
+    g = torch.Generator(device="cuda").manual_seed(5)
+    heads, page, kv_len = (10, 2, 128), 64, [2500, 2400]
+    k, v, table = gpu_cache(g, kv_len, heads, page)
+    q = torch.randn((2 * new, 1280), generator=g, device="cuda").to(torch.float16)
+    row0 = np.array([0, new, 2 * new])
+    v[int(table[0][1500 // page]), 1, 1500 % page, 77] = math.inf
+    out = run_attn(hip, q, k, v, table, row0, kv_len, None, heads, "f16", page)
+    for h in range(5, 10):
+        assert bool((out[:new, h * 128 + 77] == math.inf).all())
+    out[:new, 640:][:, 77::128] = 0
+    clean = v.clone()
+    clean[int(table[0][1500 // page]), 1, 1500 % page, 77] = 0
+    want = run_attn(hip, q, k, clean, table, row0, kv_len, None, heads, "f16", page)
+    want[:new, 640:][:, 77::128] = 0
+    # request 0's KV head 1 goes through the plain loop: other orders of the same sums of 2500 terms
+    assert bool(((out - want).abs() <= 2 * 2900 * 2.0 ** -24 * 5).all())
+    assert torch.equal(out[new:], want[new:]) and torch.equal(out[:new, :640], want[:new, :640])
+
+
 @pytest.mark.parametrize("heads,S,new", [((20, 4, 256), 3, 1), ((10, 2, 128), 2, 33), ((4, 4, 64), 40, 1)], ids=str)
 def test_attention_long_caches(hip, heads, S, new):
     """Lengths that are split over many workgroups, one request much longer than the others; against 64 bits on the
@@ -515,30 +611,12 @@ def test_attention_long_caches(hip, heads, S, new):
     torch = _torch()
     H, HK, D = heads
     g = torch.Generator(device="cuda").manual_seed(S)
-    page, kind = 64, "f16"
     kv_len = [20011] + [97 + 301 * s for s in range(1, S)]
-    held = [-(-n // page) for n in kv_len]
-    pages = sum(held)
-    perm = torch.randperm(pages, generator=g, device="cuda").cpu().numpy()
-    table, at = np.full((S, max(held)), -1), 0
-    for s in range(S):
-        table[s, :held[s]] = perm[at:at + held[s]]
-        at += held[s]
-    k, v = (torch.randn((pages, HK, page, D), generator=g, device="cuda").to(torch.float16) for _ in range(2))
+    k, v, table = gpu_cache(g, kv_len, heads, 64)
     q = torch.randn((S * new, H * D), generator=g, device="cuda").to(torch.float16)
     row0 = np.arange(S + 1) * new
-    out = run_attn(hip, q, k, v, table, row0, kv_len, None, heads, kind, page)[:, :H * D].double()
-    for s in range(S):
-        L = kv_len[s]
-        ids = torch.from_numpy(table[s, :held[s]]).cuda()
-        kk, vv = (c[ids].double().transpose(0, 1).reshape(HK, -1, D)[:, :L] for c in (k, v))
-        seen = torch.ones((new, L), dtype=torch.bool, device="cuda").tril(L - new)
-        for h in range(H):
-            qq = q[s * new:(s + 1) * new, h * D:(h + 1) * D].double()
-            p = torch.softmax((qq @ kk[h // (H // HK)].T * D ** -0.5).masked_fill(~seen, -math.inf), -1)
-            want, size = p @ vv[h // (H // HK)], p @ vv[h // (H // HK)].abs()
-            d = (out[s * new:(s + 1) * new, h * D:(h + 1) * D] - want).abs()
-            assert bool((d <= ((L + 2 * D + 200) * 2.0 ** -24 + 2.0 ** -20) * size).all()), (s, h, float(d.max()))
+    out = run_attn(hip, q, k, v, table, row0, kv_len, None, heads, "f16", 64)
+    against_gpu64(out, q, k, v, table, row0, kv_len, heads, 64)
 
 
 # ---- sampling ----
@@ -647,6 +725,31 @@ def test_sample_far_apart_and_wide(hip):
                         np.concatenate([np.full((3, 2990), -40.0), rng.standard_normal((3, 10))], 1)])
     for args in (dict(), dict(k=20, p=0.9), dict(p=0.999), dict(T=100.0, p=0.7), dict(T=0.01, mp=0.1)):
         check_sample(hip, x, u=rng.random(9).astype(np.float32), **args)
+
+
+def test_sample_many_equal_logits_of_a_large_row(hip):
+    """More logits in a border's bin than candidates are held: the row is done by its own workgroup alone."""
+    rng = np.random.default_rng(14)
+    x = np.round(rng.standard_normal((5, 100003)))
+    check_sample(hip, x, k=[30000, 0, 30000, 1, 0], p=[1, 0.4, 0.4, 0.9, 1], mp=[0, 0, 0, 0, 0.01],
+                 u=rng.random(5).astype(np.float32))
+
+
+def test_sample_the_largest_vocabulary(hip):
+    rng = np.random.default_rng(15)
+    x = 2 * rng.standard_normal((3, 1 << 20))
+    check_sample(hip, x, k=[0, 900, 0], p=[0.7, 0.9, 1.0], u=[0.2, 0.5, 0.8])
+
+
+@pytest.mark.parametrize("k", [1, 2, 7, 8, 9, 500, 2000])
+def test_sample_sorted_and_clustered_logits(hip, k):
+    """The largest logits all next to each other: the maxima of 128 say little, top-k has to be exact all the same."""
+    rng = np.random.default_rng(16)
+    V = 30000
+    up = np.sort(2 * rng.standard_normal(V))
+    one = rng.standard_normal(V)
+    one[5000:5128] += 40
+    check_sample(hip, np.stack([up, up[::-1], one, one]), k=k, p=[1, 0.9, 1, 0.99], u=[0.1, 0.6, 0.9, 0.999])
 
 
 def test_sample_without_logprob_and_same_result_twice(hip):
