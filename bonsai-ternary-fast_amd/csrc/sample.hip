@@ -46,6 +46,7 @@ constexpr int kSum = 256, kTop = 128;             // logits of a partial sum (a 
 constexpr int kMaxV = 1 << 20;
 constexpr double kOne = 8796093022208.0;          // 2^43: the weight of the largest
 constexpr double kFar = 31.0;                     // exp(-31) is below half a unit
+constexpr double kMost = 1.8e19;                  // above 2^20 weights of one, and fits 64 bits
 
 __device__ __forceinline__ uint32_t key_of(float x) { return (uint32_t)(argmax_key(x, 0) >> 32); }
 __device__ __forceinline__ float of_key(uint32_t k) { return __uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k); }
@@ -544,7 +545,7 @@ __device__ void walk(const btf_sampling& a, const float* x, int m, const Row& r,
   for (int i = j0; i < j1; ++i) mine += kept(i, rank);
   const u64 end = block_scan<kPickThreads>(mine, sh.part, &total);
   const double u = a.u[m];
-  u64 at = u > 0.0 ? (u64)fmin(u * (double)total, 9.0e18) : 0;
+  u64 at = u > 0.0 ? (u64)fmin(u * (double)total, kMost) : 0;
   if (at >= total) at = total - 1;
   if (end > at && end - mine <= at) {
     u64 s = end - mine;
@@ -747,7 +748,7 @@ __global__ void __launch_bounds__(kPickThreads) sample_pick_kernel(btf_sampling 
     if (i < per && tid * per + i < nsum) ps += sh.c.sum[tid * per + i];
   u64 end = block_scan<kPickThreads>(ps, sh.part, &total);
   const double u = a.u[m];
-  u64 at = u > 0.0 ? (u64)fmin(u * (double)total, 9.0e18) : 0;
+  u64 at = u > 0.0 ? (u64)fmin(u * (double)total, kMost) : 0;
   if (at >= total) at = total - 1;
   if (end > at && end - ps <= at) {
     u64 before = end - ps;

@@ -741,6 +741,11 @@ def test_sample_the_largest_vocabulary(hip):
     check_sample(hip, x, k=[0, 900, 0], p=[0.7, 0.9, 1.0], u=[0.2, 0.5, 0.8])
 
 
+def test_sample_the_largest_sum(hip):
+    """2^20 weights of one: sums up to 2^63."""
+    check_sample(hip, np.zeros((4, 1 << 20)), p=[1, 1, 0.999, 0.999], u=[0.99, 1 - 2.0 ** -24, 0.99, 1 - 2.0 ** -24])
+
+
 @pytest.mark.parametrize("k", [1, 2, 7, 8, 9, 500, 2000])
 def test_sample_sorted_and_clustered_logits(hip, k):
     """The largest logits all next to each other: the maxima of 128 say little, top-k has to be exact all the same."""
