@@ -133,7 +133,7 @@ __device__ bool find(const btf_paged_attention& a, const btf_kv_cache& kv, int i
   auto read = [&](int s, int& r0, int& n, int& len, int& full) {
     r0 = n = len = full = 0;
     if (s < a.S) {
-      r0 = a.row0[s];
+      r0 = max(a.row0[s], 0);
       n = min(a.row0[s + 1], a.T) - r0;
       full = a.kv_len[s];
       len = (int)max(0ll, min((long long)full, cap));
@@ -495,11 +495,11 @@ __device__ __forceinline__ u32x2 read_tr(const void* p) {
 // LDS, the other buffer's too (2048 rows over 6143 keys 602 us).
 __device__ __forceinline__ void to_lds(const void* base, uint32_t off, const void* to) {
   const uint32_t lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char*)to;
-  asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(off), "s"(base), "{m0}"(__builtin_amdgcn_readfirstlane(lds)));
+  asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(off), "s"(base), "{m0}"(__builtin_amdgcn_readfirstlane(lds)) : "memory");
 }
 __device__ __forceinline__ void to_lds(const void* from, const void* to) {
   const uint32_t lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char*)to;
-  asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(from), "{m0}"(__builtin_amdgcn_readfirstlane(lds)));
+  asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(from), "{m0}"(__builtin_amdgcn_readfirstlane(lds)) : "memory");
 }
 __device__ __forceinline__ void landed() { asm volatile("s_waitcnt vmcnt(0)" : : : "memory"); }
 
