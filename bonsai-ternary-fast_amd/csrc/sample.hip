@@ -170,15 +170,17 @@ __device__ __forceinline__ float cut_below(int bin, const Row& r) {
   return __double2float_rd(c - fabs(c) * 1e-12);  // (NaN, nothing skipped, where the maximum is infinite)
 }
 
-// fn(the thread's four logits, their indices, how many there are) for every round of a part, by all threads.
+// fn(the thread's four logits, their indices, how many there are; NaN behind them) for every round of a part, by all
+// threads.
 template <class F>
 __device__ __forceinline__ void over_part(const float* x, int i0, int i1, F fn) {
   constexpr int AHEAD = 2;  // rounds whose loads are on their way together
   for (int r = i0; r < i1; r += AHEAD * kRound) {
-    f32x4u v[AHEAD] = {};
+    f32x4u v[AHEAD];
     int n[AHEAD];
 #pragma unroll
     for (int k = 0; k < AHEAD; ++k) {
+      v[k] = f32x4u{NAN, NAN, NAN, NAN};
       const int i = r + k * kRound + 4 * (int)threadIdx.x;
       n[k] = min(4, i1 - i);
       if (n[k] == 4) v[k] = *reinterpret_cast<const f32x4u*>(x + i);
@@ -228,23 +230,35 @@ __global__ void __launch_bounds__(kPartThreads) sample_top_kernel(btf_sampling a
   if (blockIdx.x == 0 && threadIdx.x == 0) s.ncand = 0, s.done = 0;
   const bool tops = a.top_k && a.top_k[m] > 0;
   uint32_t* top = s.tops(a.V);
-  u64 best = 0;
+  const float* x0 = a.logits + (size_t)m * a.ldl;
+  // Four logits at a time: their largest as a key, their smallest, and where the thread's largest key came first; its
+  // index is found at the end.
+  uint32_t most = 0;
+  int at = 0;
   float lo = INFINITY;
-  over_part(a.logits + (size_t)m * a.ldl, i0, i1, [&](f32x4u x, int i, int n) {
-    uint32_t most = 0;
+  over_part(x0, i0, i1, [&](f32x4u x, int i, int n) {
+    uint32_t k = key_of(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])));
+    float least = fminf(fminf(x[0], x[1]), fminf(x[2], x[3]));
+    if (__any(least == -INFINITY)) {
+      least = INFINITY;
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (j < n) {
-        const u64 k = argmax_key(x[j], i + j);
-        best = key_max(best, k);
-        most = max(most, (uint32_t)(k >> 32));
-        if (x[j] > -INFINITY) lo = fminf(lo, x[j]);
-      }
+      for (int j = 0; j < 4; ++j)
+        if (x[j] > -INFINITY) least = fminf(least, x[j]);
+    }
+    lo = fminf(lo, least);
+    if (k > most) most = k, at = i;
     if (tops) {
-      most = half_max(most);
-      if ((threadIdx.x & 31) == 0 && n > 0) top[i / kTop] = most;
+      k = half_max(k);
+      if ((threadIdx.x & 31) == 0 && n > 0) top[i / kTop] = k;
     }
   });
+  u64 best = 0;
+  if (most) {
+    const float v = of_key(most);
+    int j = 0;
+    while (j < 3 && !(x0[at + j] == v)) ++j;  // (one of the four is it)
+    best = (u64)most << 32 | (uint32_t)~(uint32_t)(at + j);
+  }
   best = wave_max_key(best);
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) lo = fminf(lo, __shfl_xor(lo, o, 64));
@@ -763,7 +777,7 @@ __global__ void __launch_bounds__(kPickThreads) sample_pick_kernel(btf_sampling 
   __syncthreads();
   if (tid >= 64) return;
   // one wave walks them, four a lane
-  const int i0 = (int)sh.sh[0] * kSum + 4 * tid;
+  const int i0 = (int)min(sh.sh[0], (u64)nsum - 1) * kSum + 4 * tid;
   at = sh.sh[1];
   const u64 kth = sh.kth;  // the last that stays; 0: all of the bins before lo, and nothing else
   u64 wt[4], mine = 0;
