@@ -51,30 +51,40 @@ constexpr double kMost = 1.8e19;                  // above 2^20 weights of one, 
 __device__ __forceinline__ uint32_t key_of(float x) { return (uint32_t)(argmax_key(x, 0) >> 32); }
 __device__ __forceinline__ float of_key(uint32_t k) { return __uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k); }
 
-// exp(-d) in units of 2^-43, for 0 <= d < kFar: with n the nearest whole number to
-// -d / ln 2 and r = -d - n ln 2 (ln 2 in two parts), the polynomial of degree 9 that
-// agrees with exp at the Chebyshev points of |r| <= ln 2 / 2 (2e-14 off, a third of
-// the unit's half), scaled by its exponent; rounded to a whole number by adding 2^52.
-__device__ __forceinline__ u64 weight_at(double d) {
+// exp(-d) in units of 2^-43 as a whole number, for d >= 0 (0 from 30.6 on, and for NaN): with n the nearest whole number
+// to -d / ln 2 and r = -d - n ln 2 (ln 2 in two parts), the polynomial of degree 9 that agrees with exp at the Chebyshev
+// points of |r| <= ln 2 / 2 (2e-14 off, a third of the unit's half) times 2^43, scaled by 2^n and rounded.
+__device__ __forceinline__ double weight_f(double d) {
+  d = fmin(d, 64.0);
   const double n = rint(d * -1.4426950408889634);
   const double r = fma(n, -2.3190468138462996e-17, fma(n, -0.6931471805599453, -d));
-  double p = 2.7632640690513381e-06;
-  p = fma(p, r, 2.4884459768350122e-05);
-  p = fma(p, r, 0.00019841190647512536);
-  p = fma(p, r, 0.0013888801749621653);
-  p = fma(p, r, 0.0083333333673116239);
-  p = fma(p, r, 0.041666667040552129);
-  p = fma(p, r, 0.16666666666615648);
-  p = fma(p, r, 0.49999999999438588);
-  p = fma(p, r, 1.0000000000000013);
-  p = fma(p, r, 1.0000000000000135);
-  const double v = ldexp(p, (int)n + 43) + 4503599627370496.0;
-  return (u64)__double_as_longlong(v) & 0xfffffffffffffull;
+  double p = kOne * 2.7632640690513381e-06;
+  p = fma(p, r, kOne * 2.4884459768350122e-05);
+  p = fma(p, r, kOne * 0.00019841190647512536);
+  p = fma(p, r, kOne * 0.0013888801749621653);
+  p = fma(p, r, kOne * 0.0083333333673116239);
+  p = fma(p, r, kOne * 0.041666667040552129);
+  p = fma(p, r, kOne * 0.16666666666615648);
+  p = fma(p, r, kOne * 0.49999999999438588);
+  p = fma(p, r, kOne * 1.0000000000000013);
+  p = fma(p, r, kOne * 1.0000000000000135);
+  return rint(ldexp(p, (int)n));
 }
+// A whole number below 2^52 as 64 bits.
+__device__ __forceinline__ u64 whole(double v) { return (u64)__double_as_longlong(v + 4503599627370496.0) & 0xfffffffffffffull; }
+__device__ __forceinline__ u64 weight_at(double d) { return whole(weight_f(d)); }
 
 // Distance of a logit to the row's largest in units of the temperature; kFar or more (or NaN): no weight.
 __device__ __forceinline__ double distance(float x, float top, double inv_t) {
   return x == top ? 0.0 : ((double)top - (double)x) * inv_t;
+}
+// The same for the data passes, without its comparison: where the largest is infinite, `finite` makes the logits equal to
+// it 0 and the others NaN, and the largest 0.
+__device__ __forceinline__ f32x4u finite(f32x4u x, float top) {
+  if (fabsf(top) == INFINITY)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x[j] = x[j] == top ? 0.f : NAN;
+  return x;
 }
 __device__ __forceinline__ u64 weight(float x, float top, double inv_t) {
   const double d = distance(x, top, inv_t);
@@ -170,18 +180,37 @@ __device__ __forceinline__ float cut_below(int bin, const Row& r) {
   return __double2float_rd(c - fabs(c) * 1e-12);  // (NaN, nothing skipped, where the maximum is infinite)
 }
 
-// fn(the thread's four logits, their indices, how many there are; NaN behind them) for every round of a part, by all
-// threads.
+// Rounds of part [i0, i1) in which the wave's 256 logits hold one that is not below `cut`, by the maxima of 128: bit 2 r
+// for round r. By whole waves.
+constexpr uint32_t kAllRounds = 0x55555555u;
+static_assert(kMaxPart / kRound <= 16, "two bits a round");
+__device__ __forceinline__ uint32_t rounds_from(const uint32_t* top, int i0, int i1, float cut) {
+  const int lane = threadIdx.x & 63, i = i0 + (lane >> 1) * kRound + (threadIdx.x >> 6) * kSum + (lane & 1) * kTop;
+  bool live = false;
+  if (i < i1) {
+    const uint32_t k = top[i / kTop];
+    live = k != 0 && !(of_key(k) < cut);
+  }
+  const uint32_t b = (uint32_t)__ballot(live);
+  return (b | b >> 1) & kAllRounds;
+}
+
+// fn(the thread's four logits, their indices, how many there are; NaN behind them) for the rounds of a part that `rounds`
+// names, by whole waves.
 template <class F>
-__device__ __forceinline__ void over_part(const float* x, int i0, int i1, F fn) {
+__device__ __forceinline__ void over_part(const float* x, int i0, int i1, uint32_t rounds, F fn) {
   constexpr int AHEAD = 2;  // rounds whose loads are on their way together
-  for (int r = i0; r < i1; r += AHEAD * kRound) {
+  rounds &= (uint32_t)((1ull << 2 * ((i1 - i0 + kRound - 1) / kRound)) - 1);
+  while (rounds) {
     f32x4u v[AHEAD];
-    int n[AHEAD];
+    int n[AHEAD], at[AHEAD];
 #pragma unroll
     for (int k = 0; k < AHEAD; ++k) {
       v[k] = f32x4u{NAN, NAN, NAN, NAN};
-      const int i = r + k * kRound + 4 * (int)threadIdx.x;
+      n[k] = 0, at[k] = i1;
+      if (!rounds) continue;
+      const int i = at[k] = i0 + (__builtin_ctz(rounds) >> 1) * kRound + 4 * (int)threadIdx.x;
+      rounds &= rounds - 1;
       n[k] = min(4, i1 - i);
       if (n[k] == 4) v[k] = *reinterpret_cast<const f32x4u*>(x + i);
       else
@@ -190,25 +219,26 @@ __device__ __forceinline__ void over_part(const float* x, int i0, int i1, F fn) 
     }
 #pragma unroll
     for (int k = 0; k < AHEAD; ++k)
-      if (r + k * kRound < i1) fn(v[k], r + k * kRound + 4 * (int)threadIdx.x, n[k]);
+      if (__any(n[k] > 0)) fn(v[k], at[k], n[k]);
   }
 }
 
 // Sum over the wave, in every lane. (Halves by DPP within 16 lanes, then the row swaps.)
-__device__ __forceinline__ u64 wave_sum_u64(u64 v) {
-  auto add = [&](uint32_t lo, uint32_t hi) { v += (u64)hi << 32 | lo; };
-  add(dpp_i<0xB1>((int)v), dpp_i<0xB1>((int)(v >> 32)));
-  add(dpp_i<0x4E>((int)v), dpp_i<0x4E>((int)(v >> 32)));
-  add(dpp_i<0x141>((int)v), dpp_i<0x141>((int)(v >> 32)));
-  add(dpp_i<0x140>((int)v), dpp_i<0x140>((int)(v >> 32)));
+__device__ __forceinline__ double wave_sum_f64(double v) {
+  auto half = [&](int h) { return h ? (int)((u64)__double_as_longlong(v) >> 32) : (int)__double_as_longlong(v); };
+  auto join = [](uint32_t lo, uint32_t hi) { return __longlong_as_double((long long)((u64)hi << 32 | lo)); };
+  v += join(dpp_i<0xB1>(half(0)), dpp_i<0xB1>(half(1)));
+  v += join(dpp_i<0x4E>(half(0)), dpp_i<0x4E>(half(1)));
+  v += join(dpp_i<0x141>(half(0)), dpp_i<0x141>(half(1)));
+  v += join(dpp_i<0x140>(half(0)), dpp_i<0x140>(half(1)));
   {
-    const auto a = __builtin_amdgcn_permlane16_swap((uint32_t)v, (uint32_t)v, false, false);
-    const auto b = __builtin_amdgcn_permlane16_swap((uint32_t)(v >> 32), (uint32_t)(v >> 32), false, false);
-    v = ((u64)b[0] << 32 | a[0]) + ((u64)b[1] << 32 | a[1]);
+    const auto a = __builtin_amdgcn_permlane16_swap(half(0), half(0), false, false);
+    const auto b = __builtin_amdgcn_permlane16_swap(half(1), half(1), false, false);
+    v = join(a[0], b[0]) + join(a[1], b[1]);
   }
-  const auto a = __builtin_amdgcn_permlane32_swap((uint32_t)v, (uint32_t)v, false, false);
-  const auto b = __builtin_amdgcn_permlane32_swap((uint32_t)(v >> 32), (uint32_t)(v >> 32), false, false);
-  return ((u64)b[0] << 32 | a[0]) + ((u64)b[1] << 32 | a[1]);
+  const auto a = __builtin_amdgcn_permlane32_swap(half(0), half(0), false, false);
+  const auto b = __builtin_amdgcn_permlane32_swap(half(1), half(1), false, false);
+  return join(a[0], b[0]) + join(a[1], b[1]);
 }
 // Largest of each half of the wave, in its lanes.
 __device__ __forceinline__ uint32_t half_max(uint32_t v) {
@@ -228,7 +258,7 @@ __global__ void __launch_bounds__(kPartThreads) sample_top_kernel(btf_sampling a
   Scratch& s = scratch_of(a, m);
   for (int i = blockIdx.x * kPartThreads + threadIdx.x; i < kBins; i += gridDim.x * kPartThreads) s.sum[i] = 0, s.cnt[i] = 0;
   if (blockIdx.x == 0 && threadIdx.x == 0) s.ncand = 0, s.done = 0;
-  const bool tops = a.top_k && a.top_k[m] > 0;
+  const bool tops = a.top_k || a.top_p;  // what the next launches skip by
   uint32_t* top = s.tops(a.V);
   const float* x0 = a.logits + (size_t)m * a.ldl;
   // Four logits at a time: their largest as a key, their smallest, and where the thread's largest key came first; its
@@ -236,7 +266,7 @@ __global__ void __launch_bounds__(kPartThreads) sample_top_kernel(btf_sampling a
   uint32_t most = 0;
   int at = 0;
   float lo = INFINITY;
-  over_part(x0, i0, i1, [&](f32x4u x, int i, int n) {
+  over_part(x0, i0, i1, kAllRounds, [&](f32x4u x, int i, int n) {
     uint32_t k = key_of(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])));
     float least = fminf(fminf(x[0], x[1]), fminf(x[2], x[3]));
     if (__any(least == -INFINITY)) {
@@ -344,12 +374,24 @@ __global__ void __launch_bounds__(kPartThreads) sample_hist_kernel(btf_sampling 
   const bool weigh = r.p < 1.f;
   int deep = kBins - 1;
   if (r.k) {  // the deepest bin that top-k reaches, by the maxima of 128
+    // (the maxima of 1024 where there are twice as many of them as top-k keeps, or more: an eighth of the work of those
+    // of 128, and hardly deeper)
     const uint32_t* top = s.tops(a.V);
-    const int nt = (a.V + kTop - 1) / kTop;
+    const int nt = (a.V + kTop - 1) / kTop, by = 2 * r.k <= nt / 8 ? 8 : 1;
     if (r.k < nt) {
-      for (int i = threadIdx.x; i < nt; i += kPartThreads) {
-        const double d = distance(of_key(top[i]), r.top, r.inv_t);
-        if (top[i] && d < kFar) atomicAdd(&cnt[bin_of(d, r)], 1u);
+      for (int i = threadIdx.x * by; i < nt; i += kPartThreads * by) {
+        uint32_t k = 0;
+        if (by == 8) {
+          uint32_t t[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) t[j] = top[min(i + j, nt - 1)];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) k = max(k, t[j]);
+        } else {
+          k = top[i];
+        }
+        const double d = distance(of_key(k), r.top, r.inv_t);
+        if (k && d < kFar) atomicAdd(&cnt[bin_of(d, r)], 1u);
       }
       __syncthreads();
       constexpr int PER = kBins / kPartThreads;
@@ -368,25 +410,23 @@ __global__ void __launch_bounds__(kPartThreads) sample_hist_kernel(btf_sampling 
     }
   }
   const float cut = cut_below(deep, r);
-  over_part(a.logits + (size_t)m * a.ldl, i0, i1, [&](f32x4u x, int, int n) {
-    bool in[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) in[j] = j < n && !(x[j] < cut);
-    if (!__any(in[0] | in[1] | in[2] | in[3])) return;
-    u64 w[4];
+  const double top0 = fabsf(r.top) == INFINITY ? 0.0 : (double)r.top;
+  const uint32_t rounds = deep < kBins - 1 ? rounds_from(s.tops(a.V), i0, i1, cut) : kAllRounds;
+  over_part(a.logits + (size_t)m * a.ldl, i0, i1, rounds, [&](f32x4u x, int, int) {
+    if (!__any(!(x[0] < cut) | !(x[1] < cut) | !(x[2] < cut) | !(x[3] < cut))) return;
+    x = finite(x, r.top);
+    double w[4];
     int bin[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {  // (without branches, so that the four go through the arithmetic together)
-      const double d = distance(x[j], r.top, r.inv_t);
-      in[j] = in[j] & (d < kFar);
-      w[j] = weight_at(in[j] ? d : 0.0);
-      bin[j] = bin_of(in[j] ? d : 0.0, r);
-      in[j] = in[j] & (bin[j] <= deep) & (w[j] != 0);
+      const double d = fmin((top0 - (double)x[j]) * r.inv_t, 64.0);
+      w[j] = weight_f(d);
+      bin[j] = bin_of(d, r);
     }
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      if (!in[j]) continue;
-      if (weigh) atomicAdd(reinterpret_cast<unsigned long long*>(&sum[bin[j]]), (unsigned long long)w[j]);
+      if (!((w[j] != 0.0) & (bin[j] <= deep))) continue;
+      if (weigh) atomicAdd(reinterpret_cast<unsigned long long*>(&sum[bin[j]]), (unsigned long long)whole(w[j]));
       if (r.k) atomicAdd(&cnt[bin[j]], 1u);
     }
   });
@@ -427,44 +467,52 @@ __global__ void __launch_bounds__(kPartThreads) sample_border_kernel(btf_samplin
   __syncthreads();
   u64* psum = s.psum();
   const float cut = cut_below(b.lo < kBins ? max(b.hi, b.kb < kBins ? b.kb : 0) : kBins - 1, r);
-  over_part(a.logits + (size_t)m * a.ldl, i0, i1, [&](f32x4u x, int i, int n) {
-    bool in[4], stays[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) in[j] = j < n && !(x[j] < cut);
-    u64 mine = 0;
-    if (__any(in[0] | in[1] | in[2] | in[3])) {
+  // In units of bins: what is below lo stays, candidates are below end
+  const double top0 = fabsf(r.top) == INFINITY ? 0.0 : (double)r.top, floor_w = (double)r.floor_w;
+  const int deep = max(b.hi, b.kb < kBins ? b.kb : -1);
+  const double lo = b.lo < kBins ? (double)b.lo : INFINITY, end = deep < kBins - 1 ? (double)(deep + 1) : INFINITY;
+  uint32_t rounds = kAllRounds;
+  if (b.lo < kBins) {
+    rounds = rounds_from(s.tops(a.V), i0, i1, cut);
+    const int lane = threadIdx.x & 63, i = i0 + lane * kRound + (threadIdx.x >> 6) * kSum;  // a lane for each round
+    if (lane < kMaxPart / kRound && i < i1 && !(rounds >> 2 * lane & 1)) psum[i / kSum] = 0;
+  }
+  over_part(a.logits + (size_t)m * a.ldl, i0, i1, rounds, [&](f32x4u x, int i, int n) {
+    double mine = 0.0;  // (whole numbers; 256 of them stay below 2^52)
+    if (__any(!(x[0] < cut) | !(x[1] < cut) | !(x[2] < cut) | !(x[3] < cut))) {
+      const f32x4u y = finite(x, r.top);
       double d[4];
-      bool any = false;
+      bool stays[4], any = false, cands = false;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        d[j] = distance(x[j], r.top, r.inv_t);
-        in[j] = in[j] & (d[j] < kFar);
-        d[j] = in[j] ? d[j] : 0.0;
-        const int bin = bin_of(d[j], r);
-        stays[j] = in[j] & (bin < b.lo);
-        in[j] = in[j] & (bin >= b.lo) & ((bin <= b.hi) | (bin == b.kb));
+        d[j] = fmin((top0 - (double)y[j]) * r.inv_t, 64.0);
+        const double at = d[j] * r.scale;
+        stays[j] = at < lo;
         any |= stays[j];
+        cands |= !stays[j] & (at < end) & (d[j] < kFar);
       }
       if (__any(any))
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const u64 w = weight_at(d[j]);
-          mine += (stays[j] & (w >= r.floor_w)) ? w : 0;
+          const double w = weight_f(d[j]);
+          mine += stays[j] & (w >= floor_w) ? w : 0.0;
         }
+      if (cands)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if (!in[j]) continue;
-        const uint32_t k = atomicAdd(&n_cand, 1u);
-        if (k < kHere) {
-          cand[k][0] = __float_as_uint(x[j]), cand[k][1] = (uint32_t)(i + j);
-        } else {  // (more than a part's share)
-          const uint32_t g = atomicAdd(&s.ncand, 1u);
-          if (g < kCand) s.cand[g][0] = __float_as_uint(x[j]), s.cand[g][1] = (uint32_t)(i + j);
+        for (int j = 0; j < 4; ++j) {
+          const int bin = bin_of(d[j], r);
+          if (stays[j] | !(d[j] < kFar) | !((bin <= b.hi) | (bin == b.kb))) continue;
+          const uint32_t k = atomicAdd(&n_cand, 1u);
+          if (k < kHere) {
+            cand[k][0] = __float_as_uint(x[j]), cand[k][1] = (uint32_t)(i + j);
+          } else {  // (more than a part's share)
+            const uint32_t g = atomicAdd(&s.ncand, 1u);
+            if (g < kCand) s.cand[g][0] = __float_as_uint(x[j]), s.cand[g][1] = (uint32_t)(i + j);
+          }
         }
-      }
     }
-    if (__any(mine != 0)) mine = wave_sum_u64(mine);
-    if ((threadIdx.x & 63) == 0 && n > 0) psum[i / kSum] = mine;
+    if (__any(mine != 0.0)) mine = wave_sum_f64(mine);
+    if ((threadIdx.x & 63) == 0 && n > 0) psum[i / kSum] = whole(mine);
   });
   __syncthreads();
   const uint32_t here = min(n_cand, (uint32_t)kHere);
@@ -493,7 +541,7 @@ struct Pick {
   u64 part[kPickThreads / 64];
   u64 sh[8];
   u64 kth;
-  uint32_t n;
+  uint32_t n, before;
 };
 
 // The smallest key at which the count (by_count) or the weight of the logits from
@@ -602,6 +650,68 @@ __device__ void pick_alone(const btf_sampling& a, const float* x, int m, const R
   walk(a, x, m, r, key, ties, sh);
 }
 
+// The borders in the sorted candidates, PER consecutive ones a thread: what stays of them is added to its parts.
+template <int PER>
+__device__ __forceinline__ void pick_borders(Pick& sh, const Row& r, const Borders& b, uint32_t n) {
+  const uint32_t at0 = threadIdx.x * PER;
+  u64 w[PER], ws = 0, all, key[PER];
+  int bin[PER];
+  uint32_t before = 0;  // bins before top-k's border
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    w[i] = 0, bin[i] = kBins, key[i] = 0;
+    if (at0 + i < n) {
+      key[i] = sh.c.key[at0 + i];
+      const double d = distance(of_key((uint32_t)(key[i] >> 32)), r.top, r.inv_t);
+      w[i] = weight_at(d), bin[i] = bin_of(d, r);
+    }
+    ws += w[i];
+    before += bin[i] < b.kb && at0 + i < n;
+  }
+  const bool by_k = b.kb < kBins;
+  if (by_k && before) atomicAdd(&sh.before, before);
+  const u64 w0 = block_scan<kPickThreads>(ws, sh.part, &all) - ws;  // (waits: sh.before is complete)
+  // top-k: of bin kb the first k_left, and the weights of the top-k
+  uint32_t n_stay = n;
+  u64 w_top = b.below_kb;
+  if (by_k) {
+    const uint32_t n_before = sh.before;
+    n_stay = n_before + b.k_left;
+    u64 at = w0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      if (at0 + i == n_before) sh.sh[2] = at;
+      at += w[i];
+      if (at0 + i + 1 == n_stay) sh.sh[3] = at;
+    }
+    __syncthreads();  // (n_before < n_stay <= n: both are set)
+    w_top += sh.sh[3] - sh.sh[2];
+  }
+  if (r.p < 1.f) {
+    const double want = (double)r.p * (double)w_top;
+    u64 at = b.below_lo + w0;
+    uint32_t stay = 0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      // the list is without gaps up to bin hi, behind which nothing stays
+      const bool first = b.below_lo == 0 && at0 + i == 0;
+      stay += at0 + i < n && bin[i] <= b.hi && (first || (double)at < want);
+      at += w[i];
+    }
+    u64 sum;
+    block_scan<kPickThreads>(stay, sh.part, &sum);
+    n_stay = min(n_stay, (uint32_t)sum);
+  }
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    if (at0 + i >= n_stay) break;
+    const int idx = argmax_key_index(key[i]);
+    if (w[i] >= r.floor_w) atomicAdd(reinterpret_cast<unsigned long long*>(&sh.c.sum[idx / kSum]), (unsigned long long)w[i]);
+    if (at0 + i == n_stay - 1) sh.kth = key[i];
+  }
+  __syncthreads();
+}
+
 __global__ void __launch_bounds__(kPickThreads) sample_pick_kernel(btf_sampling a) {
   __shared__ Pick sh;
   const int m = blockIdx.x, tid = threadIdx.x;
@@ -624,7 +734,7 @@ __global__ void __launch_bounds__(kPickThreads) sample_pick_kernel(btf_sampling 
   const int nsum = (a.V + kSum - 1) / kSum;
   const u64* psum = s.psum();
   for (int i = tid; i < nsum; i += kPickThreads) sh.c.sum[i] = psum[i];
-  if (tid == 0) sh.kth = 0, sh.n = 0;
+  if (tid == 0) sh.kth = 0, sh.n = 0, sh.before = 0;
   constexpr int PER = kCand / kPickThreads;
   const bool by_k = b.kb < kBins;
   if (n > 64 && b.lo == b.hi && (by_k ? b.lo == b.kb && r.p == 1.f : true)) {
@@ -677,82 +787,46 @@ __global__ void __launch_bounds__(kPickThreads) sample_pick_kernel(btf_sampling 
   } else {
     for (int i = tid; i < (int)n; i += kPickThreads) sh.c.key[i] = argmax_key(__uint_as_float(s.cand[i][0]), (int)s.cand[i][1]);
   }
-  // candidates in order, by a bitonic sort of the next power of two of them
-  int size2 = 1;
+  // candidates in order
+  int size2 = 32;
   while (size2 < (int)n) size2 *= 2;
+  const bool few = size2 <= kPickThreads;
+  uint32_t* rank = reinterpret_cast<uint32_t*>(sh.c.fine);
   for (int i = n + tid; i < size2; i += kPickThreads) sh.c.key[i] = 0;
+  if (tid < kPickThreads) rank[tid] = 0;
   __syncthreads();
-  // (a wave's pairs of a pass with j <= 64 lie in 128 keys that no other wave touches in such a pass: its LDS accesses
-  // are in order, so only passes over longer distances need the workgroup to wait)
-  bool far = false;
-  for (int k = 2; k <= size2; k *= 2)
-    for (int j = k / 2; j > 0; j /= 2) {
-      if (far || j > 64) __syncthreads();
-      far = j > 64;
-      for (int i = tid; i < size2 / 2; i += kPickThreads) {
-        const int lo = 2 * i - (i & (j - 1)), hi = lo + j;  // falling order in the end
-        const u64 x0 = sh.c.key[lo], x1 = sh.c.key[hi];
-        if ((x0 < x1) == ((lo & k) == 0)) sh.c.key[lo] = x1, sh.c.key[hi] = x0;
+  if (few) {
+    // by their ranks: how many keys are larger, counted by kPickThreads / size2 threads for each (75 candidates: 0.5 us;
+    // the passes of a sort wait for each other, 5 us)
+    const int c = tid & (size2 - 1), share = size2 * size2 / kPickThreads, j0 = tid / size2 * share;
+    const u64 key = sh.c.key[c];
+    uint32_t larger = 0;
+#pragma unroll 4
+    for (int j = j0; j < j0 + share; ++j) larger += sh.c.key[j] > key;
+    if (c < (int)n && larger) atomicAdd(&rank[c], larger);
+    __syncthreads();
+    if (tid < (int)n) sh.c.key[rank[tid]] = key;  // (tid < n: c is tid; every key has been read)
+  } else {
+    // by a bitonic sort. (a wave's pairs of a pass with j <= 64 lie in 128 keys that no other wave touches in such a pass:
+    // its LDS accesses are in order, so only passes over longer distances need the workgroup to wait)
+    bool far = false;
+    for (int k = 2; k <= size2; k *= 2)
+      for (int j = k / 2; j > 0; j /= 2) {
+        if (far || j > 64) __syncthreads();
+        far = j > 64;
+        for (int i = tid; i < size2 / 2; i += kPickThreads) {
+          const int lo = 2 * i - (i & (j - 1)), hi = lo + j;  // falling order in the end
+          const u64 x0 = sh.c.key[lo], x1 = sh.c.key[hi];
+          if ((x0 < x1) == ((lo & k) == 0)) sh.c.key[lo] = x1, sh.c.key[hi] = x0;
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
       }
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-      __builtin_amdgcn_wave_barrier();
-    }
-  __syncthreads();
-  // prefix sums of their weights, consecutive ones a thread
-  u64 w[PER], ws = 0, w_all;
-  int bin[PER];
-#pragma unroll
-  for (int i = 0; i < PER; ++i) {
-    const int at = tid * PER + i;
-    w[i] = 0, bin[i] = kBins;
-    if (at < (int)n) {
-      const double d = distance(of_key((uint32_t)(sh.c.key[at] >> 32)), r.top, r.inv_t);
-      w[i] = weight_at(d), bin[i] = bin_of(d, r);
-    }
-    ws += w[i];
-  }
-  const u64 w0 = block_scan<kPickThreads>(ws, sh.part, &w_all) - ws;
-  // top-k: of bin kb the first k_left; its place in the list and the weights before it
-  uint32_t n_before = 0, n_stay = n;
-  u64 w_top = b.below_kb;  // weights of the top-k
-  if (b.kb < kBins) {
-    u64 c = 0, n_b, in = 0, w_in;
-#pragma unroll
-    for (int i = 0; i < PER; ++i) c += bin[i] < b.kb;
-    block_scan<kPickThreads>(c, sh.part, &n_b);
-    n_before = (uint32_t)n_b;
-    n_stay = n_before + b.k_left;
-#pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      const uint32_t at = tid * PER + i;
-      if (at >= n_before && at < n_stay) in += w[i];
-    }
-    block_scan<kPickThreads>(in, sh.part, &w_in);
-    w_top += w_in;
-  }
-  if (r.p < 1.f) {
-    const double want = (double)r.p * (double)w_top;
-    u64 c = 0, stay, at = b.below_lo + w0;
-#pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      // the list is without gaps up to bin hi, behind which nothing stays
-      const bool first = b.below_lo == 0 && tid == 0 && i == 0;
-      c += bin[i] <= b.hi && (first || (double)at < want);
-      at += w[i];
-    }
-    block_scan<kPickThreads>(c, sh.part, &stay);
-    n_stay = min(n_stay, (uint32_t)stay);
-  }
-  // what stays of them, added to its parts
-#pragma unroll
-  for (int i = 0; i < PER; ++i) {
-    const uint32_t at = tid * PER + i;
-    if (at >= n_stay) break;
-    const int idx = argmax_key_index(sh.c.key[at]);
-    if (w[i] >= r.floor_w) atomicAdd(reinterpret_cast<unsigned long long*>(&sh.c.sum[idx / kSum]), (unsigned long long)w[i]);
-    if (at == n_stay - 1) sh.kth = sh.c.key[at];
   }
   __syncthreads();
+  if (n == 0) {  // no border: nothing but the parts
+  } else if (few) pick_borders<1>(sh, r, b, n);
+  else pick_borders<kCand / kPickThreads>(sh, r, b, n);
   // the kSum logits in which the sum passes u times the total
   constexpr int SPER = kMaxV / kSum / kPickThreads;
   const int per = (nsum + kPickThreads - 1) / kPickThreads;  // at most SPER
