@@ -51,12 +51,16 @@ constexpr double kMost = 1.8e19;                  // above 2^20 weights of one, 
 __device__ __forceinline__ uint32_t key_of(float x) { return (uint32_t)(argmax_key(x, 0) >> 32); }
 __device__ __forceinline__ float of_key(uint32_t k) { return __uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k); }
 
-// exp(-d) in units of 2^-43 as a whole number, for d >= 0 (0 from 30.6 on, and for NaN): with n the nearest whole number
-// to -d / ln 2 and r = -d - n ln 2 (ln 2 in two parts), the polynomial of degree 9 that agrees with exp at the Chebyshev
-// points of |r| <= ln 2 / 2 (2e-14 off, a third of the unit's half) times 2^43, scaled by 2^n and rounded.
-__device__ __forceinline__ double weight_f(double d) {
+// exp(-d) in units of 2^-43 as a whole number plus 2^52 (its low 52 bits), for d >= 0 (no units from 30.6 on, and for
+// NaN): with n the nearest whole number to -d / ln 2 and r = -d - n ln 2 (ln 2 in two parts), the polynomial of degree 9
+// that agrees with exp at the Chebyshev points of |r| <= ln 2 / 2 (2e-14 off, a third of the unit's half) times 2^43,
+// scaled by 2^n in its exponent. Whole numbers come from adding 2^52 and 1.5 2^52: products and sums run at full rate,
+// conversions and the rounding instruction do not.
+constexpr double kWhole = 4503599627370496.0;
+__device__ __forceinline__ double weight_bits(double d) {
   d = fmin(d, 64.0);
-  const double n = rint(d * -1.4426950408889634);
+  const double t = fma(d, -1.4426950408889634, 1.5 * kWhole);
+  const double n = t - 1.5 * kWhole;
   const double r = fma(n, -2.3190468138462996e-17, fma(n, -0.6931471805599453, -d));
   double p = kOne * 2.7632640690513381e-06;
   p = fma(p, r, kOne * 2.4884459768350122e-05);
@@ -68,11 +72,12 @@ __device__ __forceinline__ double weight_f(double d) {
   p = fma(p, r, kOne * 0.49999999999438588);
   p = fma(p, r, kOne * 1.0000000000000013);
   p = fma(p, r, kOne * 1.0000000000000135);
-  return rint(ldexp(p, (int)n));
+  const u64 b = (u64)__double_as_longlong(p) + ((u64)(uint32_t)__double_as_longlong(t) << 52);
+  return __longlong_as_double((long long)b) + kWhole;
 }
-// A whole number below 2^52 as 64 bits.
-__device__ __forceinline__ u64 whole(double v) { return (u64)__double_as_longlong(v + 4503599627370496.0) & 0xfffffffffffffull; }
-__device__ __forceinline__ u64 weight_at(double d) { return whole(weight_f(d)); }
+__device__ __forceinline__ u64 low52(double v) { return (u64)__double_as_longlong(v) & 0xfffffffffffffull; }
+__device__ __forceinline__ u64 whole(double v) { return low52(v + kWhole); }  // of a whole number below 2^52
+__device__ __forceinline__ u64 weight_at(double d) { return low52(weight_bits(d)); }
 
 // Distance of a logit to the row's largest in units of the temperature; kFar or more (or NaN): no weight.
 __device__ __forceinline__ double distance(float x, float top, double inv_t) {
@@ -101,12 +106,25 @@ struct Row {
   float p;                       // 1: no top-p
 };
 
+// The same in every lane, which the compiler does not know of what it loads.
+__device__ __forceinline__ uint32_t same(uint32_t v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ u64 same(u64 v) { return (u64)same((uint32_t)(v >> 32)) << 32 | same((uint32_t)v); }
+__device__ __forceinline__ double same(double v) { return __longlong_as_double((long long)same((u64)__double_as_longlong(v))); }
+__device__ __forceinline__ Row same(const Row& r) {
+  return {(bool)same((uint32_t)r.greedy), __uint_as_float(same(__float_as_uint(r.top))), same(r.inv_t), same(r.scale),
+          same(r.floor_w), (int)same((uint32_t)r.k), __uint_as_float(same(__float_as_uint(r.p)))};
+}
+
 // Where the borders lie, by bins: [0, lo) stays whole; candidates are in [lo, hi] and kb.
 struct Borders {
   int lo, hi, kb;         // kBins: none
   uint32_t k_left;        // top-k: how many of bin kb stay
   u64 below_lo, below_kb; // weights of the bins before lo, before kb
 };
+__device__ __forceinline__ Borders same(const Borders& b) {
+  return {(int)same((uint32_t)b.lo), (int)same((uint32_t)b.hi), (int)same((uint32_t)b.kb), same(b.k_left), same(b.below_lo),
+          same(b.below_kb)};
+}
 
 struct Scratch {
   u64 sum[kBins];
@@ -362,8 +380,17 @@ __global__ void __launch_bounds__(kPartThreads) sample_hist_kernel(btf_sampling 
   __shared__ bool last;
   const int m = blockIdx.y, i0 = blockIdx.x * size, i1 = min(a.V, i0 + size);
   Scratch& s = scratch_of(a, m);
+  // (the first maxima are on their way while the settings are worked out)
+  const uint32_t* top = s.tops(a.V);
+  const int nt = (a.V + kTop - 1) / kTop;
+  uint32_t t[8] = {};
+  auto fetch = [&](int i) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) t[j] = i + j * kPartThreads < nt ? top[i + j * kPartThreads] : 0;
+  };
+  if (a.top_k && a.top_k[m] > 0) fetch(threadIdx.x);
   u64 best;
-  const Row r = settings(a, s, m, gridDim.x, &best);
+  const Row r = same(settings(a, s, m, gridDim.x, &best));
   if (r.greedy || (r.k == 0 && r.p == 1.f)) {
     if (blockIdx.x == 0 && threadIdx.x == 0) s.row = r, s.best = best, s.borders = Borders{kBins, -1, kBins, 0, 0, 0};
     return;
@@ -374,24 +401,22 @@ __global__ void __launch_bounds__(kPartThreads) sample_hist_kernel(btf_sampling 
   const bool weigh = r.p < 1.f;
   int deep = kBins - 1;
   if (r.k) {  // the deepest bin that top-k reaches, by the maxima of 128
-    // (the maxima of 1024 where there are twice as many of them as top-k keeps, or more: an eighth of the work of those
-    // of 128, and hardly deeper)
-    const uint32_t* top = s.tops(a.V);
-    const int nt = (a.V + kTop - 1) / kTop, by = 2 * r.k <= nt / 8 ? 8 : 1;
     if (r.k < nt) {
-      for (int i = threadIdx.x * by; i < nt; i += kPartThreads * by) {
-        uint32_t k = 0;
-        if (by == 8) {
-          uint32_t t[8];
-#pragma unroll
-          for (int j = 0; j < 8; ++j) t[j] = top[min(i + j, nt - 1)];
-#pragma unroll
-          for (int j = 0; j < 8; ++j) k = max(k, t[j]);
-        } else {
-          k = top[i];
-        }
+      // (the maxima of 1024 logits, in eight places, where there are twice as many of them as top-k keeps, or more: an
+      // eighth of the work of those of 128, and hardly deeper)
+      const bool by8 = 2 * r.k <= nt / 8;
+      auto count = [&](uint32_t k) {
         const double d = distance(of_key(k), r.top, r.inv_t);
         if (k && d < kFar) atomicAdd(&cnt[bin_of(d, r)], 1u);
+      };
+      for (int i = threadIdx.x; i < nt; i += 8 * kPartThreads) {
+        if (i >= 8 * kPartThreads) fetch(i);
+        if (by8) {
+          count(max(max(max(t[0], t[1]), max(t[2], t[3])), max(max(t[4], t[5]), max(t[6], t[7]))));
+        } else {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) count(t[j]);
+        }
       }
       __syncthreads();
       constexpr int PER = kBins / kPartThreads;
@@ -411,22 +436,22 @@ __global__ void __launch_bounds__(kPartThreads) sample_hist_kernel(btf_sampling 
   }
   const float cut = cut_below(deep, r);
   const double top0 = fabsf(r.top) == INFINITY ? 0.0 : (double)r.top;
-  const uint32_t rounds = deep < kBins - 1 ? rounds_from(s.tops(a.V), i0, i1, cut) : kAllRounds;
+  const uint32_t rounds = deep < kBins - 1 ? rounds_from(top, i0, i1, cut) : kAllRounds;
   over_part(a.logits + (size_t)m * a.ldl, i0, i1, rounds, [&](f32x4u x, int, int) {
     if (!__any(!(x[0] < cut) | !(x[1] < cut) | !(x[2] < cut) | !(x[3] < cut))) return;
     x = finite(x, r.top);
-    double w[4];
+    u64 w[4];
     int bin[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {  // (without branches, so that the four go through the arithmetic together)
       const double d = fmin((top0 - (double)x[j]) * r.inv_t, 64.0);
-      w[j] = weight_f(d);
+      w[j] = weight_at(d);
       bin[j] = bin_of(d, r);
     }
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      if (!((w[j] != 0.0) & (bin[j] <= deep))) continue;
-      if (weigh) atomicAdd(reinterpret_cast<unsigned long long*>(&sum[bin[j]]), (unsigned long long)whole(w[j]));
+      if (!((w[j] != 0) & (bin[j] <= deep))) continue;
+      if (weigh) atomicAdd(reinterpret_cast<unsigned long long*>(&sum[bin[j]]), (unsigned long long)w[j]);
       if (r.k) atomicAdd(&cnt[bin[j]], 1u);
     }
   });
@@ -457,9 +482,9 @@ __global__ void __launch_bounds__(kPartThreads) sample_border_kernel(btf_samplin
   Row r;
   Borders b = {kBins, -1, kBins, 0, 0, 0};
   if (a.top_k || a.top_p) {
-    r = s.row, b = s.borders;
+    r = same(s.row), b = same(s.borders);
   } else {  // no launch before this one has found them
-    r = settings(a, s, m, gridDim.x, &best);
+    r = same(settings(a, s, m, gridDim.x, &best));
     if (blockIdx.x == 0 && threadIdx.x == 0) s.row = r, s.best = best, s.borders = b;
   }
   if (r.greedy) return;
@@ -470,7 +495,7 @@ __global__ void __launch_bounds__(kPartThreads) sample_border_kernel(btf_samplin
   // In units of bins: what is below lo stays, candidates are below end
   const double top0 = fabsf(r.top) == INFINITY ? 0.0 : (double)r.top, floor_w = (double)r.floor_w;
   const int deep = max(b.hi, b.kb < kBins ? b.kb : -1);
-  const double lo = b.lo < kBins ? (double)b.lo : INFINITY, end = deep < kBins - 1 ? (double)(deep + 1) : INFINITY;
+  const double lo = b.lo < kBins ? (double)b.lo : INFINITY, end = fmin(deep < kBins - 1 ? (double)(deep + 1) : INFINITY, kFar * r.scale);
   uint32_t rounds = kAllRounds;
   if (b.lo < kBins) {
     rounds = rounds_from(s.tops(a.V), i0, i1, cut);
@@ -489,19 +514,19 @@ __global__ void __launch_bounds__(kPartThreads) sample_border_kernel(btf_samplin
         const double at = d[j] * r.scale;
         stays[j] = at < lo;
         any |= stays[j];
-        cands |= !stays[j] & (at < end) & (d[j] < kFar);
+        cands |= !stays[j] & (at < end);
       }
       if (__any(any))
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const double w = weight_f(d[j]);
-          mine += stays[j] & (w >= floor_w) ? w : 0.0;
+          const double w = weight_bits(d[j]) - kWhole;
+          mine += (stays[j] & (w >= floor_w)) ? w : 0.0;
         }
       if (cands)
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const int bin = bin_of(d[j], r);
-          if (stays[j] | !(d[j] < kFar) | !((bin <= b.hi) | (bin == b.kb))) continue;
+          if (stays[j] | !(d[j] * r.scale < end) | !((bin <= b.hi) | (bin == b.kb))) continue;
           const uint32_t k = atomicAdd(&n_cand, 1u);
           if (k < kHere) {
             cand[k][0] = __float_as_uint(x[j]), cand[k][1] = (uint32_t)(i + j);
