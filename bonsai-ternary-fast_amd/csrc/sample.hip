@@ -160,6 +160,19 @@ __host__ __device__ inline Parts parts_of(int M, int V) {
   return {(V + size - 1) / size, size};
 }
 
+// Smallest of the wave, in every lane.
+__device__ __forceinline__ float wave_min(float v) {
+  auto at = [&](int x) { return __int_as_float(x); };
+  v = fminf(v, at(dpp_i<0xB1>(__float_as_int(v))));
+  v = fminf(v, at(dpp_i<0x4E>(__float_as_int(v))));
+  v = fminf(v, at(dpp_i<0x141>(__float_as_int(v))));
+  v = fminf(v, at(dpp_i<0x140>(__float_as_int(v))));
+  auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = fminf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fminf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+}
+
 // Settings of row m; `best` its largest key. By every thread of the workgroup, which waits here.
 __device__ Row settings(const btf_sampling& a, const Scratch& s, int m, int parts, u64* best) {
   u64 b = 0;
@@ -167,8 +180,7 @@ __device__ Row settings(const btf_sampling& a, const Scratch& s, int m, int part
   const int lane = threadIdx.x & 63;
   for (int i = lane; i < parts; i += 64) b = key_max(b, s.pmax[i]), lo = fminf(lo, s.pmin[i]);
   b = wave_max_key(b);
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) lo = fminf(lo, __shfl_xor(lo, o, 64));
+  lo = wave_min(lo);
   Row r;
   const float t = a.temperature ? a.temperature[m] : 1.f;
   r.greedy = !(t > 0.f) || b == 0;
@@ -308,8 +320,7 @@ __global__ void __launch_bounds__(kPartThreads) sample_top_kernel(btf_sampling a
     best = (u64)most << 32 | (uint32_t)~(uint32_t)(at + j);
   }
   best = wave_max_key(best);
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) lo = fminf(lo, __shfl_xor(lo, o, 64));
+  lo = wave_min(lo);
   if ((threadIdx.x & 63) == 0) wk[threadIdx.x >> 6] = best, wm[threadIdx.x >> 6] = lo;
   __syncthreads();
   if (threadIdx.x == 0) {
