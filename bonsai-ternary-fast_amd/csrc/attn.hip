@@ -149,7 +149,7 @@ __device__ bool find(const btf_paged_attention& a, const btf_kv_cache& kv, int i
   const int C = max(kStep, __builtin_amdgcn_readfirstlane((int)(work / (float)(target(R) * kStep) + 1.f)) * kStep);
   int items = 0, slots = 0;  // before the chunk
   for (int s0 = 0; s0 < a.S; s0 += 64) {
-    read(s0 + lane, r0, n, len, full);
+    if (a.S > 64) read(s0 + lane, r0, n, len, full);  // (up to 64 requests are still there)
     const int tiles = n > 0 ? (n * G + R - 1) / R : 0, pieces = max(1, (len + C - 1) / C);
     const int mine = kv.heads * tiles * pieces, cut = pieces > 1 ? mine : 0;
     const int upto = wave_scan_i(mine), cuts = wave_scan_i(cut);
