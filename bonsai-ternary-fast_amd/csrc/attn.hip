@@ -30,6 +30,17 @@
 // -infinity, V of keys behind the end is cleared. Where V or a score is not
 // finite all the same (0 * infinity in a product), the item's result shows it,
 // and the item is done again one row at a time by the plain loop.
+//
+// Which kernel: by the rows that a request has on average for a KV head (tile_rows).
+// Up to 16 or 32 (one new token, few heads more), attn_stream_kernel as above: bound
+// by HBM once the cache is long (one token each of 32 requests, 2.7 GB of cache: 465
+// us, 5.8 TB/s), by the chain of reads when it is short (one token over 4097: 14 us,
+// find 1.1, pages and first block 3.4, products 1.8, the waves' join 1.5, the pieces'
+// join 3.7). More rows, attn_tile_kernel below: bound by the issue of matrix and vector
+// instructions (64-row trees of 8 requests 182 us, matrix units 46 % busy and vector
+// 43 %; 2048 rows of heads of 256 over 8191 keys 482-493 us: 4.5e11 operations with
+// both parts of P, 0.97 PFLOP/s, 46 % and 30 %). The join of the pieces takes 5 to 28
+// us of these: without pieces 512 tiles of unlike length end one after another.
 #include <string>
 
 #include "../../include/btf/hip_abi.h"

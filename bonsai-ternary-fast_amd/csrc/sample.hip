@@ -7,22 +7,28 @@
 // (units of 2^-43, in 64 bits), so no sum depends on its order.
 //
 // Four launches over the row, cut into parts of 2048 to 16384 logits:
-//  * top: the parts' largest key and smallest logit; with top-k also the largest key
-//    of every 128 logits;
+//  * top: the parts' largest key and smallest logit, and the largest key of every 128
+//    logits, by which the next launches skip what lies below all that they look for;
 //  * hist (rows with top-k or top-p): weights (top-p) and counts (top-k) by 1024 bins
 //    of the distance to the maximum, in LDS, then added to the row's. With top-k only
-//    the bins down to the one in which the k-th largest of the 128-logit maxima lies:
-//    k logits are at least as large;
-//  * border: from the bins, those in which a border can lie. top-k's is the bin in
-//    which the count passes k; top-p's lies between the bins in which the sum passes p
-//    times the least and the most that the top-k may weigh. Below them everything
-//    stays: its weights are summed for every 256 logits. What lies in them is written
-//    out, logit and index, as candidates;
-//  * pick: one workgroup per row sorts the candidates (a bin of a row of 248320
+//    the bins down to the one in which the k-th largest of the maxima lies: k logits
+//    are at least as large. The row's last workgroup finds from the bins those in which
+//    a border can lie: top-k's is the bin in which the count passes k; top-p's lies
+//    between the bins in which the sum passes p times the least and the most that the
+//    top-k may weigh;
+//  * border: below those bins everything stays: its weights are summed for every 256
+//    logits. What lies in them is written out, logit and index, as candidates;
+//  * pick: one workgroup per row puts the candidates in order (a bin of a row of 248320
 //    normal logits holds 1500 of them at most), finds the borders exactly, adds
 //    what stays to its 256 logits, and walks those in which the sum passes u.
 // A row whose border bins hold more than kCand logits (many equal ones) is done by
 // that workgroup alone, eight key bits at a time.
+//
+// What bounds it: one row waits, for four launches and the chain of reads in each (248320
+// logits: 26 us; top 3.6, hist 8.4, border 4.3, pick 6.3). Many rows read the logits three
+// times, 10 us a pass for 48 rows of 248320 at the copy rate, and where there is no top-k work
+// out every logit's weight in each of two (36 vector instructions): 59 us (top 12.3, hist 20.9,
+// border 14.5, pick 9.2).
 #include <cmath>
 #include <string>
 
@@ -152,8 +158,8 @@ struct Parts {
   int n, size;  // size a multiple of kRound
 };
 __host__ __device__ inline Parts parts_of(int M, int V) {
-  // about 2048 workgroups over the rows: eight to a CU, as many as there is room for (48 rows of 248320 in 73.9 us with
-  // 1024, 67.4 with 2048, 71.5 with 4096)
+  // about 2048 workgroups over the rows: eight to a CU, as many as there is room for (48 rows of 248320 in 64.9 us with
+  // 1024, 59.1 with 2048, 59.7 with 2560; 130 of 50257 in 50.1, 45.6 and 46.5)
   int want = (2048 + M - 1) / M;
   int size = (V + want - 1) / want;
   size = size < kMinPart ? kMinPart : size > kMaxPart ? kMaxPart : (size + kRound - 1) / kRound * kRound;
