@@ -874,6 +874,79 @@ def check_step(L, dense):
             dense[s][j] = k[table[s, j // L.page], :, j % L.page].copy()
 
 
+# strides with which the last page, token or head starts beyond 2^32 bytes
+FAR = [(16, lambda HK, D, page: (2 ** 30 + 64, page * D, D)), (256, lambda HK, D, page: (HK * D, D, 2 ** 24)),
+       (32, lambda HK, D, page: (page * D, 2 ** 31, D))]
+
+
+def far_cache(shape, strides, kind, fill=None):
+    """Two caches of (pages, heads, tokens, dim) at these strides, as flat arrays and as views of what the strides reach."""
+    torch = _torch()
+    flat = [torch.empty(sum((n - 1) * st for n, st in zip(shape, (*strides, 1))) + 1, dtype=kind_of(kind), device="cuda")
+            for _ in range(2)]
+    view = [torch.as_strided(f, shape, (*strides, 1)) for f in flat]
+    for i, w in enumerate(view):
+        w.copy_(fill[i]) if fill else w.zero_()
+    return flat, view
+
+
+@pytest.mark.parametrize("page,strides", FAR, ids=["pages", "tokens", "heads"])
+@pytest.mark.parametrize("new", [1, 3, 90])
+def test_attention_offsets_beyond_32_bits(hip, page, strides, new):
+    rng = np.random.default_rng(page + new)
+    heads, kind = (8, 2, 128), "f16"
+    kv_len = [3 * page + 7] if page < 256 else [page + 9]
+    new = min(new, kv_len[0])
+    q, k, v, table, row0 = attn_inputs(rng, kv_len, [new], heads, kind, page)
+    flat, view = far_cache(k.shape, strides(2, 128, page), kind, (k, v))
+    out = run_attn(hip, q, *flat, table, row0, kv_len, None, heads, kind, page, pages=k.shape[0], strides=strides(2, 128, page))
+    check_attn(out, q, k, v, table, row0, kv_len, None, heads, kind, page)
+
+
+def test_attention_rows_beyond_32_bits(hip):
+    """Rows of q and out that lie gigabytes apart."""
+    torch = _torch()
+    rng = np.random.default_rng(16)
+    heads, kind, page, kv_len, ld = (4, 2, 64), "bf16", 16, [40], 2 ** 29 + 8
+    q, k, v, table, row0 = attn_inputs(rng, kv_len, [6], heads, kind, page)
+    far_q = torch.as_strided(torch.empty(5 * ld + 256, dtype=q.dtype, device="cuda"), (6, 256), (ld, 1)).copy_(q)
+    far_o = torch.as_strided(torch.empty(5 * ld + 256, dtype=torch.float32, device="cuda"), (6, 256), (ld, 1))
+    kv = hip.KvCache(k, v, hip.CacheType[kind], page, 2, 64, k.shape[0], 2 * page * 64, page * 64, 64)
+    hip.launch_paged_attention(hip.PagedAttention(
+        S=1, T=6, heads=4, q=far_q, ldq=ld, table=ints(table), ldt=table.shape[1], row0=ints(row0), kv_len=ints(kv_len),
+        scale=0.125, out=far_o, ldo=ld, ws=words(hip.paged_attention_ws_bytes(1, 6, 4, kv))), kv, stream())
+    torch.cuda.synchronize()
+    check_attn(far_o.contiguous(), q, k, v, table, row0, kv_len, None, heads, kind, page, scale=0.125)
+
+
+@pytest.mark.parametrize("page,strides", FAR, ids=["pages", "tokens", "heads"])
+def test_rope_offsets_beyond_32_bits(hip, page, strides):
+    rng = np.random.default_rng(page)
+    H, HK, D, kind, pages = 2, 2, 128, "bf16", 5 if page < 256 else 2
+    flat, view = far_cache((pages, HK, page, D), strides(HK, D, page), kind)
+    T = 24
+    qkv, slot = rope_inputs(rng, T, H, HK, D, page, kind)[:2]
+    slot = rng.permutation(pages * page)[:T]
+    if pages * page - 1 not in slot:  # (no slot twice)
+        slot[0] = pages * page - 1
+    pos, (turns, _) = rng.integers(0, 999, T), hip.rope_table(64, 1e4)
+    q = run_rope(hip, qkv, slot, flat, pages, pos, turns, H, HK, D, page, kind, 64, "half", strides=strides(HK, D, page))
+    got = [w.contiguous() for w in view]
+    check_rope(q, got, [w.new_zeros(w.shape) for w in got], qkv, slot, pos, turns, H, HK, D, page, kind, 64, "half")
+
+
+def test_sample_rows_beyond_32_bits(hip):
+    torch = _torch()
+    rng = np.random.default_rng(17)
+    x, ld = (2 * rng.standard_normal((3, 5000))).astype(np.float32), 2 ** 30 + 1
+    far = torch.as_strided(torch.empty(2 * ld + 5000, dtype=torch.float32, device="cuda"), (3, 5000), (ld, 1)).copy_(dev(x))
+    tok, u = torch.full((3,), -5, dtype=torch.int32, device="cuda"), np.array([0.1, 0.5, 0.9], np.float32)
+    hip.launch_sample(hip.Sampling(M=3, V=5000, logits=far, ldl=ld, top_k=ints([0, 40, 0]), top_p=dev(np.array([1, 1, 0.8], np.float32)),
+                                   u=dev(u), token=tok, ws=words(hip.sample_ws_bytes(3, 5000))), stream())
+    want = [ref.sample(x[m], 1.0, [0, 40, 0][m], np.float32([1, 1, 0.8][m]), 0.0, u[m])[0] for m in range(3)]
+    assert host(tok).tolist() == want
+
+
 @pytest.mark.parametrize("graph", [False, True], ids=["eager", "captured"])
 def test_serving_steps(hip, graph):
     """Prompt, drafted trees, single tokens and idle requests in turn; one graph captured once serves every step."""
