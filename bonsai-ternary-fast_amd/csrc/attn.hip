@@ -37,7 +37,7 @@
 // us, 5.8 TB/s), by the chain of reads when it is short (one token over 4097: 14 us,
 // find 1.1, pages and first block 3.4, products 1.8, the waves' join 1.5, the pieces'
 // join 3.7). More rows, attn_tile_kernel below: bound by the issue of matrix and vector
-// instructions (64-row trees of 8 requests 182 us, matrix units 46 % busy and vector
+// instructions (64-row trees of 8 requests 175-182 us, matrix units 46 % busy and vector
 // 43 %; 2048 rows of heads of 256 over 8191 keys 482-493 us: 4.5e11 operations with
 // both parts of P, 0.97 PFLOP/s, 46 % and 30 %). The join of the pieces takes 5 to 28
 // us of these: without pieces 512 tiles of unlike length end one after another.
@@ -60,6 +60,12 @@ constexpr int kKeys = 32;      // keys of a block
 constexpr int kStep = kWaves * kKeys;
 // Items that a launch is cut into, for tiles of R rows.
 constexpr int target(int R) { return R <= 32 ? 1536 : 1024; }
+// Of launches with less work, pieces of up to `least` keys where that leaves one for each of the 512 workgroups that the
+// card holds at once: a tile of many rows costs more to begin, leave and join than a few blocks of keys (694 rows of 24
+// heads of 256 behind 157 tokens 57 us in pieces of 128 keys, 47 so; trees of up to 57 nodes of three requests over 6000
+// keys 63 and 48, of 49 nodes of five requests, heads of 64, 26 and 27). Few rows: the smallest pieces.
+constexpr int least(int R) { return R <= 32 ? kStep : 512; }
+constexpr int kPlaces = 512;
 
 template <bool BF>
 __device__ __forceinline__ float from16(uint16_t h) {
@@ -157,7 +163,9 @@ __device__ bool find(const btf_paged_attention& a, const btf_kv_cache& kv, int i
     if (n > 0) work += (float)((n * G + R - 1) / R) * (float)len;
   }
   work = wave_sum_f(work) * (float)kv.heads;
-  const int C = max(kStep, __builtin_amdgcn_readfirstlane((int)(work / (float)(target(R) * kStep) + 1.f)) * kStep);
+  work /= (float)kStep;  // (in the smallest pieces)
+  const int C = kStep * __builtin_amdgcn_readfirstlane(
+                            max((int)(work / (float)target(R) + 1.f), min(least(R) / kStep, (int)(work / (float)kPlaces + 1.f))));
   int items = 0, slots = 0;  // before the chunk
   for (int s0 = 0; s0 < a.S; s0 += 64) {
     if (a.S > 64) read(s0 + lane, r0, n, len, full);  // (up to 64 requests are still there)
