@@ -530,7 +530,6 @@ __device__ __forceinline__ int fresh_tid() {
   return t;
 }
 
-constexpr int tile_R(int D) { return D == 256 ? 64 : 128; }
 // The launch's arguments, read again: what only the end needs is not kept in scalar registers over the loop.
 struct Args {
   btf_paged_attention a;
@@ -545,12 +544,12 @@ __device__ __forceinline__ Args fresh_args() {
   return g;
 }
 
-template <int D, bool BF>
+template <int D, bool BF, int RT>
 __global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2)))
     attn_tile_kernel(Args args) {
   const btf_paged_attention& a = args.a;
   const btf_kv_cache& kv = args.kv;
-  constexpr int NW = kWaves, R = tile_R(D), RW = R / NW, RT = RW / 16;
+  constexpr int NW = kWaves, RW = 16 * RT, R = NW * RW;
   constexpr int KS = D / 32;
   constexpr int DT = D / 16;            // dim tiles of the values
   constexpr int DB = 4, KB = 2;         // ... read at a time, and steps of K
@@ -854,10 +853,12 @@ __global__ void __launch_bounds__(64 * kJoinWaves) attn_join_kernel(btf_paged_at
 }
 
 // Rows of an item's tile, by the rows that a request has on average for a KV head. (32 rows of heads of 256 do not
-// fit a wave's registers with K and V there too.)
+// fit a wave's registers with K and V there too, nor do two tiles of 16 a wave in attn_tile_kernel.)
 int tile_rows(int S, int T, int heads, const btf_kv_cache& kv) {
   const int64_t rows = (int64_t)T * (heads / kv.heads);
-  return rows <= 16 * (int64_t)S ? 16 : rows <= 32 * (int64_t)S && kv.dim < 256 ? 32 : tile_R(kv.dim);
+  if (rows <= 16 * (int64_t)S) return 16;
+  if (kv.dim == 256) return 64;
+  return rows <= 32 * (int64_t)S ? 32 : rows <= 64 * (int64_t)S ? 64 : 128;
 }
 
 template <int D, bool BF>
@@ -867,26 +868,33 @@ int attn_go(const btf_paged_attention& a, const btf_kv_cache& kv, hipStream_t st
   // items: one for each tile and target(R) more, or all the pieces that the table has room for
   const int64_t room = ((int64_t)a.ldt * kv.page + kStep - 1) / kStep, most = tiles * kv.heads;
   const dim3 grid((unsigned)(most * room < most + target(R) ? most * room : most + target(R))), blk(64 * kWaves);
-  if (R == 16) hipLaunchKernelGGL((attn_stream_kernel<D, BF, 1>), grid, blk, 0, st, a, kv);
-  else if constexpr (D < 256) {
-    if (R == 32) hipLaunchKernelGGL((attn_stream_kernel<D, BF, 2>), grid, blk, 0, st, a, kv);
-  }
-  if (R == tile_R(D)) hipLaunchKernelGGL((attn_tile_kernel<D, BF>), grid, dim3(64 * kWaves), 0, st, Args{a, kv});
-  const int rc = launch_status("attn kernel");
-  if (rc != BTF_OK) return rc;
-  // one wave a row from 2048 rows of heads on
+  // one wave a row of the join from 2048 rows of heads on
   const bool one = (int64_t)a.T * a.heads >= 2048;
-  const dim3 join(a.T, one ? (a.heads + kJoinWaves - 1) / kJoinWaves : a.heads), jblk(64 * kJoinWaves);
-  auto go = [&](auto few, auto many) {
-    if (one) hipLaunchKernelGGL(many, join, jblk, 0, st, a, kv);
-    else hipLaunchKernelGGL(few, join, jblk, 0, st, a, kv);
+  const dim3 join(a.T, one ? (a.heads + kJoinWaves - 1) / kJoinWaves : a.heads);
+  int rc = BTF_OK;
+  auto joined = [&](auto few, auto many) {
+    rc = launch_status("attn kernel");
+    if (rc != BTF_OK) return;
+    if (one) hipLaunchKernelGGL(many, join, dim3(64 * kJoinWaves), 0, st, a, kv);
+    else hipLaunchKernelGGL(few, join, dim3(64 * kJoinWaves), 0, st, a, kv);
+    rc = launch_status("attn_join_kernel");
   };
-  if (R == 16) go(attn_join_kernel<D, 16, false>, attn_join_kernel<D, 16, true>);
-  else if constexpr (D < 256) {
-    if (R == 32) go(attn_join_kernel<D, 32, false>, attn_join_kernel<D, 32, true>);
+  if (R == 16) {
+    hipLaunchKernelGGL((attn_stream_kernel<D, BF, 1>), grid, blk, 0, st, a, kv);
+    joined(attn_join_kernel<D, 16, false>, attn_join_kernel<D, 16, true>);
+  } else if (R == 64) {
+    hipLaunchKernelGGL((attn_tile_kernel<D, BF, 1>), grid, blk, 0, st, Args{a, kv});
+    joined(attn_join_kernel<D, 64, false>, attn_join_kernel<D, 64, true>);
+  } else if constexpr (D < 256) {
+    if (R == 32) {
+      hipLaunchKernelGGL((attn_stream_kernel<D, BF, 2>), grid, blk, 0, st, a, kv);
+      joined(attn_join_kernel<D, 32, false>, attn_join_kernel<D, 32, true>);
+    } else {
+      hipLaunchKernelGGL((attn_tile_kernel<D, BF, 2>), grid, blk, 0, st, Args{a, kv});
+      joined(attn_join_kernel<D, 128, false>, attn_join_kernel<D, 128, true>);
+    }
   }
-  if (R == tile_R(D)) go(attn_join_kernel<D, tile_R(D), false>, attn_join_kernel<D, tile_R(D), true>);
-  return launch_status("attn_join_kernel");
+  return rc;
 }
 
 }  // namespace
