@@ -495,7 +495,7 @@ __global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_e
 }
 
 // ---- many rows: K and V through LDS ----
-// A workgroup's 4 waves have 32 rows each (two MFMA tiles, which share every operand
+// A workgroup's 4 waves have 16 or 32 rows each (RT MFMA tiles, which share every operand
 // of K and V; one for heads of 256, whose sums take twice the registers) and walk the
 // same keys, 32 at a time, from two buffers in LDS: the next block is on its way to
 // one while the other is worked on. K's rows lie in the order of the score tiles'
@@ -853,12 +853,17 @@ __global__ void __launch_bounds__(64 * kJoinWaves) attn_join_kernel(btf_paged_at
 }
 
 // Rows of an item's tile, by the rows that a request has on average for a KV head. (32 rows of heads of 256 do not
-// fit a wave's registers with K and V there too, nor do two tiles of 16 a wave in attn_tile_kernel.)
+// fit a wave's registers with K and V there too, nor do two tiles of 16 a wave in attn_tile_kernel.) 128 rows read K and V
+// half as often as 64, which leave room for three workgroups a CU instead of two and half the work in an item: heads of
+// 64 gain by 64 rows throughout (2000 rows over 6000 keys, 16 heads, 131 us in tiles of 128, 119 in tiles of 64), heads
+// of 128 up to two such tiles (120 rows over 4000 keys 31 and 25, over 16000 143 and 149; 200 rows over 6000 45 and 52,
+// 512 over 16500 276 and 350).
 int tile_rows(int S, int T, int heads, const btf_kv_cache& kv) {
   const int64_t rows = (int64_t)T * (heads / kv.heads);
   if (rows <= 16 * (int64_t)S) return 16;
   if (kv.dim == 256) return 64;
-  return rows <= 32 * (int64_t)S ? 32 : rows <= 64 * (int64_t)S ? 64 : 128;
+  if (rows <= 32 * (int64_t)S) return 32;
+  return kv.dim == 64 || rows <= 128 * (int64_t)S ? 64 : 128;
 }
 
 template <int D, bool BF>
@@ -889,7 +894,7 @@ int attn_go(const btf_paged_attention& a, const btf_kv_cache& kv, hipStream_t st
     if (R == 32) {
       hipLaunchKernelGGL((attn_stream_kernel<D, BF, 2>), grid, blk, 0, st, a, kv);
       joined(attn_join_kernel<D, 32, false>, attn_join_kernel<D, 32, true>);
-    } else {
+    } else if constexpr (D == 128) {
       hipLaunchKernelGGL((attn_tile_kernel<D, BF, 2>), grid, blk, 0, st, Args{a, kv});
       joined(attn_join_kernel<D, 128, false>, attn_join_kernel<D, 128, true>);
     }
