@@ -37,10 +37,10 @@
 // us, 5.8 TB/s), by the chain of reads when it is short (one token over 4097: 14 us,
 // find 1.1, pages and first block 3.4, products 1.8, the waves' join 1.5, the pieces'
 // join 3.7). More rows, attn_tile_kernel below: bound by the issue of matrix and vector
-// instructions (64-row trees of 8 requests 175-182 us, matrix units 46 % busy and vector
-// 43 %; 2048 rows of heads of 256 over 8191 keys 482-493 us: 4.5e11 operations with
-// both parts of P, 0.97 PFLOP/s, 46 % and 30 %). The join of the pieces takes 5 to 28
-// us of these: without pieces 512 tiles of unlike length end one after another.
+// instructions (trees of up to 64 nodes of 8 requests 175 us, matrix units 46 % busy and
+// vector 43 %; 2048 rows of heads of 256 over 8191 keys 481-493 us: 4.5e11 operations
+// with both parts of P, 0.97 PFLOP/s, 46 % and 30 %). The join of the pieces takes 5 to
+// 28 us of these: without pieces 512 tiles of unlike length end one after another.
 #include <string>
 
 #include "../../include/btf/hip_abi.h"
@@ -63,8 +63,10 @@ constexpr int target(int R) { return R <= 32 ? 1536 : 1024; }
 // Of launches with less work, pieces of up to `least` keys where that leaves one for each of the 512 workgroups that the
 // card holds at once: a tile of many rows costs more to begin, leave and join than a few blocks of keys (694 rows of 24
 // heads of 256 behind 157 tokens 57 us in pieces of 128 keys, 47 so; trees of up to 57 nodes of three requests over 6000
-// keys 63 and 48, of 49 nodes of five requests, heads of 64, 26 and 27). Few rows: the smallest pieces.
-constexpr int least(int R) { return R <= 32 ? kStep : 512; }
+// keys 63 and 48, of 49 nodes of five requests, heads of 64, 26 and 27; 25 rows of one request over 16000 keys, 8 KV
+// heads of 128, 33 and 24). Up to 16 rows the smallest pieces (the smallest calls, 11.5 us, take 13 in pieces of 256 or
+// 512 keys).
+constexpr int least(int R) { return R <= 16 ? kStep : 512; }
 constexpr int kPlaces = 512;
 
 template <bool BF>
