@@ -604,7 +604,9 @@ def test_attention_infinities_in_a_long_cache(hip, new):
     assert torch.equal(out[new:], want[new:]) and torch.equal(out[:new, :640], want[:new, :640])
 
 
-@pytest.mark.parametrize("heads,S,new", [((20, 4, 256), 3, 1), ((10, 2, 128), 2, 33), ((4, 4, 64), 40, 1)], ids=str)
+@pytest.mark.parametrize("heads,S,new", [((20, 4, 256), 3, 1), ((10, 2, 128), 2, 33), ((4, 4, 64), 40, 1), ((10, 2, 128), 2, 11),
+                                         ((8, 8, 64), 3, 70), ((10, 2, 128), 3, 5), ((14, 2, 64), 2, 4), ((20, 4, 256), 2, 30)],
+                         ids=str)
 def test_attention_long_caches(hip, heads, S, new):
     """Lengths that are split over many workgroups, one request much longer than the others; against 64 bits on the
     GPU. The tolerance is the worst case of the 32-bit sums over the keys."""
