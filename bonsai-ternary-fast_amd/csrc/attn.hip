@@ -295,7 +295,8 @@ __device__ __forceinline__ u32x4 signed_q(u32x4 q, float scale) {
 }
 
 template <int D, bool BF, int RT>
-__global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(D < 256 ? 2 : 1))) attn_stream_kernel(btf_paged_attention a, btf_kv_cache kv) {
+__global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(D < 256 ? 2 : 1)))
+    attn_stream_kernel(btf_paged_attention a, btf_kv_cache kv) {
   constexpr int R = 16 * RT;             // rows of a tile
   constexpr int KS = D / 32;             // steps over the dims in Q K^T
   constexpr int VD = D < 128 ? D / 16 : 8;  // dims that a lane reads of a key of V
@@ -913,7 +914,7 @@ int64_t paged_attention_ws_bytes(int S, int T, int heads, const btf_kv_cache& kv
   return (int64_t)2 * target(R) * R * (kv.dim + 2) * 4;
 }
 
-int paged_attention(const btf_paged_attention& a, const btf_kv_cache& kv, hipStream_t st, const DevState& ds) {
+int paged_attention(const btf_paged_attention& a, const btf_kv_cache& kv, hipStream_t st) {
   const bool bf = kv.type == BTF_BF16;
   if (kv.dim == 64) return bf ? attn_go<64, true>(a, kv, st) : attn_go<64, false>(a, kv, st);
   if (kv.dim == 128) return bf ? attn_go<128, true>(a, kv, st) : attn_go<128, false>(a, kv, st);

@@ -247,8 +247,8 @@ int page_plan(const btf_page_plan& a, hipStream_t st);
 int rope_table(int n_rot, double base, const btf_rope_scale* sc, double* turns, float* mscale);  // host only
 int rope_cache(const btf_rope_cache& a, const btf_kv_cache& kv, bool vec, hipStream_t st);
 int64_t paged_attention_ws_bytes(int S, int T, int heads, const btf_kv_cache& kv);
-int paged_attention(const btf_paged_attention& a, const btf_kv_cache& kv, hipStream_t st, const DevState& ds);
+int paged_attention(const btf_paged_attention& a, const btf_kv_cache& kv, hipStream_t st);
 int64_t sample_ws_bytes(int M, int V);
-int sample(const btf_sampling& a, hipStream_t st, const DevState& ds);
+int sample(const btf_sampling& a, hipStream_t st);
 
 }  // namespace btfhip

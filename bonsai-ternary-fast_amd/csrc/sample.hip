@@ -931,7 +931,7 @@ __global__ void __launch_bounds__(kPickThreads) sample_pick_kernel(btf_sampling 
 
 int64_t sample_ws_bytes(int M, int V) { return (int64_t)M * scratch_bytes(V); }
 
-int sample(const btf_sampling& a, hipStream_t st, const DevState& ds) {
+int sample(const btf_sampling& a, hipStream_t st) {
   const Parts p = parts_of(a.M, a.V);
   for (int m0 = 0; m0 < a.M; m0 += 65535) {  // (rows are the grid's second dimension)
     btf_sampling b = a;

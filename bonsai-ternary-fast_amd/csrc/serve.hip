@@ -121,9 +121,8 @@ int btf_hip_launch_paged_attention(const btf_paged_attention* a, const btf_kv_ca
   if (!(a->scale == a->scale)) return bad("paged_attention", "scale is not a number");
   if (paged_attention_ws_bytes(a->S, a->T, a->heads, *kv) > 0 && (!a->ws || !aligned(a->ws, 16)))
     return bad("paged_attention", "ws must be 16-byte aligned scratch");
-  const DevState* ds = current_state();
-  if (!ds) return BTF_ERR_NOT_INIT;
-  return paged_attention(*a, *kv, static_cast<hipStream_t>(stream), *ds);
+  if (!current_state()) return BTF_ERR_NOT_INIT;
+  return paged_attention(*a, *kv, static_cast<hipStream_t>(stream));
 }
 
 int64_t btf_hip_sample_ws_bytes(int M, int V) { return M > 0 && V > 0 ? sample_ws_bytes(M, V) : 0; }
@@ -136,9 +135,8 @@ int btf_hip_launch_sample(const btf_sampling* a, btf_stream_t stream) {
   if (a->M > 1 && a->ldl < a->V) return bad("sample", "ldl < V");
   if (!a->logits || !a->u || !a->token) return bad("sample", "null pointer");
   if (sample_ws_bytes(a->M, a->V) > 0 && (!a->ws || !aligned(a->ws, 8))) return bad("sample", "ws must be 8-byte aligned scratch");
-  const DevState* ds = current_state();
-  if (!ds) return BTF_ERR_NOT_INIT;
-  return sample(*a, static_cast<hipStream_t>(stream), *ds);
+  if (!current_state()) return BTF_ERR_NOT_INIT;
+  return sample(*a, static_cast<hipStream_t>(stream));
 }
 
 }  // extern "C"
