@@ -24,7 +24,8 @@
 //
 // Probabilities are 32-bit; as MFMA takes 16-bit factors they are carried in
 // parts, p = hi + lo (+ lo2 for bf16), each the rounding of what the parts
-// before leave: 22 and 24 bits. One part would put 2^-12 or 2^-9 on fp32 output.
+// before leave: 22 and 24 bits (fp16: as far as its small end allows, see softmax_block).
+// One part would put 2^-11 or 2^-8 on fp32 output.
 //
 // What a row does not see takes no part, whatever it holds: masked scores become
 // -infinity, V of keys behind the end is cleared. Where V or a score is not
@@ -236,25 +237,48 @@ __device__ void plain_row(const btf_paged_attention& a, const btf_kv_cache& kv, 
 }
 
 // A block's scores s of the lane's row before their scale (tiles 0 and 1: keys 8 g ..
-// 8 g + 7): the running maximum m (in powers of two, as the scores times c2 > 0 are),
-// the lane's share of the sum, the values so far scaled to the new maximum, and the
-// probabilities in 16-bit parts. m follows the maximum only when that is more than
-// kLag above it, so that the values are rarely scaled: probabilities reach 2^kLag,
-// which changes nothing in their relative rounding.
-constexpr float kLag = 8.f;
+// 8 g + 7): the running base m (in powers of two, as the scores times c2 > 0 are), the
+// lane's share of the sum and the values so far scaled to the new base, and the
+// probabilities 2^(score - m) in 16-bit parts. The base follows the scores only when it
+// has to, so that the values are rarely scaled. Sums and values go with it: the joins
+// need not know where it is.
+// bf16: the running maximum, moved when it is more than kLag below. A part has the
+// exponents of 32 bits: a probability of any size has all of its bits.
+// fp16: a part ends at 2^-25, so the base stays near the block, not near the row's
+// maximum: else a key that takes nearly all of the weight leaves every later key a few
+// bits or none (one 11 above 690 others, its V 0: 1e-3 of the output was lost). It is a
+// whole number (scaling is exact) and moves when the block's largest probability leaves
+// [2^-kLow, 2^15]: up to make that 2^11, down to 2^7. A probability is then off by 2^-22
+// of itself or 2^-20 of the largest of its block's 32 keys. Blocks more than kFar below
+// the highest base are not followed, so sums stay below 2^71 times the number of keys.
+// It costs scaling, the more the wider a row's scores are spread (2048 rows over 8191
+// keys, heads of 256, queries and keys normal: 499 -> 504 us, with twice the spread 495
+// -> 510, with four times 485 -> 521, part of it the power of fewer zeros).
+constexpr float kLag = 8.f, kLow = 5.f, kFar = 48.f;
 template <bool BF, int PARTS, int N>
-__device__ __forceinline__ void softmax_block(const f32x4 (&s)[2], float c2, float& m, float& l, f32x4 (&o)[N],
+__device__ __forceinline__ void softmax_block(const f32x4 (&s)[2], float c2, float& m, float& high, float& l, f32x4 (&o)[N],
                                               u32x4 (&p)[PARTS]) {
   const float mx = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
                          fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
   const float mn = groups_max(mx) * c2;
-  if (__any(mn > m + kLag)) {
-    const float to = fmaxf(m, mn);
-    const float c = to == -INFINITY ? 1.f : fast_exp2(m - to);
+  auto rebase = [&](float to, float c) {
     l *= c;
 #pragma unroll
     for (int i = 0; i < N; ++i) o[i] *= c;
     m = to;
+  };
+  if (BF) {
+    if (__any(mn > m + kLag)) {
+      const float to = fmaxf(m, mn);
+      rebase(to, to == -INFINITY ? 1.f : fast_exp2(m - to));
+    }
+  } else if (__any(fabsf(mn - m - 0.5f * (15.f - kLow)) > 0.5f * (15.f + kLow))) {
+    const bool up = mn > m + 15.f, down = mn < m - kLow && mn > high - kFar;
+    if (__any(up | down)) {
+      const float to = up ? floorf(mn) - 11.f : down ? floorf(mn) - 7.f : m;
+      high = fmaxf(high, to);
+      rebase(to, to == m ? 1.f : fast_exp2(m - to));
+    }
   }
   const float base = m == -INFINITY ? 0.f : m;
   float x[8];
@@ -338,10 +362,10 @@ __global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_e
     for (int ks = 0; ks < KS; ++ks) qf[rt][ks] = live ? signed_q(*reinterpret_cast<const u32x4*>(x + 32 * ks), a.scale) : u32x4{0, 0, 0, 0};
   }
   f32x4 o[RT][VG * VD];
-  float m[RT], l[RT];
+  float m[RT], high[RT], l[RT];
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
-    m[rt] = -INFINITY, l[rt] = 0.f;
+    m[rt] = high[rt] = -INFINITY, l[rt] = 0.f;
 #pragma unroll
     for (int i = 0; i < VG * VD; ++i) o[rt][i] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
@@ -409,7 +433,7 @@ __global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_e
     // the running maximum and sum; probabilities in 16-bit parts, keys 8 g .. 8 g + 7
     u32x4 p[RT][PARTS];
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt) softmax_block<BF, PARTS>(s[rt], c2, m[rt], l[rt], o[rt], p[rt]);
+    for (int rt = 0; rt < RT; ++rt) softmax_block<BF, PARTS>(s[rt], c2, m[rt], high[rt], l[rt], o[rt], p[rt]);
     // O^T += V^T P^T: dim VD c16 + e of each lane group's eight keys
 #pragma unroll
     for (int i = 0; i < VG; ++i)
@@ -587,10 +611,10 @@ __global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_e
       qf[rt][ks] = live ? signed_q(*reinterpret_cast<const u32x4*>(x + 32 * ks), a.scale) : u32x4{0, 0, 0, 0};
   }
   f32x4 o[RT][DT];
-  float m[RT], l[RT];
+  float m[RT], high[RT], l[RT];
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
-    m[rt] = -INFINITY, l[rt] = 0.f;
+    m[rt] = high[rt] = -INFINITY, l[rt] = 0.f;
 #pragma unroll
     for (int i = 0; i < DT; ++i) o[rt][i] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
@@ -701,7 +725,7 @@ __global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_e
       }
     }
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt) softmax_block<BF, PARTS>(s[rt], c2, m[rt], l[rt], o[rt], p[rt]);
+    for (int rt = 0; rt < RT; ++rt) softmax_block<BF, PARTS>(s[rt], c2, m[rt], high[rt], l[rt], o[rt], p[rt]);
   };
   auto values = [&](int buf) {  // O^T += V^T P^T
     const char* bv = reinterpret_cast<const char*>(sh_v[buf]);

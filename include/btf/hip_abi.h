@@ -536,7 +536,9 @@ int btf_hip_launch_rope_cache(const btf_rope_cache* a, const btf_kv_cache* kv, b
  * whose id in table is not in [0, pages) are not seen. A row that sees nothing,
  * or nothing but scores of -infinity, gives zeros. What a row does not see has
  * no effect on it, infinities and NaN included. out is fp32, as launch_prep
- * takes it; products are of 16-bit values, everything else is in 32 bits.
+ * takes it; products are of 16-bit values, everything else is in 32 bits. The
+ * probabilities take part in their products in 16-bit parts: bf16 with 24 bits,
+ * fp16 with 22, or off by 2^-20 of the largest of the same 32 keys.
  * ws: paged_attention_ws_bytes of device scratch for the launch's S, T and
  * heads, 16-byte aligned, one for each stream that launches. It need not be
  * cleared. The bytes for S = 1 and the largest T serve every launch. */
