@@ -487,11 +487,12 @@ class Sampling:
 _call.bind(*[C.cast(f, C.c_void_p).value for f in (_launch_prep, _launch_gemv, _launch_gemv_ptq1_0, _launch_gemv_ex)],
            Q8Act, Hx, GemvSeg)
 _kv_layout, _plan_layout, _rope_layout, _attn_layout, _sample_layout = (
-    _call.layout(_cls, tuple((_f, {C.c_int: "i", C.c_int64: "q", C.c_float: "f", C.c_void_p: "p"}[_t],
-                              getattr(_c_struct, _n).offset)
-                             for _f, (_n, _t) in zip(_cls.__dataclass_fields__, _c_struct._fields_)), C.sizeof(_c_struct))
-    for _cls, _c_struct in ((KvCache, _KvCache), (PagePlan, _PagePlan), (RopeCache, _RopeCache),
-                            (PagedAttention, _PagedAttention), (Sampling, _Sampling)))
+    _call.layout(_slot, _cls, tuple((_f, {C.c_int: "i", C.c_int64: "q", C.c_float: "f", C.c_void_p: "p"}[_t],
+                                     getattr(_c_struct, _n).offset)
+                                    for _f, (_n, _t) in zip(_cls.__dataclass_fields__, _c_struct._fields_)),
+                 C.sizeof(_c_struct))
+    for _slot, (_cls, _c_struct) in enumerate(((KvCache, _KvCache), (PagePlan, _PagePlan), (RopeCache, _RopeCache),
+                                               (PagedAttention, _PagedAttention), (Sampling, _Sampling))))
 _addr_page_plan, _addr_rope_cache, _addr_paged_attention, _addr_sample = (
     C.cast(f, C.c_void_p).value for f in (_launch_page_plan, _launch_rope_cache, _launch_paged_attention, _launch_sample))
 

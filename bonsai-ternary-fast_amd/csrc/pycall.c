@@ -201,13 +201,15 @@ static int do_gemv_ex(PyObject* const* v, int* status) {
 }
 
 /* ---- launches that take one argument struct, or two (a serving step's operators) ----
- * layout(cls, fields, size) describes the C struct of a class of btf_hip.py:
- * fields = ((name, kind, offset), ...), kind i int, q int64, f float, p pointer. */
+ * layout(slot, cls, fields, size) describes the C struct of a class of btf_hip.py:
+ * fields = ((name, kind, offset), ...), kind i int, q int64, f float, p pointer. A slot
+ * is taken over by whoever describes it last (btf_hip.py executed again, under its own or
+ * another name): objects of the classes before then go the ctypes path. */
 #define MAX_LAYOUTS 8
 #define MAX_FIELDS 24
 #define MAX_STRUCT 256
 typedef struct {
-  PyObject* cls;
+  PyObject* cls; /* NULL: empty */
   Py_ssize_t n;
   struct {
     PyObject* name;
@@ -216,31 +218,46 @@ typedef struct {
   } f[MAX_FIELDS];
 } layout_t;
 static layout_t layouts[MAX_LAYOUTS];
-static int n_layouts;
+
+static void drop(layout_t* L) {
+  for (Py_ssize_t i = 0; i < L->n; ++i) Py_DECREF(L->f[i].name);
+  Py_XDECREF(L->cls);
+}
 
 static PyObject* py_layout(PyObject* self, PyObject* const* v, Py_ssize_t n) {
-  if (n != 3 || !PyTuple_CheckExact(v[1]) || PyTuple_GET_SIZE(v[1]) > MAX_FIELDS || PyLong_AsSsize_t(v[2]) > MAX_STRUCT ||
-      n_layouts == MAX_LAYOUTS) {
-    if (!PyErr_Occurred()) PyErr_SetString(PyExc_ValueError, "layout(cls, fields, size)");
+  layout_t L = {0};
+  Py_ssize_t slot = -1, size = -1;
+  if (n == 4 && PyLong_Check(v[0]) && PyTuple_CheckExact(v[2]) && PyLong_Check(v[3])) {
+    slot = PyLong_AsSsize_t(v[0]);
+    size = PyLong_AsSsize_t(v[3]);
+    if (PyErr_Occurred()) return NULL;
+  }
+  if (slot < 0 || slot >= MAX_LAYOUTS || size < 0 || size > MAX_STRUCT || PyTuple_GET_SIZE(v[2]) > MAX_FIELDS) {
+    PyErr_SetString(PyExc_ValueError, "layout(slot, cls, fields, size)");
     return NULL;
   }
-  layout_t* L = &layouts[n_layouts];
-  for (L->n = 0; L->n < PyTuple_GET_SIZE(v[1]); ++L->n) {
+  for (; L.n < PyTuple_GET_SIZE(v[2]); ++L.n) {
     const char *name, *kind;
     Py_ssize_t off;
-    if (!PyArg_ParseTuple(PyTuple_GET_ITEM(v[1], L->n), "ssn", &name, &kind, &off)) return NULL;
-    if (off < 0 || off + 8 > MAX_STRUCT) {
-      PyErr_SetString(PyExc_ValueError, "layout: offset");
-      return NULL;
-    }
-    L->f[L->n].name = PyUnicode_InternFromString(name);
-    if (!L->f[L->n].name) return NULL;
-    L->f[L->n].kind = kind[0];
-    L->f[L->n].offset = off;
+    PyObject* f = PyTuple_GET_ITEM(v[2], L.n);
+    if (!PyTuple_CheckExact(f) || !PyArg_ParseTuple(f, "ssn", &name, &kind, &off)) goto bad;
+    const Py_ssize_t bytes = kind[0] == 'i' || kind[0] == 'f' ? 4 : kind[0] == 'q' || kind[0] == 'p' ? 8 : 0;
+    if (!bytes || off < 0 || off > size - bytes) goto bad;
+    L.f[L.n].name = PyUnicode_InternFromString(name);
+    if (!L.f[L.n].name) goto bad;
+    L.f[L.n].kind = kind[0];
+    L.f[L.n].offset = off;
   }
-  Py_INCREF(v[0]);
-  L->cls = v[0];
-  return PyLong_FromLong(n_layouts++);
+  Py_INCREF(v[1]);
+  L.cls = v[1];
+  layout_t old = layouts[slot];
+  layouts[slot] = L;
+  drop(&old);
+  return PyLong_FromSsize_t(slot);
+bad:
+  if (!PyErr_Occurred()) PyErr_SetString(PyExc_ValueError, "layout: a field is (name, kind, offset) inside the struct");
+  drop(&L);
+  return NULL;
 }
 
 static int read_struct(PyObject* o, int which, char* to) {
@@ -279,7 +296,7 @@ static int do_launch(PyObject* const* v, int* status) {
   if (!f) return PyErr_Occurred() ? RAISED : OTHER;
   TRY(read_int(v[1], &la));
   TRY(read_int(v[3], &lb));
-  if (la < 0 || la >= n_layouts || lb < -1 || lb >= n_layouts) return OTHER;
+  if (la < 0 || la >= MAX_LAYOUTS || lb < -1 || lb >= MAX_LAYOUTS) return OTHER;
   TRY(read_struct(v[2], la, a));
   if (lb >= 0) TRY(read_struct(v[4], lb, b));
   TRY(read_stream(v[5], &st));

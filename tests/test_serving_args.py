@@ -235,3 +235,56 @@ def test_native_calls_leave_other_forms_to_ctypes():
     import ctypes
     with pytest.raises(ctypes.ArgumentError):
         h.launch_sample(PLAN)
+
+
+@pytest.mark.skipif(not os.path.exists(h.CALL_PATH), reason="native launch calls not built")
+@pytest.mark.parametrize("how", ["reload", "second name"])
+def test_module_executed_again(how):
+    """btf_hip executed twice in one process, by importlib.reload or under another name: launches of both go through, the
+    newer one's by the native calls, and as often as one likes."""
+    code = f"""
+import gc, importlib, importlib.util, sys
+sys.path.insert(0, {os.path.dirname(h.__file__)!r})
+import btf_hip
+first = btf_hip
+for i in range(9):
+    if {how == "reload"}:
+        old = first.Sampling(M=1, V=0)
+        new = importlib.reload(btf_hip)
+    else:
+        spec = importlib.util.spec_from_file_location("again%d" % i, btf_hip.__file__)
+        new = importlib.util.module_from_spec(spec)
+        sys.modules[spec.name] = new
+        spec.loader.exec_module(new)
+        old = first.Sampling(M=1, V=0)
+    gc.collect()
+    args = lambda m, a: (m._addr_sample, m._sample_layout, a, -1, None, None)
+    assert new._call.launch(*args(new, new.Sampling(M=1, V=0))) == {ARGS}
+    assert new._call.launch(*args(new, old)) is NotImplemented
+    for m in (first, new):
+        for call in (lambda: m.launch_sample(m.Sampling(M=1, V=0)), lambda: m.launch_rope_cache(m.RopeCache(T=1), None),
+                     lambda: m.launch_paged_attention(m.PagedAttention(S=1, T=1), m.KvCache()),
+                     lambda: m.launch_page_plan(m.PagePlan(S=1, T=-1))):
+            try:
+                call()
+            except RuntimeError:
+                continue
+            raise SystemExit("not refused")
+print("done")
+"""
+    r = subprocess.run([os.sys.executable, "-c", code], capture_output=True, text=True, timeout=120)
+    assert r.returncode == 0 and "done" in r.stdout, r.stderr[-2000:]
+
+
+@pytest.mark.skipif(not os.path.exists(h.CALL_PATH), reason="native launch calls not built")
+@pytest.mark.parametrize("args", [(), (0, h.Sampling, ()), (-1, h.Sampling, (), 8), (8, h.Sampling, (), 8), (0, h.Sampling, [], 8),
+                                  (0, h.Sampling, (), 257), (0, h.Sampling, (), -1), (5, h.Sampling, (("M", "i", 253),), 256),
+                                  (5, h.Sampling, (("M", "i", -8),), 8), (5, h.Sampling, (("M", "i"),), 8), (5, h.Sampling, ("M",), 8),
+                                  (5, h.Sampling, (("M", "", 0),), 8), (5, h.Sampling, (("M", "i", 0),) * 25, 8),
+                                  (2 ** 70, h.Sampling, (), 8)], ids=str)
+def test_layouts_refused(args):
+    """A refused registration changes nothing: the launches still read their structs, slot 5 is still empty."""
+    with pytest.raises((ValueError, TypeError, OverflowError)):
+        h._call.layout(*args)
+    assert h._call.launch(h._addr_sample, h._sample_layout, dataclasses.replace(SAMPLE, V=0), -1, None, None) == ARGS
+    assert h._call.launch(h._addr_sample, 5, SAMPLE, -1, None, None) is NotImplemented
