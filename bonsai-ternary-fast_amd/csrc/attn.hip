@@ -308,10 +308,12 @@ __device__ __forceinline__ void mask_block(f32x4 (&s)[2], int key0, int end, int
   }
 }
 
-// The scale of the scores in powers of two, as a positive number (the sign goes to Q;
-// a scale of zero becomes one that leaves every finite score at zero).
+// The scale of the scores in powers of two, as a positive number: the sign goes to Q, and
+// zero, with which a masked score's infinity would be NaN, becomes the smallest number
+// there is, 2^-149 (2^128 times that, the largest score, is 2^-21 away from zero: a
+// weight's relative error of 3e-7 at most).
 __device__ __forceinline__ float scale2(float scale) {
-  return fmaxf(fabsf(scale) * 1.4426950408889634f, 1.17549435e-38f);
+  return fmaxf(fabsf(scale) * 1.4426950408889634f, 1.40129846e-45f);
 }
 __device__ __forceinline__ u32x4 signed_q(u32x4 q, float scale) {
   const uint32_t f = scale < 0.f ? 0x80008000u : 0u;

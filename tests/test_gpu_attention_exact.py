@@ -124,3 +124,33 @@ def test_two_keys(hip, form, kind):
 def tree_of_nothing(n):
     """Rows that see none of the new ones: the cache alone."""
     return np.zeros(2 * n, np.uint64)
+
+
+@pytest.mark.parametrize("form", FORMS, ids=IDS)
+@pytest.mark.parametrize("scale", [0.0, -0.0, 1e-44, 3e-39, -3e-39, 1.17e-38])
+def test_scales_next_to_zero(hip, form, scale):
+    """bf16 scores of 2^126 times a scale below the smallest normal number, or of zero: weights that are equal for zero,
+    and as the formula has them else."""
+    import torch
+    heads, n = form
+    H, HK, D = heads
+    rng = np.random.default_rng(n)
+    q, k, v, table, row0, kv_len, page = case(rng, 2, n, 128, heads, "bf16", 0, 0)
+    q.zero_()
+    k.zero_()
+    q[:, ::D] = 2.0 ** 63
+    k[..., 0] = torch.from_numpy(rng.choice([-2.0 ** 63, 0.0, 2.0 ** 63], tuple(k.shape[:-1]))).cuda()
+    out = run_attn(hip, q, k, v, table, row0, kv_len, None, heads, "bf16", page, scale=scale).double().cpu().numpy()
+    s = float(np.float32(scale))
+    kk, vv = k.double().cpu().numpy(), v.double().cpu().numpy()
+    for r in range(2 * n):
+        t, L = table[r // n], 128 + r % n + 1
+        a, b = (np.moveaxis(c[t], 1, 0).reshape(HK, -1, D)[:, :L] for c in (kk, vv))
+        for h in range(H):
+            w = np.exp(2.0 ** 63 * a[h // (H // HK), :, 0] * s)
+            w /= w.sum()
+            want = w @ b[h // (H // HK)]
+            # The scale's product with log2 e is a multiple of 2^-149, as the smallest stand-in for zero is: scores up to
+            # 2^126 are off by up to 2^-23 times ln 2 each, the weights by twice that. Sums of 190 positive terms in
+            # three parts each, and the exponentials.
+            assert np.all(np.abs(out[r, h * D:(h + 1) * D] - want) <= want * (2 * 2.0 ** -23 + (3 * 190 + 40) * U))
