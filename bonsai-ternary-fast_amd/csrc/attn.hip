@@ -896,12 +896,16 @@ int tile_rows(int S, int T, int heads, const btf_kv_cache& kv) {
   return kv.dim == 64 || rows <= 128 * (int64_t)S ? 64 : 128;
 }
 
+// (request, KV head, row tile) of a launch, at most: a request's last tile may be a part of one.
+int64_t most_tiles(int S, int T, int heads, const btf_kv_cache& kv) {
+  return ((int64_t)T * (heads / kv.heads) / tile_rows(S, T, heads, kv) + S) * kv.heads;
+}
+
 template <int D, bool BF>
 int attn_go(const btf_paged_attention& a, const btf_kv_cache& kv, hipStream_t st) {
   const int R = tile_rows(a.S, a.T, a.heads, kv);
-  const int64_t tiles = (int64_t)a.T * (a.heads / kv.heads) / R + a.S;  // at most
   // items: one for each tile and target(R) more, or all the pieces that the table has room for
-  const int64_t room = ((int64_t)a.ldt * kv.page + kStep - 1) / kStep, most = tiles * kv.heads;
+  const int64_t room = ((int64_t)a.ldt * kv.page + kStep - 1) / kStep, most = most_tiles(a.S, a.T, a.heads, kv);
   const dim3 grid((unsigned)(most * room < most + target(R) ? most * room : most + target(R))), blk(64 * kWaves);
   // One wave a row of the join from 2048 rows of heads on: 20 of them, one token over 4097 keys, 17.6 us by one wave each
   // and 14.4 by four; 640 466.9 and 465.1; 13 thousand, trees of 8 requests, 180 and 197; 41 thousand 484 and 560.
@@ -934,6 +938,10 @@ int attn_go(const btf_paged_attention& a, const btf_kv_cache& kv, hipStream_t st
 }
 
 }  // namespace
+
+int64_t paged_attention_most_items(int S, int T, int heads, const btf_kv_cache& kv) {
+  return most_tiles(S, T, heads, kv) + target(tile_rows(S, T, heads, kv));
+}
 
 // Cut requests have at most 2 target(R) items: a piece of them holds at least C / 2 keys on average, and C is at least
 // all the work over target(R).

@@ -246,6 +246,7 @@ int pos_add(int* d_pos, int M, hipStream_t st);
 int page_plan(const btf_page_plan& a, hipStream_t st);
 int rope_table(int n_rot, double base, const btf_rope_scale* sc, double* turns, float* mscale);  // host only
 int rope_cache(const btf_rope_cache& a, const btf_kv_cache& kv, bool vec, hipStream_t st);
+int64_t paged_attention_most_items(int S, int T, int heads, const btf_kv_cache& kv);
 int64_t paged_attention_ws_bytes(int S, int T, int heads, const btf_kv_cache& kv);
 int paged_attention(const btf_paged_attention& a, const btf_kv_cache& kv, hipStream_t st);
 int64_t sample_ws_bytes(int M, int V);

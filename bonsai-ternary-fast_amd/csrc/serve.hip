@@ -12,6 +12,10 @@ namespace {
 
 bool aligned(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
 
+// A grid has at most 2^32 - 1 threads along x and 65535 workgroups along y.
+constexpr int kMaxGroups = (1 << 24) - 1;  // of 256 threads
+constexpr int kMaxY = 65535;
+
 int bad(const char* who, const char* what) { return fail(BTF_ERR_ARGS, std::string(who) + ": " + what); }
 
 int check_kv(const btf_kv_cache* kv, const char* who, bool need_data) {
@@ -48,6 +52,7 @@ int btf_hip_launch_page_plan(const btf_page_plan* a, btf_stream_t stream) {
     return bad("page_plan", "null pointer");
   if ((a->parent == nullptr) != (a->tree == nullptr)) return bad("page_plan", "parent and tree go together");
   if (!aligned(a->tree, 8)) return bad("page_plan", "tree must be 8-byte aligned");
+  if (a->S >= 1 << 26 || a->T > kMaxY * 1024) return bad("page_plan", "more requests or rows than a launch takes");
   if (!current_state()) return BTF_ERR_NOT_INIT;
   return page_plan(*a, static_cast<hipStream_t>(stream));
 }
@@ -87,6 +92,8 @@ int btf_hip_launch_rope_cache(const btf_rope_cache* a, const btf_kv_cache* kv, b
   if (a->n_rot && (!a->turns || !a->pos)) return bad("rope_cache", "null turns or pos");
   if (!aligned(a->turns, 8) || !aligned(a->q, 4) || !aligned(a->k, 4) || !aligned(a->v, 4) || !aligned(a->q_out, 2))
     return bad("rope_cache", "pointers must have their types' alignment");
+  if (a->T > kMaxGroups || (q ? a->heads : 0) + (k ? (int64_t)2 * kv->heads : 0) > kMaxY)
+    return bad("rope_cache", "more rows or heads than a launch takes");
   if (!current_state()) return BTF_ERR_NOT_INIT;
   // Vector accesses where every head's pairs start at a multiple of their size
   const bool pairs = a->layout == BTF_ROPE_PAIRS;
@@ -116,6 +123,8 @@ int btf_hip_launch_paged_attention(const btf_paged_attention* a, const btf_kv_ca
     return bad("paged_attention", "out must be 16-byte aligned with ldo % 4 == 0 and ldo >= heads * dim");
   if (a->heads > 65535 || (int64_t)a->T * a->heads > 0x7fffffff)
     return bad("paged_attention", "heads above 65535, or rows times heads above 2^31");
+  if (a->T > kMaxGroups || paged_attention_most_items(a->S, a->T, a->heads, *kv) > kMaxGroups)
+    return bad("paged_attention", "more rows or requests than a launch takes");
   if (a->ldt < 1) return bad("paged_attention", "ldt must be at least 1");
   if (!aligned(a->tree, 8)) return bad("paged_attention", "tree must be 8-byte aligned");
   if (!(a->scale == a->scale)) return bad("paged_attention", "scale is not a number");

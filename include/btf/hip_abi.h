@@ -458,7 +458,7 @@ typedef struct btf_kv_cache {
  *    its ancestors; a request of more than BTF_TREE_NODES rows is a prompt
  *    (pos = ctx[s] + i, tree 0). */
 typedef struct btf_page_plan {
-  int S, T;              /* requests, rows */
+  int S, T;              /* requests (below 2^26), rows (below 2^26 - 1023) */
   int page;              /* tokens of a page: a power of two */
   int ldt;               /* page ids that a row of table holds */
   int64_t pages;         /* pages of the cache */
@@ -508,7 +508,7 @@ int btf_hip_rope_table(int n_rot, double base, const btf_rope_scale* scale, doub
  * row0 + S gives them. */
 enum { BTF_ROPE_HALF = 0, BTF_ROPE_PAIRS = 1 };
 typedef struct btf_rope_cache {
-  int T, heads;         /* rows, Q heads */
+  int T, heads;         /* rows (below 2^24), Q heads (all heads together up to 65535) */
   const float* q;       /* [T][ldq] */
   int ldq;
   const float* k;       /* [T][ldk] */
@@ -543,7 +543,8 @@ int btf_hip_launch_rope_cache(const btf_rope_cache* a, const btf_kv_cache* kv, b
  * heads, 16-byte aligned, one for each stream that launches. It need not be
  * cleared. The bytes for S = 1 and the largest T serve every launch. */
 typedef struct btf_paged_attention {
-  int S, T, heads;       /* requests, rows, Q heads */
+  int S, T, heads;       /* requests, rows (below 2^24, T * heads below 2^31), Q heads (up to 65535);
+                            KV heads times (S and the row tiles) below 2^24 - 1536 */
   const void* q;         /* [T][ldq], 16 bits of kv->type, 16-byte aligned, ldq % 8 == 0 */
   int ldq;
   const int* table;      /* [S][ldt] */

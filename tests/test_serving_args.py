@@ -288,3 +288,25 @@ def test_layouts_refused(args):
         h._call.layout(*args)
     assert h._call.launch(h._addr_sample, h._sample_layout, dataclasses.replace(SAMPLE, V=0), -1, None, None) == ARGS
     assert h._call.launch(h._addr_sample, 5, SAMPLE, -1, None, None) is NotImplemented
+
+
+@pytest.mark.parametrize("op,change,kv", [
+    ("plan", dict(S=1 << 26), {}), ("plan", dict(S=2 ** 31 - 1), {}), ("plan", dict(T=65535 * 1024 + 1), {}),
+    ("plan", dict(T=2 ** 31 - 1), {}), ("rope", dict(T=1 << 24), {}), ("rope", dict(T=2 ** 31 - 1), {}),
+    ("rope", dict(heads=65528, ldq=2 ** 31 - 1, ldqo=2 ** 31 - 1), {}),
+    ("rope", dict(ldk=2 ** 31 - 1, ldv=2 ** 31 - 1), dict(heads=32768)),
+    ("attn", dict(T=1 << 24), {}), ("attn", dict(S=1 << 22), {}), ("attn", dict(S=1 << 26), {}),
+    ("attn", dict(S=2 ** 31 - 1, heads=65535, ldq=2 ** 31 - 8, ldo=2 ** 31 - 4), dict(heads=65535, dim=64, tok_stride=64)),
+    # 2^32 items and 1536: a grid that would wrap to 1536
+    ("attn", dict(S=1 << 26, T=1, heads=64, ldq=64 * 64, ldo=64 * 64), dict(heads=64, dim=64, tok_stride=64))], ids=str)
+def test_launches_beyond_the_grid_refused(op, change, kv):
+    """Before the first kernel, since a launch of several could otherwise stop after it, and a grid could wrap."""
+    assert launch(op, dataclasses.replace(VALID[op], **change), dataclasses.replace(KV, **kv)) == ARGS
+
+
+@pytest.mark.parametrize("op,change,kv", [
+    ("plan", dict(S=(1 << 26) - 1), {}), ("plan", dict(T=65535 * 1024), {}), ("rope", dict(T=(1 << 24) - 1), {}),
+    ("rope", dict(heads=65527, ldq=2 ** 31 - 1, ldqo=2 ** 31 - 1), {}), ("attn", dict(T=(1 << 24) - 1, S=1), {}),
+    ("attn", dict(S=4000000), {})], ids=str)
+def test_the_largest_launches(op, change, kv):
+    assert launch(op, dataclasses.replace(VALID[op], **change), dataclasses.replace(KV, **kv)) == NOT_INIT
