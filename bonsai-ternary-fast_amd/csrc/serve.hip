@@ -1,6 +1,7 @@
 // serve.hip -- the extern "C" boundary of a serving step's operators
 // (include/btf/hip_abi.h): host-side argument checks, as in abi.hip before any
 // HIP call.
+#include <cmath>
 #include <string>
 
 #include "../../include/btf/hip_abi.h"
@@ -60,14 +61,17 @@ int btf_hip_launch_page_plan(const btf_page_plan* a, btf_stream_t stream) {
 int btf_hip_rope_table(int n_rot, double base, const btf_rope_scale* sc, double* turns, float* mscale) {
   if (!turns || !mscale) return bad("rope_table", "null output");
   if (n_rot < 2 || n_rot % 2) return bad("rope_table", "n_rot must be even and positive");
-  if (!(base > 1.0)) return bad("rope_table", "base must be above 1");
+  if (!(base > 1.0) || std::isinf(base)) return bad("rope_table", "base must be above 1 and finite");
   if (sc && sc->kind != BTF_ROPE_NONE) {
     if (sc->kind != BTF_ROPE_LINEAR && sc->kind != BTF_ROPE_NTK && sc->kind != BTF_ROPE_YARN)
       return bad("rope_table", "unknown scaling");
-    if (!(sc->factor >= 1.0)) return bad("rope_table", "factor must be at least 1");
+    if (!(sc->factor >= 1.0) || std::isinf(sc->factor)) return bad("rope_table", "factor must be at least 1 and finite");
     if (sc->kind == BTF_ROPE_NTK && n_rot < 4) return bad("rope_table", "ntk needs n_rot > 2");
-    if (sc->kind == BTF_ROPE_YARN && !(sc->trained > 0.0 && sc->beta_slow > 0.0 && sc->beta_fast > sc->beta_slow))
-      return bad("rope_table", "yarn needs trained > 0 and beta_fast > beta_slow > 0");
+    if (sc->kind == BTF_ROPE_NTK && std::isinf(base * std::pow(sc->factor, (double)n_rot / (n_rot - 2))))
+      return bad("rope_table", "ntk makes the base infinite");
+    if (sc->kind == BTF_ROPE_YARN && !(sc->trained > 0.0 && std::isfinite(sc->trained) && sc->beta_slow > 0.0 &&
+                                       sc->beta_fast > sc->beta_slow && std::isfinite(sc->beta_fast)))
+      return bad("rope_table", "yarn needs finite trained > 0 and beta_fast > beta_slow > 0");
   }
   return rope_table(n_rot, base, sc, turns, mscale);
 }

@@ -491,7 +491,7 @@ int btf_hip_launch_page_plan(const btf_page_plan* a, btf_stream_t stream);
 enum { BTF_ROPE_NONE = 0, BTF_ROPE_LINEAR = 1, BTF_ROPE_NTK = 2, BTF_ROPE_YARN = 3 };
 typedef struct btf_rope_scale {
   int kind;
-  double factor;               /* >= 1 */
+  double factor;               /* >= 1, finite as all of these */
   double trained;              /* yarn: trained context */
   double beta_fast, beta_slow; /* yarn: 32 and 1 by custom */
 } btf_rope_scale;

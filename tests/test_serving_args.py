@@ -310,3 +310,23 @@ def test_launches_beyond_the_grid_refused(op, change, kv):
     ("attn", dict(S=4000000), {})], ids=str)
 def test_the_largest_launches(op, change, kv):
     assert launch(op, dataclasses.replace(VALID[op], **change), dataclasses.replace(KV, **kv)) == NOT_INIT
+
+
+@pytest.mark.parametrize("n_rot,base,scale", [
+    (64, math.inf, None), (64, 1e4, h.RopeScale(h.RopeScaling.linear, math.inf)), (64, 1e4, h.RopeScale(h.RopeScaling.ntk, math.inf)),
+    (64, 1e4, h.RopeScale(h.RopeScaling.ntk, 1e305)), (64, 1e4, h.RopeScale(h.RopeScaling.yarn, math.inf, 4096.0)),
+    (64, 1e4, h.RopeScale(h.RopeScaling.yarn, 2.0, math.inf)), (64, 1e4, h.RopeScale(h.RopeScaling.yarn, 2.0, 4096.0, math.inf)),
+    (64, 1e4, h.RopeScale(h.RopeScaling.yarn, 2.0, 4096.0, math.inf, math.inf)),
+    (64, 1e4, h.RopeScale(h.RopeScaling.yarn, 2.0, math.nan)), (64, 1e4, h.RopeScale(h.RopeScaling.yarn, 2.0, 4096.0, math.nan))],
+    ids=str)
+def test_rope_tables_of_infinite_numbers_refused(n_rot, base, scale):
+    """A base, a factor, a context or turns that are not finite (or a base that ntk makes so) would give frequencies of zero."""
+    with pytest.raises(RuntimeError, match="rope_table"):
+        h.rope_table(n_rot, base, scale)
+
+
+def test_rope_tables_of_large_numbers():
+    for scale in (None, h.RopeScale(h.RopeScaling.linear, 1e6), h.RopeScale(h.RopeScaling.ntk, 1e6),
+                  h.RopeScale(h.RopeScaling.yarn, 1e6, 1e9, 1e8, 1e-8), h.RopeScale(h.RopeScaling.none, math.inf)):
+        turns, m = h.rope_table(128, 1e30, scale)
+        assert all(0 < t < 0.16 for t in turns) and turns == sorted(turns, reverse=True) and 1 <= m < 3
