@@ -91,6 +91,8 @@ int btf_hip_launch_rope_cache(const btf_rope_cache* a, const btf_kv_cache* kv, b
   if (k && ((int64_t)a->ldk < (int64_t)kv->heads * D || (int64_t)a->ldv < (int64_t)kv->heads * D))
     return bad("rope_cache", "ldk or ldv below the heads' values");
   if (k && !a->slot) return bad("rope_cache", "k needs slots");
+  if (k && ((kv->heads > 1 && kv->head_stride < D) || (kv->pages > 1 && kv->page_stride < D)))
+    return bad("rope_cache", "heads or pages of the cache overlap");
   if (a->n_rot < 0 || a->n_rot > D || a->n_rot % 2) return bad("rope_cache", "n_rot must be even, in [0, dim]");
   if (a->layout != BTF_ROPE_HALF && a->layout != BTF_ROPE_PAIRS) return bad("rope_cache", "unknown layout");
   if (a->n_rot && (!a->turns || !a->pos)) return bad("rope_cache", "null turns or pos");

@@ -504,7 +504,8 @@ int btf_hip_rope_table(int n_rot, double base, const btf_rope_scale* scale, doub
  * BTF_ROPE_HALF turns the pairs (i, i + n_rot / 2), BTF_ROPE_PAIRS (2i, 2i + 1):
  * (a cos - b sin, a sin + b cos) * mscale, the angle pos * turns[i] turns.
  * q (with q_out) or k and v may be NULL: left out. A slot outside the cache
- * is not written; two rows with the same slot leave either's values there. rows (optional): the rows to do are min(*rows, T), as
+ * is not written; two rows with the same slot leave either's values there. Heads
+ * and pages of the cache that overlap (strides below dim) are refused. rows (optional): the rows to do are min(*rows, T), as
  * row0 + S gives them. */
 enum { BTF_ROPE_HALF = 0, BTF_ROPE_PAIRS = 1 };
 typedef struct btf_rope_cache {

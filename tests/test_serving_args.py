@@ -330,3 +330,14 @@ def test_rope_tables_of_large_numbers():
                   h.RopeScale(h.RopeScaling.yarn, 1e6, 1e9, 1e8, 1e-8), h.RopeScale(h.RopeScaling.none, math.inf)):
         turns, m = h.rope_table(128, 1e30, scale)
         assert all(0 < t < 0.16 for t in turns) and turns == sorted(turns, reverse=True) and 1 <= m < 3
+
+
+@pytest.mark.parametrize("change", [dict(head_stride=248), dict(head_stride=0), dict(page_stride=0), dict(page_stride=248)], ids=str)
+def test_rope_refuses_caches_whose_heads_or_pages_overlap(change):
+    """They would be written over one another; the attention may read them."""
+    assert launch("rope", ROPE, dataclasses.replace(KV, **change)) == ARGS
+    assert launch("attn", ATTN, dataclasses.replace(KV, **change)) == NOT_INIT
+    q_only = dataclasses.replace(ROPE, k=None, v=None)
+    assert launch("rope", q_only, dataclasses.replace(KV, **change)) == NOT_INIT
+    one = dataclasses.replace(KV, heads=1, pages=1, **change)
+    assert launch("rope", ROPE, one) == NOT_INIT
