@@ -154,3 +154,55 @@ def test_scales_next_to_zero(hip, form, scale):
             # 2^126 are off by up to 2^-23 times ln 2 each, the weights by twice that. Sums of 190 positive terms in
             # three parts each, and the exponentials.
             assert np.all(np.abs(out[r, h * D:(h + 1) * D] - want) <= want * (2 * 2.0 ** -23 + (3 * 190 + 40) * U))
+
+
+@pytest.mark.parametrize("heads,new,tree", [((20, 4, 256), [1, 1, 1], False), ((20, 4, 256), [20, 3, 31], True), ((10, 2, 256), [90, 1, 70], False),
+                                            ((8, 8, 128), [1, 1, 1], False), ((8, 2, 128), [6, 2, 8], True), ((8, 2, 128), [64, 9, 40], True),
+                                            ((10, 2, 128), [150, 64, 1], False), ((4, 2, 64), [1, 2, 1], True),
+                                            ((14, 2, 64), [4, 4, 3], False), ((8, 2, 64), [64, 33, 64], True)], ids=str)
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+def test_long_caches_in_which_each_row_looks_for_a_key(hip, heads, new, tree, kind):
+    """Caches of thousands of keys, cut into pieces and joined; each row and head's query is twice some key, before its
+    request's rows, among them or one that it must not see, so that a few keys carry its output wherever they lie."""
+    import torch
+    from test_gpu_serving import gpu_cache, trees
+    H, HK, D = heads
+    G, page = H // HK, 16
+    g = torch.Generator(device="cuda").manual_seed(sum(new))
+    rng = np.random.default_rng(sum(new))
+    ctx = [9011, 700, 2500]
+    kv_len = [c + n for c, n in zip(ctx, new)]
+    k, v, table = gpu_cache(g, kv_len, heads, page)
+    k, v = k.to(kind_of(kind)), v.to(kind_of(kind))
+    row0 = np.cumsum([0] + new)
+    bits = trees(rng, new, sum(new)) if tree else None
+    dense = []
+    for s, L in enumerate(kv_len):
+        ids = torch.from_numpy(table[s, :-(-L // page)]).cuda().long()
+        dense.append([c[ids].transpose(0, 1).reshape(HK, -1, D)[:, :L] for c in (k, v)])
+    q = torch.zeros((sum(new), H, D), dtype=kind_of(kind), device="cuda")
+    for s, L in enumerate(kv_len):
+        for r in range(int(row0[s]), int(row0[s + 1])):
+            at = torch.from_numpy(np.where(rng.random(H) < 0.5, rng.integers(0, L, H), rng.integers(ctx[s] - 40, L, H))).cuda()
+            q[r] = 2 * dense[s][0][torch.arange(H, device="cuda") // G, at]
+    q = q.reshape(-1, H * D)
+    out = run_attn(hip, q, k, v, table, row0, kv_len, bits, heads, kind, page).double()
+    for s, L in enumerate(kv_len):
+        a, b = int(row0[s]), int(row0[s + 1])
+        j = torch.arange(L, device="cuda")
+        i = torch.arange(b - a, device="cuda")[:, None]
+        seen = j - ctx[s] <= i
+        if tree:
+            own = torch.from_numpy(bits[a:b].view(np.int64)).cuda()[:, None] >> (j - ctx[s]).clamp(0, 63) & 1
+            seen = (j < ctx[s]) | (own == 1)
+        for h in range(H):
+            kk, vv = (c[h // G].double() for c in dense[s])
+            qq = q[a:b, h * D:(h + 1) * D].double()
+            x, size = qq @ kk.T * D ** -0.5, qq.abs() @ kk.abs().T * D ** -0.5
+            p = torch.softmax(x.masked_fill(~seen, -math.inf), -1)
+            # Scores: sums of D products, the scale and the exponent; the sums over the keys (pieces of at most 512 keys
+            # in three parts, 72 pieces joined); the parts; fp16's small end, 2^-20 of a block's largest for its 32 keys.
+            e = 2 * U * ((D + 8) * size.amax(-1, keepdim=True) + 8 * x.abs().amax(-1, keepdim=True)) + (3 * 512 + 200) * U + PARTS[kind]
+            tol = e * (p @ vv.abs()) + (32 * 2.0 ** -20 * vv.abs().max() if kind == "f16" else 0)
+            d = (out[a:b, h * D:(h + 1) * D] - p @ vv).abs() - tol
+            assert float(d.max()) <= 0, (s, h, float(d.max()))
