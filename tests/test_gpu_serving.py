@@ -748,6 +748,28 @@ def test_sample_the_largest_sum(hip):
     check_sample(hip, np.zeros((4, 1 << 20)), p=[1, 1, 0.999, 0.999], u=[0.99, 1 - 2.0 ** -24, 0.99, 1 - 2.0 ** -24])
 
 
+def test_sample_more_rows_than_a_grid_has(hip):
+    """66001 rows, in two launches of each kernel; settings by the row."""
+    rng = np.random.default_rng(18)
+    M, V = 66001, 7
+    x = (2 * rng.standard_normal((M, V))).astype(np.float32)
+    T, k = rng.choice([0.0, 0.7, 1.5], M).astype(np.float32), rng.choice([0, 1, 3], M).astype(np.int32)
+    p, mp = rng.choice([0.4, 0.9, 1.0], M).astype(np.float32), rng.choice([0.0, 0.2], M).astype(np.float32)
+    u = rng.random(M).astype(np.float32)
+    tok, lp = run_sample(hip, x, T, k, p, mp, u)
+    for m in list(range(0, M, 97)) + list(range(65500, 65580)) + [M - 1]:
+        want = ref.sample(x[m], T[m], k[m], p[m], mp[m], u[m])
+        assert tok[m] == want[0] and abs(lp[m] - want[1]) <= 2.0 ** -23 * abs(want[1]) + V * 2.0 ** -42 + 1e-7, (m, want)
+
+
+def test_sample_a_flat_row_beside_one_far_logit(hip):
+    """A finite logit far below the others makes the bins wide: more logits lie in the border's than candidates are held."""
+    rng = np.random.default_rng(19)
+    x = rng.standard_normal((3, 248320)).astype(np.float32)
+    x[:, 77] = -1e4
+    check_sample(hip, x, T=2.0, p=[0.7, 0.5, 0.7], k=[0, 0, 200000], u=[0.1, 0.5, 0.9])
+
+
 @pytest.mark.parametrize("k", [1, 2, 7, 8, 9, 500, 2000])
 def test_sample_sorted_and_clustered_logits(hip, k):
     """The largest logits all next to each other: the maxima of 128 say little, top-k has to be exact all the same."""
