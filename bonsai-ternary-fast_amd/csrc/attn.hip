@@ -30,7 +30,9 @@
 // What a row does not see takes no part, whatever it holds: masked scores become
 // -infinity, V of keys behind the end is cleared. Where V or a score is not
 // finite all the same (0 * infinity in a product), the item's result shows it,
-// and the item is done again one row at a time by the plain loop.
+// and the item (attn_tile_kernel: the wave's rows of it) is done again one row at a time
+// by the plain loop: right, and slow (one NaN in V that all rows see: one token over
+// 4097 keys 15 -> 150 us, 2048 rows over 8191 0.5 -> 130 ms).
 //
 // Which kernel: by the rows that a request has on average for a KV head (tile_rows).
 // Up to 16 or 32 (one new token, few heads more), attn_stream_kernel as above: bound
@@ -39,8 +41,8 @@
 // find 1.1, pages and first block 3.4, products 1.8, the waves' join 1.5, the pieces'
 // join 3.7). More rows, attn_tile_kernel below: bound by the issue of matrix and vector
 // instructions (trees of up to 64 nodes of 8 requests 175 us, matrix units 46 % busy and
-// vector 43 %; 2048 rows of heads of 256 over 8191 keys 481-493 us: 4.5e11 operations
-// with both parts of P, 0.97 PFLOP/s, 46 % and 30 %). The join of the pieces takes 5 to
+// vector 43 %; 2048 rows of heads of 256 over 8191 keys 490-508 us: 4.5e11 operations
+// with both parts of P, 0.91 PFLOP/s, 45 % and 30 %). The join of the pieces takes 5 to
 // 28 us of these: without pieces 512 tiles of unlike length end one after another.
 #include <string>
 
@@ -61,8 +63,9 @@ constexpr int kKeys = 32;      // keys of a block
 constexpr int kStep = kWaves * kKeys;
 // Items that a launch is cut into, for tiles of R rows.
 constexpr int target(int R) { return R <= 32 ? 1536 : 1024; }
-// Of launches with less work, pieces of up to `least` keys where that leaves one for each of the 512 workgroups that the
-// card holds at once: a tile of many rows costs more to begin, leave and join than a few blocks of keys (694 rows of 24
+// Of launches with less work, pieces of up to `least` keys where that leaves one for each of 512 workgroups, the two a CU
+// that every instance has room for (attn_tile_kernel with tiles of 64 rows has room for three at heads of 128, five at 64;
+// one number serves all): a tile of many rows costs more to begin, leave and join than a few blocks of keys (694 rows of 24
 // heads of 256 behind 157 tokens 57 us in pieces of 128 keys, 47 so; trees of up to 57 nodes of three requests over 6000
 // keys 63 and 48, of 49 nodes of five requests, heads of 64, 26 and 27; 25 rows of one request over 16000 keys, 8 KV
 // heads of 128, 33 and 24). Up to 16 rows the smallest pieces (the smallest calls, 11.5 us, take 13 in pieces of 256 or
@@ -294,8 +297,10 @@ __device__ __forceinline__ void softmax_block(const f32x4 (&s)[2], float c2, flo
 }
 
 // Scores of keys key0 .. key0 + 7 that the row (new token tok, -1: none) does not see become -infinity; there are keys
-// up to end. A tree's row sees its bits of the new tokens, another's those up to its own. (All by selects: the lanes
-// differ in everything here, and a branch for each of 16 scores costs more than the arithmetic.)
+// up to end. A tree's row sees its bits of the new tokens, another's those up to its own. All by selects: the lanes
+// differ in everything here, and a branch for each of 16 scores costs more than the arithmetic. A form with branches has
+// also been seen to lose the causal mask in one build (the tests of prompts failed; the cause was not found): keep the
+// selects.
 __device__ __forceinline__ void mask_block(f32x4 (&s)[2], int key0, int end, int ctx, bool tree, int tok,
                                            unsigned long long bits) {
   const int upto = tree ? ctx - 1 : ctx + tok, nj = key0 - ctx;
@@ -887,7 +892,9 @@ __global__ void __launch_bounds__(64 * kJoinWaves) attn_join_kernel(btf_paged_at
 // 64 gain by 64 rows throughout (2000 rows over 6000 keys, 16 heads, 131 us in tiles of 128, 119 in tiles of 64), heads
 // of 128 up to two such tiles (120 rows over 4000 keys 31 and 25, over 16000 143 and 149; 200 over 6000 45 and 52, 2560
 // over 16500 276 and 350). Up to 32 rows attn_stream_kernel: 30 rows of 32 requests over up to 32768 keys 489, in tiles of
-// 64 rows 545.
+// 64 rows 545. Rows are those of the launch: one prompt piece beside many single tokens puts
+// these into its tiles, too (512 rows behind 2048 tokens and 31 single tokens over 7000 to 16000 keys, 20 / 4 heads of 256:
+// 323 us, 71 + 282 apart; 2048 rows, 40 / 8 heads of 128: 619, 267 + 289 apart).
 int tile_rows(int S, int T, int heads, const btf_kv_cache& kv) {
   const int64_t rows = (int64_t)T * (heads / kv.heads);
   if (rows <= 16 * (int64_t)S) return 16;

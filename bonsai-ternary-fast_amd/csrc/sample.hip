@@ -19,13 +19,15 @@
 //  * border: below those bins everything stays: its weights are summed for every 256
 //    logits. What lies in them is written out, logit and index, as candidates;
 //  * pick: one workgroup per row puts the candidates in order (a bin of a row of 248320
-//    normal logits holds 1500 of them at most), finds the borders exactly, adds
+//    normal logits spread over less than 32 temperatures holds 1500 at most), finds the borders exactly, adds
 //    what stays to its 256 logits, and walks those in which the sum passes u.
-// A row whose border bins hold more than kCand logits (many equal ones) is done by
-// that workgroup alone, eight key bits at a time.
+// A row whose border bins hold more than kCand logits (many equal ones, or a
+// flat row beside one logit far below, which makes the bins 1/32 of the temperature wide)
+// is done by that workgroup alone, eight key bits at a time: right, and slow (248320
+// normal logits at temperature 2, one of -10^4, top-p 0.7: 1.0 ms instead of 30 us).
 //
 // What bounds it: one row waits, for four launches and the chain of reads in each (248320
-// logits: 26 us; top 3.6, hist 8.4, border 4.3, pick 6.3). Many rows read the logits three
+// logits: 19 to 25 us a call; on the GPU top 3.6, hist 8.4, border 4.3, pick 6.3). Many rows read the logits three
 // times, 10 us a pass for 48 rows of 248320 at the copy rate, and where there is no top-k work
 // out every logit's weight in each of two (36 vector instructions): 59 us (top 12.3, hist 20.9,
 // border 14.5, pick 9.2).

@@ -505,8 +505,8 @@ int btf_hip_rope_table(int n_rot, double base, const btf_rope_scale* scale, doub
  * (a cos - b sin, a sin + b cos) * mscale, the angle pos * turns[i] turns.
  * q (with q_out) or k and v may be NULL: left out. A slot outside the cache
  * is not written; two rows with the same slot leave either's values there. Heads
- * and pages of the cache that overlap (strides below dim) are refused. rows (optional): the rows to do are min(*rows, T), as
- * row0 + S gives them. */
+ * and pages of the cache that overlap (strides below dim) are refused. rows
+ * (optional): the rows to do are min(*rows, T), as row0 + S gives them. */
 enum { BTF_ROPE_HALF = 0, BTF_ROPE_PAIRS = 1 };
 typedef struct btf_rope_cache {
   int T, heads;         /* rows (below 2^24), Q heads (all heads together up to 65535) */
@@ -542,7 +542,10 @@ int btf_hip_launch_rope_cache(const btf_rope_cache* a, const btf_kv_cache* kv, b
  * fp16 with 22, or off by 2^-20 of the largest of the same 32 keys.
  * ws: paged_attention_ws_bytes of device scratch for the launch's S, T and
  * heads, 16-byte aligned, one for each stream that launches. It need not be
- * cleared. The bytes for S = 1 and the largest T serve every launch. */
+ * cleared. The bytes for S = 1 and the largest T serve every launch: 13 MB (few
+ * rows, heads of 64) to 137 MB (prompts, heads of 128 or 256), whatever the lengths.
+ * The kernel's tiles follow T / S: a launch of one prompt piece and many single
+ * tokens, or of many spare rows, takes the prompt's. */
 typedef struct btf_paged_attention {
   int S, T, heads;       /* requests, rows (below 2^24, T * heads below 2^31), Q heads (up to 65535);
                             KV heads times (S and the row tiles) below 2^24 - 1536 */
