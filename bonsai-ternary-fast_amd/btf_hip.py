@@ -40,7 +40,7 @@ else:
     class _call:
         """No native calls: every launch takes the ctypes path."""
         prep = gemv = gemv_ptq1_0 = gemv_ex = staticmethod(lambda *args: NotImplemented)
-        launch = staticmethod(lambda *args: NotImplemented)
+        launch = launch_list = staticmethod(lambda *args: NotImplemented)
         bind = layout = staticmethod(lambda *args: None)
 
 BTF_OK, BTF_ERR_ARGS, BTF_ERR_DEVICE, BTF_ERR_LAUNCH, BTF_ERR_NOT_INIT = 0, 1, 2, 3, 4
@@ -127,6 +127,48 @@ class _Sampling(C.Structure):
                 ("u", C.c_void_p), ("token", C.c_void_p), ("logprob", C.c_void_p), ("ws", C.c_void_p)]
 
 
+class _PageFork(C.Structure):
+    _fields_ = [("F", C.c_int), ("S", C.c_int), ("page", C.c_int), ("ldt", C.c_int), ("pages", C.c_int64),
+                ("src", C.c_void_p), ("dst", C.c_void_p), ("tokens", C.c_void_p), ("free_list", C.c_void_p),
+                ("n_free", C.c_void_p), ("table", C.c_void_p), ("held", C.c_void_p), ("shared", C.c_void_p),
+                ("got", C.c_void_p), ("copy_from", C.c_void_p), ("copy_to", C.c_void_p), ("copy_tokens", C.c_void_p)]
+
+
+class _PageCopy(C.Structure):
+    _fields_ = [("n", C.c_int), ("from_", C.c_void_p), ("to", C.c_void_p), ("tokens", C.c_void_p), ("layers", C.c_int),
+                ("layer_stride", C.c_int64)]
+
+
+class _PageFree(C.Structure):
+    _fields_ = [("S", C.c_int), ("page", C.c_int), ("ldt", C.c_int), ("pages", C.c_int64), ("keep", C.c_void_p),
+                ("table", C.c_void_p), ("held", C.c_void_p), ("shared", C.c_void_p), ("free_list", C.c_void_p),
+                ("n_free", C.c_void_p), ("ws", C.c_void_p)]
+
+
+class _CacheMove(C.Structure):
+    _fields_ = [("S", C.c_int), ("T", C.c_int), ("table", C.c_void_p), ("ldt", C.c_int), ("to_table", C.c_void_p),
+                ("ldt_to", C.c_int), ("first", C.c_void_p), ("tree", C.c_void_p), ("leaf", C.c_void_p),
+                ("source", C.c_void_p), ("source0", C.c_void_p), ("kv_len", C.c_void_p), ("layers", C.c_int),
+                ("layer_stride", C.c_int64)]
+
+
+class _SharedAttention(C.Structure):
+    _fields_ = _PagedAttention._fields_ + [("groups", C.c_int), ("group0", C.c_void_p), ("lead", C.c_void_p),
+                                           ("shared", C.c_void_p)]
+
+
+class _LoraSeg(C.Structure):
+    _fields_ = [("a", C.c_void_p), ("b", C.c_void_p), ("a_stride", C.c_int64), ("b_stride", C.c_int64), ("N", C.c_int),
+                ("y", C.c_void_p), ("ldy", C.c_int)]
+
+
+class _Lora(C.Structure):
+    _fields_ = [("S", C.c_int), ("T", C.c_int), ("K", C.c_int), ("rank", C.c_int), ("adapters", C.c_int),
+                ("type", C.c_int), ("mode", C.c_int), ("row0", C.c_void_p), ("adapter", C.c_void_p),
+                ("ranks", C.c_void_p), ("scale", C.c_void_p), ("x", C.c_void_p), ("ldx", C.c_int), ("out", C.c_void_p),
+                ("ldo", C.c_int), ("ws", C.c_void_p)]
+
+
 class _GgufHeader(C.Structure):
     _fields_ = [("version", C.c_uint32), ("alignment", C.c_uint64), ("data_offset", C.c_uint64),
                 ("file_bytes", C.c_uint64), ("n_tensors", C.c_int64), ("n_kv", C.c_int64)]
@@ -175,6 +217,16 @@ _launch_paged_attention = _decl("btf_hip_launch_paged_attention",
                                 [C.POINTER(_PagedAttention), C.POINTER(_KvCache), _vp])
 _sample_ws_bytes = _decl("btf_hip_sample_ws_bytes", [_i, _i], _i64)
 _launch_sample = _decl("btf_hip_launch_sample", [C.POINTER(_Sampling), _vp])
+_launch_page_fork = _decl("btf_hip_launch_page_fork", [C.POINTER(_PageFork), _vp])
+_launch_page_copy = _decl("btf_hip_launch_page_copy", [C.POINTER(_PageCopy), C.POINTER(_KvCache), _vp])
+_page_free_ws_bytes = _decl("btf_hip_page_free_ws_bytes", [_i, _i], _i64)
+_launch_page_free = _decl("btf_hip_launch_page_free", [C.POINTER(_PageFree), _vp])
+_launch_cache_move = _decl("btf_hip_launch_cache_move", [C.POINTER(_CacheMove), C.POINTER(_KvCache), _vp])
+_shared_attention_ws_bytes = _decl("btf_hip_shared_attention_ws_bytes", [_i, _i, _i, C.POINTER(_KvCache)], _i64)
+_launch_shared_attention = _decl("btf_hip_launch_shared_attention",
+                                 [C.POINTER(_SharedAttention), C.POINTER(_KvCache), _vp])
+_lora_ws_bytes = _decl("btf_hip_lora_ws_bytes", [_i, _i, _i, _i, _i], _i64)
+_launch_lora = _decl("btf_hip_launch_lora", [C.POINTER(_Lora), C.POINTER(_LoraSeg), _i, _vp])
 _launch_gemv_ex = _decl("btf_hip_launch_gemv_ex", [C.POINTER(_GemvSeg), _i, _i, _i, C.POINTER(_Q8Act), _vp, _i, _i,
                                                     C.POINTER(_Q8Act), _vp])
 _launch_gemv_ptq1_0 = _decl("btf_hip_launch_gemv_ptq1_0",
@@ -245,6 +297,9 @@ ABI_SYMBOLS = (
     "btf_hip_launch_page_plan", "btf_hip_rope_table", "btf_hip_launch_rope_cache",
     "btf_hip_paged_attention_ws_bytes", "btf_hip_launch_paged_attention", "btf_hip_sample_ws_bytes",
     "btf_hip_launch_sample",
+    "btf_hip_launch_page_fork", "btf_hip_launch_page_copy", "btf_hip_page_free_ws_bytes", "btf_hip_launch_page_free",
+    "btf_hip_launch_cache_move", "btf_hip_shared_attention_ws_bytes", "btf_hip_launch_shared_attention",
+    "btf_hip_lora_ws_bytes", "btf_hip_launch_lora",
 )
 
 
@@ -482,19 +537,161 @@ class Sampling:
         return _struct(self, _Sampling)
 
 
+@dataclass
+class PageFork:
+    """Arguments of launch_page_fork (btf_page_fork); n_free, table, held and shared are updated in place."""
+    F: int = 0
+    S: int = 0
+    page: int = 64
+    ldt: int = 0
+    pages: int = 0
+    src: object = None          # i32 [F]
+    dst: object = None          # i32 [F]
+    tokens: object = None       # i32 [F]
+    free: object = None         # i32, at least *n_free
+    n_free: object = None       # i32 [1]
+    table: object = None        # i32 [S][ldt]
+    held: object = None         # i32 [S]
+    shared: object = None       # i32 [pages]
+    got: object = None          # i32 [F]
+    copy_from: object = None    # i32 [F]
+    copy_to: object = None      # i32 [F]
+    copy_tokens: object = None  # i32 [F]
+
+    def _c(self):
+        return _struct(self, _PageFork)
+
+
+@dataclass
+class PageCopy:
+    """Arguments of launch_page_copy (btf_page_copy)."""
+    n: int = 0
+    source: object = None  # i32 [n] (btf_page_copy.from)
+    to: object = None      # i32 [n]
+    tokens: object = None  # i32 [n] or None
+    layers: int = 1
+    layer_stride: int = 0
+
+    def _c(self):
+        return _struct(self, _PageCopy)
+
+
+@dataclass
+class PageFree:
+    """Arguments of launch_page_free (btf_page_free); all but keep is updated in place."""
+    S: int = 0
+    page: int = 64
+    ldt: int = 0
+    pages: int = 0
+    keep: object = None    # i32 [S]
+    table: object = None   # i32 [S][ldt]
+    held: object = None    # i32 [S]
+    shared: object = None  # i32 [pages] or None
+    free: object = None    # i32 [pages]
+    n_free: object = None  # i32 [1]
+    ws: object = None      # page_free_ws_bytes
+
+    def _c(self):
+        return _struct(self, _PageFree)
+
+
+@dataclass
+class CacheMove:
+    """Arguments of launch_cache_move (btf_cache_move): tree and leaf, or source and source0."""
+    S: int = 0
+    T: int = 0
+    table: object = None     # i32 [S][ldt]
+    ldt: int = 0
+    to_table: object = None  # i32 [S][ldt_to] or None
+    ldt_to: int = 0
+    first: object = None     # i32 [S]
+    tree: object = None      # i64 [T] or None
+    leaf: object = None      # i32 [S]
+    source: object = None    # i32 [T] or None
+    source0: object = None   # i32 [S + 1]
+    kv_len: object = None    # i32 [S] or None
+    layers: int = 1
+    layer_stride: int = 0
+
+    def _c(self):
+        return _struct(self, _CacheMove)
+
+
+@dataclass
+class SharedAttention(PagedAttention):
+    """Arguments of launch_shared_attention (btf_shared_attention): those of PagedAttention and the groups."""
+    groups: int = 0
+    group0: object = None  # i32 [groups + 1]
+    lead: object = None    # i32 [groups]
+    shared: object = None  # i32 [groups]
+
+    def _c(self):
+        return _struct(self, _SharedAttention)
+
+
+@dataclass
+class LoraSeg:
+    """One projection's adapters and its output (btf_lora_seg)."""
+    a: object = None   # 16 bits [adapters][rank][K]
+    b: object = None   # 16 bits [adapters][N][rank]
+    a_stride: int = 0
+    b_stride: int = 0
+    N: int = 0
+    y: object = None   # f32 [T][ldy]
+    ldy: int = 0
+
+    def _c(self):
+        return _struct(self, _LoraSeg)
+
+
+@dataclass
+class Lora:
+    """Arguments of launch_lora (btf_lora); type: a CacheType, mode: kAdd or kSwiglu."""
+    S: int = 0
+    T: int = 0
+    K: int = 0
+    rank: int = 0
+    adapters: int = 0
+    type: int = CacheType.f16
+    mode: int = GemvMode.kAdd
+    row0: object = None     # i32 [S + 1]
+    adapter: object = None  # i32 [S]
+    ranks: object = None    # i32 [adapters] or None
+    scale: object = None    # f32 [adapters] or None
+    x: object = None        # f32 [T][ldx]
+    ldx: int = 0
+    out: object = None      # f32 [T][ldo], kSwiglu
+    ldo: int = 0
+    ws: object = None       # lora_ws_bytes
+
+    def _c(self):
+        return _struct(self, _Lora)
+
+
 # The launchers below go through the native calls of _btf_call; arguments that
 # those do not read (NotImplemented) take the ctypes path.
 _call.bind(*[C.cast(f, C.c_void_p).value for f in (_launch_prep, _launch_gemv, _launch_gemv_ptq1_0, _launch_gemv_ex)],
            Q8Act, Hx, GemvSeg)
+_layouts = {
+    _cls: _call.layout(_slot, _cls, tuple((_f, {C.c_int: "i", C.c_int64: "q", C.c_float: "f", C.c_void_p: "p"}[_t],
+                                           getattr(_c_struct, _n).offset)
+                                          for _f, (_n, _t) in zip(_cls.__dataclass_fields__, _c_struct._fields_)),
+                       C.sizeof(_c_struct), _table)
+    for _table, _slots in enumerate((
+        ((KvCache, _KvCache), (PagePlan, _PagePlan), (RopeCache, _RopeCache), (PagedAttention, _PagedAttention),
+         (Sampling, _Sampling)),
+        ((PageFork, _PageFork), (PageCopy, _PageCopy), (PageFree, _PageFree), (CacheMove, _CacheMove),
+         (SharedAttention, _SharedAttention), (Lora, _Lora), (LoraSeg, _LoraSeg))))
+    for _slot, (_cls, _c_struct) in enumerate(_slots)}
 _kv_layout, _plan_layout, _rope_layout, _attn_layout, _sample_layout = (
-    _call.layout(_slot, _cls, tuple((_f, {C.c_int: "i", C.c_int64: "q", C.c_float: "f", C.c_void_p: "p"}[_t],
-                                     getattr(_c_struct, _n).offset)
-                                    for _f, (_n, _t) in zip(_cls.__dataclass_fields__, _c_struct._fields_)),
-                 C.sizeof(_c_struct))
-    for _slot, (_cls, _c_struct) in enumerate(((KvCache, _KvCache), (PagePlan, _PagePlan), (RopeCache, _RopeCache),
-                                               (PagedAttention, _PagedAttention), (Sampling, _Sampling))))
+    _layouts[_cls] for _cls in (KvCache, PagePlan, RopeCache, PagedAttention, Sampling))
+_fork_layout, _copy_layout, _free_layout, _move_layout, _shared_layout, _lora_layout, _lora_seg_layout = (
+    _layouts[_cls] for _cls in (PageFork, PageCopy, PageFree, CacheMove, SharedAttention, Lora, LoraSeg))
 _addr_page_plan, _addr_rope_cache, _addr_paged_attention, _addr_sample = (
     C.cast(f, C.c_void_p).value for f in (_launch_page_plan, _launch_rope_cache, _launch_paged_attention, _launch_sample))
+_addr_page_fork, _addr_page_copy, _addr_page_free, _addr_cache_move, _addr_shared_attention, _addr_lora = (
+    C.cast(f, C.c_void_p).value for f in (_launch_page_fork, _launch_page_copy, _launch_page_free, _launch_cache_move,
+                                          _launch_shared_attention, _launch_lora))
 
 
 def kernels_init(device: int = 0) -> None:
@@ -649,6 +846,106 @@ def launch_sample(a: Sampling, stream=None) -> None:
 
 def launch_sample_raw(a: Sampling, stream=None) -> int:
     return _launch_sample(C.byref(a._c()) if a is not None else None, _stream(stream))
+
+
+def launch_page_fork(a: PageFork, stream=None) -> None:
+    """Request rows that begin as copies of others, whole pages shared (btf_hip_launch_page_fork)."""
+    rc = _call.launch(_addr_page_fork, _fork_layout, a, -1, None, stream)
+    if rc is not NotImplemented:
+        if rc:
+            _check(rc)
+        return
+    _check(launch_page_fork_raw(a, stream))
+
+
+def launch_page_fork_raw(a: PageFork, stream=None) -> int:
+    return _launch_page_fork(C.byref(a._c()) if a is not None else None, _stream(stream))
+
+
+def launch_page_copy(a: PageCopy, kv: KvCache, stream=None) -> None:
+    """Pages copied in every layer (btf_hip_launch_page_copy)."""
+    rc = _call.launch(_addr_page_copy, _copy_layout, a, _kv_layout, kv, stream)
+    if rc is not NotImplemented:
+        if rc:
+            _check(rc)
+        return
+    _check(launch_page_copy_raw(a, kv, stream))
+
+
+def launch_page_copy_raw(a: PageCopy, kv: KvCache, stream=None) -> int:
+    return _launch_page_copy(C.byref(a._c()) if a is not None else None, C.byref(kv._c()) if kv is not None else None,
+                             _stream(stream))
+
+
+def page_free_ws_bytes(S: int, ldt: int) -> int:
+    return int(_page_free_ws_bytes(S, ldt))
+
+
+def launch_page_free(a: PageFree, stream=None) -> None:
+    """Pages behind what the requests keep go back to the free list (btf_hip_launch_page_free)."""
+    rc = _call.launch(_addr_page_free, _free_layout, a, -1, None, stream)
+    if rc is not NotImplemented:
+        if rc:
+            _check(rc)
+        return
+    _check(launch_page_free_raw(a, stream))
+
+
+def launch_page_free_raw(a: PageFree, stream=None) -> int:
+    return _launch_page_free(C.byref(a._c()) if a is not None else None, _stream(stream))
+
+
+def launch_cache_move(a: CacheMove, kv: KvCache, stream=None) -> None:
+    """Tokens that stay are moved together in every layer (btf_hip_launch_cache_move)."""
+    rc = _call.launch(_addr_cache_move, _move_layout, a, _kv_layout, kv, stream)
+    if rc is not NotImplemented:
+        if rc:
+            _check(rc)
+        return
+    _check(launch_cache_move_raw(a, kv, stream))
+
+
+def launch_cache_move_raw(a: CacheMove, kv: KvCache, stream=None) -> int:
+    return _launch_cache_move(C.byref(a._c()) if a is not None else None, C.byref(kv._c()) if kv is not None else None,
+                              _stream(stream))
+
+
+def shared_attention_ws_bytes(S: int, T: int, heads: int, kv: KvCache) -> int:
+    return int(_shared_attention_ws_bytes(S, T, heads, C.byref(kv._c())))
+
+
+def launch_shared_attention(a: SharedAttention, kv: KvCache, stream=None) -> None:
+    """launch_paged_attention with shared prefixes read once (btf_hip_launch_shared_attention)."""
+    rc = _call.launch(_addr_shared_attention, _shared_layout, a, _kv_layout, kv, stream)
+    if rc is not NotImplemented:
+        if rc:
+            _check(rc)
+        return
+    _check(launch_shared_attention_raw(a, kv, stream))
+
+
+def launch_shared_attention_raw(a: SharedAttention, kv: KvCache, stream=None) -> int:
+    return _launch_shared_attention(C.byref(a._c()) if a is not None else None,
+                                    C.byref(kv._c()) if kv is not None else None, _stream(stream))
+
+
+def lora_ws_bytes(S: int, T: int, K: int, rank: int, nseg: int) -> int:
+    return int(_lora_ws_bytes(S, T, K, rank, nseg))
+
+
+def launch_lora(a: Lora, segs, stream=None) -> None:
+    """Low-rank adapters of many requests beside a shared projection (btf_hip_launch_lora). `segs`: 1..3 LoraSeg."""
+    rc = _call.launch_list(_addr_lora, _lora_layout, a, _lora_seg_layout, segs, stream)
+    if rc is not NotImplemented:
+        if rc:
+            _check(rc)
+        return
+    _check(launch_lora_raw(a, segs, len(segs), stream))
+
+
+def launch_lora_raw(a: Lora, segs, nseg: int, stream=None) -> int:
+    arr = (_LoraSeg * max(1, len(segs)))(*[s._c() for s in segs]) if segs else None
+    return _launch_lora(C.byref(a._c()) if a is not None else None, arr, nseg, _stream(stream))
 
 
 def launch_gemv_ex(segs, K: int, M: int, a: Q8Act = None, x=None, ldx: int = 0,

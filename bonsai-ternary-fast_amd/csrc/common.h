@@ -251,5 +251,15 @@ int64_t paged_attention_ws_bytes(int S, int T, int heads, const btf_kv_cache& kv
 int paged_attention(const btf_paged_attention& a, const btf_kv_cache& kv, hipStream_t st);
 int64_t sample_ws_bytes(int M, int V);
 int sample(const btf_sampling& a, hipStream_t st);
+int page_fork(const btf_page_fork& a, hipStream_t st);
+int page_copy(const btf_page_copy& a, const btf_kv_cache& kv, hipStream_t st);
+int64_t page_free_ws_bytes(int S, int ldt);
+int page_free(const btf_page_free& a, hipStream_t st);
+int cache_move(const btf_cache_move& a, const btf_kv_cache& kv, hipStream_t st);
+int64_t shared_attention_most_items(int S, int T, int heads, const btf_kv_cache& kv);
+int64_t shared_attention_ws_bytes(int S, int T, int heads, const btf_kv_cache& kv);
+int shared_attention(const btf_shared_attention& a, const btf_kv_cache& kv, hipStream_t st);
+int64_t lora_ws_bytes(int S, int T, int K, int rank, int nseg);
+int lora(const btf_lora& a, const btf_lora_seg* segs, int nseg, hipStream_t st);
 
 }  // namespace btfhip

@@ -1,0 +1,405 @@
+// lora.hip -- low-rank adapters of many requests beside a shared projection
+// (btf_hip_launch_lora; gfx950): y += scale B (A x), each request's rows with its
+// own A [rank][K] and B [N][rank].
+//
+// Two launches. lora_shrink: h = A x, a tile of rows of one request by a slice of K a
+// workgroup; its waves take every fourth 64 columns, join in LDS, and leave the slice's
+// sums in the workspace. lora_expand: the slices' sums in order, times scale, then
+// B h for a tile of rows and a run of outputs, added to y (or through silu(g) u).
+// No sum's order depends on which workgroup comes first.
+//
+// Products on 16x16x32 bf16 MFMA with exact factors: a 32-bit x is the sum of three
+// bf16 numbers (8 bits each, cut off, not rounded, so that no part overflows), h
+// likewise, an fp16 weight of two. All products of parts are taken, so only the sums
+// round, in 32 bits. (The three parts cost less than a third of 32-bit MFMA would, and
+// where few rows have an adapter nothing but its bytes counts.) Infinite x or weights give NaN.
+//
+// Bound by HBM where rows or adapters are many, by latency of the two launches where few.
+#include <string>
+
+#include "../../include/btf/hip_abi.h"
+#include "common.h"
+
+namespace btfhip {
+namespace {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 b8 __attribute__((ext_vector_type(8)));
+
+constexpr int kThreads = 256;
+constexpr int kWaves = kThreads / 64;
+constexpr int kBlockK = 64;       // columns of a wave's step
+constexpr int kGroups = 512;      // workgroups that a launch is cut into, at least
+constexpr int kChunk = 256;       // outputs of a workgroup, or a multiple
+
+struct Segs {
+  btf_lora_seg s[3];
+};
+
+__device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8, a), __builtin_bit_cast(b8, b), c, 0, 0, 0);
+}
+
+// The upper halves of two 32-bit numbers (bf16, cut off), and what they leave.
+__device__ __forceinline__ uint32_t cut2(float& x, float& y) {
+  const uint32_t a = __float_as_uint(x), b = __float_as_uint(y);
+  x -= __uint_as_float(a & 0xffff0000u);
+  y -= __uint_as_float(b & 0xffff0000u);
+  return __builtin_amdgcn_perm(b, a, 0x07060302u);
+}
+// Eight numbers as three times eight bf16.
+__device__ __forceinline__ void cut3(f32x4 lo, f32x4 hi, u32x4 (&p)[3]) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    float x = j < 2 ? lo[2 * j] : hi[2 * j - 4], y = j < 2 ? lo[2 * j + 1] : hi[2 * j - 3];
+    p[0][j] = cut2(x, y);
+    p[1][j] = cut2(x, y);
+    p[2][j] = cut2(x, y);
+  }
+}
+// Eight weights as one or two times eight bf16.
+template <bool BF>
+__device__ __forceinline__ void weights(u32x4 v, u32x4 (&w)[BF ? 1 : 2]) {
+  if constexpr (BF) {
+    w[0] = v;
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      float x = h2f((uint16_t)v[j]), y = h2f((uint16_t)(v[j] >> 16));
+      w[0][j] = cut2(x, y);
+      w[1][j] = cut2(x, y);
+    }
+  }
+}
+
+// Inclusive sum over the lanes.
+__device__ __forceinline__ int wave_scan(int v) {
+  v += dpp_i<0x111>(v);
+  v += dpp_i<0x112>(v);
+  v += dpp_i<0x114>(v);
+  v += dpp_i<0x118>(v);
+  const int t0 = __builtin_amdgcn_readlane(v, 15), t1 = __builtin_amdgcn_readlane(v, 31), t2 = __builtin_amdgcn_readlane(v, 47);
+  const int row = (threadIdx.x & 63) >> 4;
+  return v + (row > 0 ? t0 : 0) + (row > 1 ? t1 : 0) + (row > 2 ? t2 : 0);
+}
+
+// Tile `id` of R rows of the requests, found by every wave for itself: its first row and
+// rows, its adapter (-1: none) and that one's rank. False: there is no such tile.
+struct Tile {
+  int row, n, adapter, rank;
+};
+template <int R>
+__device__ bool find(const btf_lora& a, int id, Tile& t) {
+  const int lane = threadIdx.x & 63;
+  int before = 0;
+  for (int s0 = 0; s0 < a.S; s0 += 64) {
+    int r0 = 0, n = 0;
+    if (s0 + lane < a.S) {
+      r0 = max(a.row0[s0 + lane], 0);
+      n = min(a.row0[s0 + lane + 1], a.T) - r0;
+    }
+    const int mine = n > 0 ? (n + R - 1) / R : 0, upto = before + wave_scan(mine);
+    const unsigned long long who = __ballot(mine > 0 && id >= upto - mine && id < upto);
+    if (who) {
+      const int l = __builtin_ctzll(who), k = id - __builtin_amdgcn_readlane(upto - mine, l);
+      t.row = __builtin_amdgcn_readlane(r0, l) + k * R;
+      t.n = min(__builtin_amdgcn_readlane(n, l) - k * R, R);
+      t.adapter = a.adapter[s0 + l];
+      if (t.adapter < 0 || t.adapter >= a.adapters) t.adapter = -1;
+      t.rank = t.adapter < 0 ? 0 : a.ranks ? min(max(a.ranks[t.adapter], 0), a.rank) : a.rank;
+      return true;
+    }
+    before = __builtin_amdgcn_readlane(upto, 63);
+  }
+  return false;
+}
+
+// h of row `row`, rank 0, slice k of K.
+__device__ __forceinline__ float* h_of(const btf_lora& a, int nseg, int k, int seg, int row) {
+  return static_cast<float*>(a.ws) + ((size_t)(k * nseg + seg) * a.T + row) * a.rank;
+}
+
+// RT tiles of 16 rows by NT tiles of 16 ranks. grid: (tile, slice of K), (segment, NT tiles of ranks).
+template <bool BF, int RT, int NT>
+__global__ void __launch_bounds__(kThreads, 2) lora_shrink_kernel(btf_lora a, Segs segs, int nseg, int slices, int slice) {
+  constexpr int R = 16 * RT, LD = 16 * NT + 4;
+  __shared__ float sh[kWaves][R][LD];
+  Tile t;
+  const int k = blockIdx.x % slices, seg = blockIdx.y % nseg, first = blockIdx.y / nseg * 16 * NT;
+  if (!find<R>(a, blockIdx.x / slices, t) || first >= t.rank) return;  // the whole workgroup
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, c16 = lane & 15, g = lane >> 4;
+  const btf_lora_seg& s = segs.s[seg];
+  const int end = min(a.K, (k + 1) * slice);
+  // lane's columns of a step: 16 g .. 16 g + 15; its row of x in each tile, its rank's row of A
+  const float* x = a.x + (size_t)(t.row + c16) * a.ldx + 16 * g;
+  const uint16_t* m = static_cast<const uint16_t*>(s.a) + (size_t)t.adapter * s.a_stride + (size_t)(first + c16) * a.K + 16 * g;
+  f32x4 acc[RT][NT];
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+    for (int n = 0; n < NT; ++n) acc[rt][n] = f32x4{0.f, 0.f, 0.f, 0.f};
+  f32x4 xv[RT][4];
+  u32x4 av[NT][2];
+  auto load = [&](int kb) {
+    const bool in = kb + 16 * g < end;  // (K is a multiple of 32: a lane's columns are all there or none)
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        av[n][u] = u32x4{0, 0, 0, 0};
+        if (in && first + 16 * n + c16 < t.rank)
+          av[n][u] = *reinterpret_cast<const u32x4*>(m + (size_t)(16 * n) * a.K + kb + 8 * u);
+      }
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        xv[rt][u] = f32x4{0.f, 0.f, 0.f, 0.f};
+        if (in && 16 * rt + c16 < t.n)
+          xv[rt][u] = *reinterpret_cast<const f32x4*>(x + (size_t)(16 * rt) * a.ldx + kb + 4 * u);
+      }
+  };
+  // Few rows: the next step's loads are on their way while this one is worked on. Many: a wave's loads are 16 KB
+  // anyway, and its registers are the rows'.
+  constexpr bool kAhead = RT == 1;
+  constexpr int kStep = kBlockK * kWaves;
+  int kb = k * slice + kBlockK * w;
+  if (kAhead && kb < end) load(kb);
+  for (; kb < end; kb += kStep) {
+    if (!kAhead) load(kb);
+    u32x4 xp[kAhead ? 2 : 1][RT][3], ap[kAhead ? 2 : 1][NT][BF ? 1 : 2];
+    auto cut = [&](int u, int at) {
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) cut3(xv[rt][2 * u], xv[rt][2 * u + 1], xp[at][rt]);
+#pragma unroll
+      for (int n = 0; n < NT; ++n) weights<BF>(av[n][u], ap[at][n]);
+    };
+    auto multiply = [&](int at) {
+#pragma unroll
+      for (int p = 0; p < 3; ++p)
+#pragma unroll
+        for (int q = 0; q < (BF ? 1 : 2); ++q)
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) acc[rt][n] = mfma(ap[at][n][q], xp[at][rt][p], acc[rt][n]);
+    };
+    if constexpr (kAhead) {
+      cut(0, 0);
+      cut(1, 1);
+      if (kb + kStep < end) load(kb + kStep);
+      multiply(0);
+      multiply(1);
+    } else {
+      cut(0, 0);
+      multiply(0);
+      cut(1, 0);
+      multiply(0);
+    }
+  }
+  // the waves' sums (lane: row c16, ranks 4 g .. 4 g + 3)
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+    for (int n = 0; n < NT; ++n) *reinterpret_cast<f32x4*>(&sh[w][16 * rt + c16][16 * n + 4 * g]) = acc[rt][n];
+  __syncthreads();
+  constexpr int Q = 4 * NT;  // fours of ranks in a row
+  for (int i = threadIdx.x; i < t.n * Q; i += kThreads) {
+    const int r = i / Q, c = 4 * (i % Q);
+    if (first + c >= a.rank) continue;  // (a.rank is a multiple of 8)
+    f32x4 v = *reinterpret_cast<const f32x4*>(&sh[0][r][c]);
+#pragma unroll
+    for (int j = 1; j < kWaves; ++j) v += *reinterpret_cast<const f32x4*>(&sh[j][r][c]);
+    *reinterpret_cast<f32x4*>(h_of(a, nseg, k, seg, t.row + r) + first + c) = v;
+  }
+}
+
+// Row of h's parts in LDS, in bf16: the ranks in steps of 32, and 16 bytes so that rows lie in other banks.
+__host__ __device__ constexpr int parts_ld(int rank) { return (rank + 31) / 32 * 32 + 8; }
+
+// RT tiles of 16 rows by `chunk` outputs. GLU: both segments, into out.
+template <bool BF, int RT, bool GLU, bool VEC>
+__global__ void __launch_bounds__(kThreads, 2) lora_expand_kernel(btf_lora a, Segs segs, int nseg, int slices, int chunk, int chunks) {
+  constexpr int R = 16 * RT, NS = GLU ? 2 : 1;
+  constexpr int TN = GLU && RT > 1 ? 1 : GLU || RT > 1 ? 2 : 4;  // tiles of 16 outputs of a wave at a time
+  extern __shared__ uint16_t sh_h[];         // [segment][part][row][parts_ld]
+  Tile t;
+  if (!find<R>(a, blockIdx.x / chunks, t) || (!GLU && t.rank == 0)) return;  // the whole workgroup
+  int c = blockIdx.x % chunks, seg = 0;
+  if (!GLU)
+    while (seg < nseg - 1 && c >= (segs.s[seg].N + chunk - 1) / chunk) c -= (segs.s[seg].N + chunk - 1) / chunk, ++seg;
+  const int N = segs.s[seg].N, ld = parts_ld(a.rank), steps = (t.rank + 31) / 32;
+  const float scale = t.adapter >= 0 && a.scale ? a.scale[t.adapter] : 1.f;
+  // h, scaled, in parts
+  for (int i = threadIdx.x; i < NS * R * steps * 8; i += kThreads) {
+    const int q = 4 * (i % (steps * 8)), r = i / (steps * 8) % R, sg = i / (steps * 8) / R;
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+    if (r < t.n && q < t.rank) {
+      for (int k = 0; k < slices; ++k) v += *reinterpret_cast<const f32x4*>(h_of(a, nseg, k, GLU ? sg : seg, t.row + r) + q);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] = q + j < t.rank ? v[j] * scale : 0.f;
+    }
+    float x[4] = {v[0], v[1], v[2], v[3]};
+#pragma unroll
+    for (int p = 0; p < 3; ++p) {
+      const uint32_t lo = cut2(x[0], x[1]), hi = cut2(x[2], x[3]);
+      *reinterpret_cast<uint2*>(sh_h + (size_t)((sg * 3 + p) * R + r) * ld + q) = uint2{lo, hi};
+    }
+  }
+  __syncthreads();
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, c16 = lane & 15, g = lane >> 4;
+  const int n1 = min(N, (c + 1) * chunk);
+  for (int n0 = c * chunk + 16 * TN * w; n0 < n1; n0 += 16 * TN * kWaves) {
+    // y of the lane's row in each tile: outputs n0 + 16 i + 4 g .. + 3
+    f32x4 y[NS][TN][RT];
+#pragma unroll
+    for (int sg = 0; sg < NS; ++sg)
+#pragma unroll
+      for (int i = 0; i < TN; ++i)
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+          const btf_lora_seg& s = segs.s[GLU ? sg : seg];
+          const int n = n0 + 16 * i + 4 * g, r = 16 * rt + c16;
+          const float* p = s.y + (size_t)(t.row + r) * s.ldy + n;
+          y[sg][i][rt] = f32x4{0.f, 0.f, 0.f, 0.f};
+          if (r < t.n) {
+            if (VEC && n + 3 < n1) {
+              y[sg][i][rt] = *reinterpret_cast<const f32x4*>(p);
+            } else {
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+                if (n + j < n1) y[sg][i][rt][j] = p[j];
+            }
+          }
+        }
+#pragma unroll
+    for (int sg = 0; sg < NS; ++sg) {
+      const btf_lora_seg& s = segs.s[GLU ? sg : seg];
+      const uint16_t* b = static_cast<const uint16_t*>(s.b) + (size_t)max(t.adapter, 0) * s.b_stride + (size_t)(n0 + c16) * a.rank + 8 * g;
+      f32x4 d[TN][RT];
+#pragma unroll
+      for (int i = 0; i < TN; ++i)
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) d[i][rt] = f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int k = 0; k < steps; ++k) {
+        const int left = t.rank - 32 * k - 8 * g;  // ranks from the lane's first on
+        u32x4 bv[TN];
+#pragma unroll
+        for (int i = 0; i < TN; ++i) {
+          bv[i] = u32x4{0, 0, 0, 0};
+          if (left > 0 && n0 + 16 * i + c16 < n1) bv[i] = *reinterpret_cast<const u32x4*>(b + (size_t)(16 * i) * a.rank + 32 * k);
+#pragma unroll
+          for (int j = 0; j < 4; ++j)  // what lies behind the adapter's rank
+            bv[i][j] &= left > 2 * j + 1 ? 0xffffffffu : left > 2 * j ? 0xffffu : 0u;
+        }
+        u32x4 hp[RT][3];
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+          for (int p = 0; p < 3; ++p)
+            hp[rt][p] = *reinterpret_cast<const u32x4*>(sh_h + (size_t)((sg * 3 + p) * R + 16 * rt + c16) * ld + 32 * k + 8 * g);
+#pragma unroll
+        for (int i = 0; i < TN; ++i) {
+          u32x4 bp[BF ? 1 : 2];
+          weights<BF>(bv[i], bp);
+#pragma unroll
+          for (int p = 0; p < 3; ++p)
+#pragma unroll
+            for (int q = 0; q < (BF ? 1 : 2); ++q)
+#pragma unroll
+              for (int rt = 0; rt < RT; ++rt) d[i][rt] = mfma(bp[q], hp[rt][p], d[i][rt]);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < TN; ++i)
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) y[sg][i][rt] += d[i][rt];
+    }
+#pragma unroll
+    for (int i = 0; i < TN; ++i)
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) {
+        const int n = n0 + 16 * i + 4 * g, r = 16 * rt + c16;
+        f32x4 v = y[0][i][rt];
+        if (GLU) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) v[j] = v[j] / (1.0f + expf(-v[j])) * y[NS - 1][i][rt][j];
+        }
+        float* p = GLU ? a.out + (size_t)(t.row + r) * a.ldo + n : segs.s[seg].y + (size_t)(t.row + r) * segs.s[seg].ldy + n;
+        if (r < t.n) {
+          if (VEC && n + 3 < n1) {
+            *reinterpret_cast<f32x4*>(p) = v;
+          } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              if (n + j < n1) p[j] = v[j];
+          }
+        }
+      }
+  }
+}
+
+// Rows of a tile: 64 where requests have more than 16 on average, as far as the parts of h fit 64 KB of LDS.
+int tile_rows(int S, int T, int rank, int together) {
+  return (int64_t)T > 16 * (int64_t)S && rank * together <= 128 ? 64 : 16;
+}
+
+bool vec4(const float* p, int ld) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ld % 4 == 0; }
+
+template <bool BF, int RT>
+int lora_go(const btf_lora& a, const Segs& segs, int nseg, hipStream_t st) {
+  constexpr int R = 16 * RT;
+  const int tiles = a.T / R + a.S;
+  const int nt = a.rank <= 16 ? 1 : a.rank <= 32 ? 2 : 4, groups = (a.rank + 16 * nt - 1) / (16 * nt);
+  // slices of K: enough for kGroups workgroups, each at least one step of its waves long
+  const int step = kBlockK * kWaves, most = (a.K + step - 1) / step;
+  int slices = (kGroups + tiles * nseg * groups - 1) / (tiles * nseg * groups);
+  slices = slices < most ? slices : most;
+  const int slice = ((a.K + slices - 1) / slices + step - 1) / step * step;
+  slices = (a.K + slice - 1) / slice;
+  const dim3 grid((unsigned)tiles * slices, nseg * groups), blk(kThreads);
+  if (nt == 1) hipLaunchKernelGGL((lora_shrink_kernel<BF, RT, 1>), grid, blk, 0, st, a, segs, nseg, slices, slice);
+  else if (nt == 2) hipLaunchKernelGGL((lora_shrink_kernel<BF, RT, 2>), grid, blk, 0, st, a, segs, nseg, slices, slice);
+  else hipLaunchKernelGGL((lora_shrink_kernel<BF, RT, 4>), grid, blk, 0, st, a, segs, nseg, slices, slice);
+  const int rc = launch_status("lora_shrink_kernel");
+  if (rc != BTF_OK) return rc;
+  const bool glu = a.mode == BTF_GEMV_SWIGLU;
+  int outs = 0;
+  bool vec = true;
+  for (int i = 0; i < nseg; ++i) vec = vec && vec4(segs.s[i].y, segs.s[i].ldy), outs += glu && i ? 0 : segs.s[i].N;
+  if (glu) vec = vec && vec4(a.out, a.ldo);
+  int chunk = kChunk;
+  while (chunk < 4 * kChunk && (int64_t)tiles * (outs / (2 * chunk)) >= kGroups) chunk *= 2;
+  int chunks = 0;
+  for (int i = 0; i < (glu ? 1 : nseg); ++i) chunks += (segs.s[i].N + chunk - 1) / chunk;
+  const size_t lds = (size_t)(glu ? 2 : 1) * 3 * R * parts_ld(a.rank) * 2;
+  const dim3 eg((unsigned)tiles * chunks);
+  auto expand = [&](auto kernel) { hipLaunchKernelGGL(kernel, eg, blk, lds, st, a, segs, nseg, slices, chunk, chunks); };
+  if (glu && vec) expand(lora_expand_kernel<BF, RT, true, true>);
+  else if (glu) expand(lora_expand_kernel<BF, RT, true, false>);
+  else if (vec) expand(lora_expand_kernel<BF, RT, false, true>);
+  else expand(lora_expand_kernel<BF, RT, false, false>);
+  return launch_status("lora_expand_kernel");
+}
+
+}  // namespace
+
+// slices * T * nseg is at most nseg * T + kGroups * 64 (tiles >= T / 64), and slices at most K / 256, rounded up.
+int64_t lora_ws_bytes(int S, int T, int K, int rank, int nseg) {
+  (void)S;
+  const int64_t most = (K + kBlockK * kWaves - 1) / (kBlockK * kWaves), rows = (int64_t)nseg * T;
+  const int64_t all = rows * most, cut = rows + kGroups * 64;
+  return (all < cut ? all : cut) * rank * 4;
+}
+
+int lora(const btf_lora& a, const btf_lora_seg* s, int nseg, hipStream_t st) {
+  Segs segs{};
+  for (int i = 0; i < nseg; ++i) segs.s[i] = s[i];
+  const bool bf = a.type == BTF_BF16;
+  if (tile_rows(a.S, a.T, a.rank, a.mode == BTF_GEMV_SWIGLU ? 2 : 1) == 64)
+    return bf ? lora_go<true, 4>(a, segs, nseg, st) : lora_go<false, 4>(a, segs, nseg, st);
+  return bf ? lora_go<true, 1>(a, segs, nseg, st) : lora_go<false, 1>(a, segs, nseg, st);
+}
+
+}  // namespace btfhip

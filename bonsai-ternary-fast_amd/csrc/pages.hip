@@ -1,0 +1,384 @@
+// pages.hip -- cache pages that several requests hold, and tokens that change
+// their places (btf_hip_launch_page_fork, _page_copy, _page_free, _cache_move;
+// gfx950).
+//
+// fork and free are integers: which row holds which page, and how many rows hold a
+// page beyond one (shared). Counts change by 32-bit atomic additions, whose order
+// does not show in the sums. Pages go back in an order that does not depend on the
+// threads' either: after all counts have been lowered, those of the pages to give
+// back are below zero; each place (row, page of the row) that gives one up puts the
+// smallest mark, INT_MIN + its number, there, and the one whose mark stays owns the
+// page. Its number among the owners is a prefix sum.
+//
+// copy and move are bytes. A wave's lanes take runs of 128 bytes (a cache line) or
+// more of a token's values; up to eight 16-byte loads a thread are on their way
+// before the first store.
+#include <climits>
+#include <string>
+
+#include "../../include/btf/hip_abi.h"
+#include "common.h"
+
+namespace btfhip {
+namespace {
+
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+// ---- fork ----
+constexpr int kForkThreads = 1024;
+// Page ids of all forks that the deciding workgroup copies itself.
+constexpr int kForkSmall = 2048;
+
+// Fork f's ids of whole pages, j0, j0 + step, ...
+__device__ __forceinline__ void fork_row(const btf_page_fork& a, int src, int dst, int whole, int j0, int step) {
+  const int* from = a.table + (size_t)src * a.ldt;
+  int* to = a.table + (size_t)dst * a.ldt;
+  for (int j = j0; j < whole; j += step) {
+    const int p = from[j];
+    to[j] = p;
+    if (p >= 0 && p < a.pages) __hip_atomic_fetch_add(a.shared + p, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+}
+
+template <bool ROWS>
+__global__ void __launch_bounds__(kForkThreads) page_fork_kernel(btf_page_fork a) {
+  __shared__ uint64_t part[kForkThreads / 64];
+  __shared__ int sh_dst[kForkThreads], sh_src[kForkThreads], sh_whole[kForkThreads];
+  const int f = threadIdx.x;
+  const bool live = f < a.F;
+  const int s = live ? a.src[f] : -1, d = live ? a.dst[f] : -1, n = live ? a.tokens[f] : -1;
+  const long long free0 = max(*a.n_free, 0);
+  bool sound = s >= 0 && s < a.S && d >= 0 && d < a.S && s != d && n >= 0;
+  if (sound) {
+    const int hs = a.held[s];
+    sound = hs <= a.ldt && n <= (long long)hs * a.page && a.held[d] == 0;
+  }
+  sh_dst[f] = sound ? d : -1;
+  sh_src[f] = s;
+  __syncthreads();  // (all of held, and *n_free, has been read)
+  bool taken = false;
+  for (int i = 0; i < (sound ? f : 0); ++i) taken |= sh_dst[i] == d;
+  sound = sound && !taken;
+  const int whole = sound ? n / a.page : 0;
+  const bool part_page = sound && n % a.page != 0;
+  uint64_t all;
+  const long long upto = (long long)block_scan<kForkThreads>(part_page, part, &all);
+  const bool ok = sound && (!part_page || upto <= free0);
+  sh_whole[f] = ok ? whole : 0;
+  if (live) {
+    int from = -1, to = -1;
+    if (ok && part_page) {
+      from = a.table[(size_t)s * a.ldt + whole];
+      to = a.free_list[free0 - upto];
+      a.table[(size_t)d * a.ldt + whole] = to;
+    }
+    if (ok) a.held[d] = whole + part_page;
+    a.got[f] = ok ? n : -1;
+    a.copy_from[f] = from;
+    a.copy_to[f] = to;
+    a.copy_tokens[f] = ok && part_page ? n % a.page : 0;
+  }
+  if (f == 0) *a.n_free = (int)(free0 - min((long long)all, free0));  // (each takes one: the first ones are served)
+  if (!ROWS) return;
+  __syncthreads();
+  for (int i = f >> 6; i < a.F; i += kForkThreads / 64) fork_row(a, sh_src[i], sh_dst[i], sh_whole[i], f & 63, 64);
+}
+
+__global__ void __launch_bounds__(256) page_fork_rows_kernel(btf_page_fork a) {
+  const int f = blockIdx.x, n = a.got[f];
+  if (n > 0) fork_row(a, a.src[f], a.dst[f], min(n / a.page, a.ldt), blockIdx.y * 256 + threadIdx.x, gridDim.y * 256);
+}
+
+// ---- free ----
+constexpr int kFreeThreads = 1024;
+constexpr int kFreeEach = 4;                          // places of a thread
+constexpr int kFreeChunk = kFreeThreads * kFreeEach;  // ... of a workgroup
+
+// Place e = s * ldt + j gives up its page (`in`); the page's id, -1: none that the cache has.
+struct Place {
+  bool in;
+  int page;
+};
+__device__ __forceinline__ Place place_of(const btf_page_free& a, const int* held, int e) {
+  Place p{false, -1};
+  if (e >= a.S * a.ldt) return p;
+  const int s = e / a.ldt, j = e - s * a.ldt;
+  const int keep = max(a.keep[s], 0), first = (int)(((long long)keep + a.page - 1) / a.page);
+  p.in = j >= first && j < held[s];
+  if (p.in) {
+    p.page = a.table[e];
+    if (p.page >= a.pages || p.page < 0) p.page = -1;
+  }
+  return p;
+}
+__device__ __forceinline__ void lower(const btf_page_free& a, int page) {
+  if (page >= 0) __hip_atomic_fetch_add(a.shared + page, -1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ int count_of(const btf_page_free& a, int page) {
+  return __hip_atomic_load(a.shared + page, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ void mark(const btf_page_free& a, int page, int e) {
+  // (a count below zero is more than -2^29, a mark less than INT_MIN + 2^29)
+  if (page >= 0 && count_of(a, page) < 0)
+    __hip_atomic_fetch_min(a.shared + page, INT_MIN + e, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ bool owns(const btf_page_free& a, int page, int e) {
+  return page >= 0 && (!a.shared || count_of(a, page) == INT_MIN + e);
+}
+// The places' pages go to the list, which has n0 entries, `behind` of the call's after them.
+__device__ __forceinline__ void give_back(const btf_page_free& a, const Place (&p)[kFreeEach], unsigned own, int e0,
+                                          long long n0, long long behind) {
+#pragma unroll
+  for (int i = kFreeEach - 1; i >= 0; --i) {
+    if (own >> i & 1) {
+      if (n0 + behind < a.pages) a.free_list[n0 + behind] = p[i].page;
+      ++behind;
+      if (a.shared) a.shared[p[i].page] = 0;
+    }
+    if (p[i].in) a.table[e0 + i] = -1;
+  }
+}
+__device__ __forceinline__ int stays(const btf_page_free& a, int held, int s) {
+  return (int)min((long long)held, ((long long)max(a.keep[s], 0) + a.page - 1) / a.page);
+}
+
+// All of it by one workgroup: up to kFreeChunk places.
+__global__ void __launch_bounds__(kFreeThreads) page_free_small_kernel(btf_page_free a) {
+  __shared__ uint64_t part[kFreeThreads / 64];
+  const int e0 = threadIdx.x * kFreeEach;
+  const long long n0 = min((long long)max(*a.n_free, 0), (long long)a.pages);
+  Place p[kFreeEach];
+#pragma unroll
+  for (int i = 0; i < kFreeEach; ++i) p[i] = place_of(a, a.held, e0 + i);
+  if (a.shared) {
+#pragma unroll
+    for (int i = 0; i < kFreeEach; ++i) lower(a, p[i].page);
+    __threadfence();
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kFreeEach; ++i) mark(a, p[i].page, e0 + i);
+    __threadfence();
+    __syncthreads();
+  }
+  unsigned own = 0;
+#pragma unroll
+  for (int i = 0; i < kFreeEach; ++i) own |= (unsigned)owns(a, p[i].page, e0 + i) << i;
+  uint64_t all;
+  const uint64_t upto = block_scan<kFreeThreads>(__popc(own), part, &all);  // (and all have read what is written below)
+  give_back(a, p, own, e0, n0, (long long)(all - upto));
+  for (int s = threadIdx.x; s < a.S; s += kFreeThreads) a.held[s] = stays(a, a.held[s], s);
+  if (threadIdx.x == 0) *a.n_free = (int)min(n0 + (long long)all, (long long)a.pages);
+}
+
+// The same in four launches, a workgroup for each kFreeChunk places. ws: owners of each
+// chunk, then held and *n_free as they were (the last launch writes them while other
+// workgroups read).
+__global__ void __launch_bounds__(kFreeThreads) page_free_lower_kernel(btf_page_free a) {
+  const int e0 = blockIdx.x * kFreeChunk + threadIdx.x * kFreeEach;
+#pragma unroll
+  for (int i = 0; i < kFreeEach; ++i) lower(a, place_of(a, a.held, e0 + i).page);
+}
+__global__ void __launch_bounds__(kFreeThreads) page_free_mark_kernel(btf_page_free a) {
+  const int e0 = blockIdx.x * kFreeChunk + threadIdx.x * kFreeEach;
+#pragma unroll
+  for (int i = 0; i < kFreeEach; ++i) mark(a, place_of(a, a.held, e0 + i).page, e0 + i);
+}
+__global__ void __launch_bounds__(kFreeThreads) page_free_count_kernel(btf_page_free a) {
+  __shared__ uint64_t part[kFreeThreads / 64];
+  int* owners = static_cast<int*>(a.ws);
+  const int e0 = blockIdx.x * kFreeChunk + threadIdx.x * kFreeEach;
+  uint64_t n = 0, all;
+#pragma unroll
+  for (int i = 0; i < kFreeEach; ++i) {
+    n += owns(a, place_of(a, a.held, e0 + i).page, e0 + i);
+    if (e0 + i < a.S * a.ldt && (e0 + i) % a.ldt == 0) owners[gridDim.x + (e0 + i) / a.ldt] = a.held[(e0 + i) / a.ldt];
+  }
+  (void)block_scan<kFreeThreads>(n, part, &all);
+  if (threadIdx.x == 0) owners[blockIdx.x] = (int)all;
+  if (blockIdx.x == 0 && threadIdx.x == 0) owners[gridDim.x + a.S] = *a.n_free;
+}
+__global__ void __launch_bounds__(kFreeThreads) page_free_kernel(btf_page_free a) {
+  __shared__ uint64_t part[kFreeThreads / 64];
+  const int* owners = static_cast<const int*>(a.ws);
+  const int* held = owners + gridDim.x;
+  const int e0 = blockIdx.x * kFreeChunk + threadIdx.x * kFreeEach;
+  const long long n0 = min((long long)max(held[a.S], 0), (long long)a.pages);
+  Place p[kFreeEach];
+  unsigned own = 0;
+#pragma unroll
+  for (int i = 0; i < kFreeEach; ++i) {
+    p[i] = place_of(a, held, e0 + i);
+    own |= (unsigned)owns(a, p[i].page, e0 + i) << i;
+  }
+  uint64_t later = 0, behind, all;  // owners of the chunks behind this one
+  for (int c = blockIdx.x + 1 + threadIdx.x; c < (int)gridDim.x; c += kFreeThreads) later += owners[c];
+  (void)block_scan<kFreeThreads>(later, part, &behind);
+  const uint64_t upto = block_scan<kFreeThreads>(__popc(own), part, &all);
+  give_back(a, p, own, e0, n0, (long long)(behind + all - upto));
+#pragma unroll
+  for (int i = 0; i < kFreeEach; ++i)
+    if (e0 + i < a.S * a.ldt && (e0 + i) % a.ldt == 0) a.held[(e0 + i) / a.ldt] = stays(a, held[(e0 + i) / a.ldt], (e0 + i) / a.ldt);
+  if (blockIdx.x == 0 && threadIdx.x == 0) *a.n_free = (int)min(n0 + (long long)(behind + all), (long long)a.pages);
+}
+
+// ---- copy ----
+constexpr int kCopyThreads = 256;
+constexpr int kInFlight = 8;  // 16-byte loads of a thread before its first store
+
+// One (entry, K or V, head) of a layer: up to a page's tokens.
+__global__ void __launch_bounds__(kCopyThreads) page_copy_kernel(btf_page_copy a, btf_kv_cache kv) {
+  const int h = blockIdx.x % kv.heads, rest = blockIdx.x / kv.heads, i = rest >> 1;
+  const int from = a.from[i], to = a.to[i], n = min(a.tokens ? a.tokens[i] : kv.page, kv.page);
+  if (from < 0 || from >= kv.pages || to < 0 || to >= kv.pages || from == to || n <= 0) return;
+  uint16_t* base = static_cast<uint16_t*>(rest & 1 ? kv.v : kv.k) + (size_t)blockIdx.y * a.layer_stride + (size_t)h * kv.head_stride;
+  const uint16_t* x = base + (size_t)from * kv.page_stride;
+  uint16_t* y = base + (size_t)to * kv.page_stride;
+  const int sh = __builtin_ctz(kv.dim) - 3, mask = (1 << sh) - 1, end = n << sh;  // 16-byte chunks
+  auto at = [&](int c) { return (size_t)(c >> sh) * kv.tok_stride + 8 * (c & mask); };
+  for (int c0 = threadIdx.x; c0 < end; c0 += kCopyThreads * kInFlight) {
+    u32x4 v[kInFlight];
+#pragma unroll
+    for (int u = 0; u < kInFlight; ++u)
+      if (c0 + u * kCopyThreads < end) v[u] = *reinterpret_cast<const u32x4*>(x + at(c0 + u * kCopyThreads));
+#pragma unroll
+    for (int u = 0; u < kInFlight; ++u)
+      if (c0 + u * kCopyThreads < end) *reinterpret_cast<u32x4*>(y + at(c0 + u * kCopyThreads)) = v[u];
+  }
+}
+
+// ---- move ----
+// In place a token's new place may be another's old one, but never that of a later
+// token of the list (places ascend, none goes up). A workgroup has one 128-byte run of
+// the values of one (request, K or V, head, layer) for all tokens: it reads a batch,
+// waits until all of its threads have theirs, writes it, and goes on. So no two
+// workgroups touch the same bytes, and nothing is overwritten before it was read.
+template <int N, bool TREE>
+__global__ void __launch_bounds__(N) cache_move_kernel(btf_cache_move a, btf_kv_cache kv) {
+  const int runs = kv.dim / 64;
+  int id = blockIdx.x;
+  const int run = id % runs;
+  id /= runs;
+  const int h = id % kv.heads;
+  id /= kv.heads;
+  const int s = id >> 1;
+  const int first = a.first[s];
+  unsigned long long bits = 0;
+  int lo = 0, n;
+  if (TREE) {
+    const int leaf = a.leaf[s];
+    if (leaf >= 0 && leaf < a.T) bits = a.tree[leaf];
+    n = __popcll(bits);
+  } else {
+    lo = max(a.source0[s], 0);
+    n = max(min(a.source0[s + 1], a.T) - lo, 0);
+  }
+  if (blockIdx.y == 0 && run == 0 && h == 0 && !(id & 1) && threadIdx.x == 0 && a.kv_len) a.kv_len[s] = first + n;
+  uint16_t* base = static_cast<uint16_t*>(id & 1 ? kv.v : kv.k) + (size_t)blockIdx.y * a.layer_stride +
+                   (size_t)h * kv.head_stride + 64 * run + 8 * (threadIdx.x & 7);
+  const int* tab = a.table + (size_t)s * a.ldt;
+  const int* tab_to = a.to_table ? a.to_table + (size_t)s * a.ldt_to : tab;
+  const int ld_to = a.to_table ? a.ldt_to : a.ldt;
+  const int sh = __builtin_ctz(kv.page);
+  // where a place's values are, counted from base; -1: not in the table or the cache
+  auto where = [&](const int* t, int ld, long long place) -> long long {
+    if (place < 0 || place >= (long long)ld << sh) return -1;
+    const int p = t[place >> sh];
+    return p < 0 || p >= kv.pages ? -1 : p * (long long)kv.page_stride + (place & (kv.page - 1)) * (long long)kv.tok_stride;
+  };
+  constexpr int kAtOnce = N / 8;  // tokens
+  constexpr int kMine = TREE ? 2 : kInFlight;
+  for (int i0 = 0; i0 < n; i0 += kAtOnce * kMine) {
+    u32x4 v[kMine];
+    long long to[kMine];
+#pragma unroll
+    for (int u = 0; u < kMine; ++u) {
+      const int i = i0 + u * kAtOnce + (threadIdx.x >> 3);
+      to[u] = -1;
+      if (i < n) {
+        long long from;
+        if (TREE) {  // the i-th set bit
+          unsigned long long b = bits;
+          int k = i, pos = 0;
+#pragma unroll
+          for (int half = 32; half; half >>= 1) {
+            const int c = __popcll(b & ((1ull << half) - 1));
+            if (k >= c) k -= c, pos += half, b >>= half;
+          }
+          from = (long long)first + pos;
+        } else {
+          from = a.source[lo + i];
+        }
+        const long long dst = (long long)first + i;
+        if (a.to_table || from != dst) {
+          const long long x = where(tab, a.ldt, from);
+          if (x >= 0) to[u] = where(tab_to, ld_to, dst);
+          if (to[u] >= 0) v[u] = *reinterpret_cast<const u32x4*>(base + x);
+        }
+      }
+    }
+    // every thread's loads have arrived before any thread stores
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < kMine; ++u)
+      if (to[u] >= 0) *reinterpret_cast<u32x4*>(base + to[u]) = v[u];
+  }
+}
+
+int free_chunks(int S, int ldt) { return (int)(((int64_t)S * ldt + kFreeChunk - 1) / kFreeChunk); }
+
+}  // namespace
+
+int page_fork(const btf_page_fork& a, hipStream_t st) {
+  if ((int64_t)a.F * a.ldt <= kForkSmall) {
+    hipLaunchKernelGGL(page_fork_kernel<true>, dim3(1), dim3(kForkThreads), 0, st, a);
+    return launch_status("page_fork_kernel");
+  }
+  hipLaunchKernelGGL(page_fork_kernel<false>, dim3(1), dim3(kForkThreads), 0, st, a);
+  const int rc = launch_status("page_fork_kernel");
+  if (rc != BTF_OK) return rc;
+  const int y = (a.ldt + 255) / 256;
+  hipLaunchKernelGGL(page_fork_rows_kernel, dim3(a.F, y < 64 ? y : 64), dim3(256), 0, st, a);
+  return launch_status("page_fork_rows_kernel");
+}
+
+int64_t page_free_ws_bytes(int S, int ldt) {
+  const int n = free_chunks(S, ldt);
+  return n <= 1 ? 0 : ((int64_t)n + S + 1) * 4;
+}
+
+int page_free(const btf_page_free& a, hipStream_t st) {
+  const int n = free_chunks(a.S, a.ldt);
+  if (n <= 1) {
+    hipLaunchKernelGGL(page_free_small_kernel, dim3(1), dim3(kFreeThreads), 0, st, a);
+    return launch_status("page_free_small_kernel");
+  }
+  if (a.shared) {
+    hipLaunchKernelGGL(page_free_lower_kernel, dim3(n), dim3(kFreeThreads), 0, st, a);
+    int rc = launch_status("page_free_lower_kernel");
+    if (rc != BTF_OK) return rc;
+    hipLaunchKernelGGL(page_free_mark_kernel, dim3(n), dim3(kFreeThreads), 0, st, a);
+    rc = launch_status("page_free_mark_kernel");
+    if (rc != BTF_OK) return rc;
+  }
+  hipLaunchKernelGGL(page_free_count_kernel, dim3(n), dim3(kFreeThreads), 0, st, a);
+  int rc = launch_status("page_free_count_kernel");
+  if (rc != BTF_OK) return rc;
+  hipLaunchKernelGGL(page_free_kernel, dim3(n), dim3(kFreeThreads), 0, st, a);
+  return launch_status("page_free_kernel");
+}
+
+int page_copy(const btf_page_copy& a, const btf_kv_cache& kv, hipStream_t st) {
+  hipLaunchKernelGGL(page_copy_kernel, dim3(2 * a.n * kv.heads, a.layers), dim3(kCopyThreads), 0, st, a, kv);
+  return launch_status("page_copy_kernel");
+}
+
+int cache_move(const btf_cache_move& a, const btf_kv_cache& kv, hipStream_t st) {
+  const dim3 grid(2 * a.S * kv.heads * (kv.dim / 64), a.layers);
+  // A tree's path in batches of 16 tokens, a list in batches of 1024.
+  if (a.tree) hipLaunchKernelGGL((cache_move_kernel<64, true>), grid, dim3(64), 0, st, a, kv);
+  else hipLaunchKernelGGL((cache_move_kernel<1024, false>), grid, dim3(1024), 0, st, a, kv);
+  return launch_status("cache_move_kernel");
+}
+
+}  // namespace btfhip

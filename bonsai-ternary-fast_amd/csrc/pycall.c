@@ -200,17 +200,19 @@ static int do_gemv_ex(PyObject* const* v, int* status) {
   return OK;
 }
 
-/* ---- launches that take one argument struct, or two (a serving step's operators) ----
- * layout(slot, cls, fields, size) describes the C struct of a class of btf_hip.py:
+/* ---- launches that take one argument struct, two, or one and a list of structs (a serving step's operators) ----
+ * layout(slot, cls, fields, size, table=0) describes the C struct of a class of btf_hip.py
+ * and returns its number (8 slots in each of two tables):
  * fields = ((name, kind, offset), ...), kind i int, q int64, f float, p pointer. A slot
  * is taken over by whoever describes it last (btf_hip.py executed again, under its own or
  * another name): objects of the classes before then go the ctypes path. */
-#define MAX_LAYOUTS 8
+#define TABLE 8    /* slots of a table */
+#define MAX_LAYOUTS 16
 #define MAX_FIELDS 24
 #define MAX_STRUCT 256
 typedef struct {
   PyObject* cls; /* NULL: empty */
-  Py_ssize_t n;
+  Py_ssize_t n, size;
   struct {
     PyObject* name;
     char kind;
@@ -226,14 +228,15 @@ static void drop(layout_t* L) {
 
 static PyObject* py_layout(PyObject* self, PyObject* const* v, Py_ssize_t n) {
   layout_t L = {0};
-  Py_ssize_t slot = -1, size = -1;
-  if (n == 4 && PyLong_Check(v[0]) && PyTuple_CheckExact(v[2]) && PyLong_Check(v[3])) {
+  Py_ssize_t slot = -1, size = -1, table = 0;
+  if ((n == 4 || (n == 5 && PyLong_Check(v[4]))) && PyLong_Check(v[0]) && PyTuple_CheckExact(v[2]) && PyLong_Check(v[3])) {
     slot = PyLong_AsSsize_t(v[0]);
     size = PyLong_AsSsize_t(v[3]);
+    if (n == 5) table = PyLong_AsSsize_t(v[4]);
     if (PyErr_Occurred()) return NULL;
   }
-  if (slot < 0 || slot >= MAX_LAYOUTS || size < 0 || size > MAX_STRUCT || PyTuple_GET_SIZE(v[2]) > MAX_FIELDS) {
-    PyErr_SetString(PyExc_ValueError, "layout(slot, cls, fields, size)");
+  if (slot < 0 || slot >= TABLE || table < 0 || table >= MAX_LAYOUTS / TABLE || size < 0 || size > MAX_STRUCT || PyTuple_GET_SIZE(v[2]) > MAX_FIELDS) {
+    PyErr_SetString(PyExc_ValueError, "layout(slot, cls, fields, size, table=0)");
     return NULL;
   }
   for (; L.n < PyTuple_GET_SIZE(v[2]); ++L.n) {
@@ -250,6 +253,8 @@ static PyObject* py_layout(PyObject* self, PyObject* const* v, Py_ssize_t n) {
   }
   Py_INCREF(v[1]);
   L.cls = v[1];
+  L.size = size;
+  slot += TABLE * table;
   layout_t old = layouts[slot];
   layouts[slot] = L;
   drop(&old);
@@ -307,6 +312,36 @@ static int do_launch(PyObject* const* v, int* status) {
   return OK;
 }
 
+/* launch_list(function address, layout of a, a, layout of the list's elements, list of 1 .. 3, stream) */
+static int do_launch_list(PyObject* const* v, int* status) {
+  _Alignas(8) char a[MAX_STRUCT] = {0}, b[MAX_SEGS * MAX_STRUCT] = {0};
+  btf_stream_t st;
+  int la, lb;
+  if (!PyLong_CheckExact(v[0])) return OTHER;
+  void* f = PyLong_AsVoidPtr(v[0]);
+  if (!f) return PyErr_Occurred() ? RAISED : OTHER;
+  TRY(read_int(v[1], &la));
+  TRY(read_int(v[3], &lb));
+  if (la < 0 || la >= MAX_LAYOUTS || lb < 0 || lb >= MAX_LAYOUTS) return OTHER;
+  TRY(read_struct(v[2], la, a));
+  if (!PyList_CheckExact(v[4]) && !PyTuple_CheckExact(v[4])) return OTHER;
+  const Py_ssize_t n = PySequence_Fast_GET_SIZE(v[4]);
+  if (n < 1 || n > MAX_SEGS) return OTHER;
+  for (Py_ssize_t i = 0; i < n; ++i) {
+    if (i >= PySequence_Fast_GET_SIZE(v[4])) return OTHER; /* (as in read_segs) */
+    PyObject* s = PySequence_Fast_GET_ITEM(v[4], i);
+    Py_INCREF(s);
+    const int rc = read_struct(s, lb, b + i * layouts[lb].size);
+    Py_DECREF(s);
+    if (rc != OK) return rc;
+  }
+  TRY(read_stream(v[5], &st));
+  Py_BEGIN_ALLOW_THREADS
+  *status = ((int (*)(const void*, const void*, int, btf_stream_t))f)(a, b, (int)n, st);
+  Py_END_ALLOW_THREADS
+  return OK;
+}
+
 static int args(Py_ssize_t got, Py_ssize_t want) {
   if (got == want) return 1;
   PyErr_Format(PyExc_TypeError, "%zd arguments, got %zd", want, got);
@@ -317,6 +352,12 @@ static PyObject* py_launch(PyObject* self, PyObject* const* v, Py_ssize_t n) {
   int status = 0;
   if (!args(n, 6)) return NULL;
   const int rc = do_launch(v, &status);
+  return answer(rc, status);
+}
+static PyObject* py_launch_list(PyObject* self, PyObject* const* v, Py_ssize_t n) {
+  int status = 0;
+  if (!args(n, 6)) return NULL;
+  const int rc = do_launch_list(v, &status);
   return answer(rc, status);
 }
 static PyObject* py_prep(PyObject* self, PyObject* const* v, Py_ssize_t n) {
@@ -375,6 +416,7 @@ static PyMethodDef methods[] = {
     {"gemv_ex", (PyCFunction)(void (*)(void))py_gemv_ex, METH_FASTCALL, NULL},
     {"layout", (PyCFunction)(void (*)(void))py_layout, METH_FASTCALL, NULL},
     {"launch", (PyCFunction)(void (*)(void))py_launch, METH_FASTCALL, NULL},
+    {"launch_list", (PyCFunction)(void (*)(void))py_launch_list, METH_FASTCALL, NULL},
     {NULL, NULL, 0, NULL}};
 
 static struct PyModuleDef module = {PyModuleDef_HEAD_INIT, "_btf_call", NULL, -1, methods, NULL, NULL, NULL, NULL};

@@ -37,6 +37,38 @@ int check_kv(const btf_kv_cache* kv, const char* who, bool need_data) {
   return BTF_OK;
 }
 
+// What the attentions ask of the arguments that they have in common.
+template <class A>
+int check_attention(const A* a, const btf_kv_cache* kv, const char* who) {
+  const int rc = check_kv(kv, who, true);
+  if (rc != BTF_OK) return rc;
+  if (a->heads < 1 || a->heads % kv->heads) return bad(who, "heads must be a multiple of the KV heads");
+  if (!a->q || !a->table || !a->row0 || !a->kv_len || !a->out) return bad(who, "null pointer");
+  if (!aligned(a->q, 16) || a->ldq % 8 || (int64_t)a->ldq < (int64_t)a->heads * kv->dim)
+    return bad(who, "q must be 16-byte aligned with ldq % 8 == 0 and ldq >= heads * dim");
+  if (!aligned(a->out, 16) || a->ldo % 4 || (int64_t)a->ldo < (int64_t)a->heads * kv->dim)
+    return bad(who, "out must be 16-byte aligned with ldo % 4 == 0 and ldo >= heads * dim");
+  if (a->heads > 65535 || (int64_t)a->T * a->heads > 0x7fffffff)
+    return bad(who, "heads above 65535, or rows times heads above 2^31");
+  if (a->ldt < 1) return bad(who, "ldt must be at least 1");
+  if (!aligned(a->tree, 8)) return bad(who, "tree must be 8-byte aligned");
+  if (!(a->scale == a->scale)) return bad(who, "scale is not a number");
+  if (!a->ws || !aligned(a->ws, 16)) return bad(who, "ws must be 16-byte aligned scratch");
+  return BTF_OK;
+}
+
+// A cache that is written, in several layers.
+int check_layers(const btf_kv_cache* kv, int layers, int64_t stride, const char* who) {
+  const int rc = check_kv(kv, who, true);
+  if (rc != BTF_OK) return rc;
+  if (layers < 1 || layers > kMaxY) return bad(who, "layers must be in [1, 65535]");
+  if ((kv->heads > 1 && kv->head_stride < kv->dim) || (kv->pages > 1 && kv->page_stride < kv->dim) ||
+      (layers > 1 && stride < kv->dim))
+    return bad(who, "heads, pages or layers of the cache overlap");
+  if (layers > 1 && stride % 8) return bad(who, "layer_stride must be a multiple of 8 values");
+  return BTF_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -119,23 +151,10 @@ int64_t btf_hip_paged_attention_ws_bytes(int S, int T, int heads, const btf_kv_c
 int btf_hip_launch_paged_attention(const btf_paged_attention* a, const btf_kv_cache* kv, btf_stream_t stream) {
   if (!a) return bad("paged_attention", "null arguments");
   if (a->S <= 0 || a->T <= 0) return BTF_OK;
-  const int rc = check_kv(kv, "paged_attention", true);
+  const int rc = check_attention(a, kv, "paged_attention");
   if (rc != BTF_OK) return rc;
-  if (a->heads < 1 || a->heads % kv->heads) return bad("paged_attention", "heads must be a multiple of the KV heads");
-  if (!a->q || !a->table || !a->row0 || !a->kv_len || !a->out) return bad("paged_attention", "null pointer");
-  if (!aligned(a->q, 16) || a->ldq % 8 || (int64_t)a->ldq < (int64_t)a->heads * kv->dim)
-    return bad("paged_attention", "q must be 16-byte aligned with ldq % 8 == 0 and ldq >= heads * dim");
-  if (!aligned(a->out, 16) || a->ldo % 4 || (int64_t)a->ldo < (int64_t)a->heads * kv->dim)
-    return bad("paged_attention", "out must be 16-byte aligned with ldo % 4 == 0 and ldo >= heads * dim");
-  if (a->heads > 65535 || (int64_t)a->T * a->heads > 0x7fffffff)
-    return bad("paged_attention", "heads above 65535, or rows times heads above 2^31");
   if (a->T > kMaxGroups || paged_attention_most_items(a->S, a->T, a->heads, *kv) > kMaxGroups)
     return bad("paged_attention", "more rows or requests than a launch takes");
-  if (a->ldt < 1) return bad("paged_attention", "ldt must be at least 1");
-  if (!aligned(a->tree, 8)) return bad("paged_attention", "tree must be 8-byte aligned");
-  if (!(a->scale == a->scale)) return bad("paged_attention", "scale is not a number");
-  if (paged_attention_ws_bytes(a->S, a->T, a->heads, *kv) > 0 && (!a->ws || !aligned(a->ws, 16)))
-    return bad("paged_attention", "ws must be 16-byte aligned scratch");
   if (!current_state()) return BTF_ERR_NOT_INIT;
   return paged_attention(*a, *kv, static_cast<hipStream_t>(stream));
 }
@@ -152,6 +171,122 @@ int btf_hip_launch_sample(const btf_sampling* a, btf_stream_t stream) {
   if (sample_ws_bytes(a->M, a->V) > 0 && (!a->ws || !aligned(a->ws, 8))) return bad("sample", "ws must be 8-byte aligned scratch");
   if (!current_state()) return BTF_ERR_NOT_INIT;
   return sample(*a, static_cast<hipStream_t>(stream));
+}
+
+int btf_hip_launch_page_fork(const btf_page_fork* a, btf_stream_t stream) {
+  if (!a) return bad("page_fork", "null arguments");
+  if (a->F <= 0) return BTF_OK;
+  if (a->F > 1024) return bad("page_fork", "more than 1024 forks");
+  if (a->S < 1) return bad("page_fork", "no rows of table");
+  if (a->page < 1 || (a->page & (a->page - 1))) return bad("page_fork", "page must be a power of two");
+  if (a->ldt < 1) return bad("page_fork", "ldt must be at least 1");
+  if (a->pages < 1 || a->pages > (int64_t)0x7fffffff / a->page) return bad("page_fork", "pages * page must be in [1, 2^31)");
+  if (!a->src || !a->dst || !a->tokens || !a->free_list || !a->n_free || !a->table || !a->held || !a->shared || !a->got ||
+      !a->copy_from || !a->copy_to || !a->copy_tokens)
+    return bad("page_fork", "null pointer");
+  if (!current_state()) return BTF_ERR_NOT_INIT;
+  return page_fork(*a, static_cast<hipStream_t>(stream));
+}
+
+int btf_hip_launch_page_copy(const btf_page_copy* a, const btf_kv_cache* kv, btf_stream_t stream) {
+  if (!a) return bad("page_copy", "null arguments");
+  if (a->n <= 0) return BTF_OK;
+  const int rc = check_layers(kv, a->layers, a->layer_stride, "page_copy");
+  if (rc != BTF_OK) return rc;
+  if (!a->from || !a->to) return bad("page_copy", "null pointer");
+  if ((int64_t)2 * a->n * kv->heads > kMaxGroups) return bad("page_copy", "more entries times heads than a launch takes");
+  if (!current_state()) return BTF_ERR_NOT_INIT;
+  return page_copy(*a, *kv, static_cast<hipStream_t>(stream));
+}
+
+int64_t btf_hip_page_free_ws_bytes(int S, int ldt) {
+  return S > 0 && ldt > 0 && (int64_t)S * ldt < 1 << 29 ? page_free_ws_bytes(S, ldt) : 0;
+}
+
+int btf_hip_launch_page_free(const btf_page_free* a, btf_stream_t stream) {
+  if (!a) return bad("page_free", "null arguments");
+  if (a->S <= 0) return BTF_OK;
+  if (a->page < 1 || (a->page & (a->page - 1))) return bad("page_free", "page must be a power of two");
+  if (a->ldt < 1) return bad("page_free", "ldt must be at least 1");
+  if ((int64_t)a->S * a->ldt >= 1 << 29) return bad("page_free", "S * ldt must be below 2^29");
+  if (a->pages < 1 || a->pages > (int64_t)0x7fffffff / a->page) return bad("page_free", "pages * page must be in [1, 2^31)");
+  if (!a->keep || !a->table || !a->held || !a->free_list || !a->n_free) return bad("page_free", "null pointer");
+  if (page_free_ws_bytes(a->S, a->ldt) > 0 && (!a->ws || !aligned(a->ws, 4)))
+    return bad("page_free", "ws must be 4-byte aligned scratch");
+  if (!current_state()) return BTF_ERR_NOT_INIT;
+  return page_free(*a, static_cast<hipStream_t>(stream));
+}
+
+int btf_hip_launch_cache_move(const btf_cache_move* a, const btf_kv_cache* kv, btf_stream_t stream) {
+  if (!a) return bad("cache_move", "null arguments");
+  if (a->S <= 0) return BTF_OK;
+  const int rc = check_layers(kv, a->layers, a->layer_stride, "cache_move");
+  if (rc != BTF_OK) return rc;
+  if (a->T < 0) return bad("cache_move", "negative T");
+  if (!a->table || !a->first) return bad("cache_move", "null pointer");
+  if ((a->tree != nullptr) == (a->source != nullptr)) return bad("cache_move", "either tree or source");
+  if (a->tree ? !a->leaf : !a->source0) return bad("cache_move", "tree needs leaf, source needs source0");
+  if (!aligned(a->tree, 8)) return bad("cache_move", "tree must be 8-byte aligned");
+  if (a->ldt < 1 || (a->to_table && a->ldt_to < 1)) return bad("cache_move", "ldt must be at least 1");
+  if ((int64_t)2 * a->S * kv->heads * (kv->dim / 64) > kMaxGroups / 4)
+    return bad("cache_move", "more requests times heads than a launch takes");
+  if (!current_state()) return BTF_ERR_NOT_INIT;
+  return cache_move(*a, *kv, static_cast<hipStream_t>(stream));
+}
+
+int64_t btf_hip_shared_attention_ws_bytes(int S, int T, int heads, const btf_kv_cache* kv) {
+  if (S <= 0 || T <= 0 || check_kv(kv, "shared_attention_ws_bytes", false) != BTF_OK || heads < 1 || heads % kv->heads)
+    return 0;
+  return shared_attention_ws_bytes(S, T, heads, *kv);
+}
+
+int btf_hip_launch_shared_attention(const btf_shared_attention* a, const btf_kv_cache* kv, btf_stream_t stream) {
+  if (!a) return bad("shared_attention", "null arguments");
+  if (a->S <= 0 || a->T <= 0) return BTF_OK;
+  const int rc = check_attention(a, kv, "shared_attention");
+  if (rc != BTF_OK) return rc;
+  if (a->groups < 0 || a->groups > a->S) return bad("shared_attention", "groups must be in [0, S]");
+  if (a->groups && (!a->group0 || !a->lead || !a->shared)) return bad("shared_attention", "null pointer of the groups");
+  if (a->T > kMaxGroups || shared_attention_most_items(a->S, a->T, a->heads, *kv) > kMaxGroups)
+    return bad("shared_attention", "more rows or requests than a launch takes");
+  if (!current_state()) return BTF_ERR_NOT_INIT;
+  return shared_attention(*a, *kv, static_cast<hipStream_t>(stream));
+}
+
+int64_t btf_hip_lora_ws_bytes(int S, int T, int K, int rank, int nseg) {
+  if (S <= 0 || T <= 0 || K <= 0 || rank <= 0 || rank > 256 || nseg < 1 || nseg > 3) return 0;
+  return lora_ws_bytes(S, T, K, rank, nseg);
+}
+
+int btf_hip_launch_lora(const btf_lora* a, const btf_lora_seg* segs, int nseg, btf_stream_t stream) {
+  if (!a) return bad("lora", "null arguments");
+  if (a->S <= 0 || a->T <= 0) return BTF_OK;
+  if (nseg < 1 || nseg > 3 || !segs) return bad("lora", "1..3 segments");
+  if (a->mode != BTF_GEMV_ADD && a->mode != BTF_GEMV_SWIGLU) return bad("lora", "mode must be add or swiglu");
+  const bool glu = a->mode == BTF_GEMV_SWIGLU;
+  if (glu && (nseg != 2 || segs[0].N != segs[1].N)) return bad("lora", "swiglu takes two segments of the same N");
+  if (a->K < 32 || a->K % 32) return bad("lora", "K must be a positive multiple of 32");
+  if (a->rank < 8 || a->rank % 8 || a->rank > 256) return bad("lora", "rank must be a multiple of 8 up to 256");
+  if (a->adapters < 0) return bad("lora", "negative number of adapters");
+  if (a->type != BTF_F16 && a->type != BTF_BF16) return bad("lora", "unknown type");
+  if (!a->row0 || !a->adapter || !a->x) return bad("lora", "null pointer");
+  if (!aligned(a->x, 16) || a->ldx % 4 || a->ldx < a->K) return bad("lora", "x must be 16-byte aligned with ldx % 4 == 0 and ldx >= K");
+  if (glu && (!a->out || !aligned(a->out, 4) || a->ldo < segs[0].N)) return bad("lora", "swiglu needs out with ldo >= N");
+  int64_t outs = 0;
+  for (int i = 0; i < nseg; ++i) {
+    const btf_lora_seg& g = segs[i];
+    if (g.N < 1) return bad("lora", "a segment needs outputs");
+    if (!g.y || !aligned(g.y, 4) || g.ldy < g.N) return bad("lora", "y must be given with ldy >= N");
+    if (a->adapters && (!g.a || !g.b)) return bad("lora", "null adapters");
+    if (!aligned(g.a, 16) || !aligned(g.b, 16)) return bad("lora", "a and b must be 16-byte aligned");
+    if (g.a_stride < 0 || g.b_stride < 0 || g.a_stride % 8 || g.b_stride % 8)
+      return bad("lora", "adapter strides must be multiples of 8 values");
+    outs += g.N;
+  }
+  if (a->S > kMaxGroups / 4 || a->T > kMaxGroups / 4 || outs > 1 << 24) return bad("lora", "more requests, rows or outputs than a launch takes");
+  if (!a->ws || !aligned(a->ws, 16)) return bad("lora", "ws must be 16-byte aligned scratch");
+  if (!current_state()) return BTF_ERR_NOT_INIT;
+  return lora(*a, segs, nseg, static_cast<hipStream_t>(stream));
 }
 
 }  // extern "C"

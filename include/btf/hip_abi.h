@@ -593,6 +593,199 @@ typedef struct btf_sampling {
 int64_t btf_hip_sample_ws_bytes(int M, int V);
 int btf_hip_launch_sample(const btf_sampling* a, btf_stream_t stream);
 
+/* ---- requests that share --------------------------------------------------
+ * Samples of one prompt, beams and requests behind one long instruction hold the
+ * same cache pages. shared[p] counts the holders of page p beyond one: 0 for a
+ * page that one request holds and for a free page, so launch_page_plan, which
+ * knows nothing of it, hands out pages that are counted right. A shared page is
+ * full and is not written again: a request writes behind its last token only.
+ * All lengths and ids are device data, as above. */
+
+/* Request rows of `table` that begin as copies of others: fork f makes row dst[f]
+ * hold the first tokens[f] tokens of row src[f]. Its whole pages are shared
+ * (their ids copied, shared + 1); where the tokens end inside a page, the fork
+ * gets a page of its own from the end of the free list (the first fork that needs
+ * one free_list[*n_free - 1]) and copy_from, copy_to, copy_tokens[f] say what
+ * launch_page_copy then has to copy in every layer (-1, -1, 0: nothing).
+ * got[f] = tokens[f], held[dst[f]] = its pages; held, *n_free, shared and table
+ * are updated in place. A fork is refused (got -1, nothing changes) if src or dst
+ * is not in [0, S), they are the same, tokens[f] is negative or passes
+ * held[src] * page, held[src] passes ldt, held[dst] is not 0 before the call, an
+ * earlier fork of the call that is not refused for these reasons has the same
+ * dst, or the free pages do not reach for it and those before it (then every
+ * later fork that needs a page is refused, too). So a row that a fork of the call
+ * begins is no source in the same call. */
+typedef struct btf_page_fork {
+  int F, S;              /* forks (up to 1024), rows of table */
+  int page;              /* tokens of a page: a power of two */
+  int ldt;               /* page ids that a row of table holds */
+  int64_t pages;         /* pages of the cache */
+  const int* src;        /* [F] */
+  const int* dst;        /* [F] */
+  const int* tokens;     /* [F] */
+  const int* free_list;  /* page ids, at least *n_free */
+  int* n_free;           /* [1] */
+  int* table;            /* [S][ldt] */
+  int* held;             /* [S] */
+  int* shared;           /* [pages] */
+  int* got;              /* [F] */
+  int* copy_from;        /* [F] */
+  int* copy_to;          /* [F] */
+  int* copy_tokens;      /* [F] */
+} btf_page_fork;
+int btf_hip_launch_page_fork(const btf_page_fork* a, btf_stream_t stream);
+
+/* K and V of the first tokens[i] tokens (NULL: all) of page from[i] to page to[i],
+ * in every layer: layer l's cache lies l * layer_stride values behind kv's.
+ * Entries whose ids are not in [0, pages) or are the same are left out. A page
+ * that two entries write, or that one writes and another reads, holds either's
+ * values. Layers, heads and pages that overlap (strides below dim) are refused. */
+typedef struct btf_page_copy {
+  int n;                 /* entries: n * KV heads below 2^23 */
+  const int* from;       /* [n] */
+  const int* to;         /* [n] */
+  const int* tokens;     /* [n] or NULL */
+  int layers;            /* 1 .. 65535 */
+  int64_t layer_stride;  /* values, a multiple of 8 (layers > 1) */
+} btf_page_copy;
+int btf_hip_launch_page_copy(const btf_page_copy* a, const btf_kv_cache* kv, btf_stream_t stream);
+
+/* Gives back what the requests hold behind their first keep[s] tokens (0 or less:
+ * all; a request that stays as it is has any number from held[s] * page on): the
+ * pages' ids in table become -1, held[s] the pages that stay, a page that others
+ * hold loses a count of shared, and a page that nobody holds any more goes to the
+ * end of the free list. They go there in the opposite order of their places (a
+ * page that several rows give up: at its first), so that giving back what a plan
+ * or forks have just handed out leaves the list as it was. shared NULL: no page
+ * has two holders. held[s] is taken as at most ldt; ids that are not in [0, pages)
+ * are dropped; the list never gets more than `pages` entries. A page given up more
+ * often in one call than it has holders goes back once.
+ * ws: page_free_ws_bytes of device scratch, 4-byte aligned, one for each stream that
+ * launches; it need not be cleared, and the bytes for the largest S and ldt serve all. */
+typedef struct btf_page_free {
+  int S, page, ldt;      /* S * ldt below 2^29 */
+  int64_t pages;
+  const int* keep;       /* [S] */
+  int* table;            /* [S][ldt] */
+  int* held;             /* [S] */
+  int* shared;           /* [pages] or NULL */
+  int* free_list;        /* [pages] */
+  int* n_free;           /* [1] */
+  void* ws;
+} btf_page_free;
+int64_t btf_hip_page_free_ws_bytes(int S, int ldt);
+int btf_hip_launch_page_free(const btf_page_free* a, btf_stream_t stream);
+
+/* Tokens that stay are moved together, K and V, in every layer (as page_copy): the
+ * i-th kept token of request s goes to place first[s] + i, and kv_len[s]
+ * (optional) = first[s] + their number. Which are kept:
+ *  - tree and leaf: those whose bit tree[leaf[s]] has (the row leaf[s] of the step
+ *    and its ancestors, as launch_page_plan gives them; a leaf not in [0, T): none),
+ *    bit j being place first[s] + j: the accepted path of a drafted tree;
+ *  - source and source0: the places source[source0[s]] .. source[source0[s+1] - 1]
+ *    (as far as there are T), a cache that drops tokens.
+ * Places are looked up in the rows of table, where they go to in those of to_table;
+ * NULL: table, in place. In place the listed places have to ascend and none may lie
+ * before the place that it goes to (else some tokens hold another's values), and
+ * pages from first[s] on must not be shared: a request that shares them moves its
+ * tokens to pages of its own, which no row that is read has. Tokens whose place or
+ * page is not in the table or the cache stay out. */
+typedef struct btf_cache_move {
+  int S;
+  int T;                  /* rows of tree, or entries of source */
+  const int* table;       /* [S][ldt] */
+  int ldt;
+  const int* to_table;    /* [S][ldt_to] or NULL */
+  int ldt_to;
+  const int* first;       /* [S] */
+  const uint64_t* tree;   /* [T] or NULL */
+  const int* leaf;        /* [S] with tree */
+  const int* source;      /* [T] or NULL */
+  const int* source0;     /* [S + 1] with source */
+  int* kv_len;            /* [S] or NULL */
+  int layers;             /* 1 .. 65535 */
+  int64_t layer_stride;   /* values, a multiple of 8 (layers > 1) */
+} btf_cache_move;
+int btf_hip_launch_cache_move(const btf_cache_move* a, const btf_kv_cache* kv, btf_stream_t stream);
+
+/* launch_paged_attention for requests of which some share a prefix: what it gives,
+ * with the prefix read and multiplied once for all rows of a group. Group g is
+ * requests group0[g] .. group0[g+1] - 1; the first shared[g] tokens of theirs are
+ * the tokens in row lead[g] of table (one of the S rows: the same pages as in the
+ * members' rows, or pages with the same values). Requests before group0[0] or from
+ * group0[groups] on are attended to alone, as is a member that has less than
+ * shared[g] tokens before its new rows (a refused one gives zeros, as there), and
+ * all of a group whose lead is not in [0, S). group0 has to ascend, in [0, S].
+ * The other arguments, trees and masks are launch_paged_attention's. ws:
+ * shared_attention_ws_bytes of device scratch for the launch's S, T and heads,
+ * 16-byte aligned, one for each stream that launches; it need not be cleared, and
+ * the bytes for the largest S and T serve every launch of these heads. */
+typedef struct btf_shared_attention {
+  int S, T, heads;
+  const void* q;
+  int ldq;
+  const int* table;
+  int ldt;
+  const int* row0;
+  const int* kv_len;
+  const uint64_t* tree;
+  float scale;
+  float* out;
+  int ldo;
+  void* ws;
+  int groups;            /* 0 .. S */
+  const int* group0;     /* [groups + 1] */
+  const int* lead;       /* [groups] */
+  const int* shared;     /* [groups] tokens */
+} btf_shared_attention;
+int64_t btf_hip_shared_attention_ws_bytes(int S, int T, int heads, const btf_kv_cache* kv);
+int btf_hip_launch_shared_attention(const btf_shared_attention* a, const btf_kv_cache* kv, btf_stream_t stream);
+
+/* Low-rank adapters of the requests beside a projection that all share: for the rows
+ * row0[s] .. row0[s+1] - 1 of a request with adapter id = adapter[s] in [0, adapters)
+ * and each of 1 to 3 segments,
+ *  BTF_GEMV_ADD:    y += scale[id] * B_id (A_id x);
+ *  BTF_GEMV_SWIGLU: (two segments of the same N: gate and up, as launch_gemv stored
+ *   them) out = silu(g + its delta) * (u + its delta); g and u stay. out may be the
+ *   gate's y itself.
+ * Other ids: no delta. x is the projection's input before its transform and
+ * quantization (launch_prep's xn_out), fp32. A_id: `rank` rows of K values at
+ * a + id * a_stride, B_id: N rows of `rank` values at b + id * b_stride, of which
+ * the adapter uses the first ranks[id] (NULL: all; clamped to [0, rank]); what lies
+ * behind them has no effect. Products and sums are in 32 bits. The order of a row's
+ * sums follows from K, the rank and, by the launch's tiles, S and T.
+ * Rows from row0[S] on are left as they were. ws: lora_ws_bytes of device scratch,
+ * 16-byte aligned, one for each stream that launches; it need not be cleared, and the
+ * bytes for the largest of each argument serve every launch. */
+typedef struct btf_lora_seg {
+  const void* a;         /* [adapters][rank][K], 16 bits, 16-byte aligned */
+  const void* b;         /* [adapters][N][rank], 16 bits, 16-byte aligned */
+  int64_t a_stride;      /* values between adapters, multiples of 8 */
+  int64_t b_stride;
+  int N;
+  float* y;              /* [T][ldy] */
+  int ldy;
+} btf_lora_seg;
+typedef struct btf_lora {
+  int S, T;              /* requests, rows (below 2^24) */
+  int K;                 /* a multiple of 32 */
+  int rank;              /* ranks that a and b have room for: a multiple of 8 up to 256 */
+  int adapters;
+  int type;              /* BTF_F16 or BTF_BF16 */
+  int mode;              /* BTF_GEMV_ADD or BTF_GEMV_SWIGLU */
+  const int* row0;       /* [S + 1] */
+  const int* adapter;    /* [S] */
+  const int* ranks;      /* [adapters] or NULL */
+  const float* scale;    /* [adapters] or NULL: 1 */
+  const float* x;        /* [T][ldx], 16-byte aligned, ldx % 4 == 0 */
+  int ldx;
+  float* out;            /* [T][ldo], SWIGLU */
+  int ldo;
+  void* ws;
+} btf_lora;
+int64_t btf_hip_lora_ws_bytes(int S, int T, int K, int rank, int nseg);
+int btf_hip_launch_lora(const btf_lora* a, const btf_lora_seg* segs, int nseg, btf_stream_t stream);
+
 /* Device description for reports. name must hold name_len bytes. */
 typedef struct btf_device_info {
   int cu_count;
