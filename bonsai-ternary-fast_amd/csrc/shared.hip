@@ -1,6 +1,390 @@
-#include "common.h"
+// shared.hip -- attention of requests of which some share a prefix
+// (btf_hip_launch_shared_attention; gfx950).
+//
+// A row's softmax over prefix and own keys is put together from sums over pieces
+// of the keys, (maximum, sum, values) each, so the pieces of the prefix can be done
+// for the rows of all requests that see them at once. Two roles, both with the
+// kernels of attn_core.h: a group's rows are one request of many rows over the
+// prefix, all of which they see; each request's rows go over its own keys, from
+// where the prefix ends. shared_join_kernel puts a row's pieces of both together.
+//
+// shared_plan_kernel, one workgroup, finds who takes part (a member needs the whole
+// prefix before its new rows), cuts both roles into items of like size and writes
+// down which item is whose: with up to hundreds of requests a workgroup that looked
+// for itself, as launch_paged_attention's do, would read all lengths several times.
+// The prefix counts in steps of 32 keys, a block of the kernels; what is left of it
+// is done with each member's own keys, which its row of table has, too.
+#include <string>
+
+#include "../../include/btf/hip_abi.h"
+#include "attn_core.h"
+
 namespace btfhip {
-int64_t shared_attention_most_items(int, int, int, const btf_kv_cache&) { return 0; }
-int64_t shared_attention_ws_bytes(int, int, int, const btf_kv_cache&) { return 16; }
-int shared_attention(const btf_shared_attention&, const btf_kv_cache&, hipStream_t) { return fail(BTF_ERR_LAUNCH, "shared_attention: not built"); }
+namespace {
+
+// What the plan found of a group (first in the list) or a request.
+struct alignas(64) Found {
+  int s, row0, n, len, ctx, tiles, pieces, begin;  // as Req
+  int item0, slot0, C;
+  int flags;                                       // kTree, kCut
+  int group;                                       // of a request that takes part, else -1
+  int b, e, whole;                                 // requests of a group; tokens of its prefix
+};
+constexpr int kTree = 1, kCut = 2;
+static_assert(sizeof(Found) == 64, "one line");
+
+// The parts of the workspace.
+struct Ws {
+  int* items;     // [2] of the groups, of the requests
+  Found* found;   // [groups + S]
+  int* map[2];    // [most[i]] the group or request of an item
+  int* request;   // [T] of a row, -1: none
+  float* slots[2];
+  int most[2];
+};
+
+struct Plan : Args {
+  Ws ws;
+  int groups;
+  const int *group0, *lead, *shared;
+  int R[2];       // rows of a tile
+};
+
+constexpr int kPlanThreads = 1024;
+
+// Pieces of the keys for `work` tiles times keys in all: about `items` of like size (see target and least).
+__device__ __forceinline__ int piece_keys(uint64_t work, int R, int items) {
+  const uint64_t w = work / kStep;  // in the smallest pieces
+  const uint64_t c = w / (uint64_t)items + 1, few = w / kPlaces + 1;
+  const uint64_t l = (uint64_t)(least(R) / kStep);
+  const uint64_t f = few < l ? few : l;
+  return kStep * (int)(c > f ? c : f);
 }
+
+__global__ void __launch_bounds__(kPlanThreads) shared_plan_kernel(Plan p) {
+  __shared__ uint64_t part[kPlanThreads / 64];
+  __shared__ int sh_upto[kPlanThreads], sh_row0[kPlanThreads], sh_n[kPlanThreads];
+  const btf_paged_attention& a = p.a;
+  const btf_kv_cache& kv = p.kv;
+  const int G = a.heads / kv.heads, tid = threadIdx.x;
+  const long long cap = (long long)a.ldt * kv.page;
+  auto tiles_of = [&](int n, int R) { return n > 0 ? (int)(((long long)n * G + R - 1) / R) : 0; };
+  auto row_of = [&](int s) { return min(max(a.row0[s], 0), a.T); };
+  uint64_t work[2] = {0, 0};
+  // the groups
+  for (int g = tid; g < p.groups; g += kPlanThreads) {
+    Found f{};
+    f.b = min(max(p.group0[g], 0), a.S);
+    f.e = min(max(p.group0[g + 1], f.b), a.S);
+    f.s = p.lead[g];
+    f.row0 = row_of(f.b);
+    f.n = max(row_of(f.e) - f.row0, 0);
+    const bool there = f.s >= 0 && f.s < a.S && f.n > 0;
+    f.whole = p.shared[g];
+    f.len = f.ctx = there ? (int)(min((long long)max(f.whole, 0), min(cap, 0x7fffffffll)) & ~31ll) : 0;
+    f.tiles = f.len > 0 ? tiles_of(f.n, p.R[0]) : 0;
+    f.flags = kCut;
+    f.group = -1;
+    if (!there) f.s = 0;
+    work[0] += (uint64_t)f.tiles * (uint64_t)f.len;
+    p.ws.found[g] = f;
+  }
+  for (int t = tid; t < a.T; t += kPlanThreads) p.ws.request[t] = -1;
+  __threadfence_block();
+  __syncthreads();
+  // the requests
+  Found* const mine = p.ws.found + p.groups;
+  for (int s = tid; s < a.S; s += kPlanThreads) {
+    Found f{};
+    f.s = s;
+    f.row0 = max(a.row0[s], 0);
+    f.n = max(min(a.row0[s + 1], a.T) - f.row0, 0);
+    const int full = a.kv_len[s];
+    f.len = (int)max(0ll, min((long long)full, cap));
+    f.ctx = full - f.n;
+    f.tiles = tiles_of(f.n, p.R[1]);
+    f.group = -1;
+    if (p.groups > 0 && f.n > 0) {
+      int lo = 0, hi = p.groups - 1;  // the last group that begins at s or before
+      while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (p.group0[mid] <= s) lo = mid;
+        else hi = mid - 1;
+      }
+      const Found& g = p.ws.found[lo];
+      if (s >= g.b && s < g.e && g.len > 0 && f.ctx >= g.whole && f.row0 >= g.row0 && f.row0 + f.n <= g.row0 + g.n)
+        f.group = lo, f.begin = g.len;
+    }
+    f.flags = a.tree && f.n <= BTF_TREE_NODES ? kTree : 0;
+    work[1] += (uint64_t)f.tiles * (uint64_t)max(f.len - f.begin, 0);
+    mine[s] = f;
+  }
+  uint64_t all[2];
+  (void)block_scan<kPlanThreads>(work[0], part, &all[0]);
+  (void)block_scan<kPlanThreads>(work[1], part, &all[1]);
+#pragma unroll
+  for (int role = 0; role < 2; ++role) {
+    const int count = role ? a.S : p.groups;
+    Found* const list = role ? mine : p.ws.found;
+    const int C = piece_keys(all[role] * kv.heads, p.R[role], target(p.R[role]));
+    long long items = 0, slots = 0;  // before the chunk
+    for (int i0 = 0; i0 < count; i0 += kPlanThreads) {
+      const int i = i0 + tid;
+      int own = 0, cut = 0, row0 = 0, n = 0;
+      if (i < count) {
+        const Found& f = list[i];
+        const int pieces = max(1, (f.len - f.begin + C - 1) / C);
+        own = kv.heads * f.tiles * pieces;
+        cut = role == 0 || f.group >= 0 || pieces > 1;
+        row0 = f.row0, n = f.n;
+      }
+      uint64_t chunk, cuts;
+      const int upto = (int)block_scan<kPlanThreads>((uint64_t)own, part, &chunk);
+      const int slot = (int)block_scan<kPlanThreads>((uint64_t)(cut ? own : 0), part, &cuts);
+      sh_upto[tid] = upto;
+      sh_row0[tid] = row0, sh_n[tid] = n;
+      if (i < count) {
+        Found& f = list[i];
+        f.pieces = max(1, (f.len - f.begin + C - 1) / C);
+        f.C = C;
+        f.item0 = (int)items + upto - own;
+        f.slot0 = (int)slots + slot - (cut ? own : 0);
+        if (cut) f.flags |= kCut;
+      }
+      __syncthreads();
+      for (int k = tid; k < (int)chunk; k += kPlanThreads) {
+        int lo = 0, hi = kPlanThreads - 1;  // the first one with upto > k
+        while (lo < hi) {
+          const int mid = (lo + hi) >> 1;
+          if (sh_upto[mid] > k) hi = mid;
+          else lo = mid + 1;
+        }
+        if (items + k < p.ws.most[role]) p.ws.map[role][items + k] = i0 + lo;
+      }
+      if (role)
+        for (int w = tid >> 6; w < min(kPlanThreads, count - i0); w += kPlanThreads / 64)
+          for (int r = tid & 63; r < sh_n[w]; r += 64) p.ws.request[sh_row0[w] + r] = i0 + w;
+      items += (long long)chunk;
+      slots += (long long)cuts;
+      __syncthreads();
+    }
+    if (tid == 0) p.ws.items[role] = (int)min(items, (long long)p.ws.most[role]);
+  }
+}
+
+// One role's launch as the kernels take it: a.ws is its slots.
+typedef __attribute__((address_space(4))) const Found* found_p;
+typedef __attribute__((address_space(4))) const int* ints_p;
+struct Role : Args {
+  const int *items, *map;
+  const Found* found;
+  template <int R, bool SCALAR>
+  __device__ __forceinline__ bool find(int id, Req& q) const {
+    if (id >= *(ints_p)items) return false;
+    const found_p f = (found_p)found + ((ints_p)map)[id];
+    q.s = f->s, q.row0 = f->row0, q.n = f->n, q.len = f->len, q.ctx = f->ctx;
+    q.tiles = f->tiles, q.pieces = f->pieces, q.begin = f->begin, q.C = f->C;
+    q.local = id - f->item0;
+    q.slot = f->slot0;
+    q.tree = f->flags & kTree;
+    q.cut = f->flags & kCut;
+    if (!SCALAR) {  // (in vector registers)
+      auto vector = [](int& v) { asm("" : "+v"(v)); };
+      vector(q.s), vector(q.row0), vector(q.n), vector(q.len), vector(q.ctx), vector(q.tiles), vector(q.pieces);
+      vector(q.begin), vector(q.C), vector(q.local), vector(q.slot);
+    }
+    return true;
+  }
+};
+
+// The pieces of one row of one head, the group's and its own, put together: as attn_join_kernel.
+constexpr int kJoinWaves = 4;
+template <int D, bool ONE>
+__global__ void __launch_bounds__(64 * kJoinWaves) shared_join_kernel(Plan p) {
+  constexpr int E = D / 64;                 // values of a lane
+  constexpr int BY = ONE ? 1 : kJoinWaves;  // waves of a row
+  constexpr int AT = ONE ? 4 : 8;
+  typedef float vE __attribute__((ext_vector_type(E)));
+  const btf_paged_attention& a = p.a;
+  const int s = ((ints_p)p.ws.request)[blockIdx.x];
+  if (s < 0) return;  // the whole workgroup
+  const found_p f = (found_p)p.ws.found + p.groups + s;
+  if (!(f->flags & kCut)) return;
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int G = a.heads / p.kv.heads, h = ONE ? blockIdx.y * kJoinWaves + w : blockIdx.y, kvh = h / G;
+  if (h >= a.heads) return;
+  // a role's first piece of the row, and from one to the next
+  auto first_of = [&](const found_p f, int role, size_t& step, int& r) {
+    const int R = p.R[role], row = (blockIdx.x - f->row0) * G + h % G, tile = row / R;
+    const size_t slot = (size_t)R * (D + 2);
+    r = row % R;
+    step = (size_t)f->tiles * p.kv.heads * slot;
+    return p.ws.slots[role] + ((size_t)f->slot0 + (size_t)(f->tiles - 1 - tile) * p.kv.heads + kvh) * slot;
+  };
+  int n0 = 0, r0 = 0, r1;
+  size_t step0 = 0, step1;
+  const float* base0 = nullptr;
+  if (f->group >= 0) {
+    const found_p g = (found_p)p.ws.found + f->group;
+    n0 = g->pieces;
+    base0 = first_of(g, 0, step0, r0);
+  }
+  const float* base1 = first_of(f, 1, step1, r1);
+  const int n = n0 + f->pieces, R0 = p.R[0], R1 = p.R[1];
+  auto values = [&](int i) { return i < n0 ? base0 + i * step0 + r0 * D : base1 + (i - n0) * step1 + r1 * D; };
+  auto top_of = [&](int i) { return i < n0 ? base0[i * step0 + R0 * D + r0] : base1[(i - n0) * step1 + R1 * D + r1]; };
+  auto sum_of = [&](int i) { return i < n0 ? base0[i * step0 + R0 * D + R0 + r0] : base1[(i - n0) * step1 + R1 * D + R1 + r1]; };
+  float top = -INFINITY, sum = 0.f, l0 = 0.f;
+  if (lane < n) top = top_of(lane), l0 = sum_of(lane);
+  vE x[AT];
+  auto read = [&](int i0, int i, int m) {
+#pragma unroll
+    for (int u = 0; u < AT; ++u) x[u] = *reinterpret_cast<const vE*>(values(i0 + min(i + u * BY, m - 1)) + lane * E);
+  };
+  const int first = ONE ? 0 : w;
+  read(0, first, min(64, n));
+  const float m0 = top;
+  for (int i = 64 + lane; i < n; i += 64) top = fmaxf(top, top_of(i));
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
+  const float base = top == -INFINITY ? 0.f : top;
+  vE v = vE(0.f);
+  for (int i0 = 0; i0 < n; i0 += 64) {
+    float c = 0.f;
+    if (i0 + lane < n) {
+      c = fast_exp2((i0 ? top_of(i0 + lane) : m0) - base);
+      sum += c * (i0 ? sum_of(i0 + lane) : l0);
+    }
+    const int m = min(64, n - i0);
+    for (int i = first; i < m; i += AT * BY) {
+      if (i0 + i != first) read(i0, i, m);
+#pragma unroll
+      for (int u = 0; u < AT; ++u) {
+        const int j = min(i + u * BY, m - 1);
+        const float f = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(c), j));
+        if (i + u * BY < m) v += f * x[u];
+      }
+    }
+  }
+  sum = wave_sum_f(sum);
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  float* y = a.out + (size_t)blockIdx.x * a.ldo + h * D;
+  if (ONE) {
+    *reinterpret_cast<vE*>(y + lane * E) = v * inv;
+    return;
+  }
+  __shared__ float sh[kJoinWaves][D];
+  *reinterpret_cast<vE*>(&sh[w][lane * E]) = v;
+  __syncthreads();
+  for (int d = threadIdx.x; d < D; d += 64 * kJoinWaves) {
+    float x = sh[0][d];
+#pragma unroll
+    for (int i = 1; i < kJoinWaves; ++i) x += sh[i][d];
+    y[d] = x * inv;
+  }
+}
+
+// Rows of a tile of `count` groups or requests that have T rows in all (launch_paged_attention's rule).
+int tile_rows(int count, int T, int heads, const btf_kv_cache& kv) {
+  const int64_t rows = (int64_t)T * (heads / kv.heads);
+  if (rows <= 16 * (int64_t)count) return 16;
+  if (kv.dim == 256) return 64;
+  if (rows <= 32 * (int64_t)count) return 32;
+  return kv.dim == 64 || rows <= 128 * (int64_t)count ? 64 : 128;
+}
+
+// Items of a role at most: each tile's last piece may be a part of one.
+int64_t most_items(int count, int T, int heads, const btf_kv_cache& kv, int R) {
+  return ((int64_t)T * (heads / kv.heads) / R + count) * kv.heads + target(R);
+}
+
+// Floats of a role's slots, for a launch of up to S requests and T rows, whatever tiles it takes: slots * R is at most
+// T * heads + count * KV heads * R + target(R) * R, and count * R at most 4 T * heads / KV heads for the tiles above 16.
+int64_t slot_floats(int S, int T, int heads, const btf_kv_cache& kv) {
+  const int64_t rows = (int64_t)T * heads, few = 16 * (int64_t)S * kv.heads, top = kv.dim == 128 ? 128 : 64;
+  return (rows + (few > 4 * rows ? few : 4 * rows) + target(64) * top) * (kv.dim + 2);
+}
+
+int64_t up(int64_t n) { return (n + 255) & ~(int64_t)255; }
+
+// Bytes before the slots, for up to S requests and groups.
+int64_t plan_bytes(int S, int T, int heads, const btf_kv_cache& kv) {
+  const int64_t most = most_items(S, T, heads, kv, 16) + target(16);
+  return up(64 + 2 * (int64_t)S * sizeof(Found) + 8 * most + 4 * (int64_t)T);
+}
+
+template <int D, bool BF>
+int role_go(const Role& r, int R, unsigned grid, hipStream_t st) {
+  const dim3 blk(64 * kWaves);
+  if (R == 16) {
+    hipLaunchKernelGGL((attn_stream_kernel<D, BF, 1, Role>), dim3(grid), blk, 0, st, r);
+  } else if (R == 64) {
+    hipLaunchKernelGGL((attn_tile_kernel<D, BF, 1, Role>), dim3(grid), blk, 0, st, r);
+  } else if constexpr (D < 256) {
+    if (R == 32) {
+      hipLaunchKernelGGL((attn_stream_kernel<D, BF, 2, Role>), dim3(grid), blk, 0, st, r);
+    } else if constexpr (D == 128) {
+      hipLaunchKernelGGL((attn_tile_kernel<D, BF, 2, Role>), dim3(grid), blk, 0, st, r);
+    }
+  }
+  return launch_status("shared attention kernel");
+}
+
+template <int D, bool BF>
+int shared_go(const Plan& p, hipStream_t st) {
+  hipLaunchKernelGGL(shared_plan_kernel, dim3(1), dim3(kPlanThreads), 0, st, p);
+  int rc = launch_status("shared_plan_kernel");
+  if (rc != BTF_OK) return rc;
+  const int64_t room = ((int64_t)p.a.ldt * p.kv.page + kStep - 1) / kStep;
+  for (int role = p.groups ? 0 : 1; role < 2; ++role) {
+    Role r{{p.a, p.kv}, p.ws.items + role, p.ws.map[role], role ? p.ws.found + p.groups : p.ws.found};
+    r.a.ws = p.ws.slots[role];
+    const int64_t tiles = p.ws.most[role] - target(p.R[role]);
+    rc = role_go<D, BF>(r, p.R[role], (unsigned)(tiles * room < p.ws.most[role] ? tiles * room : p.ws.most[role]), st);
+    if (rc != BTF_OK) return rc;
+  }
+  const bool one = (int64_t)p.a.T * p.a.heads >= 2048;
+  const dim3 join(p.a.T, one ? (p.a.heads + kJoinWaves - 1) / kJoinWaves : p.a.heads), blk(64 * kJoinWaves);
+  if (one) hipLaunchKernelGGL((shared_join_kernel<D, true>), join, blk, 0, st, p);
+  else hipLaunchKernelGGL((shared_join_kernel<D, false>), join, blk, 0, st, p);
+  return launch_status("shared_join_kernel");
+}
+
+}  // namespace
+
+int64_t shared_attention_most_items(int S, int T, int heads, const btf_kv_cache& kv) {
+  return most_items(S, T, heads, kv, 16) + target(16);
+}
+
+int64_t shared_attention_ws_bytes(int S, int T, int heads, const btf_kv_cache& kv) {
+  return plan_bytes(S, T, heads, kv) + 2 * up(4 * slot_floats(S, T, heads, kv));
+}
+
+int shared_attention(const btf_shared_attention& a, const btf_kv_cache& kv, hipStream_t st) {
+  Plan p{};
+  p.a = btf_paged_attention{a.S, a.T, a.heads, a.q, a.ldq, a.table, a.ldt, a.row0, a.kv_len, a.tree, a.scale, a.out, a.ldo, a.ws};
+  p.kv = kv;
+  p.groups = a.groups;
+  p.group0 = a.group0, p.lead = a.lead, p.shared = a.shared;
+  p.R[0] = tile_rows(a.groups > 0 ? a.groups : 1, a.T, a.heads, kv);
+  p.R[1] = tile_rows(a.S, a.T, a.heads, kv);
+  char* at = static_cast<char*>(a.ws);
+  p.ws.items = reinterpret_cast<int*>(at);
+  p.ws.found = reinterpret_cast<Found*>(at + 64);
+  int* ints = reinterpret_cast<int*>(p.ws.found + a.groups + a.S);
+  for (int role = 0; role < 2; ++role) {
+    p.ws.most[role] = (int)most_items(role ? a.S : a.groups, a.T, a.heads, kv, p.R[role]);
+    p.ws.map[role] = ints;
+    ints += p.ws.most[role];
+  }
+  p.ws.request = ints;
+  float* slots = reinterpret_cast<float*>(at + plan_bytes(a.S, a.T, a.heads, kv));
+  p.ws.slots[0] = slots;
+  p.ws.slots[1] = slots + up(4 * slot_floats(a.S, a.T, a.heads, kv)) / 4;
+  const bool bf = kv.type == BTF_BF16;
+  if (kv.dim == 64) return bf ? shared_go<64, true>(p, st) : shared_go<64, false>(p, st);
+  if (kv.dim == 128) return bf ? shared_go<128, true>(p, st) : shared_go<128, false>(p, st);
+  return bf ? shared_go<256, true>(p, st) : shared_go<256, false>(p, st);
+}
+
+}  // namespace btfhip

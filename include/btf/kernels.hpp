@@ -136,6 +136,40 @@ inline void launch_sample(const Sampling& a, btf_stream_t st) {
   detail::check(btf_hip_launch_sample(&a, st), "launch_sample");
 }
 
+// ---- requests that share: cache pages, prefixes, the projection beside their adapters
+using PageFork = btf_page_fork;
+using PageCopy = btf_page_copy;
+using PageFree = btf_page_free;
+using CacheMove = btf_cache_move;
+using SharedAttention = btf_shared_attention;
+using LoraSeg = btf_lora_seg;
+using Lora = btf_lora;
+inline void launch_page_fork(const PageFork& a, btf_stream_t st) {
+  detail::check(btf_hip_launch_page_fork(&a, st), "launch_page_fork");
+}
+inline void launch_page_copy(const PageCopy& a, const KvCache& kv, btf_stream_t st) {
+  detail::check(btf_hip_launch_page_copy(&a, &kv, st), "launch_page_copy");
+}
+inline size_t page_free_ws_bytes(int S, int ldt) { return (size_t)btf_hip_page_free_ws_bytes(S, ldt); }
+inline void launch_page_free(const PageFree& a, btf_stream_t st) {
+  detail::check(btf_hip_launch_page_free(&a, st), "launch_page_free");
+}
+inline void launch_cache_move(const CacheMove& a, const KvCache& kv, btf_stream_t st) {
+  detail::check(btf_hip_launch_cache_move(&a, &kv, st), "launch_cache_move");
+}
+inline size_t shared_attention_ws_bytes(int S, int T, int heads, const KvCache& kv) {
+  return (size_t)btf_hip_shared_attention_ws_bytes(S, T, heads, &kv);
+}
+inline void launch_shared_attention(const SharedAttention& a, const KvCache& kv, btf_stream_t st) {
+  detail::check(btf_hip_launch_shared_attention(&a, &kv, st), "launch_shared_attention");
+}
+inline size_t lora_ws_bytes(int S, int T, int K, int rank, int nseg) {
+  return (size_t)btf_hip_lora_ws_bytes(S, T, K, rank, nseg);
+}
+inline void launch_lora(const Lora& a, const LoraSeg* segs, int nseg, btf_stream_t st) {
+  detail::check(btf_hip_launch_lora(&a, segs, nseg, st), "launch_lora");
+}
+
 // launch_gemv with the chain's quantizes fused in (no counterpart in
 // kernels.cuh: the decoder's launch_prep + launch_gemv pairs without norm or
 // transform, src/cuda/gpu_decoder.cu:411-418): input from Q8 rows `a` or fp32
