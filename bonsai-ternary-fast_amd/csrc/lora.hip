@@ -94,18 +94,19 @@ __device__ bool find(const btf_lora& a, int id, Tile& t) {
   const int lane = threadIdx.x & 63;
   int before = 0;
   for (int s0 = 0; s0 < a.S; s0 += 64) {
-    int r0 = 0, n = 0;
+    int r0 = 0, n = 0, who = -1;
     if (s0 + lane < a.S) {
       r0 = max(a.row0[s0 + lane], 0);
       n = min(a.row0[s0 + lane + 1], a.T) - r0;
+      who = a.adapter[s0 + lane];
     }
     const int mine = n > 0 ? (n + R - 1) / R : 0, upto = before + wave_scan(mine);
-    const unsigned long long who = __ballot(mine > 0 && id >= upto - mine && id < upto);
-    if (who) {
-      const int l = __builtin_ctzll(who), k = id - __builtin_amdgcn_readlane(upto - mine, l);
+    const unsigned long long here = __ballot(mine > 0 && id >= upto - mine && id < upto);
+    if (here) {
+      const int l = __builtin_ctzll(here), k = id - __builtin_amdgcn_readlane(upto - mine, l);
       t.row = __builtin_amdgcn_readlane(r0, l) + k * R;
       t.n = min(__builtin_amdgcn_readlane(n, l) - k * R, R);
-      t.adapter = a.adapter[s0 + l];
+      t.adapter = __builtin_amdgcn_readlane(who, l);
       if (t.adapter < 0 || t.adapter >= a.adapters) t.adapter = -1;
       t.rank = t.adapter < 0 ? 0 : a.ranks ? min(max(a.ranks[t.adapter], 0), a.rank) : a.rank;
       return true;
@@ -231,28 +232,12 @@ __global__ void __launch_bounds__(kThreads, 2) lora_expand_kernel(btf_lora a, Se
     while (seg < nseg - 1 && c >= (segs.s[seg].N + chunk - 1) / chunk) c -= (segs.s[seg].N + chunk - 1) / chunk, ++seg;
   const int N = segs.s[seg].N, ld = parts_ld(a.rank), steps = (t.rank + 31) / 32;
   const float scale = t.adapter >= 0 && a.scale ? a.scale[t.adapter] : 1.f;
-  // h, scaled, in parts
-  for (int i = threadIdx.x; i < NS * R * steps * 8; i += kThreads) {
-    const int q = 4 * (i % (steps * 8)), r = i / (steps * 8) % R, sg = i / (steps * 8) / R;
-    f32x4 v = {0.f, 0.f, 0.f, 0.f};
-    if (r < t.n && q < t.rank) {
-      for (int k = 0; k < slices; ++k) v += *reinterpret_cast<const f32x4*>(h_of(a, nseg, k, GLU ? sg : seg, t.row + r) + q);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) v[j] = q + j < t.rank ? v[j] * scale : 0.f;
-    }
-    float x[4] = {v[0], v[1], v[2], v[3]};
-#pragma unroll
-    for (int p = 0; p < 3; ++p) {
-      const uint32_t lo = cut2(x[0], x[1]), hi = cut2(x[2], x[3]);
-      *reinterpret_cast<uint2*>(sh_h + (size_t)((sg * 3 + p) * R + r) * ld + q) = uint2{lo, hi};
-    }
-  }
-  __syncthreads();
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, c16 = lane & 15, g = lane >> 4;
   const int n1 = min(N, (c + 1) * chunk);
-  for (int n0 = c * chunk + 16 * TN * w; n0 < n1; n0 += 16 * TN * kWaves) {
-    // y of the lane's row in each tile: outputs n0 + 16 i + 4 g .. + 3
-    f32x4 y[NS][TN][RT];
+  // y of the lane's row in each tile (outputs n0 + 16 i + 4 g .. + 3) and 64 ranks of B from rank 32 k on
+  f32x4 y[NS][TN][RT];
+  u32x4 bv[2][NS][TN];
+  auto load_y = [&](int n0) {
 #pragma unroll
     for (int sg = 0; sg < NS; ++sg)
 #pragma unroll
@@ -273,58 +258,102 @@ __global__ void __launch_bounds__(kThreads, 2) lora_expand_kernel(btf_lora a, Se
             }
           }
         }
+  };
+  auto load_b = [&](int n0, int k) {
 #pragma unroll
-    for (int sg = 0; sg < NS; ++sg) {
-      const btf_lora_seg& s = segs.s[GLU ? sg : seg];
-      const uint16_t* b = static_cast<const uint16_t*>(s.b) + (size_t)max(t.adapter, 0) * s.b_stride + (size_t)(n0 + c16) * a.rank + 8 * g;
-      f32x4 d[TN][RT];
+    for (int u = 0; u < 2; ++u)
 #pragma unroll
-      for (int i = 0; i < TN; ++i)
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt) d[i][rt] = f32x4{0.f, 0.f, 0.f, 0.f};
-      for (int k = 0; k < steps; ++k) {
-        const int left = t.rank - 32 * k - 8 * g;  // ranks from the lane's first on
-        u32x4 bv[TN];
+      for (int sg = 0; sg < NS; ++sg) {
+        const btf_lora_seg& s = segs.s[GLU ? sg : seg];
+        const uint16_t* b = static_cast<const uint16_t*>(s.b) + (size_t)max(t.adapter, 0) * s.b_stride + (size_t)(n0 + c16) * a.rank + 8 * g;
 #pragma unroll
         for (int i = 0; i < TN; ++i) {
-          bv[i] = u32x4{0, 0, 0, 0};
-          if (left > 0 && n0 + 16 * i + c16 < n1) bv[i] = *reinterpret_cast<const u32x4*>(b + (size_t)(16 * i) * a.rank + 32 * k);
-#pragma unroll
-          for (int j = 0; j < 4; ++j)  // what lies behind the adapter's rank
-            bv[i][j] &= left > 2 * j + 1 ? 0xffffffffu : left > 2 * j ? 0xffffu : 0u;
-        }
-        u32x4 hp[RT][3];
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-          for (int p = 0; p < 3; ++p)
-            hp[rt][p] = *reinterpret_cast<const u32x4*>(sh_h + (size_t)((sg * 3 + p) * R + 16 * rt + c16) * ld + 32 * k + 8 * g);
-#pragma unroll
-        for (int i = 0; i < TN; ++i) {
-          u32x4 bp[BF ? 1 : 2];
-          weights<BF>(bv[i], bp);
-#pragma unroll
-          for (int p = 0; p < 3; ++p)
-#pragma unroll
-            for (int q = 0; q < (BF ? 1 : 2); ++q)
-#pragma unroll
-              for (int rt = 0; rt < RT; ++rt) d[i][rt] = mfma(bp[q], hp[rt][p], d[i][rt]);
+          bv[u][sg][i] = u32x4{0, 0, 0, 0};
+          if (32 * (k + u) + 8 * g < t.rank && n0 + 16 * i + c16 < n1)
+            bv[u][sg][i] = *reinterpret_cast<const u32x4*>(b + (size_t)(16 * i) * a.rank + 32 * (k + u));
         }
       }
+  };
+  int n0 = c * chunk + 16 * TN * w;
+  load_b(n0, 0);  // (on their way while h is put together)
+  load_y(n0);
+  // h, scaled, in parts
+  for (int i = threadIdx.x; i < NS * R * steps * 8; i += kThreads) {
+    const int q = 4 * (i % (steps * 8)), r = i / (steps * 8) % R, sg = i / (steps * 8) / R;
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+    if (r < t.n && q < t.rank) {
+      const float* h = h_of(a, nseg, 0, GLU ? sg : seg, t.row + r) + q;
+      const size_t next = (size_t)nseg * a.T * a.rank;
+      for (int k = 0; k < slices; k += 8) {
+        f32x4 x[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) x[u] = *reinterpret_cast<const f32x4*>(h + min(k + u, slices - 1) * next);
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+          if (k + u < slices) v += x[u];
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] = q + j < t.rank ? v[j] * scale : 0.f;
+    }
+    float x[4] = {v[0], v[1], v[2], v[3]};
+#pragma unroll
+    for (int p = 0; p < 3; ++p) {
+      const uint32_t lo = cut2(x[0], x[1]), hi = cut2(x[2], x[3]);
+      *reinterpret_cast<uint2*>(sh_h + (size_t)((sg * 3 + p) * R + r) * ld + q) = uint2{lo, hi};
+    }
+  }
+  __syncthreads();
+  while (n0 < n1) {
+    const int next = n0 + 16 * TN * kWaves;
+    f32x4 d[NS][TN][RT];
+#pragma unroll
+    for (int sg = 0; sg < NS; ++sg)
 #pragma unroll
       for (int i = 0; i < TN; ++i)
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) y[sg][i][rt] += d[i][rt];
+        for (int rt = 0; rt < RT; ++rt) d[sg][i][rt] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int k = 0; k < steps; k += 2) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        if (k + u >= steps) break;
+        const int left = t.rank - 32 * (k + u) - 8 * g;  // ranks from the lane's first on
+#pragma unroll
+        for (int sg = 0; sg < NS; ++sg) {
+          u32x4 hp[RT][3];
+#pragma unroll
+          for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+            for (int p = 0; p < 3; ++p)
+              hp[rt][p] = *reinterpret_cast<const u32x4*>(sh_h + (size_t)((sg * 3 + p) * R + 16 * rt + c16) * ld + 32 * (k + u) + 8 * g);
+#pragma unroll
+          for (int i = 0; i < TN; ++i) {
+            u32x4 v = bv[u][sg][i], bp[BF ? 1 : 2];
+#pragma unroll
+            for (int j = 0; j < 4; ++j)  // what lies behind the adapter's rank
+              v[j] &= left > 2 * j + 1 ? 0xffffffffu : left > 2 * j ? 0xffffu : 0u;
+            weights<BF>(v, bp);
+#pragma unroll
+            for (int p = 0; p < 3; ++p)
+#pragma unroll
+              for (int q = 0; q < (BF ? 1 : 2); ++q)
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt) d[sg][i][rt] = mfma(bp[q], hp[rt][p], d[sg][i][rt]);
+          }
+        }
+      }
+      if (k + 2 < steps) load_b(n0, k + 2);
     }
+    if (next < n1) load_b(next, 0);
 #pragma unroll
     for (int i = 0; i < TN; ++i)
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt) {
         const int n = n0 + 16 * i + 4 * g, r = 16 * rt + c16;
-        f32x4 v = y[0][i][rt];
+        f32x4 v = y[0][i][rt] + d[0][i][rt];
         if (GLU) {
+          const f32x4 up = y[NS - 1][i][rt] + d[NS - 1][i][rt];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) v[j] = v[j] / (1.0f + expf(-v[j])) * y[NS - 1][i][rt][j];
+          for (int j = 0; j < 4; ++j) v[j] = v[j] / (1.0f + expf(-v[j])) * up[j];
         }
         float* p = GLU ? a.out + (size_t)(t.row + r) * a.ldo + n : segs.s[seg].y + (size_t)(t.row + r) * segs.s[seg].ldy + n;
         if (r < t.n) {
@@ -337,6 +366,204 @@ __global__ void __launch_bounds__(kThreads, 2) lora_expand_kernel(btf_lora a, Se
           }
         }
       }
+    if (next < n1) load_y(next);
+    n0 = next;
+  }
+}
+
+// ---- few rows: a row or four a request, each adapter's bytes read for next to nothing ----
+// Vector arithmetic in 32 bits: for one row matrix instructions spend 15 of 16 rows on
+// nothing, and the registers that hold them are then missing for loads in flight.
+
+// Eight weights times eight numbers, added to s.
+template <bool BF>
+__device__ __forceinline__ float dot8(u32x4 w, const float* x, float s) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float lo = BF ? __uint_as_float(w[j] << 16) : h2f((uint16_t)w[j]);
+    const float hi = BF ? __uint_as_float(w[j] & 0xffff0000u) : h2f((uint16_t)(w[j] >> 16));
+    s = __builtin_fmaf(lo, x[2 * j], s);
+    s = __builtin_fmaf(hi, x[2 * j + 1], s);
+  }
+  return s;
+}
+__device__ __forceinline__ float swap16(float v) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+__device__ __forceinline__ float swap32(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+// Workgroups that a launch of few rows is cut into, at least (64 requests of one token, three segments, ranks to 64: shrink
+// and expand 38.6 us with 512, 33.8 with 1024, 36.0 with 2048).
+constexpr int kFewGroups = 1024;
+constexpr int kFewK = 512;     // columns of a wave's step, eight a lane
+constexpr int kFewRanks = 8;   // ranks of a wave at a time
+
+// R rows by the adapter's ranks. A workgroup's waves share the ranks by eights; where there are fewer than four of
+// these, several waves share one by steps of K and join in LDS. grid: (tile, slice of K), segment.
+template <bool BF, int R>
+__global__ void __launch_bounds__(kThreads, 2) lora_shrink_few_kernel(btf_lora a, Segs segs, int nseg, int slices, int slice) {
+  __shared__ float sh[kWaves][R][kFewRanks];
+  Tile t;
+  const int k = blockIdx.x % slices, seg = blockIdx.y;
+  if (!find<R>(a, blockIdx.x / slices, t) || t.rank == 0) return;  // the whole workgroup
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const btf_lora_seg& s = segs.s[seg];
+  const int end = min(a.K, (k + 1) * slice), all = (t.rank + kFewRanks - 1) / kFewRanks;
+  const int groups = all >= 4 ? 4 : all >= 2 ? 2 : 1, share = kWaves / groups;
+  for (int g0 = 0; g0 < all; g0 += groups) {
+    const int first = (g0 + w / share) * kFewRanks, ranks = min(t.rank - first, kFewRanks);
+    float acc[kFewRanks][R] = {};
+    const uint16_t* m = static_cast<const uint16_t*>(s.a) + (size_t)t.adapter * s.a_stride + (size_t)first * a.K;
+    const float* x = a.x + (size_t)t.row * a.ldx;
+    for (int kb = k * slice + w % share * kFewK; kb < end && ranks > 0; kb += share * kFewK) {
+      const bool in = kb + 8 * lane < end;
+      f32x4 xv[R][2] = {};
+      u32x4 av[kFewRanks];
+#pragma unroll
+      for (int i = 0; i < kFewRanks; ++i) {
+        av[i] = u32x4{0, 0, 0, 0};
+        if (in && i < ranks) av[i] = reinterpret_cast<const u32x4*>(m + (size_t)i * a.K + kb)[lane];
+      }
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+        if (in && r < t.n)
+#pragma unroll
+          for (int u = 0; u < 2; ++u) xv[r][u] = reinterpret_cast<const f32x4*>(x + (size_t)r * a.ldx + kb)[2 * lane + u];
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const float xs[8] = {xv[r][0][0], xv[r][0][1], xv[r][0][2], xv[r][0][3], xv[r][1][0], xv[r][1][1], xv[r][1][2], xv[r][1][3]};
+#pragma unroll
+        for (int i = 0; i < kFewRanks; ++i) acc[i][r] = dot8<BF>(av[i], xs, acc[i][r]);
+      }
+    }
+    // the lanes' sums: rank i of row r to lane i
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      float mine = 0.f;
+#pragma unroll
+      for (int i = 0; i < kFewRanks; ++i) {
+        const float v = swap32(swap16(row16_sum(acc[i][r])));
+        mine = lane == i ? v : mine;
+      }
+      if (lane < kFewRanks) sh[w][r][lane] = mine;
+    }
+    __syncthreads();
+    if (w % share == 0 && lane < ranks)
+      for (int r = 0; r < t.n; ++r) {
+        float v = sh[w][r][lane];
+        for (int j = 1; j < share; ++j) v += sh[w + j][r][lane];
+        h_of(a, nseg, k, seg, t.row + r)[first + lane] = v;
+      }
+    __syncthreads();
+  }
+}
+
+// R rows by `chunk` outputs. The lanes of 2^lg hold one row of B, eight ranks each, so that a wave's load is 1 KB in one
+// piece; kFewLoads of them are on their way at a time.
+constexpr int kFewLoads = 8;
+template <bool BF, int R, bool GLU>
+__global__ void __launch_bounds__(kThreads, 2) lora_expand_few_kernel(btf_lora a, Segs segs, int nseg, int slices, int chunk, int chunks) {
+  constexpr int NS = GLU ? 2 : 1, U = kFewLoads / NS / (R > 1 ? 2 : 1);
+  __shared__ float sh_h[NS][R][256];
+  Tile t;
+  if (!find<R>(a, blockIdx.x / chunks, t) || (!GLU && t.rank == 0)) return;  // the whole workgroup
+  int c = blockIdx.x % chunks, seg = 0;
+  if (!GLU)
+    while (seg < nseg - 1 && c >= (segs.s[seg].N + chunk - 1) / chunk) c -= (segs.s[seg].N + chunk - 1) / chunk, ++seg;
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lg = t.rank <= 8 ? 0 : 32 - __builtin_clz((t.rank + 7) / 8 - 1), per = 64 >> lg;  // outputs of a load
+  const int j = lane & ((1 << lg) - 1), n_of = lane >> lg;
+  const int n1 = min(segs.s[seg].N, (c + 1) * chunk);
+  const bool in = 8 * j < t.rank;
+  u32x4 bv[NS][U];
+  float y[NS][U][R];
+  auto load = [&](int n0) {
+#pragma unroll
+    for (int sg = 0; sg < NS; ++sg) {
+      const btf_lora_seg& s = segs.s[GLU ? sg : seg];
+      const uint16_t* b = static_cast<const uint16_t*>(s.b) + (size_t)max(t.adapter, 0) * s.b_stride + 8 * j;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int n = n0 + u * per + n_of;
+        bv[sg][u] = u32x4{0, 0, 0, 0};
+        if (in && n < n1) bv[sg][u] = *reinterpret_cast<const u32x4*>(b + (size_t)n * a.rank);
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          y[sg][u][r] = 0.f;
+          if (n < n1 && r < t.n) y[sg][u][r] = s.y[(size_t)(t.row + r) * s.ldy + n];
+        }
+      }
+    }
+  };
+  int n0 = c * chunk + w * U * per;
+  load(n0);  // (on their way while h is put together)
+  // h, scaled; behind the rank zero
+  const float scale = t.adapter >= 0 && a.scale ? a.scale[t.adapter] : 1.f;
+  const int ranks8 = 8 << lg;
+  for (int i = threadIdx.x; i < NS * R * ranks8; i += kThreads) {
+    const int q = i % ranks8, r = i / ranks8 % R, sg = i / ranks8 / R;
+    float v = 0.f;
+    if (r < t.n && q < t.rank) {
+      const float* h = h_of(a, nseg, 0, GLU ? sg : seg, t.row + r) + q;
+      const size_t next = (size_t)nseg * a.T * a.rank;
+      for (int k = 0; k < slices; k += 8) {
+        float x[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) x[u] = h[min(k + u, slices - 1) * next];
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+          if (k + u < slices) v += x[u];
+      }
+      v *= scale;
+    }
+    sh_h[sg][r][q] = v;
+  }
+  __syncthreads();
+  while (n0 < n1) {
+    float d[NS][U][R];
+#pragma unroll
+    for (int sg = 0; sg < NS; ++sg)
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        float h[8];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const f32x4 v = *reinterpret_cast<const f32x4*>(&sh_h[sg][r][8 * j + 4 * i]);
+          h[4 * i] = v[0], h[4 * i + 1] = v[1], h[4 * i + 2] = v[2], h[4 * i + 3] = v[3];
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          u32x4 b = bv[sg][u];
+#pragma unroll
+          for (int i = 0; i < 4; ++i)  // what lies behind the adapter's rank
+            b[i] &= t.rank - 8 * j > 2 * i + 1 ? 0xffffffffu : t.rank - 8 * j > 2 * i ? 0xffffu : 0u;
+          float v = dot8<BF>(b, h, 0.f);
+          if (lg > 0) v += dpp_f<0xB1>(v);
+          if (lg > 1) v += dpp_f<0x4E>(v);
+          if (lg > 2) v += dpp_f<0x141>(v);
+          if (lg > 3) v += dpp_f<0x140>(v);
+          if (lg > 4) v = swap16(v);
+          d[sg][u][r] = v + y[sg][u][r];
+        }
+      }
+    const int at = n0;
+    n0 += U * per * kWaves;
+    if (n0 < n1) load(n0);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int n = at + u * per + n_of;
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+        if (j == 0 && n < n1 && r < t.n) {
+          float v = d[0][u][r];
+          if (GLU) v = v / (1.0f + expf(-v)) * d[NS - 1][u][r];
+          (GLU ? a.out + (size_t)(t.row + r) * a.ldo : segs.s[seg].y + (size_t)(t.row + r) * segs.s[seg].ldy)[n] = v;
+        }
+    }
   }
 }
 
@@ -345,12 +572,15 @@ int tile_rows(int S, int T, int rank, int together) {
   return (int64_t)T > 16 * (int64_t)S && rank * together <= 128 ? 64 : 16;
 }
 
+// Tiles of the requests' rows, at most: a request's last one may be a part of one.
+int most_tiles(const btf_lora& a, int R) { return a.T / R + a.S < a.T ? a.T / R + a.S : a.T; }
+
 bool vec4(const float* p, int ld) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ld % 4 == 0; }
 
 template <bool BF, int RT>
 int lora_go(const btf_lora& a, const Segs& segs, int nseg, hipStream_t st) {
   constexpr int R = 16 * RT;
-  const int tiles = a.T / R + a.S;
+  const int tiles = most_tiles(a, R);
   const int nt = a.rank <= 16 ? 1 : a.rank <= 32 ? 2 : 4, groups = (a.rank + 16 * nt - 1) / (16 * nt);
   // slices of K: enough for kGroups workgroups, each at least one step of its waves long
   const int step = kBlockK * kWaves, most = (a.K + step - 1) / step;
@@ -365,8 +595,8 @@ int lora_go(const btf_lora& a, const Segs& segs, int nseg, hipStream_t st) {
   const int rc = launch_status("lora_shrink_kernel");
   if (rc != BTF_OK) return rc;
   const bool glu = a.mode == BTF_GEMV_SWIGLU;
-  int outs = 0;
   bool vec = true;
+  int outs = 0;
   for (int i = 0; i < nseg; ++i) vec = vec && vec4(segs.s[i].y, segs.s[i].ldy), outs += glu && i ? 0 : segs.s[i].N;
   if (glu) vec = vec && vec4(a.out, a.ldo);
   int chunk = kChunk;
@@ -383,6 +613,37 @@ int lora_go(const btf_lora& a, const Segs& segs, int nseg, hipStream_t st) {
   return launch_status("lora_expand_kernel");
 }
 
+template <bool BF, int R>
+int lora_few(const btf_lora& a, const Segs& segs, int nseg, hipStream_t st) {
+  const int tiles = most_tiles(a, R);
+  const int together = a.rank > 2 * kFewRanks ? 1 : a.rank > kFewRanks ? 2 : 4;  // waves that share ranks
+  const int step = kFewK * together, most = (a.K + step - 1) / step;
+  int slices = (kFewGroups + tiles * nseg - 1) / (tiles * nseg);
+  slices = slices < most ? slices : most;
+  const int slice = ((a.K + slices - 1) / slices + step - 1) / step * step;
+  slices = (a.K + slice - 1) / slice;
+  hipLaunchKernelGGL((lora_shrink_few_kernel<BF, R>), dim3((unsigned)tiles * slices, nseg), dim3(kThreads), 0, st, a, segs, nseg, slices, slice);
+  const int rc = launch_status("lora_shrink_few_kernel");
+  if (rc != BTF_OK) return rc;
+  const bool glu = a.mode == BTF_GEMV_SWIGLU;
+  int outs = 0, chunk = kChunk, chunks = 0;
+  for (int i = 0; i < (glu ? 1 : nseg); ++i) outs += segs.s[i].N;
+  while (chunk < 4 * kChunk && (int64_t)tiles * (outs / (2 * chunk)) >= kFewGroups) chunk *= 2;
+  for (int i = 0; i < (glu ? 1 : nseg); ++i) chunks += (segs.s[i].N + chunk - 1) / chunk;
+  const dim3 grid((unsigned)tiles * chunks);
+  if (glu) hipLaunchKernelGGL((lora_expand_few_kernel<BF, R, true>), grid, dim3(kThreads), 0, st, a, segs, nseg, slices, chunk, chunks);
+  else hipLaunchKernelGGL((lora_expand_few_kernel<BF, R, false>), grid, dim3(kThreads), 0, st, a, segs, nseg, slices, chunk, chunks);
+  return launch_status("lora_expand_few_kernel");
+}
+
+template <bool BF>
+int lora_any(const btf_lora& a, const Segs& segs, int nseg, hipStream_t st) {
+  if (a.T <= a.S) return lora_few<BF, 1>(a, segs, nseg, st);
+  if (a.T <= 4 * (int64_t)a.S) return lora_few<BF, 4>(a, segs, nseg, st);
+  if (tile_rows(a.S, a.T, a.rank, a.mode == BTF_GEMV_SWIGLU ? 2 : 1) == 64) return lora_go<BF, 4>(a, segs, nseg, st);
+  return lora_go<BF, 1>(a, segs, nseg, st);
+}
+
 }  // namespace
 
 // slices * T * nseg is at most nseg * T + kGroups * 64 (tiles >= T / 64), and slices at most K / 256, rounded up.
@@ -396,10 +657,7 @@ int64_t lora_ws_bytes(int S, int T, int K, int rank, int nseg) {
 int lora(const btf_lora& a, const btf_lora_seg* s, int nseg, hipStream_t st) {
   Segs segs{};
   for (int i = 0; i < nseg; ++i) segs.s[i] = s[i];
-  const bool bf = a.type == BTF_BF16;
-  if (tile_rows(a.S, a.T, a.rank, a.mode == BTF_GEMV_SWIGLU ? 2 : 1) == 64)
-    return bf ? lora_go<true, 4>(a, segs, nseg, st) : lora_go<false, 4>(a, segs, nseg, st);
-  return bf ? lora_go<true, 1>(a, segs, nseg, st) : lora_go<false, 1>(a, segs, nseg, st);
+  return a.type == BTF_BF16 ? lora_any<true>(a, segs, nseg, st) : lora_any<false>(a, segs, nseg, st);
 }
 
 }  // namespace btfhip

@@ -93,21 +93,34 @@ __global__ void __launch_bounds__(256) page_fork_rows_kernel(btf_page_fork a) {
 constexpr int kFreeThreads = 1024;
 constexpr int kFreeEach = 4;                          // places of a thread
 constexpr int kFreeChunk = kFreeThreads * kFreeEach;  // ... of a workgroup
+constexpr int kFreeMost = 16;                         // ... of a thread, where one workgroup does it all
 
-// Place e = s * ldt + j gives up its page (`in`); the page's id, -1: none that the cache has.
-struct Place {
-  bool in;
-  int page;
+// Whether places e0, e0 + 1, ... (place s * ldt + j is page j of row s) give up their pages, and the pages' ids, -1: none
+// that the cache has. (Loads without branches, so that all are on their way at once.)
+template <int EACH>
+struct Places {
+  unsigned in = 0;
+  int page[EACH];
 };
-__device__ __forceinline__ Place place_of(const btf_page_free& a, const int* held, int e) {
-  Place p{false, -1};
-  if (e >= a.S * a.ldt) return p;
-  const int s = e / a.ldt, j = e - s * a.ldt;
-  const int keep = max(a.keep[s], 0), first = (int)(((long long)keep + a.page - 1) / a.page);
-  p.in = j >= first && j < held[s];
-  if (p.in) {
-    p.page = a.table[e];
-    if (p.page >= a.pages || p.page < 0) p.page = -1;
+template <int EACH>
+__device__ __forceinline__ Places<EACH> places_of(const btf_page_free& a, const int* held, int e0) {
+  const int end = a.S * a.ldt;
+  int keep[EACH], have[EACH], j[EACH];
+  Places<EACH> p;
+#pragma unroll
+  for (int i = 0; i < EACH; ++i) {
+    const int e = min(e0 + i, end - 1), s = e / a.ldt;
+    j[i] = e - s * a.ldt;
+    keep[i] = a.keep[s];
+    have[i] = held[s];
+    p.page[i] = a.table[e];
+  }
+#pragma unroll
+  for (int i = 0; i < EACH; ++i) {
+    const int first = (int)(((long long)max(keep[i], 0) + a.page - 1) / a.page);
+    const bool in = e0 + i < end && j[i] >= first && j[i] < have[i];
+    p.in |= (unsigned)in << i;
+    if (!in || p.page[i] >= a.pages || p.page[i] < 0) p.page[i] = -1;
   }
   return p;
 }
@@ -117,52 +130,69 @@ __device__ __forceinline__ void lower(const btf_page_free& a, int page) {
 __device__ __forceinline__ int count_of(const btf_page_free& a, int page) {
   return __hip_atomic_load(a.shared + page, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
-__device__ __forceinline__ void mark(const btf_page_free& a, int page, int e) {
+__device__ __forceinline__ void mark(const btf_page_free& a, int page, int count, int e) {
   // (a count below zero is more than -2^29, a mark less than INT_MIN + 2^29)
-  if (page >= 0 && count_of(a, page) < 0)
+  if (page >= 0 && count < 0)
     __hip_atomic_fetch_min(a.shared + page, INT_MIN + e, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
-__device__ __forceinline__ bool owns(const btf_page_free& a, int page, int e) {
-  return page >= 0 && (!a.shared || count_of(a, page) == INT_MIN + e);
+// The places' counts (page 0's for a place without a page).
+template <int EACH>
+__device__ __forceinline__ void counts_of(const btf_page_free& a, const Places<EACH>& p, int (&count)[EACH]) {
+#pragma unroll
+  for (int i = 0; i < EACH; ++i) count[i] = a.shared ? count_of(a, max(p.page[i], 0)) : 0;
+}
+template <int EACH>
+__device__ __forceinline__ unsigned owned(const btf_page_free& a, const Places<EACH>& p, int e0) {
+  int count[EACH];
+  counts_of(a, p, count);
+  unsigned own = 0;
+#pragma unroll
+  for (int i = 0; i < EACH; ++i) own |= (unsigned)(p.page[i] >= 0 && (!a.shared || count[i] == INT_MIN + e0 + i)) << i;
+  return own;
 }
 // The places' pages go to the list, which has n0 entries, `behind` of the call's after them.
-__device__ __forceinline__ void give_back(const btf_page_free& a, const Place (&p)[kFreeEach], unsigned own, int e0,
+template <int EACH>
+__device__ __forceinline__ void give_back(const btf_page_free& a, const Places<EACH>& p, unsigned own, int e0,
                                           long long n0, long long behind) {
 #pragma unroll
-  for (int i = kFreeEach - 1; i >= 0; --i) {
+  for (int i = EACH - 1; i >= 0; --i) {
     if (own >> i & 1) {
-      if (n0 + behind < a.pages) a.free_list[n0 + behind] = p[i].page;
+      if (n0 + behind < a.pages) a.free_list[n0 + behind] = p.page[i];
       ++behind;
-      if (a.shared) a.shared[p[i].page] = 0;
+      if (a.shared) a.shared[p.page[i]] = 0;
     }
-    if (p[i].in) a.table[e0 + i] = -1;
+    if (p.in >> i & 1) a.table[e0 + i] = -1;
   }
 }
 __device__ __forceinline__ int stays(const btf_page_free& a, int held, int s) {
   return (int)min((long long)held, ((long long)max(a.keep[s], 0) + a.page - 1) / a.page);
 }
 
-// All of it by one workgroup: up to kFreeChunk places.
+// All memory accesses of the workgroup's threads so far are done (atomics on counts among them, which act in L2, as the
+// loads of counts do: nothing has to be written back or thrown away for these).
+__device__ __forceinline__ void all_done() {
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+}
+
+// All of it by one workgroup.
+template <int EACH>
 __global__ void __launch_bounds__(kFreeThreads) page_free_small_kernel(btf_page_free a) {
   __shared__ uint64_t part[kFreeThreads / 64];
-  const int e0 = threadIdx.x * kFreeEach;
+  const int e0 = threadIdx.x * EACH;
   const long long n0 = min((long long)max(*a.n_free, 0), (long long)a.pages);
-  Place p[kFreeEach];
-#pragma unroll
-  for (int i = 0; i < kFreeEach; ++i) p[i] = place_of(a, a.held, e0 + i);
+  const Places<EACH> p = places_of<EACH>(a, a.held, e0);
   if (a.shared) {
 #pragma unroll
-    for (int i = 0; i < kFreeEach; ++i) lower(a, p[i].page);
-    __threadfence();
-    __syncthreads();
+    for (int i = 0; i < EACH; ++i) lower(a, p.page[i]);
+    all_done();
+    int count[EACH];
+    counts_of(a, p, count);
 #pragma unroll
-    for (int i = 0; i < kFreeEach; ++i) mark(a, p[i].page, e0 + i);
-    __threadfence();
-    __syncthreads();
+    for (int i = 0; i < EACH; ++i) mark(a, p.page[i], count[i], e0 + i);
+    all_done();
   }
-  unsigned own = 0;
-#pragma unroll
-  for (int i = 0; i < kFreeEach; ++i) own |= (unsigned)owns(a, p[i].page, e0 + i) << i;
+  const unsigned own = owned(a, p, e0);
   uint64_t all;
   const uint64_t upto = block_scan<kFreeThreads>(__popc(own), part, &all);  // (and all have read what is written below)
   give_back(a, p, own, e0, n0, (long long)(all - upto));
@@ -175,22 +205,27 @@ __global__ void __launch_bounds__(kFreeThreads) page_free_small_kernel(btf_page_
 // workgroups read).
 __global__ void __launch_bounds__(kFreeThreads) page_free_lower_kernel(btf_page_free a) {
   const int e0 = blockIdx.x * kFreeChunk + threadIdx.x * kFreeEach;
+  const Places<kFreeEach> p = places_of<kFreeEach>(a, a.held, e0);
 #pragma unroll
-  for (int i = 0; i < kFreeEach; ++i) lower(a, place_of(a, a.held, e0 + i).page);
+  for (int i = 0; i < kFreeEach; ++i) lower(a, p.page[i]);
 }
 __global__ void __launch_bounds__(kFreeThreads) page_free_mark_kernel(btf_page_free a) {
   const int e0 = blockIdx.x * kFreeChunk + threadIdx.x * kFreeEach;
+  const Places<kFreeEach> p = places_of<kFreeEach>(a, a.held, e0);
+  int count[kFreeEach];
+  counts_of(a, p, count);
 #pragma unroll
-  for (int i = 0; i < kFreeEach; ++i) mark(a, place_of(a, a.held, e0 + i).page, e0 + i);
+  for (int i = 0; i < kFreeEach; ++i) mark(a, p.page[i], count[i], e0 + i);
 }
 __global__ void __launch_bounds__(kFreeThreads) page_free_count_kernel(btf_page_free a) {
   __shared__ uint64_t part[kFreeThreads / 64];
   int* owners = static_cast<int*>(a.ws);
   const int e0 = blockIdx.x * kFreeChunk + threadIdx.x * kFreeEach;
-  uint64_t n = 0, all;
+  const Places<kFreeEach> p = places_of<kFreeEach>(a, a.held, e0);
+  uint64_t all;
+  const uint64_t n = __popc(owned(a, p, e0));
 #pragma unroll
   for (int i = 0; i < kFreeEach; ++i) {
-    n += owns(a, place_of(a, a.held, e0 + i).page, e0 + i);
     if (e0 + i < a.S * a.ldt && (e0 + i) % a.ldt == 0) owners[gridDim.x + (e0 + i) / a.ldt] = a.held[(e0 + i) / a.ldt];
   }
   (void)block_scan<kFreeThreads>(n, part, &all);
@@ -203,13 +238,8 @@ __global__ void __launch_bounds__(kFreeThreads) page_free_kernel(btf_page_free a
   const int* held = owners + gridDim.x;
   const int e0 = blockIdx.x * kFreeChunk + threadIdx.x * kFreeEach;
   const long long n0 = min((long long)max(held[a.S], 0), (long long)a.pages);
-  Place p[kFreeEach];
-  unsigned own = 0;
-#pragma unroll
-  for (int i = 0; i < kFreeEach; ++i) {
-    p[i] = place_of(a, held, e0 + i);
-    own |= (unsigned)owns(a, p[i].page, e0 + i) << i;
-  }
+  const Places<kFreeEach> p = places_of<kFreeEach>(a, held, e0);
+  const unsigned own = owned(a, p, e0);
   uint64_t later = 0, behind, all;  // owners of the chunks behind this one
   for (int c = blockIdx.x + 1 + threadIdx.x; c < (int)gridDim.x; c += kFreeThreads) later += owners[c];
   (void)block_scan<kFreeThreads>(later, part, &behind);
@@ -344,13 +374,14 @@ int page_fork(const btf_page_fork& a, hipStream_t st) {
 
 int64_t page_free_ws_bytes(int S, int ldt) {
   const int n = free_chunks(S, ldt);
-  return n <= 1 ? 0 : ((int64_t)n + S + 1) * 4;
+  return n * kFreeEach <= kFreeMost ? 0 : ((int64_t)n + S + 1) * 4;
 }
 
 int page_free(const btf_page_free& a, hipStream_t st) {
   const int n = free_chunks(a.S, a.ldt);
-  if (n <= 1) {
-    hipLaunchKernelGGL(page_free_small_kernel, dim3(1), dim3(kFreeThreads), 0, st, a);
+  if (n * kFreeEach <= kFreeMost) {
+    if (n <= 1) hipLaunchKernelGGL(page_free_small_kernel<kFreeEach>, dim3(1), dim3(kFreeThreads), 0, st, a);
+    else hipLaunchKernelGGL(page_free_small_kernel<kFreeMost>, dim3(1), dim3(kFreeThreads), 0, st, a);
     return launch_status("page_free_small_kernel");
   }
   if (a.shared) {

@@ -61,62 +61,175 @@ __device__ __forceinline__ int piece_keys(uint64_t work, int R, int items) {
   return kStep * (int)(c > f ? c : f);
 }
 
+__device__ __forceinline__ int tiles_of(const Plan& p, int n, int R) {
+  return n > 0 ? (int)(((long long)n * (p.a.heads / p.kv.heads) + R - 1) / R) : 0;
+}
+__device__ __forceinline__ long long cap_of(const Plan& p) { return (long long)p.a.ldt * p.kv.page; }
+
+// A group of requests b .. e - 1 whose rows are r0 .. r1 - 1.
+__device__ __forceinline__ Found group_of(const Plan& p, int b, int e, int r0, int r1, int lead, int whole) {
+  Found f{};
+  f.b = b, f.e = e;
+  f.row0 = r0;
+  f.n = max(r1 - r0, 0);
+  const bool there = lead >= 0 && lead < p.a.S && f.n > 0;
+  f.s = there ? lead : 0;
+  f.whole = whole;
+  f.len = f.ctx = there ? (int)(min((long long)max(whole, 0), min(cap_of(p), 0x7fffffffll)) & ~31ll) : 0;
+  f.tiles = f.len > 0 ? tiles_of(p, f.n, p.R[0]) : 0;
+  f.flags = kCut;
+  f.group = -1;
+  return f;
+}
+// Request s alone.
+__device__ __forceinline__ Found request_of(const Plan& p, int s, int r0, int r1, int full) {
+  Found f{};
+  f.s = s;
+  f.row0 = max(r0, 0);
+  f.n = max(min(r1, p.a.T) - f.row0, 0);
+  f.len = (int)max(0ll, min((long long)full, cap_of(p)));
+  f.ctx = full - f.n;
+  f.tiles = tiles_of(p, f.n, p.R[1]);
+  f.flags = p.a.tree && f.n <= BTF_TREE_NODES ? kTree : 0;
+  f.group = -1;
+  return f;
+}
+__device__ __forceinline__ bool takes_part(const Found& f, const Found& g) {
+  return f.n > 0 && g.len > 0 && f.s >= g.b && f.s < g.e && f.ctx >= g.whole && f.row0 >= g.row0 && f.row0 + f.n <= g.row0 + g.n;
+}
+__device__ __forceinline__ uint64_t work_of(const Found& f) { return (uint64_t)f.tiles * (uint64_t)max(f.len - f.begin, 0); }
+// The last of n ascending numbers that is at most v (0 if none is).
+__device__ __forceinline__ int last_at_most(const int* x, int n, int v) {
+  int lo = 0, hi = n - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (x[mid] <= v) lo = mid;
+    else hi = mid - 1;
+  }
+  return lo;
+}
+
+// block_scan of two numbers a thread.
+__device__ __forceinline__ void scan2(uint64_t (&v)[2], uint64_t (&part)[2][kPlanThreads / 64], uint64_t (&all)[2]) {
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) v[i] = wave_scan_u64(v[i]);
+  __syncthreads();  // (part may still be read from the scan before)
+  if (lane == 63)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) part[i][w] = v[i];
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const uint64_t sums = wave_scan_u64(lane < kPlanThreads / 64 ? part[i][lane] : 0);
+    auto of = [&](int l) {
+      return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(sums >> 32), l) << 32 |
+             (uint32_t)__builtin_amdgcn_readlane((int)sums, l);
+    };
+    all[i] = of(kPlanThreads / 64 - 1);
+    v[i] += w ? of(w - 1) : 0;
+  }
+}
+
+// Up to 1024 requests, one a thread, with the groups and row starts in LDS: one trip to memory for all that is read.
+__global__ void __launch_bounds__(kPlanThreads) shared_plan_small_kernel(Plan p) {
+  __shared__ uint64_t part[2][kPlanThreads / 64];
+  __shared__ int sh_row0[kPlanThreads + 1], sh_group0[kPlanThreads], sh_upto[2][kPlanThreads];
+  __shared__ Found sh_group[kPlanThreads];
+  const btf_paged_attention& a = p.a;
+  const int tid = threadIdx.x;
+  const bool group = tid < p.groups, request = tid < a.S;
+  const int r0 = request ? a.row0[tid] : 0, r1 = request ? a.row0[tid + 1] : 0, full = request ? a.kv_len[tid] : 0;
+  const int b = group ? p.group0[tid] : 0, e = group ? p.group0[tid + 1] : 0, lead = group ? p.lead[tid] : 0, whole = group ? p.shared[tid] : 0;
+  if (request) sh_row0[tid] = r0;
+  if (tid == a.S - 1) sh_row0[a.S] = r1;
+  if (group) sh_group0[tid] = b;
+  __syncthreads();
+  Found f[2];
+  if (group) {
+    const int gb = min(max(b, 0), a.S), ge = min(max(e, gb), a.S);
+    auto row_of = [&](int s) { return min(max(sh_row0[s], 0), a.T); };
+    f[0] = group_of(p, gb, ge, row_of(gb), row_of(ge), lead, whole);
+    sh_group[tid] = f[0];
+  }
+  __syncthreads();
+  uint64_t v[2] = {group ? work_of(f[0]) : 0, 0}, all[2];
+  if (request) {
+    f[1] = request_of(p, tid, r0, r1, full);
+    if (p.groups > 0) {
+      const int g = last_at_most(sh_group0, p.groups, tid);
+      if (takes_part(f[1], sh_group[g])) f[1].group = g, f[1].begin = sh_group[g].len;
+    }
+    v[1] = work_of(f[1]);
+  }
+  scan2(v, part, all);
+  int own[2] = {0, 0}, cut[2] = {0, 0};
+#pragma unroll
+  for (int role = 0; role < 2; ++role)
+    if (role ? request : group) {
+      f[role].C = piece_keys(all[role] * p.kv.heads, p.R[role], target(p.R[role]));
+      f[role].pieces = max(1, (f[role].len - f[role].begin + f[role].C - 1) / f[role].C);
+      own[role] = p.kv.heads * f[role].tiles * f[role].pieces;
+      if (f[role].group >= 0 || f[role].pieces > 1) f[role].flags |= kCut;
+      cut[role] = f[role].flags & kCut ? own[role] : 0;
+    }
+#pragma unroll
+  for (int role = 0; role < 2; ++role) v[role] = (uint64_t)(uint32_t)own[role] | (uint64_t)(uint32_t)cut[role] << 32;
+  scan2(v, part, all);
+#pragma unroll
+  for (int role = 0; role < 2; ++role) {
+    sh_upto[role][tid] = (int)v[role];
+    if (role ? request : group) {
+      f[role].item0 = (int)v[role] - own[role];
+      f[role].slot0 = (int)(v[role] >> 32) - cut[role];
+      p.ws.found[role ? p.groups + tid : tid] = f[role];
+    }
+    if (tid == 0) p.ws.items[role] = min((int)all[role], p.ws.most[role]);
+  }
+  __syncthreads();
+#pragma unroll
+  for (int role = 0; role < 2; ++role)
+    for (int k = tid; k < min((int)all[role], p.ws.most[role]); k += kPlanThreads) {
+      int lo = 0, hi = (role ? a.S : p.groups) - 1;  // the first one with upto > k
+      while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (sh_upto[role][mid] > k) hi = mid;
+        else lo = mid + 1;
+      }
+      p.ws.map[role][k] = lo;
+    }
+  for (int t = tid; t < a.T; t += kPlanThreads) {
+    const int s = last_at_most(sh_row0, a.S, t);
+    p.ws.request[t] = t >= sh_row0[s] && t < sh_row0[s + 1] ? s : -1;
+  }
+}
+
+// Any number of requests and groups.
 __global__ void __launch_bounds__(kPlanThreads) shared_plan_kernel(Plan p) {
   __shared__ uint64_t part[kPlanThreads / 64];
   __shared__ int sh_upto[kPlanThreads], sh_row0[kPlanThreads], sh_n[kPlanThreads];
   const btf_paged_attention& a = p.a;
   const btf_kv_cache& kv = p.kv;
-  const int G = a.heads / kv.heads, tid = threadIdx.x;
-  const long long cap = (long long)a.ldt * kv.page;
-  auto tiles_of = [&](int n, int R) { return n > 0 ? (int)(((long long)n * G + R - 1) / R) : 0; };
+  const int tid = threadIdx.x;
   auto row_of = [&](int s) { return min(max(a.row0[s], 0), a.T); };
   uint64_t work[2] = {0, 0};
-  // the groups
   for (int g = tid; g < p.groups; g += kPlanThreads) {
-    Found f{};
-    f.b = min(max(p.group0[g], 0), a.S);
-    f.e = min(max(p.group0[g + 1], f.b), a.S);
-    f.s = p.lead[g];
-    f.row0 = row_of(f.b);
-    f.n = max(row_of(f.e) - f.row0, 0);
-    const bool there = f.s >= 0 && f.s < a.S && f.n > 0;
-    f.whole = p.shared[g];
-    f.len = f.ctx = there ? (int)(min((long long)max(f.whole, 0), min(cap, 0x7fffffffll)) & ~31ll) : 0;
-    f.tiles = f.len > 0 ? tiles_of(f.n, p.R[0]) : 0;
-    f.flags = kCut;
-    f.group = -1;
-    if (!there) f.s = 0;
-    work[0] += (uint64_t)f.tiles * (uint64_t)f.len;
+    const int b = min(max(p.group0[g], 0), a.S), e = min(max(p.group0[g + 1], b), a.S);
+    const Found f = group_of(p, b, e, row_of(b), row_of(e), p.lead[g], p.shared[g]);
+    work[0] += work_of(f);
     p.ws.found[g] = f;
   }
   for (int t = tid; t < a.T; t += kPlanThreads) p.ws.request[t] = -1;
   __threadfence_block();
   __syncthreads();
-  // the requests
   Found* const mine = p.ws.found + p.groups;
   for (int s = tid; s < a.S; s += kPlanThreads) {
-    Found f{};
-    f.s = s;
-    f.row0 = max(a.row0[s], 0);
-    f.n = max(min(a.row0[s + 1], a.T) - f.row0, 0);
-    const int full = a.kv_len[s];
-    f.len = (int)max(0ll, min((long long)full, cap));
-    f.ctx = full - f.n;
-    f.tiles = tiles_of(f.n, p.R[1]);
-    f.group = -1;
-    if (p.groups > 0 && f.n > 0) {
-      int lo = 0, hi = p.groups - 1;  // the last group that begins at s or before
-      while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (p.group0[mid] <= s) lo = mid;
-        else hi = mid - 1;
-      }
-      const Found& g = p.ws.found[lo];
-      if (s >= g.b && s < g.e && g.len > 0 && f.ctx >= g.whole && f.row0 >= g.row0 && f.row0 + f.n <= g.row0 + g.n)
-        f.group = lo, f.begin = g.len;
+    Found f = request_of(p, s, a.row0[s], a.row0[s + 1], a.kv_len[s]);
+    if (p.groups > 0) {
+      const int g = last_at_most(p.group0, p.groups, s);
+      if (takes_part(f, p.ws.found[g])) f.group = g, f.begin = p.ws.found[g].len;
     }
-    f.flags = a.tree && f.n <= BTF_TREE_NODES ? kTree : 0;
-    work[1] += (uint64_t)f.tiles * (uint64_t)max(f.len - f.begin, 0);
+    work[1] += work_of(f);
     mine[s] = f;
   }
   uint64_t all[2];
@@ -332,7 +445,8 @@ int role_go(const Role& r, int R, unsigned grid, hipStream_t st) {
 
 template <int D, bool BF>
 int shared_go(const Plan& p, hipStream_t st) {
-  hipLaunchKernelGGL(shared_plan_kernel, dim3(1), dim3(kPlanThreads), 0, st, p);
+  if (p.a.S <= kPlanThreads) hipLaunchKernelGGL(shared_plan_small_kernel, dim3(1), dim3(kPlanThreads), 0, st, p);
+  else hipLaunchKernelGGL(shared_plan_kernel, dim3(1), dim3(kPlanThreads), 0, st, p);
   int rc = launch_status("shared_plan_kernel");
   if (rc != BTF_OK) return rc;
   const int64_t room = ((int64_t)p.a.ldt * p.kv.page + kStep - 1) / kStep;

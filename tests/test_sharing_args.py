@@ -18,7 +18,7 @@ KV = h.KvCache(A, A, h.CacheType.f16, 64, 4, 256, 100, 4 * 64 * 256, 64 * 256, 2
 FORK = h.PageFork(F=3, S=8, page=64, ldt=4, pages=100, src=A, dst=A, tokens=A, free=A, n_free=A, table=A, held=A, shared=A, got=A,
                   copy_from=A, copy_to=A, copy_tokens=A)
 COPY = h.PageCopy(n=3, source=A, to=A, tokens=A, layers=2, layer_stride=1 << 20)
-FREE = h.PageFree(S=300, page=64, ldt=40, pages=100, keep=A, table=A, held=A, shared=A, free=A, n_free=A, ws=A)
+FREE = h.PageFree(S=300, page=64, ldt=60, pages=100, keep=A, table=A, held=A, shared=A, free=A, n_free=A, ws=A)
 TREE = h.CacheMove(S=2, T=8, table=A, ldt=4, first=A, tree=A, leaf=A, kv_len=A, layers=2, layer_stride=1 << 20)
 LIST = h.CacheMove(S=2, T=8, table=A, ldt=4, to_table=A, ldt_to=3, first=A, source=A, source0=A)
 SHARED = h.SharedAttention(S=2, T=8, heads=20, q=A, ldq=5120, table=A, ldt=4, row0=A, kv_len=A, tree=A, scale=0.0625, out=A,
@@ -124,7 +124,7 @@ def test_nothing_to_do(op, change):
 def test_workspaces():
     """None where nothing is launched; those of the largest launch serve the smaller ones."""
     assert h.page_free_ws_bytes(0, 8) == h.page_free_ws_bytes(8, 0) == h.page_free_ws_bytes(1 << 20, 1 << 9) == 0
-    assert h.page_free_ws_bytes(3, 40) == 0 < h.page_free_ws_bytes(300, 40) < h.page_free_ws_bytes(301, 4000)
+    assert h.page_free_ws_bytes(400, 40) == 0 < h.page_free_ws_bytes(300, 60) < h.page_free_ws_bytes(301, 4000)
     assert h.shared_attention_ws_bytes(0, 8, 20, KV) == h.shared_attention_ws_bytes(2, 8, 18, KV) == 0
     assert h.lora_ws_bytes(0, 1, 512, 16, 1) == h.lora_ws_bytes(1, 1, 512, 16, 4) == h.lora_ws_bytes(1, 1, 512, 512, 1) == 0
     for dim in (64, 128, 256):
@@ -169,7 +169,7 @@ int main() {
   try { launch_shared_attention(SharedAttention{.S = 1, .T = 1}, kv, nullptr); return 1; } catch (const std::runtime_error&) {}
   LoraSeg seg{};
   try { launch_lora(Lora{.S = 1, .T = 1}, &seg, 1, nullptr); return 1; } catch (const std::runtime_error&) {}
-  return page_free_ws_bytes(300, 40) && lora_ws_bytes(1, 1, 512, 16, 1) && !shared_attention_ws_bytes(1, 1, 1, kv) ? 0 : 1;
+  return page_free_ws_bytes(300, 60) && lora_ws_bytes(1, 1, 512, 16, 1) && !shared_attention_ws_bytes(1, 1, 1, kv) ? 0 : 1;
 }''')
     exe = tmp_path / "s"
     subprocess.run(["g++", "-std=c++20", "-I", os.path.join(ROOT, "include"), str(tmp_path / "s.cpp"), h.LIB_PATH, "-o", str(exe),
