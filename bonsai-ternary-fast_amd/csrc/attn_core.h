@@ -229,23 +229,27 @@ __device__ __forceinline__ u32x4 signed_q(u32x4 q, float scale) {
   return q ^ u32x4{f, f, f, f};
 }
 
-template <int D, bool BF, int RT, class Launch>
-__global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(D < 256 ? 2 : 1)))
-    attn_stream_kernel(Launch args) {
-  const btf_paged_attention& a = args.a;
-  const btf_kv_cache& kv = args.kv;
+// What an item's waves leave for each other.
+template <int D, int RT>
+struct StreamLds {
+  static constexpr int LD = D + 4;  // row of a wave's values, in floats
+  float o[kWaves * 16 * RT * LD];
+  float m[kWaves][16 * RT], l[kWaves][16 * RT];
+  int odd;
+};
+
+template <int D, bool BF, int RT>
+__device__ __forceinline__ void attn_stream(const btf_paged_attention& a, const btf_kv_cache& kv, const Req& q, StreamLds<D, RT>& lds) {
   constexpr int R = 16 * RT;             // rows of a tile
   constexpr int KS = D / 32;             // steps over the dims in Q K^T
   constexpr int VD = D < 128 ? D / 16 : 8;  // dims that a lane reads of a key of V
   constexpr int VG = D / (16 * VD);      // ... in so many groups of 16 lanes
   constexpr int PARTS = BF ? 3 : 2;      // 16-bit parts of a probability
-  constexpr int LD = D + 4;              // row of a wave's values in LDS, in floats
-  __shared__ float sh_o[kWaves * R * LD];
-  __shared__ float sh_m[kWaves][R], sh_l[kWaves][R];
-  __shared__ int sh_odd;
-
-  Req q;
-  if (!args.template find<R, false>(blockIdx.x, q)) return;  // the whole workgroup
+  constexpr int LD = StreamLds<D, RT>::LD;
+  auto& sh_o = lds.o;
+  auto& sh_m = lds.m;
+  auto& sh_l = lds.l;
+  int& sh_odd = lds.odd;
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int c16 = lane & 15, g = lane >> 4;
   const int G = a.heads / kv.heads;
@@ -485,11 +489,14 @@ __device__ __forceinline__ Args fresh_args() {
   return g;
 }
 
-template <int D, bool BF, int RT, class Launch>
-__global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2)))
-    attn_tile_kernel(Launch args) {
-  const btf_paged_attention& a = args.a;
-  const btf_kv_cache& kv = args.kv;
+template <int D>
+struct TileLds {
+  u32x4 k[2][kKeys * D / 8], v[2][kKeys * D / 8];
+};
+
+// SKIP: waves whose rows there are not load their share and work nothing out.
+template <int D, bool BF, int RT, bool SKIP>
+__device__ __forceinline__ void attn_tile(const btf_paged_attention& a, const btf_kv_cache& kv, const Req& q, TileLds<D>& lds) {
   constexpr int NW = kWaves, RW = 16 * RT, R = NW * RW;
   constexpr int KS = D / 32;
   constexpr int DT = D / 16;            // dim tiles of the values
@@ -497,10 +504,8 @@ __global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_e
   constexpr int PARTS = BF ? 3 : 2;
   constexpr int CH = D / 8;             // 16-byte chunks of a row
   constexpr int NC = kKeys * CH / (64 * NW);  // of a block, for each thread
-  __shared__ u32x4 sh_k[2][kKeys * CH], sh_v[2][kKeys * CH];
-
-  Req q;
-  if (!args.template find<R, true>(blockIdx.x, q)) return;  // the whole workgroup
+  auto& sh_k = lds.k;
+  auto& sh_v = lds.v;
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) & (NW - 1);
   const int c16 = lane & 15, g = lane >> 4;
   const int G = a.heads / kv.heads;
@@ -679,8 +684,10 @@ __global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_e
       look(nb + kKeys);
       load(nb, buf ^ 1);
     }
-    scores(kb, buf, h0, h1);
-    values(buf);
+    if (!SKIP || w * RW < nrows) {
+      scores(kb, buf, h0, h1);
+      values(buf);
+    }
     if (more) finish(nb, buf ^ 1);
   }
 
@@ -720,6 +727,22 @@ __global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_e
     for (int e = 0; e < E; ++e) y[lane2 * E + e] = cut ? po[e] : pl == 0.f ? 0.f : po[e] / pl;
     if (cut && lane2 == 0) slot[R * D + r] = pm, slot[R * D + R + r] = pl;
   }
+}
+
+// The kernels. args.find: the item of a workgroup, false: there is none.
+template <int D, bool BF, int RT, class Launch>
+__global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(D < 256 ? 2 : 1)))
+    attn_stream_kernel(Launch args) {
+  __shared__ StreamLds<D, RT> sh;
+  Req q;
+  if (args.template find<16 * RT, false>(blockIdx.x, q)) attn_stream<D, BF, RT>(args.a, args.kv, q, sh);
+}
+template <int D, bool BF, int RT, class Launch>
+__global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2)))
+    attn_tile_kernel(Launch args) {
+  __shared__ TileLds<D> sh;
+  Req q;
+  if (args.template find<64 * RT, true>(blockIdx.x, q)) attn_tile<D, BF, RT, false>(args.a, args.kv, q, sh);
 }
 
 }  // namespace

@@ -26,18 +26,25 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 // ---- fork ----
 constexpr int kForkThreads = 1024;
-// Page ids of all forks that the deciding workgroup copies itself.
-constexpr int kForkSmall = 2048;
+// Entries of table (forks times ldt) up to which the deciding workgroup copies the ids itself.
+constexpr int kForkSmall = 8192;
 
-// Fork f's ids of whole pages, j0, j0 + step, ...
-__device__ __forceinline__ void fork_row(const btf_page_fork& a, int src, int dst, int whole, int j0, int step) {
-  const int* from = a.table + (size_t)src * a.ldt;
-  int* to = a.table + (size_t)dst * a.ldt;
-  for (int j = j0; j < whole; j += step) {
-    const int p = from[j];
-    to[j] = p;
-    if (p >= 0 && p < a.pages) __hip_atomic_fetch_add(a.shared + p, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  }
+// Entry j of row dst becomes row src's, if it is one of its whole pages.
+constexpr int kForkEach = 4;  // entries of a thread at a time
+struct Entry {
+  int src, dst, j;  // j below zero: none
+};
+__device__ __forceinline__ void fork_entries(const btf_page_fork& a, const Entry (&e)[kForkEach]) {
+  int p[kForkEach];
+#pragma unroll
+  for (int i = 0; i < kForkEach; ++i)
+    if (e[i].j >= 0) p[i] = a.table[(size_t)e[i].src * a.ldt + e[i].j];
+#pragma unroll
+  for (int i = 0; i < kForkEach; ++i)
+    if (e[i].j >= 0) {
+      a.table[(size_t)e[i].dst * a.ldt + e[i].j] = p[i];
+      if (p[i] >= 0 && p[i] < a.pages) __hip_atomic_fetch_add(a.shared + p[i], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
 }
 
 template <bool ROWS>
@@ -81,19 +88,34 @@ __global__ void __launch_bounds__(kForkThreads) page_fork_kernel(btf_page_fork a
   if (f == 0) *a.n_free = (int)(free0 - min((long long)all, free0));  // (each takes one: the first ones are served)
   if (!ROWS) return;
   __syncthreads();
-  for (int i = f >> 6; i < a.F; i += kForkThreads / 64) fork_row(a, sh_src[i], sh_dst[i], sh_whole[i], f & 63, 64);
+  for (int k0 = f; k0 < a.F * a.ldt; k0 += kForkEach * kForkThreads) {
+    Entry e[kForkEach];
+#pragma unroll
+    for (int i = 0; i < kForkEach; ++i) {
+      const int k = k0 + i * kForkThreads, g = k < a.F * a.ldt ? k / a.ldt : 0, j = k - g * a.ldt;
+      e[i] = Entry{sh_src[g], sh_dst[g], k < a.F * a.ldt && j < sh_whole[g] ? j : -1};
+    }
+    fork_entries(a, e);
+  }
 }
 
 __global__ void __launch_bounds__(256) page_fork_rows_kernel(btf_page_fork a) {
   const int f = blockIdx.x, n = a.got[f];
-  if (n > 0) fork_row(a, a.src[f], a.dst[f], min(n / a.page, a.ldt), blockIdx.y * 256 + threadIdx.x, gridDim.y * 256);
+  if (n < a.page) return;
+  const int whole = min(n / a.page, a.ldt), src = a.src[f], dst = a.dst[f];
+  for (int j0 = blockIdx.y * 256 * kForkEach + threadIdx.x; j0 < whole; j0 += gridDim.y * 256 * kForkEach) {
+    Entry e[kForkEach];
+#pragma unroll
+    for (int i = 0; i < kForkEach; ++i) e[i] = Entry{src, dst, j0 + 256 * i < whole ? j0 + 256 * i : -1};
+    fork_entries(a, e);
+  }
 }
 
 // ---- free ----
 constexpr int kFreeThreads = 1024;
 constexpr int kFreeEach = 4;                          // places of a thread
 constexpr int kFreeChunk = kFreeThreads * kFreeEach;  // ... of a workgroup
-constexpr int kFreeMost = 16;                         // ... of a thread, where one workgroup does it all
+constexpr int kFreeMost = 8;                          // ... of a thread at most, where one workgroup does it all
 
 // Whether places e0, e0 + 1, ... (place s * ldt + j is page j of row s) give up their pages, and the pages' ids, -1: none
 // that the cache has. (Loads without branches, so that all are on their way at once.)
@@ -124,8 +146,9 @@ __device__ __forceinline__ Places<EACH> places_of(const btf_page_free& a, const 
   }
   return p;
 }
-__device__ __forceinline__ void lower(const btf_page_free& a, int page) {
-  if (page >= 0) __hip_atomic_fetch_add(a.shared + page, -1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+// Lowers the page's count; what it was.
+__device__ __forceinline__ int lower(const btf_page_free& a, int page) {
+  return page < 0 ? -1 : __hip_atomic_fetch_add(a.shared + page, -1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 __device__ __forceinline__ int count_of(const btf_page_free& a, int page) {
   return __hip_atomic_load(a.shared + page, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -179,20 +202,40 @@ __device__ __forceinline__ void all_done() {
 template <int EACH>
 __global__ void __launch_bounds__(kFreeThreads) page_free_small_kernel(btf_page_free a) {
   __shared__ uint64_t part[kFreeThreads / 64];
+  __shared__ int sh_several;
   const int e0 = threadIdx.x * EACH;
   const long long n0 = min((long long)max(*a.n_free, 0), (long long)a.pages);
   const Places<EACH> p = places_of<EACH>(a, a.held, e0);
-  if (a.shared) {
+  unsigned own = 0;
+  if (!a.shared) {
+    own = owned(a, p, e0);
+  } else {
+    // Who lowers a count from 0 gives the page back, unless other places gave up the same page: these found it above 0 (or
+    // below) and find it below 0 now. Only then the marks decide.
+    int was[EACH], count[EACH];
 #pragma unroll
-    for (int i = 0; i < EACH; ++i) lower(a, p.page[i]);
+    for (int i = 0; i < EACH; ++i) was[i] = lower(a, p.page[i]);
+    bool several = false;
+    if (threadIdx.x == 0) sh_several = 0;
     all_done();
-    int count[EACH];
-    counts_of(a, p, count);
 #pragma unroll
-    for (int i = 0; i < EACH; ++i) mark(a, p.page[i], count[i], e0 + i);
-    all_done();
+    for (int i = 0; i < EACH; ++i) count[i] = p.page[i] >= 0 && was[i] != 0 ? count_of(a, p.page[i]) : 0;
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) {
+      several |= count[i] < 0;
+      own |= (unsigned)(p.page[i] >= 0 && was[i] == 0) << i;
+    }
+    if (several) sh_several = 1;
+    __syncthreads();
+    if (sh_several) {
+      counts_of(a, p, count);
+      all_done();
+#pragma unroll
+      for (int i = 0; i < EACH; ++i) mark(a, p.page[i], count[i], e0 + i);
+      all_done();
+      own = owned(a, p, e0);
+    }
   }
-  const unsigned own = owned(a, p, e0);
   uint64_t all;
   const uint64_t upto = block_scan<kFreeThreads>(__popc(own), part, &all);  // (and all have read what is written below)
   give_back(a, p, own, e0, n0, (long long)(all - upto));
@@ -316,43 +359,64 @@ __global__ void __launch_bounds__(N) cache_move_kernel(btf_cache_move a, btf_kv_
     return p < 0 || p >= kv.pages ? -1 : p * (long long)kv.page_stride + (place & (kv.page - 1)) * (long long)kv.tok_stride;
   };
   constexpr int kAtOnce = N / 8;  // tokens
-  constexpr int kMine = TREE ? 2 : kInFlight;
-  for (int i0 = 0; i0 < n; i0 += kAtOnce * kMine) {
-    u32x4 v[kMine];
-    long long to[kMine];
+  // Two batches in flight: while one's values arrive, the places and page ids of the next are looked up; its values are
+  // under way before this one's are stored.
+  constexpr int kMine = 2;  // tokens of a thread (with more than 64 registers only one workgroup of 1024 threads fits a CU)
+  u32x4 v[2][kMine];
+  long long from[2][kMine], to[2][kMine];
+  auto look = [&](int i0, int b) {
 #pragma unroll
     for (int u = 0; u < kMine; ++u) {
       const int i = i0 + u * kAtOnce + (threadIdx.x >> 3);
-      to[u] = -1;
+      from[b][u] = to[b][u] = -1;
       if (i < n) {
-        long long from;
+        long long place;
         if (TREE) {  // the i-th set bit
-          unsigned long long b = bits;
+          unsigned long long w = bits;
           int k = i, pos = 0;
 #pragma unroll
           for (int half = 32; half; half >>= 1) {
-            const int c = __popcll(b & ((1ull << half) - 1));
-            if (k >= c) k -= c, pos += half, b >>= half;
+            const int c = __popcll(w & ((1ull << half) - 1));
+            if (k >= c) k -= c, pos += half, w >>= half;
           }
-          from = (long long)first + pos;
+          place = (long long)first + pos;
         } else {
-          from = a.source[lo + i];
+          place = a.source[lo + i];
         }
         const long long dst = (long long)first + i;
-        if (a.to_table || from != dst) {
-          const long long x = where(tab, a.ldt, from);
-          if (x >= 0) to[u] = where(tab_to, ld_to, dst);
-          if (to[u] >= 0) v[u] = *reinterpret_cast<const u32x4*>(base + x);
+        if (a.to_table || place != dst) {
+          from[b][u] = where(tab, a.ldt, place);
+          to[b][u] = where(tab_to, ld_to, dst);
         }
       }
     }
-    // every thread's loads have arrived before any thread stores
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
+  };
+  auto load = [&](int b) {
 #pragma unroll
-    for (int u = 0; u < kMine; ++u)
-      if (to[u] >= 0) *reinterpret_cast<u32x4*>(base + to[u]) = v[u];
-  }
+    for (int u = 0; u < kMine; ++u) {
+      if (from[b][u] < 0) to[b][u] = -1;
+      if (to[b][u] >= 0) v[b][u] = *reinterpret_cast<const u32x4*>(base + from[b][u]);
+    }
+  };
+  constexpr int kBatch = kAtOnce * kMine;
+  if (n <= 0) return;
+  look(0, 0);
+  load(0);
+  for (int i0 = 0; i0 < n; i0 += 2 * kBatch)
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      const int at = i0 + b * kBatch;
+      if (at >= n) break;
+      const bool more = at + kBatch < n;
+      if (more) look(at + kBatch, b ^ 1);
+      // every thread's values have arrived before any thread stores
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      __syncthreads();
+      if (more) load(b ^ 1);
+#pragma unroll
+      for (int u = 0; u < kMine; ++u)
+        if (to[b][u] >= 0) *reinterpret_cast<u32x4*>(base + to[b][u]) = v[b][u];
+    }
 }
 
 int free_chunks(int S, int ldt) { return (int)(((int64_t)S * ldt + kFreeChunk - 1) / kFreeChunk); }
@@ -367,7 +431,7 @@ int page_fork(const btf_page_fork& a, hipStream_t st) {
   hipLaunchKernelGGL(page_fork_kernel<false>, dim3(1), dim3(kForkThreads), 0, st, a);
   const int rc = launch_status("page_fork_kernel");
   if (rc != BTF_OK) return rc;
-  const int y = (a.ldt + 255) / 256;
+  const int y = (a.ldt + 256 * kForkEach - 1) / (256 * kForkEach);
   hipLaunchKernelGGL(page_fork_rows_kernel, dim3(a.F, y < 64 ? y : 64), dim3(256), 0, st, a);
   return launch_status("page_fork_rows_kernel");
 }
@@ -380,7 +444,8 @@ int64_t page_free_ws_bytes(int S, int ldt) {
 int page_free(const btf_page_free& a, hipStream_t st) {
   const int n = free_chunks(a.S, a.ldt);
   if (n * kFreeEach <= kFreeMost) {
-    if (n <= 1) hipLaunchKernelGGL(page_free_small_kernel<kFreeEach>, dim3(1), dim3(kFreeThreads), 0, st, a);
+    if ((int64_t)a.S * a.ldt <= kFreeThreads) hipLaunchKernelGGL(page_free_small_kernel<1>, dim3(1), dim3(kFreeThreads), 0, st, a);
+    else if (n <= 1) hipLaunchKernelGGL(page_free_small_kernel<kFreeEach>, dim3(1), dim3(kFreeThreads), 0, st, a);
     else hipLaunchKernelGGL(page_free_small_kernel<kFreeMost>, dim3(1), dim3(kFreeThreads), 0, st, a);
     return launch_status("page_free_small_kernel");
   }
@@ -406,7 +471,8 @@ int page_copy(const btf_page_copy& a, const btf_kv_cache& kv, hipStream_t st) {
 
 int cache_move(const btf_cache_move& a, const btf_kv_cache& kv, hipStream_t st) {
   const dim3 grid(2 * a.S * kv.heads * (kv.dim / 64), a.layers);
-  // A tree's path in batches of 16 tokens, a list in batches of 1024.
+  // A tree's path in batches of 16 tokens. A list in batches of 256 with as many threads as there are: 8 requests of up to
+  // 16384 tokens, half of which stay, 2 layers, 187 us (3.9 TB/s read and written) with 1024 threads, 247 with 512, 278 with 256.
   if (a.tree) hipLaunchKernelGGL((cache_move_kernel<64, true>), grid, dim3(64), 0, st, a, kv);
   else hipLaunchKernelGGL((cache_move_kernel<1024, false>), grid, dim3(1024), 0, st, a, kv);
   return launch_status("cache_move_kernel");

@@ -3,17 +3,19 @@
 //
 // A row's softmax over prefix and own keys is put together from sums over pieces
 // of the keys, (maximum, sum, values) each, so the pieces of the prefix can be done
-// for the rows of all requests that see them at once. Two roles, both with the
-// kernels of attn_core.h: a group's rows are one request of many rows over the
-// prefix, all of which they see; each request's rows go over its own keys, from
-// where the prefix ends. shared_join_kernel puts a row's pieces of both together.
+// for the rows of all requests that see them at once. Two roles: a group's rows are
+// one request of many rows over the prefix, all of which they see; each request's
+// rows go over its own keys, from where the prefix ends. Both are items of
+// attn_core.h, of one launch: a group's items are bound by matrix instructions, a
+// request's by HBM, and run beside each other. shared_join_kernel puts a row's pieces
+// of both together.
 //
 // shared_plan_kernel, one workgroup, finds who takes part (a member needs the whole
-// prefix before its new rows), cuts both roles into items of like size and writes
-// down which item is whose: with up to hundreds of requests a workgroup that looked
-// for itself, as launch_paged_attention's do, would read all lengths several times.
-// The prefix counts in steps of 32 keys, a block of the kernels; what is left of it
-// is done with each member's own keys, which its row of table has, too.
+// prefix before its new rows), cuts both roles into items and writes down which item
+// is whose: with up to hundreds of requests a workgroup that looked for itself, as
+// launch_paged_attention's do, would read all lengths several times. The prefix counts
+// in steps of 32 keys, a block of the kernels; what is left of it is done with each
+// member's own keys, which its row of table has, too.
 #include <string>
 
 #include "../../include/btf/hip_abi.h"
@@ -35,31 +37,37 @@ static_assert(sizeof(Found) == 64, "one line");
 
 // The parts of the workspace.
 struct Ws {
-  int* items;     // [2] of the groups, of the requests
+  int* items;     // [1]
   Found* found;   // [groups + S]
-  int* map[2];    // [most[i]] the group or request of an item
+  int* map;       // [most] the group or request of an item, as found has them
   int* request;   // [T] of a row, -1: none
-  float* slots[2];
-  int most[2];
+  float* slots;   // the groups', then the requests'
+  int most;       // items at most
 };
 
 struct Plan : Args {
   Ws ws;
   int groups;
   const int *group0, *lead, *shared;
-  int R[2];       // rows of a tile
+  int R[2];       // rows of a tile of a group, of a request
 };
 
 constexpr int kPlanThreads = 1024;
 
-// Pieces of the keys for `work` tiles times keys in all: about `items` of like size (see target and least).
-__device__ __forceinline__ int piece_keys(uint64_t work, int R, int items) {
-  const uint64_t w = work / kStep;  // in the smallest pieces
-  const uint64_t c = w / (uint64_t)items + 1, few = w / kPlaces + 1;
-  const uint64_t l = (uint64_t)(least(R) / kStep);
-  const uint64_t f = few < l ? few : l;
-  return kStep * (int)(c > f ? c : f);
+// A group's items are long and bound by matrix instructions, a
+// request's short and bound by HBM; the groups' come first. 512 workgroups run at a time, two a CU: the groups get their
+// share of these by the roles' work (a request's keys count twice, for what an item costs beside its keys), at least half,
+// the requests' items fill the rest and follow (64 requests behind 16384 keys with 250 to 1000 of their own, heads of 256:
+// the call 85 us, with 512 items of the groups 95, 192 104; a group alone 56 us in 512 items, 69 in 256).
+constexpr int kRunning = 512, kOwnItems = 384;
+__device__ __forceinline__ int piece_keys(uint64_t groups, uint64_t requests, int role) {
+  const int share = (int)(kRunning * ((float)groups / ((float)groups + 2.f * (float)requests + 1.f)));
+  const uint64_t items = role ? kOwnItems : max(share, kRunning / 2);
+  return kStep * (int)((role ? requests : groups) / (kStep * items) + 1);
 }
+// Floats of a slot, and the requests' first slot behind n of the groups'.
+__device__ __forceinline__ int64_t slot_of(const Plan& p, int role) { return (int64_t)p.R[role] * (p.kv.dim + 2); }
+__device__ __forceinline__ int slots_behind(const Plan& p, int n) { return (int)((n * slot_of(p, 0) + slot_of(p, 1) - 1) / slot_of(p, 1)); }
 
 __device__ __forceinline__ int tiles_of(const Plan& p, int n, int R) {
   return n > 0 ? (int)(((long long)n * (p.a.heads / p.kv.heads) + R - 1) / R) : 0;
@@ -167,7 +175,7 @@ __global__ void __launch_bounds__(kPlanThreads) shared_plan_small_kernel(Plan p)
 #pragma unroll
   for (int role = 0; role < 2; ++role)
     if (role ? request : group) {
-      f[role].C = piece_keys(all[role] * p.kv.heads, p.R[role], target(p.R[role]));
+      f[role].C = piece_keys(all[0] * p.kv.heads, all[1] * p.kv.heads, role);
       f[role].pieces = max(1, (f[role].len - f[role].begin + f[role].C - 1) / f[role].C);
       own[role] = p.kv.heads * f[role].tiles * f[role].pieces;
       if (f[role].group >= 0 || f[role].pieces > 1) f[role].flags |= kCut;
@@ -176,27 +184,28 @@ __global__ void __launch_bounds__(kPlanThreads) shared_plan_small_kernel(Plan p)
 #pragma unroll
   for (int role = 0; role < 2; ++role) v[role] = (uint64_t)(uint32_t)own[role] | (uint64_t)(uint32_t)cut[role] << 32;
   scan2(v, part, all);
+  const int first[2] = {0, (int)all[0]}, behind = slots_behind(p, (int)(all[0] >> 32));
 #pragma unroll
   for (int role = 0; role < 2; ++role) {
     sh_upto[role][tid] = (int)v[role];
     if (role ? request : group) {
-      f[role].item0 = (int)v[role] - own[role];
-      f[role].slot0 = (int)(v[role] >> 32) - cut[role];
+      f[role].item0 = first[role] + (int)v[role] - own[role];
+      f[role].slot0 = (role ? behind : 0) + (int)(v[role] >> 32) - cut[role];
       p.ws.found[role ? p.groups + tid : tid] = f[role];
     }
-    if (tid == 0) p.ws.items[role] = min((int)all[role], p.ws.most[role]);
   }
+  if (tid == 0) *p.ws.items = min((int)all[0] + (int)all[1], p.ws.most);
   __syncthreads();
 #pragma unroll
   for (int role = 0; role < 2; ++role)
-    for (int k = tid; k < min((int)all[role], p.ws.most[role]); k += kPlanThreads) {
+    for (int k = tid; k < min((int)all[role], p.ws.most - first[role]); k += kPlanThreads) {
       int lo = 0, hi = (role ? a.S : p.groups) - 1;  // the first one with upto > k
       while (lo < hi) {
         const int mid = (lo + hi) >> 1;
         if (sh_upto[role][mid] > k) hi = mid;
         else lo = mid + 1;
       }
-      p.ws.map[role][k] = lo;
+      p.ws.map[first[role] + k] = role ? p.groups + lo : lo;
     }
   for (int t = tid; t < a.T; t += kPlanThreads) {
     const int s = last_at_most(sh_row0, a.S, t);
@@ -235,12 +244,13 @@ __global__ void __launch_bounds__(kPlanThreads) shared_plan_kernel(Plan p) {
   uint64_t all[2];
   (void)block_scan<kPlanThreads>(work[0], part, &all[0]);
   (void)block_scan<kPlanThreads>(work[1], part, &all[1]);
+  long long items = 0, slots = 0;  // before the chunk
 #pragma unroll
   for (int role = 0; role < 2; ++role) {
     const int count = role ? a.S : p.groups;
     Found* const list = role ? mine : p.ws.found;
-    const int C = piece_keys(all[role] * kv.heads, p.R[role], target(p.R[role]));
-    long long items = 0, slots = 0;  // before the chunk
+    const int C = piece_keys(all[0] * kv.heads, all[1] * kv.heads, role);
+    if (role) slots = slots_behind(p, (int)slots);
     for (int i0 = 0; i0 < count; i0 += kPlanThreads) {
       const int i = i0 + tid;
       int own = 0, cut = 0, row0 = 0, n = 0;
@@ -272,7 +282,7 @@ __global__ void __launch_bounds__(kPlanThreads) shared_plan_kernel(Plan p) {
           if (sh_upto[mid] > k) hi = mid;
           else lo = mid + 1;
         }
-        if (items + k < p.ws.most[role]) p.ws.map[role][items + k] = i0 + lo;
+        if (items + k < p.ws.most) p.ws.map[items + k] = (role ? p.groups : 0) + i0 + lo;
       }
       if (role)
         for (int w = tid >> 6; w < min(kPlanThreads, count - i0); w += kPlanThreads / 64)
@@ -281,34 +291,74 @@ __global__ void __launch_bounds__(kPlanThreads) shared_plan_kernel(Plan p) {
       slots += (long long)cuts;
       __syncthreads();
     }
-    if (tid == 0) p.ws.items[role] = (int)min(items, (long long)p.ws.most[role]);
   }
+  if (tid == 0) *p.ws.items = (int)min(items, (long long)p.ws.most);
 }
 
-// One role's launch as the kernels take it: a.ws is its slots.
 typedef __attribute__((address_space(4))) const Found* found_p;
 typedef __attribute__((address_space(4))) const int* ints_p;
-struct Role : Args {
+
+// The launch of the items as the kernels take it: a.ws is the slots.
+struct Items : Args {
   const int *items, *map;
   const Found* found;
-  template <int R, bool SCALAR>
-  __device__ __forceinline__ bool find(int id, Req& q) const {
-    if (id >= *(ints_p)items) return false;
-    const found_p f = (found_p)found + ((ints_p)map)[id];
-    q.s = f->s, q.row0 = f->row0, q.n = f->n, q.len = f->len, q.ctx = f->ctx;
-    q.tiles = f->tiles, q.pieces = f->pieces, q.begin = f->begin, q.C = f->C;
-    q.local = id - f->item0;
-    q.slot = f->slot0;
-    q.tree = f->flags & kTree;
-    q.cut = f->flags & kCut;
-    if (!SCALAR) {  // (in vector registers)
-      auto vector = [](int& v) { asm("" : "+v"(v)); };
-      vector(q.s), vector(q.row0), vector(q.n), vector(q.len), vector(q.ctx), vector(q.tiles), vector(q.pieces);
-      vector(q.begin), vector(q.C), vector(q.local), vector(q.slot);
-    }
-    return true;
-  }
+  int groups;
 };
+
+// Item `id`, in scalar registers. False: there is none.
+__device__ __forceinline__ bool find_item(const Items& p, int id, Req& q, bool& group) {
+  if (id >= *(ints_p)p.items) return false;
+  const int v = ((ints_p)p.map)[id];
+  const found_p f = (found_p)p.found + v;
+  group = v < p.groups;
+  q.s = f->s, q.row0 = f->row0, q.n = f->n, q.len = f->len, q.ctx = f->ctx;
+  q.tiles = f->tiles, q.pieces = f->pieces, q.begin = f->begin, q.C = f->C;
+  q.slot = f->slot0;
+  q.tree = f->flags & kTree;
+  q.cut = f->flags & kCut;
+  int local = id - f->item0;
+  if (q.tiles > 1) {
+    // The tiles that read the same keys eight workgroups apart, so that they share an XCD's L2 (workgroups go to the eight
+    // XCDs in turn): pairs (piece, KV head) by eights, each with all its tiles.
+    const int heads = p.kv.heads, pairs = q.pieces * heads, at = local / (8 * q.tiles), rest = local - at * 8 * q.tiles;
+    const int wide = min(8, pairs - 8 * at), tile = rest / wide, pair = 8 * at + rest - tile * wide;
+    local = (pair / heads * q.tiles + tile) * heads + pair % heads;
+  }
+  q.local = local;
+  return true;
+}
+
+// A tile of R rows: attn_stream up to 16, attn_tile with one or two tiles of 16 a wave.
+template <int D, int R>
+struct LdsOf {
+  typedef TileLds<D> type;
+};
+template <int D>
+struct LdsOf<D, 16> {
+  typedef StreamLds<D, 1> type;
+};
+template <int D, bool BF, int R, bool TWO>
+__device__ __forceinline__ void item(const Items& p, Req& q, void* lds) {
+  const Args own = TWO ? fresh_args() : Args{p.a, p.kv};  // (two kinds of tiles: nothing kept from before the branch)
+  if constexpr (R == 16) {
+    auto vector = [](int& v) { asm("" : "+v"(v)); };  // (attn_stream has no scalar registers to spare)
+    vector(q.s), vector(q.row0), vector(q.n), vector(q.len), vector(q.ctx), vector(q.tiles), vector(q.pieces);
+    vector(q.begin), vector(q.C), vector(q.local), vector(q.slot);
+    attn_stream<D, BF, 1>(own.a, own.kv, q, *static_cast<StreamLds<D, 1>*>(lds));
+  } else {
+    attn_tile<D, BF, R / 64, true>(own.a, own.kv, q, *static_cast<TileLds<D>*>(lds));
+  }
+}
+template <int D, bool BF, int R0, int R1>
+__global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(D == 256 && R1 == 16 ? 1 : 2))) shared_kernel(Items p) {
+  constexpr size_t a = sizeof(typename LdsOf<D, R0>::type), b = sizeof(typename LdsOf<D, R1>::type);
+  __shared__ __attribute__((aligned(16))) char lds[a > b ? a : b];
+  Req q;
+  bool group;
+  if (!find_item(p, blockIdx.x, q, group)) return;  // the whole workgroup
+  if (R0 == R1 || group) item<D, BF, R0, R0 != R1>(p, q, lds);
+  else item<D, BF, R1, R0 != R1>(p, q, lds);
+}
 
 // The pieces of one row of one head, the group's and its own, put together: as attn_join_kernel.
 constexpr int kJoinWaves = 4;
@@ -332,7 +382,7 @@ __global__ void __launch_bounds__(64 * kJoinWaves) shared_join_kernel(Plan p) {
     const size_t slot = (size_t)R * (D + 2);
     r = row % R;
     step = (size_t)f->tiles * p.kv.heads * slot;
-    return p.ws.slots[role] + ((size_t)f->slot0 + (size_t)(f->tiles - 1 - tile) * p.kv.heads + kvh) * slot;
+    return p.ws.slots + ((size_t)f->slot0 + (size_t)(f->tiles - 1 - tile) * p.kv.heads + kvh) * slot;
   };
   int n0 = 0, r0 = 0, r1;
   size_t step0 = 0, step1;
@@ -397,50 +447,31 @@ __global__ void __launch_bounds__(64 * kJoinWaves) shared_join_kernel(Plan p) {
   }
 }
 
-// Rows of a tile of `count` groups or requests that have T rows in all (launch_paged_attention's rule).
+// Rows of a tile of `count` groups or requests that have T rows in all.
 int tile_rows(int count, int T, int heads, const btf_kv_cache& kv) {
   const int64_t rows = (int64_t)T * (heads / kv.heads);
   if (rows <= 16 * (int64_t)count) return 16;
-  if (kv.dim == 256) return 64;
-  if (rows <= 32 * (int64_t)count) return 32;
-  return kv.dim == 64 || rows <= 128 * (int64_t)count ? 64 : 128;
+  return kv.dim != 128 || rows <= 128 * (int64_t)count ? 64 : 128;
 }
 
 // Items of a role at most: each tile's last piece may be a part of one.
 int64_t most_items(int count, int T, int heads, const btf_kv_cache& kv, int R) {
-  return ((int64_t)T * (heads / kv.heads) / R + count) * kv.heads + target(R);
+  return ((int64_t)T * (heads / kv.heads) / R + count) * kv.heads + kRunning + kOwnItems;
 }
 
 // Floats of a role's slots, for a launch of up to S requests and T rows, whatever tiles it takes: slots * R is at most
-// T * heads + count * KV heads * R + target(R) * R, and count * R at most 4 T * heads / KV heads for the tiles above 16.
+// T * heads + count * KV heads * R + the items * R, and count * R at most 4 T * heads / KV heads for the tiles above 16
+// (64 only where a request has more than 16 rows on average, 128 where it has more than 128).
 int64_t slot_floats(int S, int T, int heads, const btf_kv_cache& kv) {
   const int64_t rows = (int64_t)T * heads, few = 16 * (int64_t)S * kv.heads, top = kv.dim == 128 ? 128 : 64;
-  return (rows + (few > 4 * rows ? few : 4 * rows) + target(64) * top) * (kv.dim + 2);
+  return (rows + (few > 4 * rows ? few : 4 * rows) + (kRunning + kOwnItems + 1) * top) * (kv.dim + 2);
 }
 
 int64_t up(int64_t n) { return (n + 255) & ~(int64_t)255; }
 
 // Bytes before the slots, for up to S requests and groups.
 int64_t plan_bytes(int S, int T, int heads, const btf_kv_cache& kv) {
-  const int64_t most = most_items(S, T, heads, kv, 16) + target(16);
-  return up(64 + 2 * (int64_t)S * sizeof(Found) + 8 * most + 4 * (int64_t)T);
-}
-
-template <int D, bool BF>
-int role_go(const Role& r, int R, unsigned grid, hipStream_t st) {
-  const dim3 blk(64 * kWaves);
-  if (R == 16) {
-    hipLaunchKernelGGL((attn_stream_kernel<D, BF, 1, Role>), dim3(grid), blk, 0, st, r);
-  } else if (R == 64) {
-    hipLaunchKernelGGL((attn_tile_kernel<D, BF, 1, Role>), dim3(grid), blk, 0, st, r);
-  } else if constexpr (D < 256) {
-    if (R == 32) {
-      hipLaunchKernelGGL((attn_stream_kernel<D, BF, 2, Role>), dim3(grid), blk, 0, st, r);
-    } else if constexpr (D == 128) {
-      hipLaunchKernelGGL((attn_tile_kernel<D, BF, 2, Role>), dim3(grid), blk, 0, st, r);
-    }
-  }
-  return launch_status("shared attention kernel");
+  return up(64 + 2 * (int64_t)S * sizeof(Found) + 8 * most_items(S, T, heads, kv, 16) + 4 * (int64_t)T);
 }
 
 template <int D, bool BF>
@@ -449,14 +480,24 @@ int shared_go(const Plan& p, hipStream_t st) {
   else hipLaunchKernelGGL(shared_plan_kernel, dim3(1), dim3(kPlanThreads), 0, st, p);
   int rc = launch_status("shared_plan_kernel");
   if (rc != BTF_OK) return rc;
-  const int64_t room = ((int64_t)p.a.ldt * p.kv.page + kStep - 1) / kStep;
-  for (int role = p.groups ? 0 : 1; role < 2; ++role) {
-    Role r{{p.a, p.kv}, p.ws.items + role, p.ws.map[role], role ? p.ws.found + p.groups : p.ws.found};
-    r.a.ws = p.ws.slots[role];
-    const int64_t tiles = p.ws.most[role] - target(p.R[role]);
-    rc = role_go<D, BF>(r, p.R[role], (unsigned)(tiles * room < p.ws.most[role] ? tiles * room : p.ws.most[role]), st);
-    if (rc != BTF_OK) return rc;
+  const Items items{{p.a, p.kv}, p.ws.items, p.ws.map, p.ws.found, p.groups};
+  auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3((unsigned)p.ws.most), dim3(64 * kWaves), 0, st, items); };
+  const int R0 = p.R[0], R1 = p.R[1];
+  if (R0 == 16) {
+    go(shared_kernel<D, BF, 16, 16>);
+  } else if (R1 == 16) {
+    if constexpr (D == 128) {
+      if (R0 == 64) go(shared_kernel<D, BF, 64, 16>);
+      else go(shared_kernel<D, BF, 128, 16>);
+    }
+  } else if (R0 == 64) {
+    go(shared_kernel<D, BF, 64, 64>);
+  } else if constexpr (D == 128) {
+    if (R1 == 64) go(shared_kernel<D, BF, 128, 64>);
+    else go(shared_kernel<D, BF, 128, 128>);
   }
+  rc = launch_status("shared_kernel");
+  if (rc != BTF_OK) return rc;
   const bool one = (int64_t)p.a.T * p.a.heads >= 2048;
   const dim3 join(p.a.T, one ? (p.a.heads + kJoinWaves - 1) / kJoinWaves : p.a.heads), blk(64 * kJoinWaves);
   if (one) hipLaunchKernelGGL((shared_join_kernel<D, true>), join, blk, 0, st, p);
@@ -467,7 +508,7 @@ int shared_go(const Plan& p, hipStream_t st) {
 }  // namespace
 
 int64_t shared_attention_most_items(int S, int T, int heads, const btf_kv_cache& kv) {
-  return most_items(S, T, heads, kv, 16) + target(16);
+  return 2 * most_items(S, T, heads, kv, 16);
 }
 
 int64_t shared_attention_ws_bytes(int S, int T, int heads, const btf_kv_cache& kv) {
@@ -476,25 +517,22 @@ int64_t shared_attention_ws_bytes(int S, int T, int heads, const btf_kv_cache& k
 
 int shared_attention(const btf_shared_attention& a, const btf_kv_cache& kv, hipStream_t st) {
   Plan p{};
-  p.a = btf_paged_attention{a.S, a.T, a.heads, a.q, a.ldq, a.table, a.ldt, a.row0, a.kv_len, a.tree, a.scale, a.out, a.ldo, a.ws};
   p.kv = kv;
   p.groups = a.groups;
   p.group0 = a.group0, p.lead = a.lead, p.shared = a.shared;
-  p.R[0] = tile_rows(a.groups > 0 ? a.groups : 1, a.T, a.heads, kv);
   p.R[1] = tile_rows(a.S, a.T, a.heads, kv);
+  p.R[0] = a.groups > 0 ? tile_rows(a.groups, a.T, a.heads, kv) : p.R[1];
+  // (heads of 64 and 256 have one kind of tile in a launch: attn_stream with 256 leaves room for one workgroup a CU only)
+  if (kv.dim != 128 && p.R[0] == 64) p.R[1] = 64;
   char* at = static_cast<char*>(a.ws);
   p.ws.items = reinterpret_cast<int*>(at);
   p.ws.found = reinterpret_cast<Found*>(at + 64);
-  int* ints = reinterpret_cast<int*>(p.ws.found + a.groups + a.S);
-  for (int role = 0; role < 2; ++role) {
-    p.ws.most[role] = (int)most_items(role ? a.S : a.groups, a.T, a.heads, kv, p.R[role]);
-    p.ws.map[role] = ints;
-    ints += p.ws.most[role];
-  }
-  p.ws.request = ints;
-  float* slots = reinterpret_cast<float*>(at + plan_bytes(a.S, a.T, a.heads, kv));
-  p.ws.slots[0] = slots;
-  p.ws.slots[1] = slots + up(4 * slot_floats(a.S, a.T, a.heads, kv)) / 4;
+  p.ws.map = reinterpret_cast<int*>(p.ws.found + a.groups + a.S);
+  p.ws.most = (int)(most_items(a.S, a.T, a.heads, kv, p.R[1]) + (a.groups ? most_items(a.groups, a.T, a.heads, kv, p.R[0]) : 0));
+  p.ws.request = p.ws.map + p.ws.most;
+  p.ws.slots = reinterpret_cast<float*>(at + plan_bytes(a.S, a.T, a.heads, kv));
+  p.a = btf_paged_attention{a.S,   a.T,    a.heads, a.q,   a.ldq, a.table,    a.ldt,
+                            a.row0, a.kv_len, a.tree, a.scale, a.out, a.ldo, p.ws.slots};
   const bool bf = kv.type == BTF_BF16;
   if (kv.dim == 64) return bf ? shared_go<64, true>(p, st) : shared_go<64, false>(p, st);
   if (kv.dim == 128) return bf ? shared_go<128, true>(p, st) : shared_go<128, false>(p, st);

@@ -132,7 +132,7 @@ def test_forks_refused(hip):
         same({**st.fork(src, dst, n), **st.values()}, ref.fork(src, dst, n, start[2], n_free, start[0], held, start[4], 16, start[5]))
 
 
-@pytest.mark.parametrize("S,ldt", [(6, 20), (300, 40), (600, 50)])  # one workgroup, one with more places a thread, several
+@pytest.mark.parametrize("S,ldt", [(6, 20), (80, 40), (150, 40), (600, 50)])  # one workgroup with one, four and eight places a thread, several
 @pytest.mark.parametrize("counted", [True, False])
 def test_free_of_what_is_wrong(hip, S, ldt, counted):
     """Ids outside the cache, rows that hold more than they have or less than nothing, a page in a row twice, pages given up

@@ -124,7 +124,7 @@ def test_nothing_to_do(op, change):
 def test_workspaces():
     """None where nothing is launched; those of the largest launch serve the smaller ones."""
     assert h.page_free_ws_bytes(0, 8) == h.page_free_ws_bytes(8, 0) == h.page_free_ws_bytes(1 << 20, 1 << 9) == 0
-    assert h.page_free_ws_bytes(400, 40) == 0 < h.page_free_ws_bytes(300, 60) < h.page_free_ws_bytes(301, 4000)
+    assert h.page_free_ws_bytes(200, 40) == 0 < h.page_free_ws_bytes(300, 60) < h.page_free_ws_bytes(301, 4000)
     assert h.shared_attention_ws_bytes(0, 8, 20, KV) == h.shared_attention_ws_bytes(2, 8, 18, KV) == 0
     assert h.lora_ws_bytes(0, 1, 512, 16, 1) == h.lora_ws_bytes(1, 1, 512, 16, 4) == h.lora_ws_bytes(1, 1, 512, 512, 1) == 0
     for dim in (64, 128, 256):
