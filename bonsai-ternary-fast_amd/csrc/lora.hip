@@ -414,51 +414,74 @@ __global__ void __launch_bounds__(kThreads, 2) lora_shrink_few_kernel(btf_lora a
   const btf_lora_seg& s = segs.s[seg];
   const int end = min(a.K, (k + 1) * slice), all = (t.rank + kFewRanks - 1) / kFewRanks;
   const int groups = all >= 4 ? 4 : all >= 2 ? 2 : 1, share = kWaves / groups;
-  for (int g0 = 0; g0 < all; g0 += groups) {
-    const int first = (g0 + w / share) * kFewRanks, ranks = min(t.rank - first, kFewRanks);
-    float acc[kFewRanks][R] = {};
-    const uint16_t* m = static_cast<const uint16_t*>(s.a) + (size_t)t.adapter * s.a_stride + (size_t)first * a.K;
-    const float* x = a.x + (size_t)t.row * a.ldx;
-    for (int kb = k * slice + w % share * kFewK; kb < end && ranks > 0; kb += share * kFewK) {
-      const bool in = kb + 8 * lane < end;
-      f32x4 xv[R][2] = {};
-      u32x4 av[kFewRanks];
+  // Steps (ranks from g0 on, columns from kb on) in turn, the next one's loads under way while one is worked on.
+  struct Step {
+    int g0, kb;
+  };
+  const int kb0 = k * slice + w % share * kFewK;
+  auto next_of = [&](Step p) { return p.kb + share * kFewK < end ? Step{p.g0, p.kb + share * kFewK} : Step{p.g0 + groups, kb0}; };
+  auto ranks_of = [&](int g0) { return min(t.rank - (g0 + w / share) * kFewRanks, kFewRanks); };
+  u32x4 av[kFewRanks];
+  f32x4 xv[R][2];
+  auto load = [&](Step p) {
+    const int first = (p.g0 + w / share) * kFewRanks, ranks = ranks_of(p.g0);
+    const uint16_t* m = static_cast<const uint16_t*>(s.a) + (size_t)t.adapter * s.a_stride + (size_t)first * a.K + p.kb;
+    const float* x = a.x + (size_t)t.row * a.ldx + p.kb;
+    const bool in = p.kb + 8 * lane < end;
 #pragma unroll
-      for (int i = 0; i < kFewRanks; ++i) {
-        av[i] = u32x4{0, 0, 0, 0};
-        if (in && i < ranks) av[i] = reinterpret_cast<const u32x4*>(m + (size_t)i * a.K + kb)[lane];
+    for (int i = 0; i < kFewRanks; ++i) {
+      av[i] = u32x4{0, 0, 0, 0};
+      if (in && i < ranks) av[i] = reinterpret_cast<const u32x4*>(m + (size_t)i * a.K)[lane];
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        xv[r][u] = f32x4{0.f, 0.f, 0.f, 0.f};
+        if (in && r < t.n) xv[r][u] = reinterpret_cast<const f32x4*>(x + (size_t)r * a.ldx)[2 * lane + u];
       }
+  };
+  Step at{0, kb0};
+  load(at);
+  float acc[kFewRanks][R] = {};
+  while (at.g0 < all) {
+    const Step next = next_of(at);
+    u32x4 ac[kFewRanks];
+    float xs[R][8];
 #pragma unroll
-      for (int r = 0; r < R; ++r)
-        if (in && r < t.n)
+    for (int i = 0; i < kFewRanks; ++i) ac[i] = av[i];
 #pragma unroll
-          for (int u = 0; u < 2; ++u) xv[r][u] = reinterpret_cast<const f32x4*>(x + (size_t)r * a.ldx + kb)[2 * lane + u];
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) xs[r][j] = xv[r][j >> 2][j & 3];
+    if (next.g0 < all) load(next);
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+      for (int i = 0; i < kFewRanks; ++i) acc[i][r] = dot8<BF>(ac[i], xs[r], acc[i][r]);
+    if (next.g0 != at.g0) {  // the lanes' sums: rank i of row r to lane i; then the waves'
+      const int first = (at.g0 + w / share) * kFewRanks, ranks = ranks_of(at.g0);
 #pragma unroll
       for (int r = 0; r < R; ++r) {
-        const float xs[8] = {xv[r][0][0], xv[r][0][1], xv[r][0][2], xv[r][0][3], xv[r][1][0], xv[r][1][1], xv[r][1][2], xv[r][1][3]};
+        float mine = 0.f;
 #pragma unroll
-        for (int i = 0; i < kFewRanks; ++i) acc[i][r] = dot8<BF>(av[i], xs, acc[i][r]);
+        for (int i = 0; i < kFewRanks; ++i) {
+          const float v = swap32(swap16(row16_sum(acc[i][r])));
+          mine = lane == i ? v : mine;
+          acc[i][r] = 0.f;
+        }
+        if (lane < kFewRanks) sh[w][r][lane] = mine;
       }
+      if (share > 1) __syncthreads();
+      if (w % share == 0 && lane < ranks)
+        for (int r = 0; r < t.n; ++r) {
+          float v = sh[w][r][lane];
+          for (int j = 1; j < share; ++j) v += sh[w + j][r][lane];
+          h_of(a, nseg, k, seg, t.row + r)[first + lane] = v;
+        }
+      if (share > 1) __syncthreads();
     }
-    // the lanes' sums: rank i of row r to lane i
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-      float mine = 0.f;
-#pragma unroll
-      for (int i = 0; i < kFewRanks; ++i) {
-        const float v = swap32(swap16(row16_sum(acc[i][r])));
-        mine = lane == i ? v : mine;
-      }
-      if (lane < kFewRanks) sh[w][r][lane] = mine;
-    }
-    __syncthreads();
-    if (w % share == 0 && lane < ranks)
-      for (int r = 0; r < t.n; ++r) {
-        float v = sh[w][r][lane];
-        for (int j = 1; j < share; ++j) v += sh[w + j][r][lane];
-        h_of(a, nseg, k, seg, t.row + r)[first + lane] = v;
-      }
-    __syncthreads();
+    at = next;
   }
 }
 
