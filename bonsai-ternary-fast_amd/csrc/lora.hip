@@ -26,6 +26,7 @@ namespace {
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 b8 __attribute__((ext_vector_type(8)));
+typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));  // (in memory: rows of y start anywhere)
 
 constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / 64;
@@ -121,20 +122,33 @@ __device__ __forceinline__ float* h_of(const btf_lora& a, int nseg, int k, int s
   return static_cast<float*>(a.ws) + ((size_t)(k * nseg + seg) * a.T + row) * a.rank;
 }
 
-// RT tiles of 16 rows by NT tiles of 16 ranks. grid: (tile, slice of K), (segment, NT tiles of ranks).
+// RT tiles of 16 rows by NT tiles of 16 ranks, those of all segments in a row: x is read and cut once for all of them.
+// grid: (tile, slice of K), NT tiles of ranks.
 template <bool BF, int RT, int NT>
 __global__ void __launch_bounds__(kThreads, 2) lora_shrink_kernel(btf_lora a, Segs segs, int nseg, int slices, int slice) {
   constexpr int R = 16 * RT, LD = 16 * NT + 4;
   __shared__ float sh[kWaves][R][LD];
   Tile t;
-  const int k = blockIdx.x % slices, seg = blockIdx.y % nseg, first = blockIdx.y / nseg * 16 * NT;
-  if (!find<R>(a, blockIdx.x / slices, t) || first >= t.rank) return;  // the whole workgroup
+  const int k = blockIdx.x % slices, of_seg = (a.rank + 15) / 16;
+  if (!find<R>(a, blockIdx.x / slices, t)) return;  // the whole workgroup
+  int seg[NT], first[NT];  // of each tile of ranks; first at or behind the adapter's rank: nothing to do
+  bool any = false;
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    const int i = blockIdx.y * NT + n;
+    seg[n] = min(i / of_seg, nseg - 1);
+    first[n] = i / of_seg < nseg ? 16 * (i % of_seg) : a.rank;
+    any |= first[n] < t.rank;
+  }
+  if (!any) return;  // the whole workgroup
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, c16 = lane & 15, g = lane >> 4;
-  const btf_lora_seg& s = segs.s[seg];
   const int end = min(a.K, (k + 1) * slice);
   // lane's columns of a step: 16 g .. 16 g + 15; its row of x in each tile, its rank's row of A
   const float* x = a.x + (size_t)(t.row + c16) * a.ldx + 16 * g;
-  const uint16_t* m = static_cast<const uint16_t*>(s.a) + (size_t)t.adapter * s.a_stride + (size_t)(first + c16) * a.K + 16 * g;
+  const uint16_t* m[NT];
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+    m[n] = static_cast<const uint16_t*>(segs.s[seg[n]].a) + (size_t)t.adapter * segs.s[seg[n]].a_stride + (size_t)(first[n] + c16) * a.K + 16 * g;
   f32x4 acc[RT][NT];
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt)
@@ -149,8 +163,7 @@ __global__ void __launch_bounds__(kThreads, 2) lora_shrink_kernel(btf_lora a, Se
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         av[n][u] = u32x4{0, 0, 0, 0};
-        if (in && first + 16 * n + c16 < t.rank)
-          av[n][u] = *reinterpret_cast<const u32x4*>(m + (size_t)(16 * n) * a.K + kb + 8 * u);
+        if (in && first[n] + c16 < t.rank) av[n][u] = *reinterpret_cast<const u32x4*>(m[n] + kb + 8 * u);
       }
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt)
@@ -205,22 +218,42 @@ __global__ void __launch_bounds__(kThreads, 2) lora_shrink_kernel(btf_lora a, Se
 #pragma unroll
     for (int n = 0; n < NT; ++n) *reinterpret_cast<f32x4*>(&sh[w][16 * rt + c16][16 * n + 4 * g]) = acc[rt][n];
   __syncthreads();
-  constexpr int Q = 4 * NT;  // fours of ranks in a row
-  for (int i = threadIdx.x; i < t.n * Q; i += kThreads) {
-    const int r = i / Q, c = 4 * (i % Q);
-    if (first + c >= a.rank) continue;  // (a.rank is a multiple of 8)
-    f32x4 v = *reinterpret_cast<const f32x4*>(&sh[0][r][c]);
+  for (int i = threadIdx.x; i < t.n * 4; i += kThreads) {
+    const int r = i / 4, c = 4 * (i % 4);
 #pragma unroll
-    for (int j = 1; j < kWaves; ++j) v += *reinterpret_cast<const f32x4*>(&sh[j][r][c]);
-    *reinterpret_cast<f32x4*>(h_of(a, nseg, k, seg, t.row + r) + first + c) = v;
+    for (int n = 0; n < NT; ++n) {
+      if (first[n] + c >= a.rank) continue;  // (a.rank is a multiple of 8)
+      f32x4 v = *reinterpret_cast<const f32x4*>(&sh[0][r][16 * n + c]);
+#pragma unroll
+      for (int j = 1; j < kWaves; ++j) v += *reinterpret_cast<const f32x4*>(&sh[j][r][16 * n + c]);
+      *reinterpret_cast<f32x4*>(h_of(a, nseg, k, seg[n], t.row + r) + first[n] + c) = v;
+    }
   }
+}
+
+// The slices' sums, in the first one's place: where there are more than kSlices, lora_expand's many workgroups would each
+// read them all (441 rows of 16544 columns in 33 slices, gate and up of 1248 outputs: the call 49 us, so 30).
+constexpr int kSlices = 8;
+__global__ void __launch_bounds__(kThreads) lora_join_kernel(float* h, int64_t n, int slices) {
+  const int64_t i = 4 * ((int64_t)blockIdx.x * kThreads + threadIdx.x);
+  if (i >= n) return;
+  f32x4 v = {0.f, 0.f, 0.f, 0.f};
+  for (int k = 0; k < slices; k += 8) {
+    f32x4 x[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) x[u] = *reinterpret_cast<const f32x4*>(h + i + min(k + u, slices - 1) * n);
+#pragma unroll
+    for (int u = 0; u < 8; ++u)
+      if (k + u < slices) v += x[u];
+  }
+  *reinterpret_cast<f32x4*>(h + i) = v;
 }
 
 // Row of h's parts in LDS, in bf16: the ranks in steps of 32, and 16 bytes so that rows lie in other banks.
 __host__ __device__ constexpr int parts_ld(int rank) { return (rank + 31) / 32 * 32 + 8; }
 
 // RT tiles of 16 rows by `chunk` outputs. GLU: both segments, into out.
-template <bool BF, int RT, bool GLU, bool VEC>
+template <bool BF, int RT, bool GLU>
 __global__ void __launch_bounds__(kThreads, 2) lora_expand_kernel(btf_lora a, Segs segs, int nseg, int slices, int chunk, int chunks) {
   constexpr int R = 16 * RT, NS = GLU ? 2 : 1;
   constexpr int TN = GLU && RT > 1 ? 1 : GLU || RT > 1 ? 2 : 4;  // tiles of 16 outputs of a wave at a time
@@ -249,8 +282,8 @@ __global__ void __launch_bounds__(kThreads, 2) lora_expand_kernel(btf_lora a, Se
           const float* p = s.y + (size_t)(t.row + r) * s.ldy + n;
           y[sg][i][rt] = f32x4{0.f, 0.f, 0.f, 0.f};
           if (r < t.n) {
-            if (VEC && n + 3 < n1) {
-              y[sg][i][rt] = *reinterpret_cast<const f32x4*>(p);
+            if (n + 3 < n1) {
+              y[sg][i][rt] = *reinterpret_cast<const f32x4_any*>(p);
             } else {
 #pragma unroll
               for (int j = 0; j < 4; ++j)
@@ -357,8 +390,8 @@ __global__ void __launch_bounds__(kThreads, 2) lora_expand_kernel(btf_lora a, Se
         }
         float* p = GLU ? a.out + (size_t)(t.row + r) * a.ldo + n : segs.s[seg].y + (size_t)(t.row + r) * segs.s[seg].ldy + n;
         if (r < t.n) {
-          if (VEC && n + 3 < n1) {
-            *reinterpret_cast<f32x4*>(p) = v;
+          if (n + 3 < n1) {
+            *reinterpret_cast<f32x4_any*>(p) = v;
           } else {
 #pragma unroll
             for (int j = 0; j < 4; ++j)
@@ -491,7 +524,7 @@ constexpr int kFewLoads = 8;
 template <bool BF, int R, bool GLU>
 __global__ void __launch_bounds__(kThreads, 2) lora_expand_few_kernel(btf_lora a, Segs segs, int nseg, int slices, int chunk, int chunks) {
   constexpr int NS = GLU ? 2 : 1, U = kFewLoads / NS / (R > 1 ? 2 : 1);
-  __shared__ float sh_h[NS][R][256];
+  __shared__ float sh_h[NS][R][256], sh_part[kThreads];
   Tile t;
   if (!find<R>(a, blockIdx.x / chunks, t) || (!GLU && t.rank == 0)) return;  // the whole workgroup
   int c = blockIdx.x % chunks, seg = 0;
@@ -524,26 +557,36 @@ __global__ void __launch_bounds__(kThreads, 2) lora_expand_few_kernel(btf_lora a
   };
   int n0 = c * chunk + w * U * per;
   load(n0);  // (on their way while h is put together)
-  // h, scaled; behind the rank zero
+  // h, scaled; behind the rank zero. Several threads share a sum over the slices: slice k goes to thread k % share.
   const float scale = t.adapter >= 0 && a.scale ? a.scale[t.adapter] : 1.f;
-  const int ranks8 = 8 << lg;
-  for (int i = threadIdx.x; i < NS * R * ranks8; i += kThreads) {
-    const int q = i % ranks8, r = i / ranks8 % R, sg = i / ranks8 / R;
+  const int lr = 3 + lg, items = NS * R << lr;
+  int share = 1;
+  while (share * 2 * items <= kThreads && share < slices) share *= 2;
+  for (int i = threadIdx.x; i < items * share; i += kThreads) {
+    const int part = i / items, e = i % items, q = e & ((1 << lr) - 1), r = (e >> lr) % R, sg = (e >> lr) / R;
     float v = 0.f;
     if (r < t.n && q < t.rank) {
       const float* h = h_of(a, nseg, 0, GLU ? sg : seg, t.row + r) + q;
       const size_t next = (size_t)nseg * a.T * a.rank;
-      for (int k = 0; k < slices; k += 8) {
+      for (int k = part; k < slices; k += 8 * share) {
         float x[8];
 #pragma unroll
-        for (int u = 0; u < 8; ++u) x[u] = h[min(k + u, slices - 1) * next];
+        for (int u = 0; u < 8; ++u) x[u] = h[min(k + u * share, slices - 1) * next];
 #pragma unroll
         for (int u = 0; u < 8; ++u)
-          if (k + u < slices) v += x[u];
+          if (k + u * share < slices) v += x[u];
       }
-      v *= scale;
     }
-    sh_h[sg][r][q] = v;
+    if (share > 1) sh_part[i] = v;
+    else sh_h[sg][r][q] = v * scale;
+  }
+  if (share > 1) {
+    __syncthreads();
+    for (int e = threadIdx.x; e < items; e += kThreads) {
+      float v = sh_part[e];
+      for (int j = 1; j < share; ++j) v += sh_part[j * items + e];
+      sh_h[(e >> lr) / R][(e >> lr) % R][e & ((1 << lr) - 1)] = v * scale;
+    }
   }
   __syncthreads();
   while (n0 < n1) {
@@ -590,38 +633,60 @@ __global__ void __launch_bounds__(kThreads, 2) lora_expand_few_kernel(btf_lora a
   }
 }
 
-// Rows of a tile: 64 where requests have more than 16 on average, as far as the parts of h fit 64 KB of LDS.
+// Rows of a tile: 64 where A and B are worth reading less often, from ranks above 32 and 1024 rows on (ranks of 64, K 17408, N
+// 5120, 8000 rows 183 us, in tiles of 16 228; ranks of 128, three segments, 2048 rows 127 and 150; 16 ranks of three segments,
+// 2048 rows 64 and 58; 1000 rows are alike), as far as requests are long and the parts of h fit 64 KB of LDS.
 int tile_rows(int S, int T, int rank, int together) {
-  return (int64_t)T > 16 * (int64_t)S && rank * together <= 128 ? 64 : 16;
+  return (int64_t)T > 16 * (int64_t)S && T >= 1024 && rank > 32 && rank * together <= 128 ? 64 : 16;
 }
 
 // Tiles of the requests' rows, at most: a request's last one may be a part of one.
 int most_tiles(const btf_lora& a, int R) { return a.T / R + a.S < a.T ? a.T / R + a.S : a.T; }
 
-bool vec4(const float* p, int ld) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ld % 4 == 0; }
+// Rows of h (a segment's, of one slice) that the workspace has room for: with tiles of at most 64 rows kGroups workgroups
+// are at most kGroups * 64 + T rows of each segment, and there are at most as many slices as steps of K.
+int64_t ws_rows(int T, int K, int nseg) {
+  const int64_t most = (K + kBlockK * kWaves - 1) / (kBlockK * kWaves), all = nseg * T * most, cut = nseg * ((int64_t)T + kGroups * 64);
+  return all < cut ? all : cut;
+}
+// Slices of K for `groups` workgroups or more of which `each` belong to a slice: of `step` columns or a multiple, and as
+// many as there is room for.
+struct Slices {
+  int n, columns;
+};
+Slices slices_of(const btf_lora& a, int nseg, int groups, int64_t each, int step) {
+  const int64_t most = (a.K + step - 1) / step, room = ws_rows(a.T, a.K, nseg) / ((int64_t)nseg * a.T);
+  int64_t n = (groups + each - 1) / each;
+  n = n < most ? n : most;
+  n = n < room ? n : room;
+  const int columns = (int)((a.K + n - 1) / n + step - 1) / step * step;
+  return {(a.K + columns - 1) / columns, columns};
+}
 
 template <bool BF, int RT>
 int lora_go(const btf_lora& a, const Segs& segs, int nseg, hipStream_t st) {
   constexpr int R = 16 * RT;
   const int tiles = most_tiles(a, R);
-  const int nt = a.rank <= 16 ? 1 : a.rank <= 32 ? 2 : 4, groups = (a.rank + 16 * nt - 1) / (16 * nt);
-  // slices of K: enough for kGroups workgroups, each at least one step of its waves long
-  const int step = kBlockK * kWaves, most = (a.K + step - 1) / step;
-  int slices = (kGroups + tiles * nseg * groups - 1) / (tiles * nseg * groups);
-  slices = slices < most ? slices : most;
-  const int slice = ((a.K + slices - 1) / slices + step - 1) / step * step;
-  slices = (a.K + slice - 1) / slice;
-  const dim3 grid((unsigned)tiles * slices, nseg * groups), blk(kThreads);
+  const int all = nseg * ((a.rank + 15) / 16), nt = all <= 2 ? all : 4, groups = (all + nt - 1) / nt;
+  const Slices sl = slices_of(a, nseg, kGroups, (int64_t)tiles * groups, kBlockK * kWaves);
+  int slices = sl.n;
+  const int slice = sl.columns;
+  const dim3 grid((unsigned)tiles * slices, groups), blk(kThreads);
   if (nt == 1) hipLaunchKernelGGL((lora_shrink_kernel<BF, RT, 1>), grid, blk, 0, st, a, segs, nseg, slices, slice);
   else if (nt == 2) hipLaunchKernelGGL((lora_shrink_kernel<BF, RT, 2>), grid, blk, 0, st, a, segs, nseg, slices, slice);
   else hipLaunchKernelGGL((lora_shrink_kernel<BF, RT, 4>), grid, blk, 0, st, a, segs, nseg, slices, slice);
-  const int rc = launch_status("lora_shrink_kernel");
+  int rc = launch_status("lora_shrink_kernel");
   if (rc != BTF_OK) return rc;
+  if (slices > kSlices) {
+    const int64_t n = (int64_t)nseg * a.T * a.rank;
+    hipLaunchKernelGGL(lora_join_kernel, dim3((unsigned)((n / 4 + kThreads - 1) / kThreads)), blk, 0, st, static_cast<float*>(a.ws), n, slices);
+    rc = launch_status("lora_join_kernel");
+    if (rc != BTF_OK) return rc;
+    slices = 1;
+  }
   const bool glu = a.mode == BTF_GEMV_SWIGLU;
-  bool vec = true;
   int outs = 0;
-  for (int i = 0; i < nseg; ++i) vec = vec && vec4(segs.s[i].y, segs.s[i].ldy), outs += glu && i ? 0 : segs.s[i].N;
-  if (glu) vec = vec && vec4(a.out, a.ldo);
+  for (int i = 0; i < (glu ? 1 : nseg); ++i) outs += segs.s[i].N;
   int chunk = kChunk;
   while (chunk < 4 * kChunk && (int64_t)tiles * (outs / (2 * chunk)) >= kGroups) chunk *= 2;
   int chunks = 0;
@@ -629,10 +694,8 @@ int lora_go(const btf_lora& a, const Segs& segs, int nseg, hipStream_t st) {
   const size_t lds = (size_t)(glu ? 2 : 1) * 3 * R * parts_ld(a.rank) * 2;
   const dim3 eg((unsigned)tiles * chunks);
   auto expand = [&](auto kernel) { hipLaunchKernelGGL(kernel, eg, blk, lds, st, a, segs, nseg, slices, chunk, chunks); };
-  if (glu && vec) expand(lora_expand_kernel<BF, RT, true, true>);
-  else if (glu) expand(lora_expand_kernel<BF, RT, true, false>);
-  else if (vec) expand(lora_expand_kernel<BF, RT, false, true>);
-  else expand(lora_expand_kernel<BF, RT, false, false>);
+  if (glu) expand(lora_expand_kernel<BF, RT, true>);
+  else expand(lora_expand_kernel<BF, RT, false>);
   return launch_status("lora_expand_kernel");
 }
 
@@ -640,11 +703,8 @@ template <bool BF, int R>
 int lora_few(const btf_lora& a, const Segs& segs, int nseg, hipStream_t st) {
   const int tiles = most_tiles(a, R);
   const int together = a.rank > 2 * kFewRanks ? 1 : a.rank > kFewRanks ? 2 : 4;  // waves that share ranks
-  const int step = kFewK * together, most = (a.K + step - 1) / step;
-  int slices = (kFewGroups + tiles * nseg - 1) / (tiles * nseg);
-  slices = slices < most ? slices : most;
-  const int slice = ((a.K + slices - 1) / slices + step - 1) / step * step;
-  slices = (a.K + slice - 1) / slice;
+  const Slices sl = slices_of(a, nseg, kFewGroups, (int64_t)tiles * nseg, kFewK * together);
+  const int slices = sl.n, slice = sl.columns;
   hipLaunchKernelGGL((lora_shrink_few_kernel<BF, R>), dim3((unsigned)tiles * slices, nseg), dim3(kThreads), 0, st, a, segs, nseg, slices, slice);
   const int rc = launch_status("lora_shrink_few_kernel");
   if (rc != BTF_OK) return rc;
@@ -669,12 +729,9 @@ int lora_any(const btf_lora& a, const Segs& segs, int nseg, hipStream_t st) {
 
 }  // namespace
 
-// slices * T * nseg is at most nseg * T + kGroups * 64 (tiles >= T / 64), and slices at most K / 256, rounded up.
 int64_t lora_ws_bytes(int S, int T, int K, int rank, int nseg) {
   (void)S;
-  const int64_t most = (K + kBlockK * kWaves - 1) / (kBlockK * kWaves), rows = (int64_t)nseg * T;
-  const int64_t all = rows * most, cut = rows + kGroups * 64;
-  return (all < cut ? all : cut) * rank * 4;
+  return ws_rows(T, K, nseg) * rank * 4;
 }
 
 int lora(const btf_lora& a, const btf_lora_seg* s, int nseg, hipStream_t st) {

@@ -282,6 +282,22 @@ def test_workspace_of_the_largest_serves_smaller_ones(hip):
         assert bool((ws[big // 4:] == GUARD).all())
 
 
+@pytest.mark.parametrize("new,K,Ns,rank", [([700, 600, 650], 7776, [40, 8, 8], 16), ([300, 1], 17408, [8, 8, 8], 32), ([600], 4096, [16], 128),
+                                           ([5, 4, 3], 17408, [8, 9, 10], 256), ([1, 2, 1], 17408, [8, 9, 10], 256)], ids=str)
+def test_nothing_is_written_behind_the_workspace(hip, new, K, Ns, rank):
+    """Many slices of K, sums of several segments."""
+    torch = _torch()
+    c = Case(new, K, Ns, "f16", rank, ranks=None, spare=0, seed=13)
+    n = hip.lora_ws_bytes(c.S, c.T, K, rank, len(Ns))
+    ws = torch.full((3 * n // 4 + 64,), GUARD, device="cuda")
+    segs = [hip.LoraSeg(a.cuda(), b.cuda(), rank * K, m * rank, m, dev(y), m) for a, b, m, y in zip(c.a, c.b, Ns, c.y)]
+    hip.launch_lora(hip.Lora(S=c.S, T=c.T, K=K, rank=rank, adapters=3, type=hip.CacheType.f16, row0=ints(c.row0), adapter=ints(c.who),
+                             scale=dev(c.scale), x=dev(c.x), ldx=K, ws=ws), segs, stream())
+    torch.cuda.synchronize()
+    assert bool((ws[n // 4:] == GUARD).all())
+    c.check_add([s.y.cpu().numpy() for s in segs])
+
+
 def test_far_adapters_and_rows(hip):
     """Adapters and rows beyond 2^32 bytes of their arrays' start."""
     torch = _torch()
