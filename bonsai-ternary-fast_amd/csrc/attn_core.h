@@ -108,6 +108,8 @@ __device__ __forceinline__ int wave_scan_i(int v) {
 // A workspace slot: R rows of D values, then R maxima, then R sums.
 template <int D, int R>
 constexpr size_t kSlot = (size_t)R * (D + 2);
+// With SKIP (attn_tile) a slot has 16, 32, .. rows, as the request's tiles need, and Req::slot counts in 16 rows.
+__device__ __forceinline__ int slot_rows(int R, int rows) { return min(R, (rows + 15) & ~15); }
 
 // Row r of the item by the plain loop over keys [k0, k1), by one wave: lane's
 // D / 64 values, the row's maximum and sum. Any input.
@@ -696,7 +698,11 @@ __device__ __forceinline__ void attn_tile(const btf_paged_attention& a, const bt
   bool odd = false;
   const int tid = fresh_tid();
   const Args end = fresh_args();
-  if (cut) slot = static_cast<float*>(end.a.ws) + (size_t)(q.slot + q.local) * kSlot<D, R>;
+  const int SR = SKIP ? slot_rows(R, q.n * G) : R;  // rows of the slot
+  if (cut) {
+    if (SKIP) slot = static_cast<float*>(end.a.ws) + (size_t)q.slot * kSlot<D, 16> + (size_t)q.local * (SR * (D + 2));
+    else slot = static_cast<float*>(end.a.ws) + (size_t)(q.slot + q.local) * kSlot<D, R>;
+  }
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
     const int r = (tid >> 6) * RW + rt * 16 + (tid & 15), row = tile * R + r, g = tid >> 4 & 3;
@@ -711,7 +717,7 @@ __device__ __forceinline__ void attn_tile(const btf_paged_attention& a, const bt
       chk += (v[0] - v[0]) + (v[1] - v[1]) + (v[2] - v[2]) + (v[3] - v[3]);
       if (live) *reinterpret_cast<f32x4*>(y + 16 * i + 4 * g) = v * f;
     }
-    if (cut && live && g == 0) slot[R * D + r] = m[rt], slot[R * D + R + r] = l[rt];
+    if (cut && live && g == 0) slot[SR * D + r] = m[rt], slot[SR * D + SR + r] = l[rt];
     odd |= !(chk == 0.f);
   }
   if (!__any(odd)) return;
@@ -725,7 +731,7 @@ __device__ __forceinline__ void attn_tile(const btf_paged_attention& a, const bt
     float* y = cut ? slot + (size_t)r * D : end.a.out + (size_t)(q.row0 + row / G) * end.a.ldo + (kvh * G + row % G) * D;
 #pragma unroll
     for (int e = 0; e < E; ++e) y[lane2 * E + e] = cut ? po[e] : pl == 0.f ? 0.f : po[e] / pl;
-    if (cut && lane2 == 0) slot[R * D + r] = pm, slot[R * D + R + r] = pl;
+    if (cut && lane2 == 0) slot[SR * D + r] = pm, slot[SR * D + SR + r] = pl;
   }
 }
 

@@ -43,6 +43,7 @@ struct Ws {
   int* request;   // [T] of a row, -1: none
   float* slots;   // the groups', then the requests'
   int most;       // items at most
+  int units;      // room for slots, in 16 rows
 };
 
 struct Plan : Args {
@@ -65,10 +66,6 @@ __device__ __forceinline__ int piece_keys(uint64_t groups, uint64_t requests, in
   const uint64_t items = role ? kOwnItems : max(share, kRunning / 2);
   return kStep * (int)((role ? requests : groups) / (kStep * items) + 1);
 }
-// Floats of a slot, and the requests' first slot behind n of the groups'.
-__device__ __forceinline__ int64_t slot_of(const Plan& p, int role) { return (int64_t)p.R[role] * (p.kv.dim + 2); }
-__device__ __forceinline__ int slots_behind(const Plan& p, int n) { return (int)((n * slot_of(p, 0) + slot_of(p, 1) - 1) / slot_of(p, 1)); }
-
 __device__ __forceinline__ int tiles_of(const Plan& p, int n, int R) {
   return n > 0 ? (int)(((long long)n * (p.a.heads / p.kv.heads) + R - 1) / R) : 0;
 }
@@ -106,6 +103,14 @@ __device__ __forceinline__ bool takes_part(const Found& f, const Found& g) {
   return f.n > 0 && g.len > 0 && f.s >= g.b && f.s < g.e && f.ctx >= g.whole && f.row0 >= g.row0 && f.row0 + f.n <= g.row0 + g.n;
 }
 __device__ __forceinline__ uint64_t work_of(const Found& f) { return (uint64_t)f.tiles * (uint64_t)max(f.len - f.begin, 0); }
+// 16 rows of a slot of f's, and what f's items take from slot0 on if they leave their sums. Row starts that do not ascend
+// can ask for more than there is (of those that do, no launch does): such a request or group is left out.
+__device__ __forceinline__ int units_of(const Plan& p, const Found& f, int role) {
+  return slot_rows(p.R[role], f.n * (p.a.heads / p.kv.heads)) >> 4;
+}
+__device__ __forceinline__ void fit(const Plan& p, Found& f, int units) {
+  if (f.slot0 < 0 || f.slot0 > p.ws.units - units) f.n = f.tiles = f.pieces = 0, f.flags &= ~kCut;
+}
 // The last of n ascending numbers that is at most v (0 if none is).
 __device__ __forceinline__ int last_at_most(const int* x, int n, int v) {
   int lo = 0, hi = n - 1;
@@ -179,18 +184,19 @@ __global__ void __launch_bounds__(kPlanThreads) shared_plan_small_kernel(Plan p)
       f[role].pieces = max(1, (f[role].len - f[role].begin + f[role].C - 1) / f[role].C);
       own[role] = p.kv.heads * f[role].tiles * f[role].pieces;
       if (f[role].group >= 0 || f[role].pieces > 1) f[role].flags |= kCut;
-      cut[role] = f[role].flags & kCut ? own[role] : 0;
+      cut[role] = f[role].flags & kCut ? own[role] * units_of(p, f[role], role) : 0;
     }
 #pragma unroll
   for (int role = 0; role < 2; ++role) v[role] = (uint64_t)(uint32_t)own[role] | (uint64_t)(uint32_t)cut[role] << 32;
   scan2(v, part, all);
-  const int first[2] = {0, (int)all[0]}, behind = slots_behind(p, (int)(all[0] >> 32));
+  const int first[2] = {0, (int)all[0]}, behind = (int)(all[0] >> 32);
 #pragma unroll
   for (int role = 0; role < 2; ++role) {
     sh_upto[role][tid] = (int)v[role];
     if (role ? request : group) {
       f[role].item0 = first[role] + (int)v[role] - own[role];
       f[role].slot0 = (role ? behind : 0) + (int)(v[role] >> 32) - cut[role];
+      fit(p, f[role], cut[role]);
       p.ws.found[role ? p.groups + tid : tid] = f[role];
     }
   }
@@ -250,7 +256,6 @@ __global__ void __launch_bounds__(kPlanThreads) shared_plan_kernel(Plan p) {
     const int count = role ? a.S : p.groups;
     Found* const list = role ? mine : p.ws.found;
     const int C = piece_keys(all[0] * kv.heads, all[1] * kv.heads, role);
-    if (role) slots = slots_behind(p, (int)slots);
     for (int i0 = 0; i0 < count; i0 += kPlanThreads) {
       const int i = i0 + tid;
       int own = 0, cut = 0, row0 = 0, n = 0;
@@ -258,12 +263,12 @@ __global__ void __launch_bounds__(kPlanThreads) shared_plan_kernel(Plan p) {
         const Found& f = list[i];
         const int pieces = max(1, (f.len - f.begin + C - 1) / C);
         own = kv.heads * f.tiles * pieces;
-        cut = role == 0 || f.group >= 0 || pieces > 1;
+        cut = role == 0 || f.group >= 0 || pieces > 1 ? own * units_of(p, f, role) : 0;
         row0 = f.row0, n = f.n;
       }
       uint64_t chunk, cuts;
       const int upto = (int)block_scan<kPlanThreads>((uint64_t)own, part, &chunk);
-      const int slot = (int)block_scan<kPlanThreads>((uint64_t)(cut ? own : 0), part, &cuts);
+      const int slot = (int)block_scan<kPlanThreads>((uint64_t)cut, part, &cuts);
       sh_upto[tid] = upto;
       sh_row0[tid] = row0, sh_n[tid] = n;
       if (i < count) {
@@ -271,8 +276,9 @@ __global__ void __launch_bounds__(kPlanThreads) shared_plan_kernel(Plan p) {
         f.pieces = max(1, (f.len - f.begin + C - 1) / C);
         f.C = C;
         f.item0 = (int)items + upto - own;
-        f.slot0 = (int)slots + slot - (cut ? own : 0);
+        f.slot0 = (int)slots + slot - cut;
         if (cut) f.flags |= kCut;
+        fit(p, f, cut);
       }
       __syncthreads();
       for (int k = tid; k < (int)chunk; k += kPlanThreads) {
@@ -317,6 +323,7 @@ __device__ __forceinline__ bool find_item(const Items& p, int id, Req& q, bool& 
   q.tree = f->flags & kTree;
   q.cut = f->flags & kCut;
   int local = id - f->item0;
+  if ((unsigned)local >= (unsigned)(q.tiles * q.pieces * p.kv.heads)) return false;  // (left out by `fit`)
   if (q.tiles > 1) {
     // The tiles that read the same keys eight workgroups apart, so that they share an XCD's L2 (workgroups go to the eight
     // XCDs in turn): pairs (piece, KV head) by eights, each with all its tiles.
@@ -377,23 +384,24 @@ __global__ void __launch_bounds__(64 * kJoinWaves) shared_join_kernel(Plan p) {
   const int G = a.heads / p.kv.heads, h = ONE ? blockIdx.y * kJoinWaves + w : blockIdx.y, kvh = h / G;
   if (h >= a.heads) return;
   // a role's first piece of the row, and from one to the next
-  auto first_of = [&](const found_p f, int role, size_t& step, int& r) {
+  auto first_of = [&](const found_p f, int role, size_t& step, int& r, int& rows) {
     const int R = p.R[role], row = (blockIdx.x - f->row0) * G + h % G, tile = row / R;
-    const size_t slot = (size_t)R * (D + 2);
+    rows = slot_rows(R, f->n * G);
+    const size_t slot = (size_t)rows * (D + 2);
     r = row % R;
     step = (size_t)f->tiles * p.kv.heads * slot;
-    return p.ws.slots + ((size_t)f->slot0 + (size_t)(f->tiles - 1 - tile) * p.kv.heads + kvh) * slot;
+    return p.ws.slots + (size_t)f->slot0 * (16 * (D + 2)) + ((size_t)(f->tiles - 1 - tile) * p.kv.heads + kvh) * slot;
   };
-  int n0 = 0, r0 = 0, r1;
+  int n0 = 0, r0 = 0, r1, R0 = 0, R1;
   size_t step0 = 0, step1;
   const float* base0 = nullptr;
   if (f->group >= 0) {
     const found_p g = (found_p)p.ws.found + f->group;
     n0 = g->pieces;
-    base0 = first_of(g, 0, step0, r0);
+    base0 = first_of(g, 0, step0, r0, R0);
   }
-  const float* base1 = first_of(f, 1, step1, r1);
-  const int n = n0 + f->pieces, R0 = p.R[0], R1 = p.R[1];
+  const float* base1 = first_of(f, 1, step1, r1, R1);
+  const int n = n0 + f->pieces;
   auto values = [&](int i) { return i < n0 ? base0 + i * step0 + r0 * D : base1 + (i - n0) * step1 + r1 * D; };
   auto top_of = [&](int i) { return i < n0 ? base0[i * step0 + R0 * D + r0] : base1[(i - n0) * step1 + R1 * D + r1]; };
   auto sum_of = [&](int i) { return i < n0 ? base0[i * step0 + R0 * D + R0 + r0] : base1[(i - n0) * step1 + R1 * D + R1 + r1]; };
@@ -459,12 +467,11 @@ int64_t most_items(int count, int T, int heads, const btf_kv_cache& kv, int R) {
   return ((int64_t)T * (heads / kv.heads) / R + count) * kv.heads + kRunning + kOwnItems;
 }
 
-// Floats of a role's slots, for a launch of up to S requests and T rows, whatever tiles it takes: slots * R is at most
-// T * heads + count * KV heads * R + the items * R, and count * R at most 4 T * heads / KV heads for the tiles above 16
-// (64 only where a request has more than 16 rows on average, 128 where it has more than 128).
-int64_t slot_floats(int S, int T, int heads, const btf_kv_cache& kv) {
-  const int64_t rows = (int64_t)T * heads, few = 16 * (int64_t)S * kv.heads, top = kv.dim == 128 ? 128 : 64;
-  return (rows + (few > 4 * rows ? few : 4 * rows) + (kRunning + kOwnItems + 1) * top) * (kv.dim + 2);
+// Slots of a launch of up to S requests and groups, in 16 rows: a tile's slot has the rows of the request or group, up to the
+// next multiple of 16 (of more than one tile, up to twice its rows), and each piece beyond a tile's first is one of the items
+// that the work is cut into.
+int64_t slot_units(int S, int T, int heads, const btf_kv_cache& kv) {
+  return (int64_t)T * heads / 4 + 2 * (int64_t)S * kv.heads + (kRunning + kOwnItems) * (kv.dim == 128 ? 8 : 4);
 }
 
 int64_t up(int64_t n) { return (n + 255) & ~(int64_t)255; }
@@ -512,7 +519,7 @@ int64_t shared_attention_most_items(int S, int T, int heads, const btf_kv_cache&
 }
 
 int64_t shared_attention_ws_bytes(int S, int T, int heads, const btf_kv_cache& kv) {
-  return plan_bytes(S, T, heads, kv) + 2 * up(4 * slot_floats(S, T, heads, kv));
+  return plan_bytes(S, T, heads, kv) + up(4 * slot_units(S, T, heads, kv) * 16 * (kv.dim + 2));
 }
 
 int shared_attention(const btf_shared_attention& a, const btf_kv_cache& kv, hipStream_t st) {
@@ -531,6 +538,7 @@ int shared_attention(const btf_shared_attention& a, const btf_kv_cache& kv, hipS
   p.ws.most = (int)(most_items(a.S, a.T, a.heads, kv, p.R[1]) + (a.groups ? most_items(a.groups, a.T, a.heads, kv, p.R[0]) : 0));
   p.ws.request = p.ws.map + p.ws.most;
   p.ws.slots = reinterpret_cast<float*>(at + plan_bytes(a.S, a.T, a.heads, kv));
+  p.ws.units = (int)slot_units(a.S, a.T, a.heads, kv);
   p.a = btf_paged_attention{a.S,   a.T,    a.heads, a.q,   a.ldq, a.table,    a.ldt,
                             a.row0, a.kv_len, a.tree, a.scale, a.out, a.ldo, p.ws.slots};
   const bool bf = kv.type == BTF_BF16;

@@ -233,6 +233,26 @@ def test_one_workspace(hip):
             assert bool(ws[big // 4:].isnan().all())
 
 
+@pytest.mark.parametrize("heads", [(32, 8, 64), (16, 8, 256), (32, 8, 128)], ids=str)
+def test_many_requests_behind_one_prefix(hip, heads):
+    """One group in tiles of many rows, its members of one row each: nothing is written behind the workspace. Then row starts
+    that do not ascend, each of whose requests claims all rows: no answer is defined, but nothing is written behind it either."""
+    torch = _torch()
+    rng = np.random.default_rng(16)
+    S, kind, page = 700, "f16", 16
+    x, kv_len = shared_inputs(rng, [0, S], [40], rng.integers(0, 9, S).tolist(), [1] * S, heads, kind, page)
+    H, HK, D = heads
+    kv = hip.KvCache(0, 0, hip.CacheType[kind], page, HK, D, 9, 8, 8, D)
+    size = hip.shared_attention_ws_bytes(S, S, H, kv)
+    ws = torch.full((size // 4 + 4096,), math.nan, device="cuda")
+    out = run_shared(hip, *x, kv_len, None, heads, kind, page, [0, S], [0], [40], ws=ws)
+    check_attn(out, *x, kv_len, None, heads, kind, page)
+    assert bool(ws[size // 4:].isnan().all())
+    q, k, v, table, row0 = x
+    out = run_shared(hip, q, k, v, table, np.resize([0, S], S + 1), [10000] * S, None, heads, kind, page, [0, S], [0], [40], ws=ws)
+    assert bool(ws[size // 4:].isnan().all()) and out.shape[0] == S
+
+
 def test_captured(hip):
     """A graph, replayed with other lengths and groups and with eager work between; equal bits call for call."""
     torch = _torch()
