@@ -12,10 +12,11 @@
 //
 // shared_plan_kernel, one workgroup, finds who takes part (a member needs the whole
 // prefix before its new rows), cuts both roles into items and writes down which item
-// is whose: with up to hundreds of requests a workgroup that looked for itself, as
-// launch_paged_attention's do, would read all lengths several times. The prefix counts
-// in steps of 32 keys, a block of the kernels; what is left of it is done with each
-// member's own keys, which its row of table has, too.
+// is whose: with hundreds of requests a workgroup that looked for itself, as
+// launch_paged_attention's do, would read all lengths several times. Up to 64 requests
+// each workgroup does that, and there is no plan. The prefix counts in steps of 32
+// keys, a block of the kernels; what is left of it is done with each member's own
+// keys, which its row of table has, too.
 #include <string>
 
 #include "../../include/btf/hip_abi.h"
@@ -51,6 +52,7 @@ struct Plan : Args {
   int groups;
   const int *group0, *lead, *shared;
   int R[2];       // rows of a tile of a group, of a request
+  bool alone;     // no launch before: find_few, and the first workgroup writes down `found` for the join
 };
 
 constexpr int kPlanThreads = 1024;
@@ -304,34 +306,108 @@ __global__ void __launch_bounds__(kPlanThreads) shared_plan_kernel(Plan p) {
 typedef __attribute__((address_space(4))) const Found* found_p;
 typedef __attribute__((address_space(4))) const int* ints_p;
 
-// The launch of the items as the kernels take it: a.ws is the slots.
-struct Items : Args {
-  const int *items, *map;
-  const Found* found;
-  int groups;
-};
+// The workgroup's tile, piece and head of the requests' or groups' item `local`.
+__device__ __forceinline__ int order_of(const Req& q, int heads, int local) {
+  if (q.tiles <= 1) return local;
+  // The tiles that read the same keys eight workgroups apart, so that they share an XCD's L2 (workgroups go to the eight
+  // XCDs in turn): pairs (piece, KV head) by eights, each with all its tiles.
+  const int pairs = q.pieces * heads, at = local / (8 * q.tiles), rest = local - at * 8 * q.tiles;
+  const int wide = min(8, pairs - 8 * at), tile = rest / wide, pair = 8 * at + rest - tile * wide;
+  return (pair / heads * q.tiles + tile) * heads + pair % heads;
+}
 
 // Item `id`, in scalar registers. False: there is none.
-__device__ __forceinline__ bool find_item(const Items& p, int id, Req& q, bool& group) {
-  if (id >= *(ints_p)p.items) return false;
-  const int v = ((ints_p)p.map)[id];
-  const found_p f = (found_p)p.found + v;
+__device__ __forceinline__ bool find_item(const Plan& p, int id, Req& q, bool& group) {
+  if (id >= *(ints_p)p.ws.items) return false;
+  const int v = ((ints_p)p.ws.map)[id];
+  const found_p f = (found_p)p.ws.found + v;
   group = v < p.groups;
   q.s = f->s, q.row0 = f->row0, q.n = f->n, q.len = f->len, q.ctx = f->ctx;
   q.tiles = f->tiles, q.pieces = f->pieces, q.begin = f->begin, q.C = f->C;
   q.slot = f->slot0;
   q.tree = f->flags & kTree;
   q.cut = f->flags & kCut;
-  int local = id - f->item0;
+  const int local = id - f->item0;
   if ((unsigned)local >= (unsigned)(q.tiles * q.pieces * p.kv.heads)) return false;  // (left out by `fit`)
-  if (q.tiles > 1) {
-    // The tiles that read the same keys eight workgroups apart, so that they share an XCD's L2 (workgroups go to the eight
-    // XCDs in turn): pairs (piece, KV head) by eights, each with all its tiles.
-    const int heads = p.kv.heads, pairs = q.pieces * heads, at = local / (8 * q.tiles), rest = local - at * 8 * q.tiles;
-    const int wide = min(8, pairs - 8 * at), tile = rest / wide, pair = 8 * at + rest - tile * wide;
-    local = (pair / heads * q.tiles + tile) * heads + pair % heads;
+  q.local = order_of(q, p.kv.heads, local);
+  return true;
+}
+
+// The same for up to 64 requests, one a lane, by the workgroup itself: one trip to memory for all that it reads, in place of
+// the plan's launch and two more trips behind it (4 requests behind 4096 keys 21.2 us, so 16.2; 64 behind 16384 85.6 and 81.9).
+constexpr int kFew = 64;
+__device__ __forceinline__ bool find_few(const Plan& p, int id, Req& q, bool& group) {
+  const btf_paged_attention& a = p.a;
+  const int lane = threadIdx.x & 63, heads = p.kv.heads;
+  const bool there[2] = {lane < p.groups, lane < a.S};
+  const int r0 = there[1] ? a.row0[lane] : 0, r1 = there[1] ? a.row0[lane + 1] : 0, full = there[1] ? a.kv_len[lane] : 0;
+  const int b = there[0] ? p.group0[lane] : 0, e = there[0] ? p.group0[lane + 1] : 0;
+  const int lead = there[0] ? p.lead[lane] : 0, whole = there[0] ? p.shared[lane] : 0;
+  const int last = __builtin_amdgcn_readlane(r1, a.S - 1);
+  auto row_of = [&](int s) {
+    const int row = __shfl(r0, s & 63, 64);  // (by all lanes)
+    return min(max(s < a.S ? row : last, 0), a.T);
+  };
+  const int gb = min(max(b, 0), a.S), ge = min(max(e, gb), a.S), g0 = row_of(gb), g1 = row_of(ge);
+  Found f[2] = {group_of(p, gb, ge, g0, g1, lead, whole), request_of(p, lane, r0, r1, full)};
+  if (p.groups > 0) {
+    int lo = 0, hi = p.groups - 1;  // last_at_most
+    while (__any(lo < hi)) {
+      const int mid = (lo + hi + 1) >> 1, v = __shfl(b, mid, 64);
+      if (lo < hi) {
+        if (v <= lane) lo = mid;
+        else hi = mid - 1;
+      }
+    }
+    Found g{};
+    g.b = __shfl(gb, lo, 64), g.e = __shfl(ge, lo, 64), g.row0 = __shfl(f[0].row0, lo, 64), g.n = __shfl(f[0].n, lo, 64);
+    g.len = __shfl(f[0].len, lo, 64), g.whole = __shfl(whole, lo, 64);
+    if (takes_part(f[1], g)) f[1].group = lo, f[1].begin = g.len;
   }
-  q.local = local;
+  uint64_t all[2], v[2];
+  auto last_of = [&](uint64_t v) {
+    return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), 63) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
+  };
+#pragma unroll
+  for (int role = 0; role < 2; ++role) all[role] = last_of(wave_scan_u64(there[role] ? work_of(f[role]) : 0));
+  int own[2], upto[2], items[2], behind = 0;
+#pragma unroll
+  for (int role = 0; role < 2; ++role) {
+    f[role].C = piece_keys(all[0] * heads, all[1] * heads, role);
+    f[role].pieces = max(1, (int)((unsigned)(f[role].len - f[role].begin + f[role].C - 1) / (unsigned)f[role].C));
+    own[role] = there[role] ? heads * f[role].tiles * f[role].pieces : 0;
+    if (f[role].group >= 0 || f[role].pieces > 1) f[role].flags |= kCut;
+    const int cut = f[role].flags & kCut ? own[role] * units_of(p, f[role], role) : 0;
+    v[role] = wave_scan_u64((uint64_t)(uint32_t)own[role] | (uint64_t)(uint32_t)cut << 32);
+    const uint64_t sum = last_of(v[role]);
+    upto[role] = (int)v[role];
+    items[role] = (int)sum;
+    f[role].slot0 = behind + (int)(v[role] >> 32) - cut;
+    behind = (int)(sum >> 32);
+    fit(p, f[role], cut);
+  }
+  if (id == 0 && threadIdx.x < 64) {
+#pragma unroll
+    for (int role = 0; role < 2; ++role)
+      if (there[role]) p.ws.found[role ? p.groups + lane : lane] = f[role];
+  }
+  group = id < items[0];
+  const int at = group ? id : id - items[0];
+  if (!group && at >= items[1]) return false;
+  const uint64_t behind_it = __ballot(group ? there[0] && upto[0] > at : there[1] && upto[1] > at);
+  if (!behind_it) return false;
+  const int l = __builtin_ctzll(behind_it);
+  auto of = [&](int x, int y) { return __builtin_amdgcn_readlane(group ? x : y, l); };
+  q.s = of(f[0].s, f[1].s), q.row0 = of(f[0].row0, f[1].row0), q.n = of(f[0].n, f[1].n);
+  q.len = of(f[0].len, f[1].len), q.ctx = of(f[0].ctx, f[1].ctx), q.tiles = of(f[0].tiles, f[1].tiles);
+  q.pieces = of(f[0].pieces, f[1].pieces), q.begin = group ? 0 : __builtin_amdgcn_readlane(f[1].begin, l);
+  q.C = of(f[0].C, f[1].C), q.slot = of(f[0].slot0, f[1].slot0);
+  const int flags = of(f[0].flags, f[1].flags);
+  q.tree = flags & kTree;
+  q.cut = flags & kCut;
+  const int local = at - of(upto[0] - own[0], upto[1] - own[1]);
+  if ((unsigned)local >= (unsigned)(q.tiles * q.pieces * heads)) return false;
+  q.local = order_of(q, heads, local);
   return true;
 }
 
@@ -345,7 +421,7 @@ struct LdsOf<D, 16> {
   typedef StreamLds<D, 1> type;
 };
 template <int D, bool BF, int R, bool TWO>
-__device__ __forceinline__ void item(const Items& p, Req& q, void* lds) {
+__device__ __forceinline__ void item(const Plan& p, Req& q, void* lds) {
   const Args own = TWO ? fresh_args() : Args{p.a, p.kv};  // (two kinds of tiles: nothing kept from before the branch)
   if constexpr (R == 16) {
     auto vector = [](int& v) { asm("" : "+v"(v)); };  // (attn_stream has no scalar registers to spare)
@@ -357,12 +433,12 @@ __device__ __forceinline__ void item(const Items& p, Req& q, void* lds) {
   }
 }
 template <int D, bool BF, int R0, int R1>
-__global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(D == 256 && R1 == 16 ? 1 : 2))) shared_kernel(Items p) {
+__global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(D == 256 && R1 == 16 ? 1 : 2))) shared_kernel(Plan p) {
   constexpr size_t a = sizeof(typename LdsOf<D, R0>::type), b = sizeof(typename LdsOf<D, R1>::type);
   __shared__ __attribute__((aligned(16))) char lds[a > b ? a : b];
   Req q;
   bool group;
-  if (!find_item(p, blockIdx.x, q, group)) return;  // the whole workgroup
+  if (!(p.alone ? find_few(p, blockIdx.x, q, group) : find_item(p, blockIdx.x, q, group))) return;  // the whole workgroup
   if (R0 == R1 || group) item<D, BF, R0, R0 != R1>(p, q, lds);
   else item<D, BF, R1, R0 != R1>(p, q, lds);
 }
@@ -376,8 +452,16 @@ __global__ void __launch_bounds__(64 * kJoinWaves) shared_join_kernel(Plan p) {
   constexpr int AT = ONE ? 4 : 8;
   typedef float vE __attribute__((ext_vector_type(E)));
   const btf_paged_attention& a = p.a;
-  const int s = ((ints_p)p.ws.request)[blockIdx.x];
-  if (s < 0) return;  // the whole workgroup
+  int s;
+  if (p.alone) {
+    const int l = threadIdx.x & 63, t = blockIdx.x;
+    const uint64_t m = __ballot(l < a.S && a.row0[min(l, a.S - 1)] <= t && t < a.row0[min(l, a.S - 1) + 1]);
+    s = 63 - __builtin_clzll(m | 1);
+    if (!m) return;  // the whole workgroup
+  } else {
+    s = ((ints_p)p.ws.request)[blockIdx.x];
+    if (s < 0) return;
+  }
   const found_p f = (found_p)p.ws.found + p.groups + s;
   if (!(f->flags & kCut)) return;
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -483,12 +567,14 @@ int64_t plan_bytes(int S, int T, int heads, const btf_kv_cache& kv) {
 
 template <int D, bool BF>
 int shared_go(const Plan& p, hipStream_t st) {
-  if (p.a.S <= kPlanThreads) hipLaunchKernelGGL(shared_plan_small_kernel, dim3(1), dim3(kPlanThreads), 0, st, p);
-  else hipLaunchKernelGGL(shared_plan_kernel, dim3(1), dim3(kPlanThreads), 0, st, p);
-  int rc = launch_status("shared_plan_kernel");
-  if (rc != BTF_OK) return rc;
-  const Items items{{p.a, p.kv}, p.ws.items, p.ws.map, p.ws.found, p.groups};
-  auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3((unsigned)p.ws.most), dim3(64 * kWaves), 0, st, items); };
+  int rc = BTF_OK;
+  if (!p.alone) {
+    if (p.a.S <= kPlanThreads) hipLaunchKernelGGL(shared_plan_small_kernel, dim3(1), dim3(kPlanThreads), 0, st, p);
+    else hipLaunchKernelGGL(shared_plan_kernel, dim3(1), dim3(kPlanThreads), 0, st, p);
+    rc = launch_status("shared_plan_kernel");
+    if (rc != BTF_OK) return rc;
+  }
+  auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3((unsigned)p.ws.most), dim3(64 * kWaves), 0, st, p); };
   const int R0 = p.R[0], R1 = p.R[1];
   if (R0 == 16) {
     go(shared_kernel<D, BF, 16, 16>);
@@ -541,6 +627,7 @@ int shared_attention(const btf_shared_attention& a, const btf_kv_cache& kv, hipS
   p.ws.units = (int)slot_units(a.S, a.T, a.heads, kv);
   p.a = btf_paged_attention{a.S,   a.T,    a.heads, a.q,   a.ldq, a.table,    a.ldt,
                             a.row0, a.kv_len, a.tree, a.scale, a.out, a.ldo, p.ws.slots};
+  p.alone = a.S <= kFew;
   const bool bf = kv.type == BTF_BF16;
   if (kv.dim == 64) return bf ? shared_go<64, true>(p, st) : shared_go<64, false>(p, st);
   if (kv.dim == 128) return bf ? shared_go<128, true>(p, st) : shared_go<128, false>(p, st);
