@@ -2,7 +2,7 @@
 // (btf_hip_launch_lora; gfx950): y += scale B (A x), each request's rows with its
 // own A [rank][K] and B [N][rank].
 //
-// Two launches. lora_shrink: h = A x, a tile of rows of one request by a slice of K a
+// Two launches (one where rows are few and A is small). lora_shrink: h = A x, a tile of rows of one request by a slice of K a
 // workgroup; its waves take every fourth 64 columns, join in LDS, and leave the slice's
 // sums in the workspace. lora_expand: the slices' sums in order, times scale, then
 // B h for a tile of rows and a run of outputs, added to y (or through silu(g) u).
@@ -14,7 +14,7 @@
 // round, in 32 bits. (The three parts cost less than a third of 32-bit MFMA would, and
 // where few rows have an adapter nothing but its bytes counts.) Infinite x or weights give NaN.
 //
-// Bound by HBM where rows or adapters are many, by latency of the two launches where few.
+// Bound by HBM where rows or adapters are many, by latency where few.
 #include <string>
 
 #include "../../include/btf/hip_abi.h"
@@ -434,24 +434,26 @@ __device__ __forceinline__ float swap32(float v) {
 constexpr int kFewGroups = 1024;
 constexpr int kFewK = 512;     // columns of a wave's step, eight a lane
 constexpr int kFewRanks = 8;   // ranks of a wave at a time
+// One launch in place of two, in which each workgroup multiplies A itself: as long as there is a CU for each and A is small
+// (one row, K and N 5120: ranks of 16 11.4 us in two launches, 8.1 so; 32 10.9 and 9.2; 64 11.5 and 12.0; eight rows, K 17408,
+// ranks of 32 11.1 and 20.2; gate and up of four rows, ranks of 8, 272 workgroups, 11.3 and 18.0).
+constexpr int kOneGroups = 256, kOneValues = 160 * 1024;
 
-// R rows by the adapter's ranks. A workgroup's waves share the ranks by eights; where there are fewer than four of
-// these, several waves share one by steps of K and join in LDS. grid: (tile, slice of K), segment.
-template <bool BF, int R>
-__global__ void __launch_bounds__(kThreads, 2) lora_shrink_few_kernel(btf_lora a, Segs segs, int nseg, int slices, int slice) {
-  __shared__ float sh[kWaves][R][kFewRanks];
-  Tile t;
-  const int k = blockIdx.x % slices, seg = blockIdx.y;
-  if (!find<R>(a, blockIdx.x / slices, t) || t.rank == 0) return;  // the whole workgroup
+// R rows by the adapter's ranks, columns k0 .. end - 1: the workgroup's W waves share the ranks by eights; where there are
+// fewer than W of these, several waves share one by steps of K and join in LDS. store(rank, row, sum) by some lane.
+template <bool BF, int R, int W, class Store>
+__device__ __forceinline__ void shrink_few(const btf_lora& a, const btf_lora_seg& s, const Tile& t, int k0, int end,
+                                           float (&sh)[W][R][kFewRanks], const Store& store) {
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const btf_lora_seg& s = segs.s[seg];
-  const int end = min(a.K, (k + 1) * slice), all = (t.rank + kFewRanks - 1) / kFewRanks;
-  const int groups = all >= 4 ? 4 : all >= 2 ? 2 : 1, share = kWaves / groups;
+  const int all = (t.rank + kFewRanks - 1) / kFewRanks;
+  int groups = 1;
+  while (2 * groups <= W && 2 * groups <= all) groups *= 2;
+  const int share = W / groups;
   // Steps (ranks from g0 on, columns from kb on) in turn, the next one's loads under way while one is worked on.
   struct Step {
     int g0, kb;
   };
-  const int kb0 = k * slice + w % share * kFewK;
+  const int kb0 = k0 + w % share * kFewK;
   auto next_of = [&](Step p) { return p.kb + share * kFewK < end ? Step{p.g0, p.kb + share * kFewK} : Step{p.g0 + groups, kb0}; };
   auto ranks_of = [&](int g0) { return min(t.rank - (g0 + w / share) * kFewRanks, kFewRanks); };
   u32x4 av[kFewRanks];
@@ -510,7 +512,7 @@ __global__ void __launch_bounds__(kThreads, 2) lora_shrink_few_kernel(btf_lora a
         for (int r = 0; r < t.n; ++r) {
           float v = sh[w][r][lane];
           for (int j = 1; j < share; ++j) v += sh[w + j][r][lane];
-          h_of(a, nseg, k, seg, t.row + r)[first + lane] = v;
+          store(first + lane, r, v);
         }
       if (share > 1) __syncthreads();
     }
@@ -518,12 +520,26 @@ __global__ void __launch_bounds__(kThreads, 2) lora_shrink_few_kernel(btf_lora a
   }
 }
 
+// grid: (tile, slice of K), segment.
+template <bool BF, int R>
+__global__ void __launch_bounds__(kThreads, 2) lora_shrink_few_kernel(btf_lora a, Segs segs, int nseg, int slices, int slice) {
+  __shared__ float sh[kWaves][R][kFewRanks];
+  Tile t;
+  const int k = blockIdx.x % slices, seg = blockIdx.y;
+  if (!find<R>(a, blockIdx.x / slices, t) || t.rank == 0) return;  // the whole workgroup
+  shrink_few<BF, R, kWaves>(a, segs.s[seg], t, k * slice, min(a.K, (k + 1) * slice), sh,
+                            [&](int q, int r, float v) { h_of(a, nseg, k, seg, t.row + r)[q] = v; });
+}
+
 // R rows by `chunk` outputs. The lanes of 2^lg hold one row of B, eight ranks each, so that a wave's load is 1 KB in one
 // piece; kFewLoads of them are on their way at a time.
+// ONE: h by the workgroup itself, in place of the launch before.
 constexpr int kFewLoads = 8;
-template <bool BF, int R, bool GLU>
-__global__ void __launch_bounds__(kThreads, 2) lora_expand_few_kernel(btf_lora a, Segs segs, int nseg, int slices, int chunk, int chunks) {
-  constexpr int NS = GLU ? 2 : 1, U = kFewLoads / NS / (R > 1 ? 2 : 1);
+constexpr int kOneWaves = 16;
+template <bool BF, int R, bool GLU, bool ONE>
+__global__ void __launch_bounds__(ONE ? 64 * kOneWaves : kThreads, ONE ? 1 : 2)
+    lora_expand_few_kernel(btf_lora a, Segs segs, int nseg, int slices, int chunk, int chunks) {
+  constexpr int NS = GLU ? 2 : 1, U = ONE ? 2 : kFewLoads / NS / (R > 1 ? 2 : 1), W = ONE ? kOneWaves : kWaves;
   __shared__ float sh_h[NS][R][256], sh_part[kThreads];
   Tile t;
   if (!find<R>(a, blockIdx.x / chunks, t) || (!GLU && t.rank == 0)) return;  // the whole workgroup
@@ -557,35 +573,48 @@ __global__ void __launch_bounds__(kThreads, 2) lora_expand_few_kernel(btf_lora a
   };
   int n0 = c * chunk + w * U * per;
   load(n0);  // (on their way while h is put together)
-  // h, scaled; behind the rank zero. Several threads share a sum over the slices: slice k goes to thread k % share.
   const float scale = t.adapter >= 0 && a.scale ? a.scale[t.adapter] : 1.f;
-  const int lr = 3 + lg, items = NS * R << lr;
-  int share = 1;
-  while (share * 2 * items <= kThreads && share < slices) share *= 2;
-  for (int i = threadIdx.x; i < items * share; i += kThreads) {
-    const int part = i / items, e = i % items, q = e & ((1 << lr) - 1), r = (e >> lr) % R, sg = (e >> lr) / R;
-    float v = 0.f;
-    if (r < t.n && q < t.rank) {
-      const float* h = h_of(a, nseg, 0, GLU ? sg : seg, t.row + r) + q;
-      const size_t next = (size_t)nseg * a.T * a.rank;
-      for (int k = part; k < slices; k += 8 * share) {
-        float x[8];
-#pragma unroll
-        for (int u = 0; u < 8; ++u) x[u] = h[min(k + u * share, slices - 1) * next];
-#pragma unroll
-        for (int u = 0; u < 8; ++u)
-          if (k + u * share < slices) v += x[u];
-      }
-    }
-    if (share > 1) sh_part[i] = v;
-    else sh_h[sg][r][q] = v * scale;
-  }
-  if (share > 1) {
+  // h, scaled; behind the rank zero.
+  if constexpr (ONE) {
+    __shared__ float sh[W][R][kFewRanks];
+    for (int i = threadIdx.x; i < NS * R * 256; i += 64 * W) (&sh_h[0][0][0])[i] = 0.f;
     __syncthreads();
-    for (int e = threadIdx.x; e < items; e += kThreads) {
-      float v = sh_part[e];
-      for (int j = 1; j < share; ++j) v += sh_part[j * items + e];
-      sh_h[(e >> lr) / R][(e >> lr) % R][e & ((1 << lr) - 1)] = v * scale;
+    if (t.rank > 0)
+#pragma unroll 1
+      for (int sg = 0; sg < NS; ++sg) {
+        const btf_lora_seg& s = segs.s[GLU ? sg : seg];
+        shrink_few<BF, R, W>(a, s, t, 0, a.K, sh, [&](int q, int r, float v) { sh_h[sg][r][q] = v * scale; });
+      }
+  } else {
+    // Several threads share a sum over the slices: slice k goes to thread k % share.
+    const int lr = 3 + lg, items = NS * R << lr;
+    int share = 1;
+    while (share * 2 * items <= kThreads && share < slices) share *= 2;
+    for (int i = threadIdx.x; i < items * share; i += kThreads) {
+      const int part = i / items, e = i % items, q = e & ((1 << lr) - 1), r = (e >> lr) % R, sg = (e >> lr) / R;
+      float v = 0.f;
+      if (r < t.n && q < t.rank) {
+        const float* h = h_of(a, nseg, 0, GLU ? sg : seg, t.row + r) + q;
+        const size_t next = (size_t)nseg * a.T * a.rank;
+        for (int k = part; k < slices; k += 8 * share) {
+          float x[8];
+#pragma unroll
+          for (int u = 0; u < 8; ++u) x[u] = h[min(k + u * share, slices - 1) * next];
+#pragma unroll
+          for (int u = 0; u < 8; ++u)
+            if (k + u * share < slices) v += x[u];
+        }
+      }
+      if (share > 1) sh_part[i] = v;
+      else sh_h[sg][r][q] = v * scale;
+    }
+    if (share > 1) {
+      __syncthreads();
+      for (int e = threadIdx.x; e < items; e += kThreads) {
+        float v = sh_part[e];
+        for (int j = 1; j < share; ++j) v += sh_part[j * items + e];
+        sh_h[(e >> lr) / R][(e >> lr) % R][e & ((1 << lr) - 1)] = v * scale;
+      }
     }
   }
   __syncthreads();
@@ -617,7 +646,7 @@ __global__ void __launch_bounds__(kThreads, 2) lora_expand_few_kernel(btf_lora a
         }
       }
     const int at = n0;
-    n0 += U * per * kWaves;
+    n0 += U * per * W;
     if (n0 < n1) load(n0);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -702,20 +731,31 @@ int lora_go(const btf_lora& a, const Segs& segs, int nseg, hipStream_t st) {
 template <bool BF, int R>
 int lora_few(const btf_lora& a, const Segs& segs, int nseg, hipStream_t st) {
   const int tiles = most_tiles(a, R);
+  const bool glu = a.mode == BTF_GEMV_SWIGLU;
+  int outs = 0, chunk = kChunk;
+  for (int i = 0; i < (glu ? 1 : nseg); ++i) outs += segs.s[i].N;
+  while (chunk < 4 * kChunk && (int64_t)tiles * (outs / (2 * chunk)) >= kFewGroups) chunk *= 2;
+  auto chunks_of = [&](int chunk) {
+    int n = 0;
+    for (int i = 0; i < (glu ? 1 : nseg); ++i) n += (segs.s[i].N + chunk - 1) / chunk;
+    return n;
+  };
+  const int chunks = chunks_of(chunk);
+  if (R == 1 && (int64_t)tiles * chunks <= kOneGroups && (int64_t)a.rank * a.K * (glu ? 2 : 1) <= kOneValues) {
+    const dim3 grid((unsigned)tiles * chunks), blk(64 * kOneWaves);
+    if (glu) hipLaunchKernelGGL((lora_expand_few_kernel<BF, 1, true, true>), grid, blk, 0, st, a, segs, nseg, 1, chunk, chunks);
+    else hipLaunchKernelGGL((lora_expand_few_kernel<BF, 1, false, true>), grid, blk, 0, st, a, segs, nseg, 1, chunk, chunks);
+    return launch_status("lora_expand_few_kernel");
+  }
   const int together = a.rank > 2 * kFewRanks ? 1 : a.rank > kFewRanks ? 2 : 4;  // waves that share ranks
   const Slices sl = slices_of(a, nseg, kFewGroups, (int64_t)tiles * nseg, kFewK * together);
   const int slices = sl.n, slice = sl.columns;
   hipLaunchKernelGGL((lora_shrink_few_kernel<BF, R>), dim3((unsigned)tiles * slices, nseg), dim3(kThreads), 0, st, a, segs, nseg, slices, slice);
   const int rc = launch_status("lora_shrink_few_kernel");
   if (rc != BTF_OK) return rc;
-  const bool glu = a.mode == BTF_GEMV_SWIGLU;
-  int outs = 0, chunk = kChunk, chunks = 0;
-  for (int i = 0; i < (glu ? 1 : nseg); ++i) outs += segs.s[i].N;
-  while (chunk < 4 * kChunk && (int64_t)tiles * (outs / (2 * chunk)) >= kFewGroups) chunk *= 2;
-  for (int i = 0; i < (glu ? 1 : nseg); ++i) chunks += (segs.s[i].N + chunk - 1) / chunk;
   const dim3 grid((unsigned)tiles * chunks);
-  if (glu) hipLaunchKernelGGL((lora_expand_few_kernel<BF, R, true>), grid, dim3(kThreads), 0, st, a, segs, nseg, slices, chunk, chunks);
-  else hipLaunchKernelGGL((lora_expand_few_kernel<BF, R, false>), grid, dim3(kThreads), 0, st, a, segs, nseg, slices, chunk, chunks);
+  if (glu) hipLaunchKernelGGL((lora_expand_few_kernel<BF, R, true, false>), grid, dim3(kThreads), 0, st, a, segs, nseg, slices, chunk, chunks);
+  else hipLaunchKernelGGL((lora_expand_few_kernel<BF, R, false, false>), grid, dim3(kThreads), 0, st, a, segs, nseg, slices, chunk, chunks);
   return launch_status("lora_expand_few_kernel");
 }
 

@@ -334,7 +334,7 @@ __device__ __forceinline__ bool find_item(const Plan& p, int id, Req& q, bool& g
 }
 
 // The same for up to 64 requests, one a lane, by the workgroup itself: one trip to memory for all that it reads, in place of
-// the plan's launch and two more trips behind it (4 requests behind 4096 keys 21.2 us, so 16.2; 64 behind 16384 85.6 and 81.9).
+// the plan's launch and two more trips behind it (4 requests behind 1000 keys 21.2 us, so 16.2; 64 behind 16384 85.6 and 81.9).
 constexpr int kFew = 64;
 __device__ __forceinline__ bool find_few(const Plan& p, int id, Req& q, bool& group) {
   const btf_paged_attention& a = p.a;

@@ -747,13 +747,13 @@ int btf_hip_launch_shared_attention(const btf_shared_attention* a, const btf_kv_
  *  BTF_GEMV_ADD:    y += scale[id] * B_id (A_id x);
  *  BTF_GEMV_SWIGLU: (two segments of the same N: gate and up, as launch_gemv stored
  *   them) out = silu(g + its delta) * (u + its delta); g and u stay. out may be the
- *   gate's y itself.
+ *   gate's y itself. Neither y nor out may overlap x.
  * Other ids: no delta. x is the projection's input before its transform and
  * quantization (launch_prep's xn_out), fp32. A_id: `rank` rows of K values at
  * a + id * a_stride, B_id: N rows of `rank` values at b + id * b_stride, of which
  * the adapter uses the first ranks[id] (NULL: all; clamped to [0, rank]); what lies
  * behind them has no effect. Products and sums are in 32 bits. The order of a row's
- * sums follows from K, the rank and, by the launch's tiles, S and T.
+ * sums follows from the sizes of the launch.
  * Rows from row0[S] on are left as they were. ws: lora_ws_bytes of device scratch,
  * 16-byte aligned, one for each stream that launches; it need not be cleared, and the
  * bytes for the largest of each argument serve every launch. */

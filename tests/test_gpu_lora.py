@@ -152,6 +152,22 @@ def test_swiglu(hip, new, K, N, rank, kind, into_gate):
         np.testing.assert_array_equal(out[c.row0[-1]:], c.y[0][c.row0[-1]:])
 
 
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("new,K,N,rank", [([1], 32, 1, 8), ([1], 5120, 300, 16), ([1], 5120, 700, 32), ([1, 1, 1], 1056, 513, 40), ([1] * 8, 96, 8, 256),
+                                          ([1, 0, 1, 1], 17408, 40, 8), ([2, 1, 0], 544, 1000, 24), ([1] * 60, 640, 1025, 128),
+                                          ([1] * 70, 1024, 1100, 64)], ids=str)
+def test_one_row_each(hip, new, K, N, rank, kind):
+    """As many rows as requests: one launch while A is small, two beyond; every number of waves that share ranks."""
+    for ranks in (None, "mixed"):
+        c = Case(new, K, [N, N, 8], kind, rank, spare=0, seed=3, ranks=ranks, pad=(8, 1))
+        c.check_add(c.run(hip)[0])
+        c = Case(new, K, [N, N], kind, rank, spare=0, seed=4, ranks=ranks, scale=ranks is None)
+        for into_gate in (False, True):
+            ys, out = c.run(hip, "swiglu", into_gate=into_gate)
+            c.check_swiglu(out)
+            np.testing.assert_array_equal(ys[1], c.y[1])
+
+
 @pytest.mark.parametrize("Ns", [[512, 96, 96], [40, 41]])
 @pytest.mark.parametrize("new", [[1, 1, 1], [50, 30]])
 @pytest.mark.parametrize("pad,shift", [((0, 0), 0), ((4, 3), 0), ((20, 4), 0), ((0, 0), 1), ((0, 4), 2)])
