@@ -63,11 +63,23 @@ constexpr int kPlanThreads = 1024;
 // the requests' items fill the rest and follow (64 requests behind 16384 keys with 250 to 1000 of their own, heads of 256:
 // the call 85 us, with 512 items of the groups 95, 192 104; a group alone 56 us in 512 items, 69 in 256).
 constexpr int kRunning = 512, kOwnItems = 384;
-__device__ __forceinline__ int piece_keys(uint64_t groups, uint64_t requests, int role) {
-  const int share = (int)(kRunning * ((float)groups / ((float)groups + 2.f * (float)requests + 1.f)));
-  const uint64_t items = role ? kOwnItems : max(share, kRunning / 2);
-  return kStep * (int)((role ? requests : groups) / (kStep * items) + 1);
+// (Sums of the work in 32 bits are off by 2^-17 at most, for which the last factor stands: there are never more items.)
+// Tiles above 16 rows, whose waves take all keys of an item, in pieces of 64 keys where that leaves no more items either and
+// makes up to 32 of a request (4 requests behind 1000 keys 16.2 us in pieces of 128, 14.3 in 64, 14.9 in 32; 6 of two groups
+// behind 6500 keys, whose rows would have 100 pieces to join, 13.8, 16.5, 16.2).
+constexpr int kHalf = kStep / 2, kMostHalves = 32;
+__device__ __forceinline__ int piece_keys(float groups, float requests, int role, int R) {
+  const float share = (float)kRunning * (groups / (groups + 2.f * requests + 1.f));
+  const float items = role ? (float)kOwnItems : fmaxf(floorf(share), (float)(kRunning / 2));
+  const float keys = (role ? requests : groups) * 1.0001f / items;
+  return R > 16 && keys <= (float)kHalf ? kHalf : kStep * (int)fminf(keys / (float)kStep + 1.f, 1e6f);
 }
+__device__ __forceinline__ void into_pieces(Found& f, int C) {
+  const int keys = f.len - f.begin;
+  f.C = C < kStep && keys > kMostHalves * kHalf ? kStep : C;
+  f.pieces = max(1, (int)((unsigned)(keys + f.C - 1) / (unsigned)f.C));
+}
+
 __device__ __forceinline__ int tiles_of(const Plan& p, int n, int R) {
   return n > 0 ? (int)(((long long)n * (p.a.heads / p.kv.heads) + R - 1) / R) : 0;
 }
@@ -79,7 +91,7 @@ __device__ __forceinline__ Found group_of(const Plan& p, int b, int e, int r0, i
   f.b = b, f.e = e;
   f.row0 = r0;
   f.n = max(r1 - r0, 0);
-  const bool there = lead >= 0 && lead < p.a.S && f.n > 0;
+  const bool there = lead >= 0 && lead < p.a.S && f.n > 0 && e - b > 1;
   f.s = there ? lead : 0;
   f.whole = whole;
   f.len = f.ctx = there ? (int)(min((long long)max(whole, 0), min(cap_of(p), 0x7fffffffll)) & ~31ll) : 0;
@@ -182,8 +194,7 @@ __global__ void __launch_bounds__(kPlanThreads) shared_plan_small_kernel(Plan p)
 #pragma unroll
   for (int role = 0; role < 2; ++role)
     if (role ? request : group) {
-      f[role].C = piece_keys(all[0] * p.kv.heads, all[1] * p.kv.heads, role);
-      f[role].pieces = max(1, (f[role].len - f[role].begin + f[role].C - 1) / f[role].C);
+      into_pieces(f[role], piece_keys((float)(all[0] * p.kv.heads), (float)(all[1] * p.kv.heads), role, p.R[role]));
       own[role] = p.kv.heads * f[role].tiles * f[role].pieces;
       if (f[role].group >= 0 || f[role].pieces > 1) f[role].flags |= kCut;
       cut[role] = f[role].flags & kCut ? own[role] * units_of(p, f[role], role) : 0;
@@ -257,15 +268,15 @@ __global__ void __launch_bounds__(kPlanThreads) shared_plan_kernel(Plan p) {
   for (int role = 0; role < 2; ++role) {
     const int count = role ? a.S : p.groups;
     Found* const list = role ? mine : p.ws.found;
-    const int C = piece_keys(all[0] * kv.heads, all[1] * kv.heads, role);
+    const int C = piece_keys((float)(all[0] * kv.heads), (float)(all[1] * kv.heads), role, p.R[role]);
     for (int i0 = 0; i0 < count; i0 += kPlanThreads) {
       const int i = i0 + tid;
       int own = 0, cut = 0, row0 = 0, n = 0;
       if (i < count) {
-        const Found& f = list[i];
-        const int pieces = max(1, (f.len - f.begin + C - 1) / C);
-        own = kv.heads * f.tiles * pieces;
-        cut = role == 0 || f.group >= 0 || pieces > 1 ? own * units_of(p, f, role) : 0;
+        Found& f = list[i];
+        into_pieces(f, C);
+        own = kv.heads * f.tiles * f.pieces;
+        cut = role == 0 || f.group >= 0 || f.pieces > 1 ? own * units_of(p, f, role) : 0;
         row0 = f.row0, n = f.n;
       }
       uint64_t chunk, cuts;
@@ -275,8 +286,6 @@ __global__ void __launch_bounds__(kPlanThreads) shared_plan_kernel(Plan p) {
       sh_row0[tid] = row0, sh_n[tid] = n;
       if (i < count) {
         Found& f = list[i];
-        f.pieces = max(1, (f.len - f.begin + C - 1) / C);
-        f.C = C;
         f.item0 = (int)items + upto - own;
         f.slot0 = (int)slots + slot - cut;
         if (cut) f.flags |= kCut;
@@ -364,26 +373,21 @@ __device__ __forceinline__ bool find_few(const Plan& p, int id, Req& q, bool& gr
     g.len = __shfl(f[0].len, lo, 64), g.whole = __shfl(whole, lo, 64);
     if (takes_part(f[1], g)) f[1].group = lo, f[1].begin = g.len;
   }
-  uint64_t all[2], v[2];
-  auto last_of = [&](uint64_t v) {
-    return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), 63) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
-  };
+  float work[2];
 #pragma unroll
-  for (int role = 0; role < 2; ++role) all[role] = last_of(wave_scan_u64(there[role] ? work_of(f[role]) : 0));
+  for (int role = 0; role < 2; ++role)
+    work[role] = wave_sum_f(there[role] ? (float)f[role].tiles * (float)max(f[role].len - f[role].begin, 0) : 0.f) * heads;
   int own[2], upto[2], items[2], behind = 0;
 #pragma unroll
   for (int role = 0; role < 2; ++role) {
-    f[role].C = piece_keys(all[0] * heads, all[1] * heads, role);
-    f[role].pieces = max(1, (int)((unsigned)(f[role].len - f[role].begin + f[role].C - 1) / (unsigned)f[role].C));
+    into_pieces(f[role], piece_keys(work[0], work[1], role, p.R[role]));
     own[role] = there[role] ? heads * f[role].tiles * f[role].pieces : 0;
     if (f[role].group >= 0 || f[role].pieces > 1) f[role].flags |= kCut;
-    const int cut = f[role].flags & kCut ? own[role] * units_of(p, f[role], role) : 0;
-    v[role] = wave_scan_u64((uint64_t)(uint32_t)own[role] | (uint64_t)(uint32_t)cut << 32);
-    const uint64_t sum = last_of(v[role]);
-    upto[role] = (int)v[role];
-    items[role] = (int)sum;
-    f[role].slot0 = behind + (int)(v[role] >> 32) - cut;
-    behind = (int)(sum >> 32);
+    const int cut = f[role].flags & kCut ? own[role] * units_of(p, f[role], role) : 0, cuts = wave_scan_i(cut);
+    upto[role] = wave_scan_i(own[role]);
+    items[role] = __builtin_amdgcn_readlane(upto[role], 63);
+    f[role].slot0 = behind + cuts - cut;
+    behind += __builtin_amdgcn_readlane(cuts, 63);
     fit(p, f[role], cut);
   }
   if (id == 0 && threadIdx.x < 64) {
@@ -546,9 +550,9 @@ int tile_rows(int count, int T, int heads, const btf_kv_cache& kv) {
   return kv.dim != 128 || rows <= 128 * (int64_t)count ? 64 : 128;
 }
 
-// Items of a role at most: each tile's last piece may be a part of one.
-int64_t most_items(int count, int T, int heads, const btf_kv_cache& kv, int R) {
-  return ((int64_t)T * (heads / kv.heads) / R + count) * kv.heads + kRunning + kOwnItems;
+// Items of the groups (role 0) or requests at most: each tile's last piece may be a part of one.
+int64_t most_items(int role, int count, int T, int heads, const btf_kv_cache& kv, int R) {
+  return ((int64_t)T * (heads / kv.heads) / R + count) * kv.heads + (role ? kOwnItems : kRunning);
 }
 
 // Slots of a launch of up to S requests and groups, in 16 rows: a tile's slot has the rows of the request or group, up to the
@@ -562,7 +566,7 @@ int64_t up(int64_t n) { return (n + 255) & ~(int64_t)255; }
 
 // Bytes before the slots, for up to S requests and groups.
 int64_t plan_bytes(int S, int T, int heads, const btf_kv_cache& kv) {
-  return up(64 + 2 * (int64_t)S * sizeof(Found) + 8 * most_items(S, T, heads, kv, 16) + 4 * (int64_t)T);
+  return up(64 + 2 * (int64_t)S * sizeof(Found) + 4 * (most_items(0, S, T, heads, kv, 16) + most_items(1, S, T, heads, kv, 16)) + 4 * (int64_t)T);
 }
 
 template <int D, bool BF>
@@ -601,7 +605,7 @@ int shared_go(const Plan& p, hipStream_t st) {
 }  // namespace
 
 int64_t shared_attention_most_items(int S, int T, int heads, const btf_kv_cache& kv) {
-  return 2 * most_items(S, T, heads, kv, 16);
+  return most_items(0, S, T, heads, kv, 16) + most_items(1, S, T, heads, kv, 16);
 }
 
 int64_t shared_attention_ws_bytes(int S, int T, int heads, const btf_kv_cache& kv) {
@@ -621,7 +625,7 @@ int shared_attention(const btf_shared_attention& a, const btf_kv_cache& kv, hipS
   p.ws.items = reinterpret_cast<int*>(at);
   p.ws.found = reinterpret_cast<Found*>(at + 64);
   p.ws.map = reinterpret_cast<int*>(p.ws.found + a.groups + a.S);
-  p.ws.most = (int)(most_items(a.S, a.T, a.heads, kv, p.R[1]) + (a.groups ? most_items(a.groups, a.T, a.heads, kv, p.R[0]) : 0));
+  p.ws.most = (int)(most_items(1, a.S, a.T, a.heads, kv, p.R[1]) + (a.groups ? most_items(0, a.groups, a.T, a.heads, kv, p.R[0]) : 0));
   p.ws.request = p.ws.map + p.ws.most;
   p.ws.slots = reinterpret_cast<float*>(at + plan_bytes(a.S, a.T, a.heads, kv));
   p.ws.units = (int)slot_units(a.S, a.T, a.heads, kv);
