@@ -13,7 +13,7 @@
 // shared_plan_kernel, one workgroup, finds who takes part (a member needs the whole
 // prefix before its new rows), cuts both roles into items and writes down which item
 // is whose: with hundreds of requests a workgroup that looked for itself, as
-// launch_paged_attention's do, would read all lengths several times. Up to 64 requests
+// launch_paged_attention's do, would read all lengths several times. Up to 128 requests
 // each workgroup does that, and there is no plan. The prefix counts in steps of 32
 // keys, a block of the kernels; what is left of it is done with each member's own
 // keys, which its row of table has, too.
@@ -52,7 +52,8 @@ struct Plan : Args {
   int groups;
   const int *group0, *lead, *shared;
   int R[2];       // rows of a tile of a group, of a request
-  bool alone;     // no launch before: find_few, and the first workgroup writes down `found` for the join
+  int G, cap;     // rows of a token and KV head; tokens that a row of table holds
+  int alone;      // no launch before: find_few of so many requests a lane, and the first workgroup writes down `found` for the join
 };
 
 constexpr int kPlanThreads = 1024;
@@ -80,10 +81,9 @@ __device__ __forceinline__ void into_pieces(Found& f, int C) {
   f.pieces = max(1, (int)((unsigned)(keys + f.C - 1) / (unsigned)f.C));
 }
 
-__device__ __forceinline__ int tiles_of(const Plan& p, int n, int R) {
-  return n > 0 ? (int)(((long long)n * (p.a.heads / p.kv.heads) + R - 1) / R) : 0;
+__device__ __forceinline__ int tiles_of(const Plan& p, int n, int R) {  // (R is a power of two)
+  return n > 0 ? (int)((unsigned)(n * p.G + R - 1) >> __builtin_ctz(R)) : 0;
 }
-__device__ __forceinline__ long long cap_of(const Plan& p) { return (long long)p.a.ldt * p.kv.page; }
 
 // A group of requests b .. e - 1 whose rows are r0 .. r1 - 1.
 __device__ __forceinline__ Found group_of(const Plan& p, int b, int e, int r0, int r1, int lead, int whole) {
@@ -94,7 +94,7 @@ __device__ __forceinline__ Found group_of(const Plan& p, int b, int e, int r0, i
   const bool there = lead >= 0 && lead < p.a.S && f.n > 0 && e - b > 1;
   f.s = there ? lead : 0;
   f.whole = whole;
-  f.len = f.ctx = there ? (int)(min((long long)max(whole, 0), min(cap_of(p), 0x7fffffffll)) & ~31ll) : 0;
+  f.len = f.ctx = there ? min(max(whole, 0), p.cap) & ~31 : 0;
   f.tiles = f.len > 0 ? tiles_of(p, f.n, p.R[0]) : 0;
   f.flags = kCut;
   f.group = -1;
@@ -106,7 +106,7 @@ __device__ __forceinline__ Found request_of(const Plan& p, int s, int r0, int r1
   f.s = s;
   f.row0 = max(r0, 0);
   f.n = max(min(r1, p.a.T) - f.row0, 0);
-  f.len = (int)max(0ll, min((long long)full, cap_of(p)));
+  f.len = max(0, min(full, p.cap));
   f.ctx = full - f.n;
   f.tiles = tiles_of(p, f.n, p.R[1]);
   f.flags = p.a.tree && f.n <= BTF_TREE_NODES ? kTree : 0;
@@ -120,7 +120,7 @@ __device__ __forceinline__ uint64_t work_of(const Found& f) { return (uint64_t)f
 // 16 rows of a slot of f's, and what f's items take from slot0 on if they leave their sums. Row starts that do not ascend
 // can ask for more than there is (of those that do, no launch does): such a request or group is left out.
 __device__ __forceinline__ int units_of(const Plan& p, const Found& f, int role) {
-  return slot_rows(p.R[role], f.n * (p.a.heads / p.kv.heads)) >> 4;
+  return slot_rows(p.R[role], f.n * p.G) >> 4;
 }
 __device__ __forceinline__ void fit(const Plan& p, Found& f, int units) {
   if (f.slot0 < 0 || f.slot0 > p.ws.units - units) f.n = f.tiles = f.pieces = 0, f.flags &= ~kCut;
@@ -342,74 +342,109 @@ __device__ __forceinline__ bool find_item(const Plan& p, int id, Req& q, bool& g
   return true;
 }
 
-// The same for up to 64 requests, one a lane, by the workgroup itself: one trip to memory for all that it reads, in place of
-// the plan's launch and two more trips behind it (4 requests behind 1000 keys 21.2 us, so 16.2; 64 behind 16384 85.6 and 81.9).
+// The same for up to 64 groups and 128 requests, one or two (N) a lane, by the workgroup itself: one trip to memory for all that it reads, in place of
+// the plan's launch and two more trips behind it (4 requests behind 1000 keys 21.2 us,
+// so 16.2; 64 behind 16384 85.6 and 81.9; 78 behind 6400 55.6 and 50.4).
 constexpr int kFew = 64;
+template <int N>
 __device__ __forceinline__ bool find_few(const Plan& p, int id, Req& q, bool& group) {
   const btf_paged_attention& a = p.a;
   const int lane = threadIdx.x & 63, heads = p.kv.heads;
-  const bool there[2] = {lane < p.groups, lane < a.S};
-  const int r0 = there[1] ? a.row0[lane] : 0, r1 = there[1] ? a.row0[lane + 1] : 0, full = there[1] ? a.kv_len[lane] : 0;
-  const int b = there[0] ? p.group0[lane] : 0, e = there[0] ? p.group0[lane + 1] : 0;
-  const int lead = there[0] ? p.lead[lane] : 0, whole = there[0] ? p.shared[lane] : 0;
-  const int last = __builtin_amdgcn_readlane(r1, a.S - 1);
+  const bool is_group = lane < p.groups;
+  int r0[N], r1[N], full[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int s = lane * N + i;
+    const bool there = s < a.S;
+    r0[i] = there ? a.row0[s] : 0, r1[i] = there ? a.row0[s + 1] : 0, full[i] = there ? a.kv_len[s] : 0;
+  }
+  const int b = is_group ? p.group0[lane] : 0, e = is_group ? p.group0[lane + 1] : 0;
+  const int lead = is_group ? p.lead[lane] : 0, whole = is_group ? p.shared[lane] : 0;
+  const int last = __builtin_amdgcn_readlane(r1[(a.S - 1) % N], (a.S - 1) / N);
   auto row_of = [&](int s) {
-    const int row = __shfl(r0, s & 63, 64);  // (by all lanes)
+    int row = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int v = __shfl(r0[i], s / N & 63, 64);  // (by all lanes)
+      if (s % N == i) row = v;
+    }
     return min(max(s < a.S ? row : last, 0), a.T);
   };
   const int gb = min(max(b, 0), a.S), ge = min(max(e, gb), a.S), g0 = row_of(gb), g1 = row_of(ge);
-  Found f[2] = {group_of(p, gb, ge, g0, g1, lead, whole), request_of(p, lane, r0, r1, full)};
-  if (p.groups > 0) {
-    int lo = 0, hi = p.groups - 1;  // last_at_most
-    while (__any(lo < hi)) {
-      const int mid = (lo + hi + 1) >> 1, v = __shfl(b, mid, 64);
-      if (lo < hi) {
-        if (v <= lane) lo = mid;
-        else hi = mid - 1;
+  Found f = group_of(p, gb, ge, g0, g1, lead, whole), r[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int s = lane * N + i;
+    r[i] = request_of(p, s, r0[i], r1[i], full[i]);
+    if (p.groups > 0) {
+      int lo = 0, hi = p.groups - 1;  // last_at_most
+      while (__any(lo < hi)) {
+        const int mid = (lo + hi + 1) >> 1, v = __shfl(b, mid, 64);
+        if (lo < hi) {
+          if (v <= s) lo = mid;
+          else hi = mid - 1;
+        }
       }
+      Found g{};
+      g.b = __shfl(gb, lo, 64), g.e = __shfl(ge, lo, 64), g.row0 = __shfl(f.row0, lo, 64), g.n = __shfl(f.n, lo, 64);
+      g.len = __shfl(f.len, lo, 64), g.whole = __shfl(whole, lo, 64);
+      if (takes_part(r[i], g)) r[i].group = lo, r[i].begin = g.len;
     }
-    Found g{};
-    g.b = __shfl(gb, lo, 64), g.e = __shfl(ge, lo, 64), g.row0 = __shfl(f[0].row0, lo, 64), g.n = __shfl(f[0].n, lo, 64);
-    g.len = __shfl(f[0].len, lo, 64), g.whole = __shfl(whole, lo, 64);
-    if (takes_part(f[1], g)) f[1].group = lo, f[1].begin = g.len;
   }
-  float work[2];
+  auto work_of_lane = [](const Found& f) { return (float)f.tiles * (float)max(f.len - f.begin, 0); };
+  float mine = 0.f;
 #pragma unroll
-  for (int role = 0; role < 2; ++role)
-    work[role] = wave_sum_f(there[role] ? (float)f[role].tiles * (float)max(f[role].len - f[role].begin, 0) : 0.f) * heads;
-  int own[2], upto[2], items[2], behind = 0;
+  for (int i = 0; i < N; ++i) mine += lane * N + i < a.S ? work_of_lane(r[i]) : 0.f;
+  const float work0 = wave_sum_f(is_group ? work_of_lane(f) : 0.f) * heads, work1 = wave_sum_f(mine) * heads;
+  into_pieces(f, piece_keys(work0, work1, 0, p.R[0]));
+  const int own0 = is_group ? heads * f.tiles * f.pieces : 0, cut0 = own0 * units_of(p, f, 0);
+  const int upto0 = wave_scan_i(own0), cuts0 = wave_scan_i(cut0);
+  f.slot0 = cuts0 - cut0;
+  fit(p, f, cut0);
+  const int C = piece_keys(work0, work1, 1, p.R[1]);
+  int own[N], cut[N], all = 0, cuts = 0;
 #pragma unroll
-  for (int role = 0; role < 2; ++role) {
-    into_pieces(f[role], piece_keys(work[0], work[1], role, p.R[role]));
-    own[role] = there[role] ? heads * f[role].tiles * f[role].pieces : 0;
-    if (f[role].group >= 0 || f[role].pieces > 1) f[role].flags |= kCut;
-    const int cut = f[role].flags & kCut ? own[role] * units_of(p, f[role], role) : 0, cuts = wave_scan_i(cut);
-    upto[role] = wave_scan_i(own[role]);
-    items[role] = __builtin_amdgcn_readlane(upto[role], 63);
-    f[role].slot0 = behind + cuts - cut;
-    behind += __builtin_amdgcn_readlane(cuts, 63);
-    fit(p, f[role], cut);
+  for (int i = 0; i < N; ++i) {
+    into_pieces(r[i], C);
+    own[i] = lane * N + i < a.S ? heads * r[i].tiles * r[i].pieces : 0;
+    if (r[i].group >= 0 || r[i].pieces > 1) r[i].flags |= kCut;
+    cut[i] = r[i].flags & kCut ? own[i] * units_of(p, r[i], 1) : 0;
+    all += own[i], cuts += cut[i];
+  }
+  const int upto1 = wave_scan_i(all);
+  int slot = __builtin_amdgcn_readlane(cuts0, 63) + wave_scan_i(cuts) - cuts;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    r[i].slot0 = slot;
+    slot += cut[i];
+    fit(p, r[i], cut[i]);
   }
   if (id == 0 && threadIdx.x < 64) {
+    if (is_group) p.ws.found[lane] = f;
 #pragma unroll
-    for (int role = 0; role < 2; ++role)
-      if (there[role]) p.ws.found[role ? p.groups + lane : lane] = f[role];
+    for (int i = 0; i < N; ++i)
+      if (lane * N + i < a.S) p.ws.found[p.groups + lane * N + i] = r[i];
   }
-  group = id < items[0];
-  const int at = group ? id : id - items[0];
-  if (!group && at >= items[1]) return false;
-  const uint64_t behind_it = __ballot(group ? there[0] && upto[0] > at : there[1] && upto[1] > at);
-  if (!behind_it) return false;
-  const int l = __builtin_ctzll(behind_it);
-  auto of = [&](int x, int y) { return __builtin_amdgcn_readlane(group ? x : y, l); };
-  q.s = of(f[0].s, f[1].s), q.row0 = of(f[0].row0, f[1].row0), q.n = of(f[0].n, f[1].n);
-  q.len = of(f[0].len, f[1].len), q.ctx = of(f[0].ctx, f[1].ctx), q.tiles = of(f[0].tiles, f[1].tiles);
-  q.pieces = of(f[0].pieces, f[1].pieces), q.begin = group ? 0 : __builtin_amdgcn_readlane(f[1].begin, l);
-  q.C = of(f[0].C, f[1].C), q.slot = of(f[0].slot0, f[1].slot0);
-  const int flags = of(f[0].flags, f[1].flags);
+  const int groups = __builtin_amdgcn_readlane(upto0, 63);
+  group = id < groups;
+  const int at = group ? id : id - groups;
+  const uint64_t behind = __ballot((group ? upto0 : upto1) > at);
+  if (!behind) return false;
+  const int l = __builtin_ctzll(behind);
+  auto of = [&](int x) { return __builtin_amdgcn_readlane(x, l); };
+  int local = at - of(group ? upto0 - own0 : upto1 - all);
+  Found x = f;
+  if (!group) {
+    x = r[0];
+#pragma unroll
+    for (int i = 1; i < N; ++i)
+      if (local >= of(own[i - 1])) local -= of(own[i - 1]), x = r[i];
+  }
+  q.s = of(x.s), q.row0 = of(x.row0), q.n = of(x.n), q.len = of(x.len), q.ctx = of(x.ctx);
+  q.tiles = of(x.tiles), q.pieces = of(x.pieces), q.begin = of(x.begin), q.C = of(x.C), q.slot = of(x.slot0);
+  const int flags = of(x.flags);
   q.tree = flags & kTree;
   q.cut = flags & kCut;
-  const int local = at - of(upto[0] - own[0], upto[1] - own[1]);
   if ((unsigned)local >= (unsigned)(q.tiles * q.pieces * heads)) return false;
   q.local = order_of(q, heads, local);
   return true;
@@ -442,7 +477,9 @@ __global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_e
   __shared__ __attribute__((aligned(16))) char lds[a > b ? a : b];
   Req q;
   bool group;
-  if (!(p.alone ? find_few(p, blockIdx.x, q, group) : find_item(p, blockIdx.x, q, group))) return;  // the whole workgroup
+  const int id = blockIdx.x;
+  const bool found = p.alone == 1 ? find_few<1>(p, id, q, group) : p.alone ? find_few<2>(p, id, q, group) : find_item(p, id, q, group);
+  if (!found) return;  // the whole workgroup
   if (R0 == R1 || group) item<D, BF, R0, R0 != R1>(p, q, lds);
   else item<D, BF, R1, R0 != R1>(p, q, lds);
 }
@@ -458,14 +495,16 @@ __global__ void __launch_bounds__(64 * kJoinWaves) shared_join_kernel(Plan p) {
   const btf_paged_attention& a = p.a;
   int s;
   if (p.alone) {
-    const int l = threadIdx.x & 63, t = blockIdx.x;
-    const uint64_t m = __ballot(l < a.S && a.row0[min(l, a.S - 1)] <= t && t < a.row0[min(l, a.S - 1) + 1]);
-    s = 63 - __builtin_clzll(m | 1);
-    if (!m) return;  // the whole workgroup
+    s = -1;
+    for (int s0 = 0; s0 < a.S; s0 += 64) {
+      const int l = min(s0 + (int)(threadIdx.x & 63), a.S - 1), t = blockIdx.x;
+      const uint64_t m = __ballot(a.row0[l] <= t && t < a.row0[l + 1]);
+      if (m) s = min(s0 + 63 - (int)__builtin_clzll(m), a.S - 1);
+    }
   } else {
     s = ((ints_p)p.ws.request)[blockIdx.x];
-    if (s < 0) return;
   }
+  if (s < 0) return;  // the whole workgroup
   const found_p f = (found_p)p.ws.found + p.groups + s;
   if (!(f->flags & kCut)) return;
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -631,7 +670,9 @@ int shared_attention(const btf_shared_attention& a, const btf_kv_cache& kv, hipS
   p.ws.units = (int)slot_units(a.S, a.T, a.heads, kv);
   p.a = btf_paged_attention{a.S,   a.T,    a.heads, a.q,   a.ldq, a.table,    a.ldt,
                             a.row0, a.kv_len, a.tree, a.scale, a.out, a.ldo, p.ws.slots};
-  p.alone = a.S <= kFew;
+  p.G = a.heads / kv.heads;
+  p.cap = (int64_t)a.ldt * kv.page < 0x7fffffff ? a.ldt * kv.page : 0x7fffffff;
+  p.alone = a.groups > kFew ? 0 : a.S <= kFew ? 1 : a.S <= 2 * kFew ? 2 : 0;
   const bool bf = kv.type == BTF_BF16;
   if (kv.dim == 64) return bf ? shared_go<64, true>(p, st) : shared_go<64, false>(p, st);
   if (kv.dim == 128) return bf ? shared_go<128, true>(p, st) : shared_go<128, false>(p, st);

@@ -206,7 +206,7 @@ def test_strides_and_spare_rows(hip):
     check_attn(out, qw, k, v, table, row0, kv_len, None, heads, kind, page)
 
 
-@pytest.mark.parametrize("S,groups", [(300, 7), (1100, 2), (1500, 1100)])
+@pytest.mark.parametrize("S,groups", [(64, 64), (65, 3), (100, 64), (127, 65), (128, 5), (129, 1), (300, 7), (1100, 2), (1500, 1100)])
 def test_many_requests(hip, S, groups):
     """More requests and groups than the plan takes at once."""
     rng = np.random.default_rng(S)
