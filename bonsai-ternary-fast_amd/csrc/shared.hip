@@ -53,6 +53,7 @@ struct Plan : Args {
   const int *group0, *lead, *shared;
   int R[2];       // rows of a tile of a group, of a request
   int G, cap;     // rows of a token and KV head; tokens that a row of table holds
+  int own;        // items that the requests' keys are cut into: kOwnItems, or kFewItems
   int alone;      // no launch before: find_few of so many requests a lane, and the first workgroup writes down `found` for the join
 };
 
@@ -63,15 +64,18 @@ constexpr int kPlanThreads = 1024;
 // share of these by the roles' work (a request's keys count twice, for what an item costs beside its keys), at least half,
 // the requests' items fill the rest and follow (64 requests behind 16384 keys with 250 to 1000 of their own, heads of 256:
 // the call 85 us, with 512 items of the groups 95, 192 104; a group alone 56 us in 512 items, 69 in 256).
-constexpr int kRunning = 512, kOwnItems = 384;
+// 256 own items where that leaves no more than run at a time (48 behind 2500 keys with 900 of their own, heads of 256, 42.4
+// us in 384, 37.2 so; the trees of 24 behind three prefixes, more items in any case, 110 and 134), and of attn_stream with heads
+// of 256, of which a CU runs one workgroup (2 requests of 8200 keys 27.1 and 20.4).
+constexpr int kRunning = 512, kOwnItems = 384, kFewItems = 256;
 // (Sums of the work in 32 bits are off by 2^-17 at most, for which the last factor stands: there are never more items.)
 // Tiles above 16 rows, whose waves take all keys of an item, in pieces of 64 keys where that leaves no more items either and
 // makes up to 32 of a request (4 requests behind 1000 keys 16.2 us in pieces of 128, 14.3 in 64, 14.9 in 32; 6 of two groups
 // behind 6500 keys, whose rows would have 100 pieces to join, 13.8, 16.5, 16.2).
 constexpr int kHalf = kStep / 2, kMostHalves = 32;
-__device__ __forceinline__ int piece_keys(float groups, float requests, int role, int R) {
+__device__ __forceinline__ int piece_keys(float groups, float requests, int role, int R, int own) {
   const float share = (float)kRunning * (groups / (groups + 2.f * requests + 1.f));
-  const float items = role ? (float)kOwnItems : fmaxf(floorf(share), (float)(kRunning / 2));
+  const float items = role ? (float)own : fmaxf(floorf(share), (float)(kRunning / 2));
   const float keys = (role ? requests : groups) * 1.0001f / items;
   return R > 16 && keys <= (float)kHalf ? kHalf : kStep * (int)fminf(keys / (float)kStep + 1.f, 1e6f);
 }
@@ -194,7 +198,7 @@ __global__ void __launch_bounds__(kPlanThreads) shared_plan_small_kernel(Plan p)
 #pragma unroll
   for (int role = 0; role < 2; ++role)
     if (role ? request : group) {
-      into_pieces(f[role], piece_keys((float)(all[0] * p.kv.heads), (float)(all[1] * p.kv.heads), role, p.R[role]));
+      into_pieces(f[role], piece_keys((float)(all[0] * p.kv.heads), (float)(all[1] * p.kv.heads), role, p.R[role], p.own));
       own[role] = p.kv.heads * f[role].tiles * f[role].pieces;
       if (f[role].group >= 0 || f[role].pieces > 1) f[role].flags |= kCut;
       cut[role] = f[role].flags & kCut ? own[role] * units_of(p, f[role], role) : 0;
@@ -268,7 +272,7 @@ __global__ void __launch_bounds__(kPlanThreads) shared_plan_kernel(Plan p) {
   for (int role = 0; role < 2; ++role) {
     const int count = role ? a.S : p.groups;
     Found* const list = role ? mine : p.ws.found;
-    const int C = piece_keys((float)(all[0] * kv.heads), (float)(all[1] * kv.heads), role, p.R[role]);
+    const int C = piece_keys((float)(all[0] * kv.heads), (float)(all[1] * kv.heads), role, p.R[role], p.own);
     for (int i0 = 0; i0 < count; i0 += kPlanThreads) {
       const int i = i0 + tid;
       int own = 0, cut = 0, row0 = 0, n = 0;
@@ -396,12 +400,19 @@ __device__ __forceinline__ bool find_few(const Plan& p, int id, Req& q, bool& gr
 #pragma unroll
   for (int i = 0; i < N; ++i) mine += lane * N + i < a.S ? work_of_lane(r[i]) : 0.f;
   const float work0 = wave_sum_f(is_group ? work_of_lane(f) : 0.f) * heads, work1 = wave_sum_f(mine) * heads;
-  into_pieces(f, piece_keys(work0, work1, 0, p.R[0]));
+  into_pieces(f, piece_keys(work0, work1, 0, p.R[0], p.own));
   const int own0 = is_group ? heads * f.tiles * f.pieces : 0, cut0 = own0 * units_of(p, f, 0);
   const int upto0 = wave_scan_i(own0), cuts0 = wave_scan_i(cut0);
   f.slot0 = cuts0 - cut0;
   fit(p, f, cut0);
-  const int C = piece_keys(work0, work1, 1, p.R[1]);
+  int C = piece_keys(work0, work1, 1, p.R[1], kFewItems);
+  if (p.own != kFewItems) {
+    float few = (float)own0;
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      few += lane * N + i < a.S ? (float)(heads * r[i].tiles) * ceilf((float)max(r[i].len - r[i].begin, 1) * __builtin_amdgcn_rcpf((float)C)) : 0.f;
+    if (wave_sum_f(few) > (float)kRunning) C = piece_keys(work0, work1, 1, p.R[1], p.own);
+  }
   int own[N], cut[N], all = 0, cuts = 0;
 #pragma unroll
   for (int i = 0; i < N; ++i) {
@@ -671,6 +682,7 @@ int shared_attention(const btf_shared_attention& a, const btf_kv_cache& kv, hipS
   p.a = btf_paged_attention{a.S,   a.T,    a.heads, a.q,   a.ldq, a.table,    a.ldt,
                             a.row0, a.kv_len, a.tree, a.scale, a.out, a.ldo, p.ws.slots};
   p.G = a.heads / kv.heads;
+  p.own = kv.dim == 256 && p.R[0] == 16 ? kFewItems : kOwnItems;
   p.cap = (int64_t)a.ldt * kv.page < 0x7fffffff ? a.ldt * kv.page : 0x7fffffff;
   p.alone = a.groups > kFew ? 0 : a.S <= kFew ? 1 : a.S <= 2 * kFew ? 2 : 0;
   const bool bf = kv.type == BTF_BF16;
