@@ -260,6 +260,7 @@ int64_t shared_attention_most_items(int S, int T, int heads, const btf_kv_cache&
 int64_t shared_attention_ws_bytes(int S, int T, int heads, const btf_kv_cache& kv);
 int shared_attention(const btf_shared_attention& a, const btf_kv_cache& kv, hipStream_t st);
 int64_t lora_ws_bytes(int S, int T, int K, int rank, int nseg);
+int64_t lora_most_groups(int S, int T, int64_t outs, int nseg);
 int lora(const btf_lora& a, const btf_lora_seg* segs, int nseg, hipStream_t st);
 
 }  // namespace btfhip

@@ -774,6 +774,12 @@ int64_t lora_ws_bytes(int S, int T, int K, int rank, int nseg) {
   return ws_rows(T, K, nseg) * rank * 4;
 }
 
+// Workgroups of a launch at most (apart from small ones, which are cut further): a tile by 1024 outputs.
+int64_t lora_most_groups(int S, int T, int64_t outs, int nseg) {
+  const int64_t tiles = T <= 4 * (int64_t)S ? T : (int64_t)T / 16 + S;
+  return tiles * (outs / (4 * kChunk) + nseg);
+}
+
 int lora(const btf_lora& a, const btf_lora_seg* s, int nseg, hipStream_t st) {
   Segs segs{};
   for (int i = 0; i < nseg; ++i) segs.s[i] = s[i];

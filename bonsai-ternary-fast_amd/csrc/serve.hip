@@ -283,7 +283,8 @@ int btf_hip_launch_lora(const btf_lora* a, const btf_lora_seg* segs, int nseg, b
       return bad("lora", "adapter strides must be multiples of 8 values");
     outs += g.N;
   }
-  if (a->S > kMaxGroups / 4 || a->T > kMaxGroups / 4 || outs > 1 << 24) return bad("lora", "more requests, rows or outputs than a launch takes");
+  if (a->S > kMaxGroups / 4 || a->T > kMaxGroups / 4 || outs > 1 << 24 || lora_most_groups(a->S, a->T, glu ? segs[0].N : outs, nseg) > kMaxGroups)
+    return bad("lora", "more requests, rows or outputs than a launch takes");
   if (!a->ws || !aligned(a->ws, 16)) return bad("lora", "ws must be 16-byte aligned scratch");
   if (!current_state()) return BTF_ERR_NOT_INIT;
   return lora(*a, segs, nseg, static_cast<hipStream_t>(stream));

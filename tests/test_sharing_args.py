@@ -93,6 +93,12 @@ def test_segments_refused(segs):
     assert h.launch_lora_raw(LORA, segs, len(segs)) == ARGS
 
 
+def test_more_workgroups_than_a_launch_takes():
+    wide = dataclasses.replace(SEG, N=20480, ldy=20480)
+    for S, T, code in ((1 << 21, 1 << 21, ARGS), (1, 1 << 22, ARGS), (1, 1 << 21, NOT_INIT), (1 << 18, 1 << 18, NOT_INIT)):
+        assert h.launch_lora_raw(dataclasses.replace(LORA, S=S, T=T), [wide], 1) == code
+
+
 def test_swiglu_segments_refused():
     for segs in ([SEG], [SEG] * 3, [SEG, dataclasses.replace(SEG, N=32)]):
         assert launch("glu", GLU, segs=segs) == ARGS
