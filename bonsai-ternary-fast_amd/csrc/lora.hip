@@ -97,8 +97,8 @@ __device__ bool find(const btf_lora& a, int id, Tile& t) {
   for (int s0 = 0; s0 < a.S; s0 += 64) {
     int r0 = 0, n = 0, who = -1;
     if (s0 + lane < a.S) {
-      r0 = max(a.row0[s0 + lane], 0);
-      n = min(a.row0[s0 + lane + 1], a.T) - r0;
+      r0 = min(max(a.row0[s0 + lane], 0), a.T);
+      n = min(max(a.row0[s0 + lane + 1], 0), a.T) - r0;
       who = a.adapter[s0 + lane];
     }
     const int mine = n > 0 ? (n + R - 1) / R : 0, upto = before + wave_scan(mine);

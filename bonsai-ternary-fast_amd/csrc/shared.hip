@@ -80,7 +80,7 @@ __device__ __forceinline__ int piece_keys(float groups, float requests, int role
   return R > 16 && keys <= (float)kHalf ? kHalf : kStep * (int)fminf(keys / (float)kStep + 1.f, 1e6f);
 }
 __device__ __forceinline__ void into_pieces(Found& f, int C) {
-  const int keys = f.len - f.begin;
+  const int keys = max(f.len - f.begin, 0);
   f.C = C < kStep && keys > kMostHalves * kHalf ? kStep : C;
   f.pieces = max(1, (int)((unsigned)(keys + f.C - 1) / (unsigned)f.C));
 }
@@ -108,10 +108,10 @@ __device__ __forceinline__ Found group_of(const Plan& p, int b, int e, int r0, i
 __device__ __forceinline__ Found request_of(const Plan& p, int s, int r0, int r1, int full) {
   Found f{};
   f.s = s;
-  f.row0 = max(r0, 0);
-  f.n = max(min(r1, p.a.T) - f.row0, 0);
+  f.row0 = min(max(r0, 0), p.a.T);
+  f.n = max(min(max(r1, 0), p.a.T) - f.row0, 0);
   f.len = max(0, min(full, p.cap));
-  f.ctx = full - f.n;
+  f.ctx = max(full, -1) - f.n;
   f.tiles = tiles_of(p, f.n, p.R[1]);
   f.flags = p.a.tree && f.n <= BTF_TREE_NODES ? kTree : 0;
   f.group = -1;

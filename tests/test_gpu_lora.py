@@ -241,6 +241,8 @@ def test_rows_that_do_not_fit(hip):
     c.check_add(c.run(hip)[0])
     c.row0 = np.array([5, 2, 6, 6])
     c.check_add(c.run(hip)[0])
+    c.row0 = np.array([-2 ** 31, 4, 2 ** 31 - 1, -2 ** 31])
+    c.check_add(c.run(hip)[0])
 
 
 @pytest.mark.parametrize("new,rank", [([1] * 20, 16), ([80, 41], 64)])

@@ -126,8 +126,31 @@ def test_members_that_do_not_take_part(hip, kind):
     q = q.clone()
     q[:2] = 0
     check_attn(out, q, *x[1:], kv_len, None, heads, kind, page)
-    none = run_shared(hip, *x, [0] * 6, None, heads, kind, page, [0, 6], [0], [100])
-    assert bool((none == 0).all())
+    for none in (0, -1, -2 ** 31):
+        assert bool((run_shared(hip, *x, [none] * 6, None, heads, kind, page, [0, 6], [0], [100]) == 0).all())
+
+
+@pytest.mark.parametrize("S", [6, 70, 130])
+def test_lengths_and_row_starts_at_the_ends_of_their_type(hip, S):
+    """Lengths below zero give zeros, ones beyond the table what it holds; a row start beyond all others leaves its request
+    the rows up to T, one below zero those from 0 on; where starts fall, the request before them is right."""
+    heads, kind, page = (10, 2, 128), "f16", 16
+    rng = np.random.default_rng(17)
+    x, kv_len = shared_inputs(rng, [0, S], [100], [4] * S, [1] * S, heads, kind, page)
+    q, k, v, table, row0 = x
+    low, high = -2 ** 31, 2 ** 31 - 1
+    full = table.shape[1] * page
+    kv_len[1], kv_len[3] = low, high
+    out = run_shared(hip, *x, kv_len, None, heads, kind, page, [0, S], [0], [100])
+    want = list(kv_len)
+    want[1], want[3] = 0, full  # (its row sees all that the table holds)
+    check_attn(out, *x, want, None, heads, kind, page)
+    row0 = row0.copy()
+    row0[0], row0[S] = low, high
+    check_attn(run_shared(hip, q, k, v, table, row0, kv_len, None, heads, kind, page, [0, S], [0], [100]), *x, want, None, heads, kind, page)
+    row0[2:] = low
+    out = run_shared(hip, q, k, v, table, row0, kv_len, None, heads, kind, page, [0, S], [0], [100])
+    check_attn(out[:1], q[:1], k, v, table, np.array([0] + [1] * S), want, None, heads, kind, page)
 
 
 @pytest.mark.parametrize("group0,lead,prefix", [
