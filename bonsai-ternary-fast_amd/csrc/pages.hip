@@ -342,8 +342,8 @@ __global__ void __launch_bounds__(N) cache_move_kernel(btf_cache_move a, btf_kv_
     if (leaf >= 0 && leaf < a.T) bits = a.tree[leaf];
     n = __popcll(bits);
   } else {
-    lo = max(a.source0[s], 0);
-    n = max(min(a.source0[s + 1], a.T) - lo, 0);
+    lo = min(max(a.source0[s], 0), a.T);
+    n = max(min(max(a.source0[s + 1], 0), a.T) - lo, 0);
   }
   if (blockIdx.y == 0 && run == 0 && h == 0 && !(id & 1) && threadIdx.x == 0 && a.kv_len) a.kv_len[s] = first + n;
   uint16_t* base = static_cast<uint16_t*>(id & 1 ? kv.v : kv.k) + (size_t)blockIdx.y * a.layer_stride +

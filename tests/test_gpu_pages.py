@@ -280,6 +280,14 @@ def test_move_of_places_that_are_none(hip):
     np.testing.assert_array_equal(n, [2, 63])
     for x, w in zip(kv, ref.move(*old, table, None, [-2, 60], [[0, 1, 2, 3], [61, 62, 63]], page)):
         np.testing.assert_array_equal(host(x.view(torch.int16)), w)
+    # starts of the lists at the ends of their type: none of request 0, the first two of request 1
+    kv, old = caches(rng, "f16", 1, pages, HK, page, D)
+    n = ints([-9, -9])
+    hip.launch_cache_move(hip.CacheMove(S=2, T=4, table=ints(table), ldt=4, first=ints([0, 0]), source=ints([18, 40, 41, 42]),
+                                        source0=ints([2 ** 31 - 1, -2 ** 31, 2]), kv_len=n), cache_of(hip, kv, "f16", HK, page, D, pages), stream())
+    assert host(n).tolist() == [0, 2]
+    for x, w in zip(kv, ref.move(*old, table, None, [0, 0], [[], [18, 40]], page)):
+        np.testing.assert_array_equal(host(x.view(torch.int16)), w)
 
 
 def test_far_pages(hip):

@@ -236,3 +236,32 @@ def test_requests_that_share(hip, kind):
         assert host(L.held).tolist() == [ref.pages_of(c, L.page) for c in ctx]
         have = paths
     assert host(L.n_free)[0] == L.pages and not host(L.shared).any()
+
+
+def test_two_streams(hip):
+    """Two loops, each with a workspace of its own, at once on two streams: what each gives alone."""
+    torch = _torch()
+    alone, loops = [Loop(hip, k) for k in ("f16", "bf16")], [Loop(hip, k) for k in ("f16", "bf16")]
+    streams = [torch.cuda.Stream() for _ in loops]
+    ctx = np.zeros(Loop.S, int)
+    for n in (0, 1):
+        for L in alone + loops:
+            fill(L, n, ctx)
+        if n:  # as the first step left them
+            ctx[1], ctx[2], ctx[5] = 30, 30, 16
+        at = ints(ctx)
+        for L in alone:
+            for part in (L.forks, lambda st, L=L: L.ctx.copy_(at), L.step, L.accept, L.give_back):
+                part(torch.cuda.current_stream().cuda_stream)
+            torch.cuda.synchronize()
+        for L, st in zip(loops, streams):
+            with torch.cuda.stream(st):
+                L.forks(st)
+                L.ctx.copy_(at)
+                for part in (L.step, L.accept, L.give_back):
+                    part(st)
+        torch.cuda.synchronize()
+        for x, y in zip(alone, loops):
+            for a, b in zip(x.state(), y.state()):
+                assert torch.equal(a.nan_to_num(9.0), b.nan_to_num(9.0))
+        ctx = host(alone[0].after).astype(int)
