@@ -713,9 +713,10 @@ int btf_hip_launch_cache_move(const btf_cache_move* a, const btf_kv_cache* kv, b
  * requests group0[g] .. group0[g+1] - 1; the first shared[g] tokens of theirs are
  * the tokens in row lead[g] of table (one of the S rows: the same pages as in the
  * members' rows, or pages with the same values). Requests before group0[0] or from
- * group0[groups] on are attended to alone, as is a member that has less than
- * shared[g] tokens before its new rows (a refused one gives zeros, as there), and
- * all of a group whose lead is not in [0, S). group0 has to ascend, in [0, S].
+ * group0[groups] on are attended to alone, through their own rows of table, as is a
+ * member that has less than shared[g] tokens before its new rows (a refused one gives
+ * zeros, as there), and all of a group of one request or whose lead is not in [0, S).
+ * group0 has to ascend, in [0, S].
  * The other arguments, trees and masks are launch_paged_attention's. ws:
  * shared_attention_ws_bytes of device scratch for the launch's S, T and heads,
  * 16-byte aligned, one for each stream that launches; it need not be cleared, and
