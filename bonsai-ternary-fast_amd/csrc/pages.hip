@@ -11,7 +11,7 @@
 // page. Its number among the owners is a prefix sum.
 //
 // copy and move are bytes. A wave's lanes take runs of 128 bytes (a cache line) or
-// more of a token's values; up to eight 16-byte loads a thread are on their way
+// more of a token's values (a move with few workgroups less); up to eight 16-byte loads a thread are on their way
 // before the first store.
 #include <climits>
 #include <string>
@@ -321,13 +321,14 @@ __global__ void __launch_bounds__(kCopyThreads) page_copy_kernel(btf_page_copy a
 
 // ---- move ----
 // In place a token's new place may be another's old one, but never that of a later
-// token of the list (places ascend, none goes up). A workgroup has one 128-byte run of
+// token of the list (places ascend, none goes up). A workgroup has one run (32 to 128 bytes) of
 // the values of one (request, K or V, head, layer) for all tokens: it reads a batch,
 // waits until all of its threads have theirs, writes it, and goes on. So no two
 // workgroups touch the same bytes, and nothing is overwritten before it was read.
-template <int N, bool TREE>
+// L lanes have a token, 16 bytes each.
+template <int N, bool TREE, int L>
 __global__ void __launch_bounds__(N) cache_move_kernel(btf_cache_move a, btf_kv_cache kv) {
-  const int runs = kv.dim / 64;
+  const int runs = kv.dim / (8 * L);
   int id = blockIdx.x;
   const int run = id % runs;
   id /= runs;
@@ -347,7 +348,7 @@ __global__ void __launch_bounds__(N) cache_move_kernel(btf_cache_move a, btf_kv_
   }
   if (blockIdx.y == 0 && run == 0 && h == 0 && !(id & 1) && threadIdx.x == 0 && a.kv_len) a.kv_len[s] = first + n;
   uint16_t* base = static_cast<uint16_t*>(id & 1 ? kv.v : kv.k) + (size_t)blockIdx.y * a.layer_stride +
-                   (size_t)h * kv.head_stride + 64 * run + 8 * (threadIdx.x & 7);
+                   (size_t)h * kv.head_stride + 8 * (L * run + (threadIdx.x & (L - 1)));
   const int* tab = a.table + (size_t)s * a.ldt;
   const int* tab_to = a.to_table ? a.to_table + (size_t)s * a.ldt_to : tab;
   const int ld_to = a.to_table ? a.ldt_to : a.ldt;
@@ -358,7 +359,7 @@ __global__ void __launch_bounds__(N) cache_move_kernel(btf_cache_move a, btf_kv_
     const int p = t[place >> sh];
     return p < 0 || p >= kv.pages ? -1 : p * (long long)kv.page_stride + (place & (kv.page - 1)) * (long long)kv.tok_stride;
   };
-  constexpr int kAtOnce = N / 8;  // tokens
+  constexpr int kAtOnce = N / L;  // tokens
   // Two batches in flight: while one's values arrive, the places and page ids of the next are looked up; its values are
   // under way before this one's are stored.
   constexpr int kMine = 2;  // tokens of a thread (with more than 64 registers only one workgroup of 1024 threads fits a CU)
@@ -367,7 +368,7 @@ __global__ void __launch_bounds__(N) cache_move_kernel(btf_cache_move a, btf_kv_
   auto look = [&](int i0, int b) {
 #pragma unroll
     for (int u = 0; u < kMine; ++u) {
-      const int i = i0 + u * kAtOnce + (threadIdx.x >> 3);
+      const int i = i0 + u * kAtOnce + threadIdx.x / L;
       from[b][u] = to[b][u] = -1;
       if (i < n) {
         long long place;
@@ -470,11 +471,18 @@ int page_copy(const btf_page_copy& a, const btf_kv_cache& kv, hipStream_t st) {
 }
 
 int cache_move(const btf_cache_move& a, const btf_kv_cache& kv, hipStream_t st) {
-  const dim3 grid(2 * a.S * kv.heads * (kv.dim / 64), a.layers);
+  const int groups = 2 * a.S * kv.heads * (kv.dim / 64);
   // A tree's path in batches of 16 tokens. A list in batches of 256 with as many threads as there are: 8 requests of up to
   // 16384 tokens, half of which stay, 2 layers, 187 us (3.9 TB/s read and written) with 1024 threads, 247 with 512, 278 with 256.
-  if (a.tree) hipLaunchKernelGGL((cache_move_kernel<64, true>), grid, dim3(64), 0, st, a, kv);
-  else hipLaunchKernelGGL((cache_move_kernel<1024, false>), grid, dim3(1024), 0, st, a, kv);
+  // Where that leaves CUs idle, shorter runs of more tokens at once: one request of 9000 tokens, heads of 256, runs of 128, 64, 32, 16
+  // bytes: 1 KV head (8 workgroups of 128 bytes) 30, 22, 19, 16 us, 4 heads (32) 42, 27, 24, 36, 8 (64) 41, 28, 30, 55, 16 (128)
+  // 46, 35, 57, 94; 160 workgroups 53 and 62 in runs of 64.
+  auto go = [&](auto kernel, int parts) { hipLaunchKernelGGL(kernel, dim3(parts * groups, a.layers), dim3(1024), 0, st, a, kv); };
+  const int64_t all = (int64_t)groups * a.layers;
+  if (a.tree) hipLaunchKernelGGL((cache_move_kernel<64, true, 8>), dim3(groups, a.layers), dim3(64), 0, st, a, kv);
+  else if (all <= 48) go(cache_move_kernel<1024, false, 2>, 4);
+  else if (all <= 128) go(cache_move_kernel<1024, false, 4>, 2);
+  else go(cache_move_kernel<1024, false, 8>, 1);
   return launch_status("cache_move_kernel");
 }
 

@@ -219,7 +219,7 @@ def run_move(hip, kv, kind, table, HK, page, D, L, pages, first, to_table=None, 
     return host(n)
 
 
-@pytest.mark.parametrize("HK,D,page,L,kind", [(4, 256, 64, 2, "f16"), (2, 128, 16, 1, "bf16"), (1, 64, 32, 3, "f16")])
+@pytest.mark.parametrize("HK,D,page,L,kind", [(8, 256, 64, 2, "bf16"), (4, 256, 64, 2, "f16"), (2, 128, 16, 1, "bf16"), (1, 64, 32, 3, "f16")])
 @pytest.mark.parametrize("hi,part", [(1, 1.0), (40, 0.5), (700, 0.9), (2500, 0.5), (2500, 1.0), (5000, 0.02)])
 @pytest.mark.parametrize("other", [False, True])
 def test_move_listed_tokens(hip, HK, D, page, L, kind, hi, part, other):
