@@ -381,13 +381,23 @@ __global__ void __launch_bounds__(kThreads, 2) lora_expand_kernel(btf_lora a, Se
     for (int i = 0; i < TN; ++i)
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt) {
-        const int n = n0 + 16 * i + 4 * g, r = 16 * rt + c16;
         f32x4 v = y[0][i][rt] + d[0][i][rt];
         if (GLU) {
           const f32x4 up = y[NS - 1][i][rt] + d[NS - 1][i][rt];
 #pragma unroll
           for (int j = 0; j < 4; ++j) v[j] = v[j] / (1.0f + expf(-v[j])) * up[j];
         }
+        d[0][i][rt] = v;
+      }
+    const int at = n0;
+    n0 = next;
+    if (n0 < n1) load_y(n0);  // (before the stores, whose ends a wait for it would include)
+#pragma unroll
+    for (int i = 0; i < TN; ++i)
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) {
+        const int n = at + 16 * i + 4 * g, r = 16 * rt + c16;
+        const f32x4 v = d[0][i][rt];
         float* p = GLU ? a.out + (size_t)(t.row + r) * a.ldo + n : segs.s[seg].y + (size_t)(t.row + r) * segs.s[seg].ldy + n;
         if (r < t.n) {
           if (n + 3 < n1) {
@@ -399,8 +409,6 @@ __global__ void __launch_bounds__(kThreads, 2) lora_expand_kernel(btf_lora a, Se
           }
         }
       }
-    if (next < n1) load_y(next);
-    n0 = next;
   }
 }
 
