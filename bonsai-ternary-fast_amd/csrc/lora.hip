@@ -33,6 +33,10 @@ constexpr int kWaves = kThreads / 64;
 constexpr int kBlockK = 64;       // columns of a wave's step
 constexpr int kGroups = 512;      // workgroups that a launch is cut into, at least
 constexpr int kChunk = 256;       // outputs of a workgroup, or a multiple
+// Workgroups below which the ranks (of few rows) and the outputs are cut further: 8 rows of five requests, ranks of 128, 547 + 2 * 109
+// outputs 26.8 us, with the ranks cut 21.2, with both 13.7; 26 rows, gate and up of 684 21.8, 20.7, 15.9; 60 rows of one request,
+// ranks of 16 14.4 and 12.5.
+constexpr int kSplit = 512;
 
 struct Segs {
   btf_lora_seg s[3];
@@ -450,7 +454,7 @@ constexpr int kOneGroups = 256, kOneValues = 160 * 1024;
 // R rows by the adapter's ranks, columns k0 .. end - 1: the workgroup's W waves share the ranks by eights; where there are
 // fewer than W of these, several waves share one by steps of K and join in LDS. store(rank, row, sum) by some lane.
 template <bool BF, int R, int W, class Store>
-__device__ __forceinline__ void shrink_few(const btf_lora& a, const btf_lora_seg& s, const Tile& t, int k0, int end,
+__device__ __forceinline__ void shrink_few(const btf_lora& a, const btf_lora_seg& s, const Tile& t, int k0, int end, int part, int parts,
                                            float (&sh)[W][R][kFewRanks], const Store& store) {
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int all = (t.rank + kFewRanks - 1) / kFewRanks;
@@ -462,7 +466,7 @@ __device__ __forceinline__ void shrink_few(const btf_lora& a, const btf_lora_seg
     int g0, kb;
   };
   const int kb0 = k0 + w % share * kFewK;
-  auto next_of = [&](Step p) { return p.kb + share * kFewK < end ? Step{p.g0, p.kb + share * kFewK} : Step{p.g0 + groups, kb0}; };
+  auto next_of = [&](Step p) { return p.kb + share * kFewK < end ? Step{p.g0, p.kb + share * kFewK} : Step{p.g0 + parts * groups, kb0}; };
   auto ranks_of = [&](int g0) { return min(t.rank - (g0 + w / share) * kFewRanks, kFewRanks); };
   u32x4 av[kFewRanks];
   f32x4 xv[R][2];
@@ -484,7 +488,8 @@ __device__ __forceinline__ void shrink_few(const btf_lora& a, const btf_lora_seg
         if (in && r < t.n) xv[r][u] = reinterpret_cast<const f32x4*>(x + (size_t)r * a.ldx)[2 * lane + u];
       }
   };
-  Step at{0, kb0};
+  Step at{part * groups, kb0};
+  if (at.g0 >= all) return;  // the whole workgroup
   load(at);
   float acc[kFewRanks][R] = {};
   while (at.g0 < all) {
@@ -528,14 +533,15 @@ __device__ __forceinline__ void shrink_few(const btf_lora& a, const btf_lora_seg
   }
 }
 
-// grid: (tile, slice of K), segment.
+// grid: (tile, slice of K), (segment, one of `parts` shares of the ranks).
 template <bool BF, int R>
-__global__ void __launch_bounds__(kThreads, 2) lora_shrink_few_kernel(btf_lora a, Segs segs, int nseg, int slices, int slice) {
+__global__ void __launch_bounds__(kThreads, 2)
+    lora_shrink_few_kernel(btf_lora a, Segs segs, int nseg, int slices, int slice, int parts) {
   __shared__ float sh[kWaves][R][kFewRanks];
   Tile t;
-  const int k = blockIdx.x % slices, seg = blockIdx.y;
+  const int k = blockIdx.x % slices, seg = blockIdx.y / parts;
   if (!find<R>(a, blockIdx.x / slices, t) || t.rank == 0) return;  // the whole workgroup
-  shrink_few<BF, R, kWaves>(a, segs.s[seg], t, k * slice, min(a.K, (k + 1) * slice), sh,
+  shrink_few<BF, R, kWaves>(a, segs.s[seg], t, k * slice, min(a.K, (k + 1) * slice), blockIdx.y % parts, parts, sh,
                             [&](int q, int r, float v) { h_of(a, nseg, k, seg, t.row + r)[q] = v; });
 }
 
@@ -591,7 +597,7 @@ __global__ void __launch_bounds__(ONE ? 64 * kOneWaves : kThreads, ONE ? 1 : 2)
 #pragma unroll 1
       for (int sg = 0; sg < NS; ++sg) {
         const btf_lora_seg& s = segs.s[GLU ? sg : seg];
-        shrink_few<BF, R, W>(a, s, t, 0, a.K, sh, [&](int q, int r, float v) { sh_h[sg][r][q] = v * scale; });
+        shrink_few<BF, R, W>(a, s, t, 0, a.K, 0, 1, sh, [&](int q, int r, float v) { sh_h[sg][r][q] = v * scale; });
       }
   } else {
     // Several threads share a sum over the slices: slice k goes to thread k % share.
@@ -726,8 +732,13 @@ int lora_go(const btf_lora& a, const Segs& segs, int nseg, hipStream_t st) {
   for (int i = 0; i < (glu ? 1 : nseg); ++i) outs += segs.s[i].N;
   int chunk = kChunk;
   while (chunk < 4 * kChunk && (int64_t)tiles * (outs / (2 * chunk)) >= kGroups) chunk *= 2;
-  int chunks = 0;
-  for (int i = 0; i < (glu ? 1 : nseg); ++i) chunks += (segs.s[i].N + chunk - 1) / chunk;
+  auto chunks_of = [&](int chunk) {
+    int n = 0;
+    for (int i = 0; i < (glu ? 1 : nseg); ++i) n += (segs.s[i].N + chunk - 1) / chunk;
+    return n;
+  };
+  while (chunk > 64 && (int64_t)tiles * chunks_of(chunk) < kSplit) chunk /= 2;
+  const int chunks = chunks_of(chunk);
   const size_t lds = (size_t)(glu ? 2 : 1) * 3 * R * parts_ld(a.rank) * 2;
   const dim3 eg((unsigned)tiles * chunks);
   auto expand = [&](auto kernel) { hipLaunchKernelGGL(kernel, eg, blk, lds, st, a, segs, nseg, slices, chunk, chunks); };
@@ -748,7 +759,7 @@ int lora_few(const btf_lora& a, const Segs& segs, int nseg, hipStream_t st) {
     for (int i = 0; i < (glu ? 1 : nseg); ++i) n += (segs.s[i].N + chunk - 1) / chunk;
     return n;
   };
-  const int chunks = chunks_of(chunk);
+  int chunks = chunks_of(chunk);
   if (R == 1 && (int64_t)tiles * chunks <= kOneGroups && (int64_t)a.rank * a.K * (glu ? 2 : 1) <= kOneValues) {
     const dim3 grid((unsigned)tiles * chunks), blk(64 * kOneWaves);
     if (glu) hipLaunchKernelGGL((lora_expand_few_kernel<BF, 1, true, true>), grid, blk, 0, st, a, segs, nseg, 1, chunk, chunks);
@@ -758,9 +769,14 @@ int lora_few(const btf_lora& a, const Segs& segs, int nseg, hipStream_t st) {
   const int together = a.rank > 2 * kFewRanks ? 1 : a.rank > kFewRanks ? 2 : 4;  // waves that share ranks
   const Slices sl = slices_of(a, nseg, kFewGroups, (int64_t)tiles * nseg, kFewK * together);
   const int slices = sl.n, slice = sl.columns;
-  hipLaunchKernelGGL((lora_shrink_few_kernel<BF, R>), dim3((unsigned)tiles * slices, nseg), dim3(kThreads), 0, st, a, segs, nseg, slices, slice);
+  int parts = 1;  // as many as give each wave its eights of ranks, where there are few workgroups
+  while (parts * 4 * kFewRanks < a.rank && (int64_t)tiles * slices * nseg * parts < kSplit) parts *= 2;
+  hipLaunchKernelGGL((lora_shrink_few_kernel<BF, R>), dim3((unsigned)tiles * slices, nseg * parts), dim3(kThreads), 0, st, a, segs, nseg, slices, slice,
+                     parts);
   const int rc = launch_status("lora_shrink_few_kernel");
   if (rc != BTF_OK) return rc;
+  while (chunk > 64 && (int64_t)tiles * chunks_of(chunk) < kSplit / 2) chunk /= 2;
+  chunks = chunks_of(chunk);
   const dim3 grid((unsigned)tiles * chunks);
   if (glu) hipLaunchKernelGGL((lora_expand_few_kernel<BF, R, true, false>), grid, dim3(kThreads), 0, st, a, segs, nseg, slices, chunk, chunks);
   else hipLaunchKernelGGL((lora_expand_few_kernel<BF, R, false, false>), grid, dim3(kThreads), 0, st, a, segs, nseg, slices, chunk, chunks);

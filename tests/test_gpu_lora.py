@@ -126,7 +126,8 @@ class Case:
 SIZES = [  # rows of each request, K, outputs, rank
     ([1], 512, [64], 16), ([1], 32, [1], 8), ([1, 1, 1, 1, 1], 5120, [512], 16), ([2, 0, 5, 16, 17], 1056, [100], 24),
     ([1] * 70, 544, [33], 8), ([100], 2048, [300], 64), ([65, 130, 1], 512, [257], 40), ([40, 3, 0, 0, 90], 96, [16], 128),
-    ([33], 17408, [64], 32), ([20, 20], 640, [700], 256), ([300], 256, [1100], 16)]
+    ([33], 17408, [64], 32), ([20, 20], 640, [700], 256), ([300], 256, [1100], 16), ([2, 1, 3], 2880, [547], 128), ([4, 0, 3], 1056, [65], 256),
+    ([12], 5120, [225], 128)]
 
 
 @pytest.mark.parametrize("kind", ["f16", "bf16"])
