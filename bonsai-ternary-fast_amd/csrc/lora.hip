@@ -260,7 +260,7 @@ __host__ __device__ constexpr int parts_ld(int rank) { return (rank + 31) / 32 *
 template <bool BF, int RT, bool GLU>
 __global__ void __launch_bounds__(kThreads, 2) lora_expand_kernel(btf_lora a, Segs segs, int nseg, int slices, int chunk, int chunks) {
   constexpr int R = 16 * RT, NS = GLU ? 2 : 1;
-  constexpr int TN = GLU && RT > 1 ? 1 : GLU || RT > 1 ? 2 : 4;  // tiles of 16 outputs of a wave at a time
+  constexpr int TN = GLU && RT > 2 ? 1 : GLU || RT > 1 ? 2 : 4;  // tiles of 16 outputs of a wave at a time
   extern __shared__ uint16_t sh_h[];         // [segment][part][row][parts_ld]
   Tile t;
   if (!find<R>(a, blockIdx.x / chunks, t) || (!GLU && t.rank == 0)) return;  // the whole workgroup
@@ -676,13 +676,6 @@ __global__ void __launch_bounds__(ONE ? 64 * kOneWaves : kThreads, ONE ? 1 : 2)
   }
 }
 
-// Rows of a tile: 64 where A and B are worth reading less often, from ranks above 32 and 1024 rows on (ranks of 64, K 17408, N
-// 5120, 8000 rows 183 us, in tiles of 16 228; ranks of 128, three segments, 2048 rows 127 and 150; 16 ranks of three segments,
-// 2048 rows 64 and 58; 1000 rows are alike), as far as requests are long and the parts of h fit 64 KB of LDS.
-int tile_rows(int S, int T, int rank, int together) {
-  return (int64_t)T > 16 * (int64_t)S && T >= 1024 && rank > 32 && rank * together <= 128 ? 64 : 16;
-}
-
 // Tiles of the requests' rows, at most: a request's last one may be a part of one.
 int most_tiles(const btf_lora& a, int R) { return a.T / R + a.S < a.T ? a.T / R + a.S : a.T; }
 
@@ -707,12 +700,11 @@ Slices slices_of(const btf_lora& a, int nseg, int groups, int64_t each, int step
 }
 
 template <bool BF, int RT>
-int lora_go(const btf_lora& a, const Segs& segs, int nseg, hipStream_t st) {
-  constexpr int R = 16 * RT;
-  const int tiles = most_tiles(a, R);
+int lora_shrink(const btf_lora& a, const Segs& segs, int nseg, int& slices, hipStream_t st) {
+  const int tiles = most_tiles(a, 16 * RT);
   const int all = nseg * ((a.rank + 15) / 16), nt = all <= 2 ? all : 4, groups = (all + nt - 1) / nt;
   const Slices sl = slices_of(a, nseg, kGroups, (int64_t)tiles * groups, kBlockK * kWaves);
-  int slices = sl.n;
+  slices = sl.n;
   const int slice = sl.columns;
   const dim3 grid((unsigned)tiles * slices, groups), blk(kThreads);
   if (nt == 1) hipLaunchKernelGGL((lora_shrink_kernel<BF, RT, 1>), grid, blk, 0, st, a, segs, nseg, slices, slice);
@@ -727,6 +719,13 @@ int lora_go(const btf_lora& a, const Segs& segs, int nseg, hipStream_t st) {
     if (rc != BTF_OK) return rc;
     slices = 1;
   }
+  return BTF_OK;
+}
+
+template <bool BF, int RT>
+int lora_expand(const btf_lora& a, const Segs& segs, int nseg, int slices, hipStream_t st) {
+  constexpr int R = 16 * RT;
+  const int tiles = most_tiles(a, R);
   const bool glu = a.mode == BTF_GEMV_SWIGLU;
   int outs = 0;
   for (int i = 0; i < (glu ? 1 : nseg); ++i) outs += segs.s[i].N;
@@ -740,7 +739,7 @@ int lora_go(const btf_lora& a, const Segs& segs, int nseg, hipStream_t st) {
   while (chunk > 64 && (int64_t)tiles * chunks_of(chunk) < kSplit) chunk /= 2;
   const int chunks = chunks_of(chunk);
   const size_t lds = (size_t)(glu ? 2 : 1) * 3 * R * parts_ld(a.rank) * 2;
-  const dim3 eg((unsigned)tiles * chunks);
+  const dim3 eg((unsigned)tiles * chunks), blk(kThreads);
   auto expand = [&](auto kernel) { hipLaunchKernelGGL(kernel, eg, blk, lds, st, a, segs, nseg, slices, chunk, chunks); };
   if (glu) expand(lora_expand_kernel<BF, RT, true>);
   else expand(lora_expand_kernel<BF, RT, false>);
@@ -787,8 +786,18 @@ template <bool BF>
 int lora_any(const btf_lora& a, const Segs& segs, int nseg, hipStream_t st) {
   if (a.T <= a.S) return lora_few<BF, 1>(a, segs, nseg, st);
   if (a.T <= 4 * (int64_t)a.S) return lora_few<BF, 4>(a, segs, nseg, st);
-  if (tile_rows(a.S, a.T, a.rank, a.mode == BTF_GEMV_SWIGLU ? 2 : 1) == 64) return lora_go<BF, 4>(a, segs, nseg, st);
-  return lora_go<BF, 1>(a, segs, nseg, st);
+  // Rows of a tile: 64 where A and B are worth reading less often, from ranks above 32 and 1024 rows on (ranks of 64, K 17408, N
+  // 5120, 8000 rows 183 us, in tiles of 16 228; ranks of 128, three segments, 2048 rows 127 and 150; 16 ranks of three segments,
+  // 2048 rows 64 and 58; 1000 rows are alike), as far as requests are long and, for B, as the parts of h fit 64 KB of LDS, or half
+  // of the rows do (ranks of 128, gate and up of 17408, 5000 rows in tiles of 32 474 us, of 16 556).
+  const bool large = (int64_t)a.T > 16 * (int64_t)a.S && a.T >= 1024 && a.rank > 32;
+  const int ranks = a.rank * (a.mode == BTF_GEMV_SWIGLU ? 2 : 1), b_rows = !large ? 16 : ranks <= 128 ? 64 : ranks <= 256 ? 32 : 16;
+  int slices;
+  const int rc = large ? lora_shrink<BF, 4>(a, segs, nseg, slices, st) : lora_shrink<BF, 1>(a, segs, nseg, slices, st);
+  if (rc != BTF_OK) return rc;
+  return b_rows == 64   ? lora_expand<BF, 4>(a, segs, nseg, slices, st)
+         : b_rows == 32 ? lora_expand<BF, 2>(a, segs, nseg, slices, st)
+                        : lora_expand<BF, 1>(a, segs, nseg, slices, st);
 }
 
 }  // namespace

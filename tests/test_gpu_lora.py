@@ -127,7 +127,7 @@ SIZES = [  # rows of each request, K, outputs, rank
     ([1], 512, [64], 16), ([1], 32, [1], 8), ([1, 1, 1, 1, 1], 5120, [512], 16), ([2, 0, 5, 16, 17], 1056, [100], 24),
     ([1] * 70, 544, [33], 8), ([100], 2048, [300], 64), ([65, 130, 1], 512, [257], 40), ([40, 3, 0, 0, 90], 96, [16], 128),
     ([33], 17408, [64], 32), ([20, 20], 640, [700], 256), ([300], 256, [1100], 16), ([2, 1, 3], 2880, [547], 128), ([4, 0, 3], 1056, [65], 256),
-    ([12], 5120, [225], 128)]
+    ([12], 5120, [225], 128), ([700, 500], 96, [130], 200), ([1100], 544, [65, 8], 72)]
 
 
 @pytest.mark.parametrize("kind", ["f16", "bf16"])
@@ -139,7 +139,7 @@ def test_add(hip, new, K, Ns, rank, kind):
 
 @pytest.mark.parametrize("kind", ["f16", "bf16"])
 @pytest.mark.parametrize("new,K,N,rank", [([1], 512, 64, 16), ([1, 2, 1], 1024, 1000, 32), ([64, 7], 512, 333, 64), ([70], 256, 128, 128),
-                                          ([1] * 9, 5120, 200, 200)], ids=str)
+                                          ([1] * 9, 5120, 200, 200), ([1100], 96, 70, 128), ([600, 500], 64, 33, 256), ([1100], 288, 130, 40)], ids=str)
 @pytest.mark.parametrize("into_gate", [False, True])
 def test_swiglu(hip, new, K, N, rank, kind, into_gate):
     c = Case(new, K, [N, N], kind, rank, seed=2)
