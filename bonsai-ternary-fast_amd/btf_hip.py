@@ -98,7 +98,7 @@ class _PagePlan(C.Structure):
                 ("ctx", C.c_void_p), ("n_new", C.c_void_p), ("held", C.c_void_p), ("parent", C.c_void_p),
                 ("free_list", C.c_void_p), ("n_free", C.c_void_p), ("table", C.c_void_p), ("held_out", C.c_void_p),
                 ("n_free_out", C.c_void_p), ("row0", C.c_void_p), ("kv_len", C.c_void_p), ("pos", C.c_void_p),
-                ("slot", C.c_void_p), ("tree", C.c_void_p)]
+                ("slot", C.c_void_p), ("tree", C.c_void_p), ("shared", C.c_void_p)]
 
 
 class _RopeScale(C.Structure):
@@ -449,6 +449,7 @@ class PagePlan:
     pos: object = None         # i32 [T]
     slot: object = None        # i32 [T]
     tree: object = None        # i64 [T] or None
+    shared: object = None      # i32 [pages] or None
 
     def _c(self):
         return _struct(self, _PagePlan)

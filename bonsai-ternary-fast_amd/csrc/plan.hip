@@ -39,6 +39,18 @@ struct Chunk {
   int ctx[kPlanThreads];        // its tokens in the cache; -1: refused
 };
 
+// Whether a page of request s that others hold, too, would take one of its new tokens ctx .. ctx + n - 1 (n > 0; it holds h
+// pages): a request that was cut back to the middle of a page. One page to look at, unless it holds more than its tokens need.
+__device__ __forceinline__ bool into_shared(const btf_page_plan& a, int s, long long ctx, long long n, long long h) {
+  const int sh = __builtin_ctz(a.page);
+  const int end = (int)min(h, ((ctx + n - 1) >> sh) + 1);
+  for (int j = (int)(ctx >> sh); j < end; ++j) {
+    const int pg = a.table[(size_t)s * a.ldt + j];
+    if (pg >= 0 && pg < a.pages && a.shared[pg] > 0) return true;
+  }
+  return false;
+}
+
 __device__ __forceinline__ void plan_requests(const btf_page_plan& a, Chunk& c, long long free0) {
   long long rows = 0, pages = 0, taken = 0;
   for (int s0 = 0; s0 < a.S; s0 += kPlanThreads) {
@@ -53,8 +65,9 @@ __device__ __forceinline__ void plan_requests(const btf_page_plan& a, Chunk& c, 
     if (live) a.row0[s] = row0;
     rows += (long long)all;
     const long long total = (ctx + nn + a.page - 1) / a.page;
-    const bool sound = live && ctx >= 0 && nn >= 0 && h >= 0 && h <= a.ldt && ctx <= h * a.page && end <= a.T &&
-                       total <= a.ldt && ctx + nn <= 0x7fffffffll;
+    bool sound = live && ctx >= 0 && nn >= 0 && h >= 0 && h <= a.ldt && ctx <= h * a.page && end <= a.T &&
+                 total <= a.ldt && ctx + nn <= 0x7fffffffll;
+    if (a.shared && sound && nn > 0) sound = !into_shared(a, s, ctx, nn, h);
     const long long want = sound ? max(total - h, 0ll) : 0;
     const long long upto = pages + (long long)block_scan<kPlanThreads>(want, c.part, &all);
     // (the served needs are the first ones: their sums are those of all needs)

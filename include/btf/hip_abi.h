@@ -444,7 +444,10 @@ typedef struct btf_kv_cache {
  *    order's first page is free_list[*n_free - 1]. A request is refused if a
  *    length is negative or passes 2^31, ctx[s] > held[s] * page, its rows pass
  *    T, its pages pass ldt, or the free pages do not reach for it and those before it (then every
- *    later request that needs a page is refused too). A refused request gets no
+ *    later request that needs a page is refused too), or, with `shared` (the counts
+ *    of launch_page_fork), if a page that it holds and its new tokens would go to has
+ *    another holder, which would then read them: such a request stays refused until it
+ *    has that page for itself (launch_page_free). A refused request gets no
  *    page, kv_len 0, and its rows position 0, slot -1 and tree 0, with which
  *    the launches below neither write the cache for it nor read it.
  *  - kv_len[s] = ctx[s] + n_new[s]; held_out, n_free_out: held and *n_free
@@ -476,6 +479,7 @@ typedef struct btf_page_plan {
   int* pos;              /* [T] */
   int* slot;             /* [T] */
   uint64_t* tree;        /* [T] or NULL (with parent) */
+  const int* shared;     /* [pages] or NULL: no page has two holders */
 } btf_page_plan;
 int btf_hip_launch_page_plan(const btf_page_plan* a, btf_stream_t stream);
 
@@ -597,8 +601,10 @@ int btf_hip_launch_sample(const btf_sampling* a, btf_stream_t stream);
  * Samples of one prompt, beams and requests behind one long instruction hold the
  * same cache pages. shared[p] counts the holders of page p beyond one: 0 for a
  * page that one request holds and for a free page, so launch_page_plan, which
- * knows nothing of it, hands out pages that are counted right. A shared page is
- * full and is not written again: a request writes behind its last token only.
+ * changes no count, hands out pages that are counted right. A shared page is full for
+ * all who hold it and is not written again, as a request writes behind its last token
+ * only. A request that is cut back to a token inside of one would write it:
+ * launch_page_plan with `shared` refuses it (see launch_page_free).
  * All lengths and ids are device data, as above. */
 
 /* Request rows of `table` that begin as copies of others: fork f makes row dst[f]
@@ -654,7 +660,12 @@ int btf_hip_launch_page_copy(const btf_page_copy* a, const btf_kv_cache* kv, btf
  * all; a request that stays as it is has any number from held[s] * page on): the
  * pages' ids in table become -1, held[s] the pages that stay, a page that others
  * hold loses a count of shared, and a page that nobody holds any more goes to the
- * end of the free list. They go there in the opposite order of their places (a
+ * end of the free list. A page that keep[s] ends in stays the request's, also one that
+ * others hold: behind a token inside of such a page it cannot go on
+ * (launch_page_plan with `shared` refuses it). To cut a request back there, fork its
+ * first keep[s] tokens into an empty row, copy (the row then has a page of its own for
+ * the last of them), and give the old row back with keep 0; the new row goes on.
+ * Pages go to the list in the opposite order of their places (a
  * page that several rows give up: at its first), so that giving back what a plan
  * or forks have just handed out leaves the list as it was. shared NULL: no page
  * has two holders. held[s] is taken as at most ldt; ids that are not in [0, pages)
