@@ -657,7 +657,8 @@ typedef struct btf_page_copy {
 int btf_hip_launch_page_copy(const btf_page_copy* a, const btf_kv_cache* kv, btf_stream_t stream);
 
 /* Gives back what the requests hold behind their first keep[s] tokens (0 or less:
- * all; a request that stays as it is has any number from held[s] * page on): the
+ * all; a request that stays as it is has any number from held[s] * page on; one that
+ * launch_page_plan refused keeps its ctx[s], its kv_len is 0): the
  * pages' ids in table become -1, held[s] the pages that stay, a page that others
  * hold loses a count of shared, and a page that nobody holds any more goes to the
  * end of the free list. A page that keep[s] ends in stays the request's, also one that
@@ -692,7 +693,8 @@ int btf_hip_launch_page_free(const btf_page_free* a, btf_stream_t stream);
  * (optional) = first[s] + their number. Which are kept:
  *  - tree and leaf: those whose bit tree[leaf[s]] has (the row leaf[s] of the step
  *    and its ancestors, as launch_page_plan gives them; a leaf not in [0, T): none),
- *    bit j being place first[s] + j: the accepted path of a drafted tree;
+ *    bit j being place first[s] + j: the accepted path of a drafted tree. (The rows of
+ *    a prompt and of a refused request have no bits: kv_len[s] = first[s], nothing moves.)
  *  - source and source0: the places source[source0[s]] .. source[source0[s+1] - 1]
  *    (as far as there are T), a cache that drops tokens.
  * Places are looked up in the rows of table, where they go to in those of to_table;

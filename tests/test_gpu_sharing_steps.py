@@ -1,5 +1,5 @@
 """GPU tests of what a serving loop over shared pages must not lose (include/btf/hip_abi.h, requests that share): a request
-cut back inside a page that others hold."""
+cut back inside a page that others hold, the pages of a request that the free list did not reach for."""
 import numpy as np
 import pytest
 
@@ -95,3 +95,87 @@ def test_a_request_cut_back_inside_a_shared_page(hip, kind):
                 want = rows[j - n] if j >= n else old[table[0, j // page], :, j % page]
                 np.testing.assert_array_equal(x[t[s, j // page], :, j % page], want)
     assert counts[t[0, 0]] == 1 and counts.sum() == 1 and ref.pages_of(keep + 3, page) == host(st.held)[2]
+
+
+class Steps:
+    """Plans, cache writes, moves and returns of three requests over a small pool, nothing of it on the host."""
+    S, T, HK, D, page, pages, ldt = 3, 128, 1, 64, 16, 8, 7
+
+    def __init__(self, hip):
+        torch = _torch()
+        self.hip, z = hip, lambda n, t=torch.int32: torch.zeros(n, dtype=t, device="cuda")  # noqa: E731
+        self.k, self.v = (torch.zeros((self.pages, self.HK, self.page, self.D), device="cuda").half() for _ in range(2))
+        self.kv = hip.KvCache(self.k, self.v, hip.CacheType.f16, self.page, self.HK, self.D, self.pages, self.HK * self.page * self.D,
+                              self.page * self.D, self.D)
+        self.table = torch.full((self.S, self.ldt), -1, dtype=torch.int32, device="cuda")
+        self.free, self.n_free, self.held, self.shared = ints(np.arange(self.pages)), ints([self.pages]), z(self.S), z(self.pages)
+        self.ctx, self.row0, self.kv_len, self.stay = z(self.S), z(self.S + 1), z(self.S), z(self.S)
+        self.pos, self.slot, self.tree = z(self.T), z(self.T), z(self.T, torch.int64)
+        self.ws = z(max(1, hip.page_free_ws_bytes(self.S, self.ldt) // 4))
+        self.wrote = 0
+
+    def step(self, n_new, parent=None):
+        """New tokens of values 1, 2, ... (what each request's should be is up to the test)."""
+        hip, HD = self.hip, self.HK * self.D
+        common = dict(S=self.S, page=self.page, ldt=self.ldt, pages=self.pages, table=self.table)
+        hip.launch_page_plan(hip.PagePlan(
+            T=self.T, ctx=self.ctx, n_new=ints(n_new), held=self.held, parent=ints(parent) if parent is not None else None, free=self.free,
+            n_free=self.n_free, held_out=self.held, n_free_out=self.n_free, row0=self.row0, kv_len=self.kv_len, pos=self.pos,
+            slot=self.slot, tree=self.tree if parent is not None else None, shared=self.shared, **common), stream())
+        x = (_torch().arange(self.T, device="cuda") + self.wrote + 1).float()[:, None].repeat(1, HD)
+        self.wrote += sum(n_new)
+        hip.launch_rope_cache(hip.RopeCache(T=self.T, heads=1, k=x, ldk=HD, v=x, ldv=HD, n_rot=2, turns=dev(np.zeros(1)), pos=self.pos,
+                                            slot=self.slot, rows=self.row0[self.S:]), self.kv, stream())
+
+    def give_back(self):
+        hip = self.hip
+        hip.launch_page_free(hip.PageFree(
+            S=self.S, page=self.page, ldt=self.ldt, pages=self.pages, keep=self.stay, table=self.table, held=self.held, shared=self.shared,
+            free=self.free, n_free=self.n_free, ws=self.ws), stream())
+
+    def tokens(self, s, n):
+        t, v = host(self.table), self.v.float().cpu().numpy()
+        return [int(v[t[s, j // self.page], 0, j % self.page, 0]) for j in range(n)]
+
+
+def test_a_refused_request_keeps_its_cache(hip):
+    """Steps without trees, what stays worked out from the plan's lengths and the tokens before: the request that the free
+    pages do not reach for has its tokens when there are pages again."""
+    L = Steps(hip)
+
+    def behind(ended=()):
+        L.stay.copy_(_torch().where(L.kv_len > 0, L.kv_len, L.ctx))
+        L.stay[list(ended)] = 0
+        L.give_back()
+        L.ctx.copy_(L.stay)
+
+    L.step([48, 32, 40])  # 3 + 2 + 3 pages: all there are
+    behind()
+    assert host(L.held).tolist() == [3, 2, 3] and host(L.n_free)[0] == 0
+    L.step([0, 1, 1])  # request 1 needs a third page
+    assert host(L.kv_len).tolist() == [48, 0, 41]
+    behind(ended=[0])
+    assert host(L.held).tolist() == [0, 2, 3] and host(L.n_free)[0] == 3 and host(L.ctx).tolist() == [0, 32, 41]
+    assert L.tokens(1, 32) == list(range(49, 81))
+    L.step([0, 1, 0])
+    assert host(L.kv_len).tolist() == [0, 33, 41] and L.tokens(1, 33) == list(range(49, 81)) + [123]
+    assert L.tokens(2, 41) == list(range(81, 121)) + [122]
+
+
+def test_a_refused_request_and_a_prompt_beside_a_tree(hip):
+    """A step with trees: the move leaves the plan's lengths as they are, says ctx for the refused request, and for the
+    prompt of more than 64 rows, whose stay is the program's to set."""
+    L = Steps(hip)
+    L.step([0, 16, 2], np.full(L.T, -1))
+    L.stay.copy_(L.kv_len)
+    L.give_back()
+    L.ctx.copy_(L.stay)
+    L.free[6:], L.n_free[0] = -1, 5  # (one page is somebody else's)
+    L.step([70, 1, 3], np.array([-1] * 72 + [0, 0] + [-1] * 54))  # 5 pages for the prompt, none left for request 1
+    hip.launch_cache_move(hip.CacheMove(S=3, T=L.T, table=L.table, ldt=L.ldt, first=L.ctx, tree=L.tree, leaf=ints([69, 70, 73]),
+                                        kv_len=L.stay), L.kv, stream())
+    assert host(L.kv_len).tolist() == [70, 0, 5] and host(L.stay).tolist() == [0, 16, 4]
+    L.stay[0] = L.kv_len[0]
+    L.give_back()
+    assert host(L.held).tolist() == [5, 1, 1] and host(L.n_free)[0] == 0
+    assert L.tokens(0, 70) == list(range(19, 89)) and L.tokens(1, 16) == list(range(1, 17)) and L.tokens(2, 4) == [17, 18, 90, 92]
