@@ -320,6 +320,25 @@ __global__ void __launch_bounds__(kCopyThreads) page_copy_kernel(btf_page_copy a
 }
 
 // ---- move ----
+// The kept tokens of request s: in a tree's bits, or list entries from `lo` on.
+struct Kept {
+  unsigned long long bits;
+  int lo, n;
+};
+template <bool TREE>
+__device__ __forceinline__ Kept kept_of(const btf_cache_move& a, int s) {
+  Kept k{0, 0, 0};
+  if (TREE) {
+    const int leaf = a.leaf[s];
+    if (leaf >= 0 && leaf < a.T) k.bits = a.tree[leaf];
+    k.n = __popcll(k.bits);
+  } else {
+    k.lo = min(max(a.source0[s], 0), a.T);
+    k.n = max(min(max(a.source0[s + 1], 0), a.T) - k.lo, 0);
+  }
+  return k;
+}
+
 // In place a token's new place may be another's old one, but never that of a later
 // token of the list (places ascend, none goes up). A workgroup has one run (32 to 128 bytes) of
 // the values of one (request, K or V, head, layer) for all tokens: it reads a batch,
@@ -336,16 +355,9 @@ __global__ void __launch_bounds__(N) cache_move_kernel(btf_cache_move a, btf_kv_
   id /= kv.heads;
   const int s = id >> 1;
   const int first = a.first[s];
-  unsigned long long bits = 0;
-  int lo = 0, n;
-  if (TREE) {
-    const int leaf = a.leaf[s];
-    if (leaf >= 0 && leaf < a.T) bits = a.tree[leaf];
-    n = __popcll(bits);
-  } else {
-    lo = min(max(a.source0[s], 0), a.T);
-    n = max(min(max(a.source0[s + 1], 0), a.T) - lo, 0);
-  }
+  const Kept kept = kept_of<TREE>(a, s);
+  const unsigned long long bits = kept.bits;
+  const int lo = kept.lo, n = kept.n;
   if (blockIdx.y == 0 && run == 0 && h == 0 && !(id & 1) && threadIdx.x == 0 && a.kv_len) a.kv_len[s] = first + n;
   uint16_t* base = static_cast<uint16_t*>(id & 1 ? kv.v : kv.k) + (size_t)blockIdx.y * a.layer_stride +
                    (size_t)h * kv.head_stride + 8 * (L * run + (threadIdx.x & (L - 1)));
@@ -420,6 +432,13 @@ __global__ void __launch_bounds__(N) cache_move_kernel(btf_cache_move a, btf_kv_
     }
 }
 
+// kv_len alone.
+template <bool TREE>
+__global__ void __launch_bounds__(256) cache_move_len_kernel(btf_cache_move a) {
+  const int s = blockIdx.x * 256 + threadIdx.x;
+  if (s < a.S) a.kv_len[s] = a.first[s] + kept_of<TREE>(a, s).n;
+}
+
 int free_chunks(int S, int ldt) { return (int)(((int64_t)S * ldt + kFreeChunk - 1) / kFreeChunk); }
 
 }  // namespace
@@ -470,7 +489,10 @@ int page_copy(const btf_page_copy& a, const btf_kv_cache& kv, hipStream_t st) {
   return launch_status("page_copy_kernel");
 }
 
-int cache_move(const btf_cache_move& a, const btf_kv_cache& kv, hipStream_t st) {
+int cache_move(const btf_cache_move& args, const btf_kv_cache& kv, hipStream_t st) {
+  btf_cache_move a = args;
+  const bool behind = a.kv_len == a.first;  // (the lengths are written when all workgroups have read what they were)
+  if (behind) a.kv_len = nullptr;
   const int groups = 2 * a.S * kv.heads * (kv.dim / 64);
   // A tree's path in batches of 16 tokens. A list in batches of 256 with as many threads as there are: 8 requests of up to
   // 16384 tokens, half of which stay, 2 layers, 187 us (3.9 TB/s read and written) with 1024 threads, 247 with 512, 278 with 256.
@@ -483,7 +505,12 @@ int cache_move(const btf_cache_move& a, const btf_kv_cache& kv, hipStream_t st) 
   else if (all <= 48) go(cache_move_kernel<1024, false, 2>, 4);
   else if (all <= 128) go(cache_move_kernel<1024, false, 4>, 2);
   else go(cache_move_kernel<1024, false, 8>, 1);
-  return launch_status("cache_move_kernel");
+  const int rc = launch_status("cache_move_kernel");
+  if (rc != BTF_OK || !behind) return rc;
+  const dim3 grid((a.S + 255) / 256), blk(256);
+  if (a.tree) hipLaunchKernelGGL(cache_move_len_kernel<true>, grid, blk, 0, st, args);
+  else hipLaunchKernelGGL(cache_move_len_kernel<false>, grid, blk, 0, st, args);
+  return launch_status("cache_move_len_kernel");
 }
 
 }  // namespace btfhip

@@ -690,7 +690,7 @@ int btf_hip_launch_page_free(const btf_page_free* a, btf_stream_t stream);
 
 /* Tokens that stay are moved together, K and V, in every layer (as page_copy): the
  * i-th kept token of request s goes to place first[s] + i, and kv_len[s]
- * (optional) = first[s] + their number. Which are kept:
+ * (optional; it may be `first` itself) = first[s] + their number. Which are kept:
  *  - tree and leaf: those whose bit tree[leaf[s]] has (the row leaf[s] of the step
  *    and its ancestors, as launch_page_plan gives them; a leaf not in [0, T): none),
  *    bit j being place first[s] + j: the accepted path of a drafted tree. (The rows of
@@ -715,7 +715,7 @@ typedef struct btf_cache_move {
   const int* leaf;        /* [S] with tree */
   const int* source;      /* [T] or NULL */
   const int* source0;     /* [S + 1] with source */
-  int* kv_len;            /* [S] or NULL */
+  int* kv_len;            /* [S] or NULL, may be first */
   int layers;             /* 1 .. 65535 */
   int64_t layer_stride;   /* values, a multiple of 8 (layers > 1) */
 } btf_cache_move;

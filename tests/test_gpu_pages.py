@@ -263,6 +263,49 @@ def test_move_accepted_paths(hip, HK, D, page, L, kind):
         np.testing.assert_array_equal(host(x.view(torch.int16)), w)
 
 
+@pytest.mark.parametrize("how", ["tree", "few", "some", "many"])  # lists: in runs of 32, 64, 128 bytes
+def test_move_with_lengths_in_place(hip, how):
+    """kv_len is `first` itself: every workgroup finds the lengths as they were, also in a graph's replays."""
+    torch = _torch()
+    rng = np.random.default_rng(len(how))
+    HK, D, page, L, S = {"tree": (8, 128, 16, 4, 40), "few": (1, 64, 16, 3, 5), "some": (1, 128, 16, 3, 8), "many": (4, 256, 16, 2, 30)}[how]
+    tokens = rng.integers(60, 120, S) + 64
+    table, *_, pages = pool(rng, tokens, S, page, 2)
+    first = [int(n) - 64 for n in tokens]
+    kv, old = caches(rng, "f16", L, pages, HK, page, D)
+    want_first = [int(rng.integers(0, f + 1)) for f in first]
+    if how == "tree":
+        want_first = first
+        tree = np.array([int(x) for x in rng.integers(0, 2 ** 63, S)], np.uint64)
+        lists = [[f + j for j in range(64) if int(b) >> j & 1] for f, b in zip(first, tree)]
+        what = dict(T=S, tree=torch.from_numpy(tree.view(np.int64)).cuda(), leaf=ints(np.arange(S)))
+    else:
+        lists = [sorted(rng.choice(np.arange(f, n), int((n - f) * 0.7), replace=False)) for f, n in zip(want_first, tokens)]
+        flat = np.concatenate(lists)
+        what = dict(T=len(flat), source=ints(flat), source0=ints(np.cumsum([0] + [len(x) for x in lists])))
+    lens, start = ints(want_first), ints(want_first)
+    a = hip.CacheMove(S=S, table=ints(table), ldt=table.shape[1], first=lens, kv_len=lens, layers=L, layer_stride=pages * HK * page * D, **what)
+    cache = cache_of(hip, kv, "f16", HK, page, D, pages)
+    want, fresh = ref.move(*old, table, None, want_first, lists, page), [x.clone() for x in kv]
+
+    def check():
+        np.testing.assert_array_equal(host(lens), [f + len(x) for f, x in zip(want_first, lists)])
+        for x, w in zip(kv, want):
+            np.testing.assert_array_equal(host(x.view(torch.int16)), w)
+    hip.launch_cache_move(a, cache, stream())
+    check()
+    g = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(g, stream=torch.cuda.Stream()):
+        hip.launch_cache_move(a, cache, torch.cuda.current_stream().cuda_stream)
+    for _ in range(3):
+        lens.copy_(start)
+        for x, f in zip(kv, fresh):
+            x.copy_(f)
+        g.replay()
+        check()
+
+
 def test_move_of_places_that_are_none(hip):
     """Places before or behind the table, pages that there are not, row starts out of range: those tokens stay out."""
     torch = _torch()
