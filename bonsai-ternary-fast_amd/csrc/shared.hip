@@ -77,7 +77,7 @@ __device__ __forceinline__ int piece_keys(float groups, float requests, int role
   const float share = (float)kRunning * (groups / (groups + 2.f * requests + 1.f));
   const float items = role ? (float)own : fmaxf(floorf(share), (float)(kRunning / 2));
   const float keys = (role ? requests : groups) * 1.0001f / items;
-  return R > 16 && keys <= (float)kHalf ? kHalf : kStep * (int)fminf(keys / (float)kStep + 1.f, 1e6f);
+  return R > 16 && keys <= (float)kHalf ? kHalf : kStep * (int)fminf(keys / (float)kStep + 1.f, 1.6e7f);  // (below 2^31)
 }
 __device__ __forceinline__ void into_pieces(Found& f, int C) {
   const int keys = max(f.len - f.begin, 0);
