@@ -58,7 +58,7 @@ namespace {
 template <int R, bool BY_ROW, bool SCALAR>
 __device__ bool find(const btf_paged_attention& a, const btf_kv_cache& kv, int id, Req& q) {
   const int lane = threadIdx.x & 63, G = a.heads / kv.heads;
-  const long long cap = (long long)a.ldt * kv.page;
+  const long long cap = min((long long)a.ldt * kv.page, (long long)kMostKeys);
   auto read = [&](int s, int& r0, int& n, int& len, int& full) {
     r0 = n = len = full = 0;
     if (s < a.S) {
@@ -81,7 +81,7 @@ __device__ bool find(const btf_paged_attention& a, const btf_kv_cache& kv, int i
   int items = 0, slots = 0;  // before the chunk
   for (int s0 = 0; s0 < a.S; s0 += 64) {
     if (a.S > 64) read(s0 + lane, r0, n, len, full);  // (up to 64 requests are still there)
-    const int tiles = n > 0 ? (n * G + R - 1) / R : 0, pieces = max(1, (len + C - 1) / C);
+    const int tiles = n > 0 ? (n * G + R - 1) / R : 0, pieces = max(1, (int)((unsigned)(len + C - 1) / (unsigned)C));
     const int mine = kv.heads * tiles * pieces, cut = pieces > 1 ? mine : 0;
     const int upto = wave_scan_i(mine), cuts = wave_scan_i(cut);
     const bool here = BY_ROW ? n > 0 && id >= r0 && id < r0 + n : mine > 0 && id >= items + upto - mine && id < items + upto;

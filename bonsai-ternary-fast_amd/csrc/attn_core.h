@@ -28,6 +28,8 @@ constexpr int target(int R) { return R <= 32 ? 1536 : 1024; }
 // 512 keys).
 constexpr int least(int R) { return R <= 16 ? kStep : 512; }
 constexpr int kPlaces = 512;
+// Keys of a request at most: the loops count some blocks beyond the last key in 32 bits.
+constexpr int kMostKeys = 0x7fffffff & ~8191;
 
 template <bool BF>
 __device__ __forceinline__ float from16(uint16_t h) {
@@ -263,7 +265,7 @@ __device__ __forceinline__ void attn_stream(const btf_paged_attention& a, const 
   // keys: [k0, k1) is the piece, cut behind the last key that any row of the tile sees; all rows see those before `all`
   const int i0 = tile * R / G, i1 = (tile * R + nrows - 1) / G;
   const int kend = tree ? q.len : max(0, min(q.len, q.ctx + i1 + 1));
-  const int k0 = q.begin + piece * q.C, k1 = min(kend, k0 + q.C);
+  const int k0 = q.begin + piece * q.C, k1 = (int)min((unsigned)kend, (unsigned)k0 + (unsigned)q.C);
   const int all = min(kend, tree ? q.ctx : q.ctx + i0 + 1);
 
   // Q^T: row c16 of row tile rt, dims 32 ks + 8 g ..
@@ -518,7 +520,7 @@ __device__ __forceinline__ void attn_tile(const btf_paged_attention& a, const bt
   const float c2 = scale2(a.scale);
   const int i0 = tile * R / G, i1 = (tile * R + nrows - 1) / G;
   const int kend = tree ? q.len : max(0, min(q.len, q.ctx + i1 + 1));
-  const int k0 = q.begin + piece * q.C, k1 = min(kend, k0 + q.C);
+  const int k0 = q.begin + piece * q.C, k1 = (int)min((unsigned)kend, (unsigned)k0 + (unsigned)q.C);
   const int all = min(kend, tree ? q.ctx : q.ctx + i0 + 1);
 
   u32x4 qf[RT][KS];

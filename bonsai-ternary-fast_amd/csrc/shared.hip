@@ -683,7 +683,7 @@ int shared_attention(const btf_shared_attention& a, const btf_kv_cache& kv, hipS
                             a.row0, a.kv_len, a.tree, a.scale, a.out, a.ldo, p.ws.slots};
   p.G = a.heads / kv.heads;
   p.own = kv.dim == 256 && p.R[0] == 16 ? kFewItems : kOwnItems;
-  p.cap = (int64_t)a.ldt * kv.page < 0x7fffffff ? a.ldt * kv.page : 0x7fffffff;
+  p.cap = (int64_t)a.ldt * kv.page < kMostKeys ? a.ldt * kv.page : kMostKeys;
   p.alone = a.groups > kFew ? 0 : a.S <= kFew ? 1 : a.S <= 2 * kFew ? 2 : 0;
   const bool bf = kv.type == BTF_BF16;
   if (kv.dim == 64) return bf ? shared_go<64, true>(p, st) : shared_go<64, false>(p, st);

@@ -558,7 +558,7 @@ typedef struct btf_paged_attention {
   const int* table;      /* [S][ldt] */
   int ldt;
   const int* row0;       /* [S + 1] */
-  const int* kv_len;     /* [S], at most ldt * page is read */
+  const int* kv_len;     /* [S], at most ldt * page, and 2^31 - 8192, is read */
   const uint64_t* tree;  /* [T] or NULL */
   float scale;
   float* out;            /* [T][ldo], 16-byte aligned, ldo % 4 == 0 */

@@ -48,6 +48,22 @@ def run(hip, kv, a, kv_len, shared):
     return host(out).reshape(a["T"], a["heads"], D)
 
 
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("n", [1, 24, 80])
+@pytest.mark.parametrize("shared", [None, 0, 2 ** 30 + 5, 2 ** 31 - 1])
+def test_lengths_at_the_end_of_their_type(hip, kind, n, shared):
+    """The last page read has the keys of score 20. Sums of the others are exact; what is left are
+    a score's rounding (20 / ln 2 in 32 bits: 2^-19), an exponential's and those of the joins, on values up to 3."""
+    kv, a, v = case(hip, kind, 1, 1, 1 if shared is None else 2, n, MOST // PAGE - 1)
+    for kv_len in (MOST, 2 ** 31 - 1):
+        out = run(hip, kv, a, [kv_len] * a["S"], shared)
+        for r in range(a["T"]):
+            last = PAGE - max(0, n - 1 - r % n - (kv_len - MOST))  # keys of the last page that the row sees
+            w = np.concatenate([np.full(PAGE, (MOST - PAGE) / PAGE), np.exp(20.0) * (np.arange(PAGE) < last)])
+            want = (w[:, None] * v[:, 0].reshape(2 * PAGE, D)).sum(0) / w.sum()
+            assert np.all(np.abs(out[r, 0] - want) <= 3 * 2.0 ** -17), (kv_len, r)
+
+
 @pytest.mark.parametrize("shared", [None, 1000])
 def test_pieces_of_many_keys(hip, shared):
     """32 KV heads over 1.9e9 keys: more than 2^27 in a piece. All scores 0."""
