@@ -206,7 +206,8 @@ __global__ void __launch_bounds__(kPlanThreads) shared_plan_small_kernel(Plan p)
 #pragma unroll
   for (int role = 0; role < 2; ++role) v[role] = (uint64_t)(uint32_t)own[role] | (uint64_t)(uint32_t)cut[role] << 32;
   scan2(v, part, all);
-  const int first[2] = {0, (int)all[0]}, behind = (int)(all[0] >> 32);
+  // (row starts that do not ascend can ask for more items than there are)
+  const int first[2] = {0, (int)min((uint32_t)all[0], (uint32_t)p.ws.most)}, behind = (int)(all[0] >> 32);
 #pragma unroll
   for (int role = 0; role < 2; ++role) {
     sh_upto[role][tid] = (int)v[role];
@@ -217,7 +218,7 @@ __global__ void __launch_bounds__(kPlanThreads) shared_plan_small_kernel(Plan p)
       p.ws.found[role ? p.groups + tid : tid] = f[role];
     }
   }
-  if (tid == 0) *p.ws.items = min((int)all[0] + (int)all[1], p.ws.most);
+  if (tid == 0) *p.ws.items = first[1] + (int)min((uint32_t)all[1], (uint32_t)(p.ws.most - first[1]));
   __syncthreads();
 #pragma unroll
   for (int role = 0; role < 2; ++role)
