@@ -222,7 +222,7 @@ __global__ void __launch_bounds__(kPlanThreads) shared_plan_small_kernel(Plan p)
   __syncthreads();
 #pragma unroll
   for (int role = 0; role < 2; ++role)
-    for (int k = tid; k < min((int)all[role], p.ws.most - first[role]); k += kPlanThreads) {
+    for (int k = tid; k < (int)min((uint32_t)all[role], (uint32_t)(p.ws.most - first[role])); k += kPlanThreads) {
       int lo = 0, hi = (role ? a.S : p.groups) - 1;  // the first one with upto > k
       while (lo < hi) {
         const int mid = (lo + hi) >> 1;
