@@ -265,7 +265,7 @@ int btf_hip_launch_lora(const btf_lora* a, const btf_lora_seg* segs, int nseg, b
   if (a->mode != BTF_GEMV_ADD && a->mode != BTF_GEMV_SWIGLU) return bad("lora", "mode must be add or swiglu");
   const bool glu = a->mode == BTF_GEMV_SWIGLU;
   if (glu && (nseg != 2 || segs[0].N != segs[1].N)) return bad("lora", "swiglu takes two segments of the same N");
-  if (a->K < 32 || a->K % 32) return bad("lora", "K must be a positive multiple of 32");
+  if (a->K < 32 || a->K % 32 || a->K > 1 << 24) return bad("lora", "K must be a multiple of 32 in [32, 2^24]");
   if (a->rank < 8 || a->rank % 8 || a->rank > 256) return bad("lora", "rank must be a multiple of 8 up to 256");
   if (a->adapters < 0) return bad("lora", "negative number of adapters");
   if (a->type != BTF_F16 && a->type != BTF_BF16) return bad("lora", "unknown type");

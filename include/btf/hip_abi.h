@@ -782,7 +782,7 @@ typedef struct btf_lora_seg {
 } btf_lora_seg;
 typedef struct btf_lora {
   int S, T;              /* requests, rows (below 2^24) */
-  int K;                 /* a multiple of 32 */
+  int K;                 /* a multiple of 32 up to 2^24 */
   int rank;              /* ranks that a and b have room for: a multiple of 8 up to 256 */
   int adapters;
   int type;              /* BTF_F16 or BTF_BF16 */

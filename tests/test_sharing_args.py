@@ -99,6 +99,14 @@ def test_more_workgroups_than_a_launch_takes():
         assert h.launch_lora_raw(dataclasses.replace(LORA, S=S, T=T), [wide], 1) == code
 
 
+@pytest.mark.parametrize("op,change,code", [
+    ("lora", dict(K=1 << 24, ldx=1 << 24), NOT_INIT), ("lora", dict(K=(1 << 24) + 32, ldx=1 << 25), ARGS),
+    ("lora", dict(K=2 ** 31 - 32, ldx=2 ** 31 - 4), ARGS)], ids=str)
+def test_counts_that_pass_32_bits_in_a_kernel(op, change, code):
+    """A loop's next column or entry is beyond the last one by a step."""
+    assert launch(op, dataclasses.replace(VALID[op], **change)) == code
+
+
 def test_swiglu_segments_refused():
     for segs in ([SEG], [SEG] * 3, [SEG, dataclasses.replace(SEG, N=32)]):
         assert launch("glu", GLU, segs=segs) == ARGS
