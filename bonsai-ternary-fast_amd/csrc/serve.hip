@@ -222,7 +222,7 @@ int btf_hip_launch_cache_move(const btf_cache_move* a, const btf_kv_cache* kv, b
   if (a->S <= 0) return BTF_OK;
   const int rc = check_layers(kv, a->layers, a->layer_stride, "cache_move");
   if (rc != BTF_OK) return rc;
-  if (a->T < 0) return bad("cache_move", "negative T");
+  if (a->T < 0 || a->T > 1 << 30) return bad("cache_move", "T must be in [0, 2^30]");
   if (!a->table || !a->first) return bad("cache_move", "null pointer");
   if ((a->tree != nullptr) == (a->source != nullptr)) return bad("cache_move", "either tree or source");
   if (a->tree ? !a->leaf : !a->source0) return bad("cache_move", "tree needs leaf, source needs source0");

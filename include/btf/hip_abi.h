@@ -705,7 +705,7 @@ int btf_hip_launch_page_free(const btf_page_free* a, btf_stream_t stream);
  * page is not in the table or the cache stay out. */
 typedef struct btf_cache_move {
   int S;
-  int T;                  /* rows of tree, or entries of source */
+  int T;                  /* rows of tree, or entries of source: up to 2^30 */
   const int* table;       /* [S][ldt] */
   int ldt;
   const int* to_table;    /* [S][ldt_to] or NULL */

@@ -101,7 +101,8 @@ def test_more_workgroups_than_a_launch_takes():
 
 @pytest.mark.parametrize("op,change,code", [
     ("lora", dict(K=1 << 24, ldx=1 << 24), NOT_INIT), ("lora", dict(K=(1 << 24) + 32, ldx=1 << 25), ARGS),
-    ("lora", dict(K=2 ** 31 - 32, ldx=2 ** 31 - 4), ARGS)], ids=str)
+    ("lora", dict(K=2 ** 31 - 32, ldx=2 ** 31 - 4), ARGS), ("list", dict(T=1 << 30), NOT_INIT), ("list", dict(T=(1 << 30) + 1), ARGS),
+    ("list", dict(T=2 ** 31 - 1), ARGS)], ids=str)
 def test_counts_that_pass_32_bits_in_a_kernel(op, change, code):
     """A loop's next column or entry is beyond the last one by a step."""
     assert launch(op, dataclasses.replace(VALID[op], **change)) == code
