@@ -704,7 +704,7 @@ int btf_hip_launch_page_free(const btf_page_free* a, btf_stream_t stream);
  * tokens to pages of its own, which no row that is read has. Tokens whose place or
  * page is not in the table or the cache stay out. */
 typedef struct btf_cache_move {
-  int S;
+  int S;                  /* S * KV heads * dim below 2^27 */
   int T;                  /* rows of tree, or entries of source: up to 2^30 */
   const int* table;       /* [S][ldt] */
   int ldt;
@@ -781,7 +781,9 @@ typedef struct btf_lora_seg {
   int ldy;
 } btf_lora_seg;
 typedef struct btf_lora {
-  int S, T;              /* requests, rows (below 2^24) */
+  int S, T;              /* requests and rows, each below 2^22; all segments' N together up to 2^24; with
+                            n = N / 1024 (SWIGLU) or the sum of N over 1024, + the segments: n * T below 2^24
+                            (T <= 4 S), else n * (T / 16 + S) */
   int K;                 /* a multiple of 32 up to 2^24 */
   int rank;              /* ranks that a and b have room for: a multiple of 8 up to 256 */
   int adapters;

@@ -108,6 +108,33 @@ def test_counts_that_pass_32_bits_in_a_kernel(op, change, code):
     assert launch(op, dataclasses.replace(VALID[op], **change)) == code
 
 
+@pytest.mark.parametrize("S,T,Ns,glu,code", [
+    ((1 << 22) - 1, (1 << 22) - 1, [64], False, NOT_INIT), (1 << 22, 1, [64], False, ARGS), (1, 1 << 22, [64], False, ARGS),
+    (1, 1, [1 << 24], False, NOT_INIT), (1, 1, [1 << 23, 1 << 23], False, NOT_INIT), (1, 1, [1 << 23, 1 << 23], True, NOT_INIT),
+    (1, 1, [(1 << 24) - 8, 9], False, ARGS), (1, 1, [(1 << 23) + 1] * 2, True, ARGS),
+    # n * T, n * (T / 16 + S)
+    (1 << 20, 1 << 20, [15 * 1024 - 1], False, NOT_INIT), (1 << 20, 1 << 20, [15 * 1024], False, ARGS),
+    (1 << 20, 1 << 20, [14 * 1024 - 1] * 2, True, NOT_INIT), (1 << 20, 1 << 20, [14 * 1024] * 2, True, ARGS),
+    (1, (1 << 22) - 16, [1024 * 61, 1024, 1024], False, ARGS), (1, (1 << 22) - 16, [1024 * 60], False, NOT_INIT)], ids=str)
+def test_limits_of_the_adapters_launches(S, T, Ns, glu, code):
+    """The header's numbers, and one more."""
+    segs = [dataclasses.replace(SEG, N=n, ldy=n) for n in Ns]
+    a = dataclasses.replace(GLU if glu else LORA, S=S, T=T, ldo=Ns[0])
+    assert h.launch_lora_raw(a, segs, len(segs)) == code
+    n = (Ns[0] if glu else sum(Ns)) // 1024 + len(Ns)
+    fits = max(S, T) < 1 << 22 and sum(Ns) <= 1 << 24 and n * (T if T <= 4 * S else T // 16 + S) < 1 << 24
+    assert code == (NOT_INIT if fits else ARGS)
+
+
+@pytest.mark.parametrize("S,heads,dim", [((1 << 17) - 1, 4, 256), (1 << 17, 4, 256), ((1 << 19) - 1, 4, 64), (1 << 19, 4, 64), (1, (1 << 20) - 1, 128),
+                                         (1, 1 << 20, 128)])
+@pytest.mark.parametrize("op", ["tree", "list"])
+def test_limits_of_a_move(op, S, heads, dim):
+    kv = dataclasses.replace(KV, heads=heads, dim=dim, tok_stride=dim, head_stride=64 * dim, page_stride=heads * 64 * dim)
+    code = NOT_INIT if S * heads * dim < 1 << 27 else ARGS
+    assert launch(op, dataclasses.replace(VALID[op], S=S, layers=1), kv) == code
+
+
 def test_swiglu_segments_refused():
     for segs in ([SEG], [SEG] * 3, [SEG, dataclasses.replace(SEG, N=32)]):
         assert launch("glu", GLU, segs=segs) == ARGS
