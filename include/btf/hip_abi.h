@@ -735,7 +735,8 @@ int btf_hip_launch_cache_move(const btf_cache_move* a, const btf_kv_cache* kv, b
  * 16-byte aligned, one for each stream that launches; it need not be cleared, and
  * the bytes for the largest S and T serve every launch of these heads. */
 typedef struct btf_shared_attention {
-  int S, T, heads;
+  int S, T, heads;       /* T below 2^24, T * heads below 2^31, heads up to 65535;
+                            2 KV heads (T * (heads / KV heads) / 16 + S) below 2^24 - 896 */
   const void* q;
   int ldq;
   const int* table;

@@ -126,6 +126,16 @@ def test_limits_of_the_adapters_launches(S, T, Ns, glu, code):
     assert code == (NOT_INIT if fits else ARGS)
 
 
+@pytest.mark.parametrize("S,T,heads,kv_heads", [
+    (1, 6710521, 20, 4), (1, 6710525, 20, 4), (8388159, 1, 1, 1), (8388160, 1, 1, 1), (1, (1 << 24) - 1, 8, 8), (1, 1 << 24, 1, 1),
+    (1 << 20, 1 << 20, 7, 7), (1 << 20, 1 << 20, 8, 8)])
+def test_limits_of_the_shared_attention(S, T, heads, kv_heads):
+    a = dataclasses.replace(SHARED, S=S, T=T, heads=heads, ldq=heads * 64, ldo=heads * 64)
+    kv = dataclasses.replace(KV, heads=kv_heads, dim=64, tok_stride=64, head_stride=64 * 64, page_stride=kv_heads * 64 * 64)
+    fits = T < 1 << 24 and 2 * kv_heads * (T * (heads // kv_heads) // 16 + S) < (1 << 24) - 896
+    assert launch("shared", a, kv) == (NOT_INIT if fits else ARGS)
+
+
 @pytest.mark.parametrize("S,heads,dim", [((1 << 17) - 1, 4, 256), (1 << 17, 4, 256), ((1 << 19) - 1, 4, 64), (1 << 19, 4, 64), (1, (1 << 20) - 1, 128),
                                          (1, 1 << 20, 128)])
 @pytest.mark.parametrize("op", ["tree", "list"])
