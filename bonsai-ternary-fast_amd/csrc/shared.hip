@@ -26,7 +26,7 @@ namespace btfhip {
 namespace {
 
 // What the plan found of a group (first in the list) or a request.
-struct alignas(64) Found {
+struct alignas(16) Found {  // (as the workspace, which need not begin at a line)
   int s, row0, n, len, ctx, tiles, pieces, begin;  // as Req
   int item0, slot0, C;
   int flags;                                       // kTree, kCut
@@ -34,7 +34,7 @@ struct alignas(64) Found {
   int b, e, whole;                                 // requests of a group; tokens of its prefix
 };
 constexpr int kTree = 1, kCut = 2;
-static_assert(sizeof(Found) == 64, "one line");
+static_assert(sizeof(Found) == 64, "as wide as a line");
 
 // The parts of the workspace.
 struct Ws {

@@ -167,6 +167,21 @@ def test_groups_that_are_wrong(hip, group0, lead, prefix):
     check_attn(out, *x, kv_len, None, heads, kind, page)
 
 
+@pytest.mark.parametrize("S", [6, 70, 130, 1100])
+def test_a_workspace_at_16_bytes(hip, S):
+    """Its start is at a multiple of 16 bytes and no more, as the header asks; nothing behind its end is written."""
+    heads, kind, page = (10, 2, 64), "f16", 16
+    rng = np.random.default_rng(S)
+    x, kv_len = shared_inputs(rng, [0, S - 1], [96], list(rng.integers(0, 40, S)), [1] * S, heads, kind, page)
+    kv = hip.KvCache(x[1], x[2], hip.CacheType[kind], page, 2, 64, x[1].shape[0], 2 * page * 64, page * 64, 64)
+    n = -(-hip.shared_attention_ws_bytes(S, S, 10, kv) // 8)
+    all_of = words(8 * (n + 66))
+    skip = 2 + all_of.data_ptr() // 8 % 2
+    out = run_shared(hip, *x, kv_len, None, heads, kind, page, [0, S - 1], [0], [96], ws=all_of[skip:])
+    assert all_of[skip:].data_ptr() % 64 == 16 and bool((all_of[:skip] == -1).all()) and bool((all_of[skip + n:] == -1).all())
+    check_attn(out, *x, kv_len, None, heads, kind, page)
+
+
 def test_the_lead_is_another_row(hip):
     """The prefix is read through the lead's row alone: other pages with the same values, the members' own left unread."""
     torch = _torch()
