@@ -669,7 +669,8 @@ int btf_hip_launch_page_copy(const btf_page_copy* a, const btf_kv_cache* kv, btf
  * Pages go to the list in the opposite order of their places (a
  * page that several rows give up: at its first), so that giving back what a plan
  * or forks have just handed out leaves the list as it was. shared NULL: no page
- * has two holders. held[s] is taken as at most ldt; ids that are not in [0, pages)
+ * has two holders. Where held[s] passes ldt, the row's ldt pages are looked at, and
+ * held[s] is lowered to what keep[s] needs, if that is less; ids that are not in [0, pages)
  * are dropped; the list never gets more than `pages` entries. A page given up more
  * often in one call than it has holders goes back once.
  * ws: page_free_ws_bytes of device scratch, 4-byte aligned, one for each stream that
