@@ -769,7 +769,10 @@ int btf_hip_launch_shared_attention(const btf_shared_attention* a, const btf_kv_
  * a + id * a_stride, B_id: N rows of `rank` values at b + id * b_stride, of which
  * the adapter uses the first ranks[id] (NULL: all; clamped to [0, rank]); what lies
  * behind them has no effect. Products and sums are in 32 bits. The order of a row's
- * sums follows from the sizes of the launch.
+ * sums follows from the sizes of the launch and the adapter's rank, not from the other
+ * rows' values. What the weights or the row's x have of infinities comes out as infinity
+ * or as NaN, by the sizes of the launch; a row's x reaches no other row. Segments' y do not
+ * overlap.
  * Rows from row0[S] on are left as they were. ws: lora_ws_bytes of device scratch,
  * 16-byte aligned, one for each stream that launches; it need not be cleared, and the
  * bytes for the largest of each argument serve every launch. */
