@@ -169,6 +169,27 @@ def test_one_row_each(hip, new, K, N, rank, kind):
             np.testing.assert_array_equal(ys[1], c.y[1])
 
 
+# A workgroup's outputs in several passes: rows of 16, 32 and 64 a tile, chunks of 512 and 1024 outputs, the last of each in
+# part; the forms of a row and of four; the one launch of a row and a small A.
+PASSES = [([600, 500], 64, 8213, 16), ([1100], 96, 7700, 200), ([1300, 900], 64, 7701, 40), ([700, 401], 64, 7703, 72), ([1, 1030], 32, 15001, 136),
+          ([1] * 70, 96, 8001, 128), ([2] * 40, 64, 9301, 24), ([1], 640, 700, 256), ([1, 1, 1], 640, 513, 128), ([1, 1], 320, 1000, 248)]
+
+
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("new,K,N,rank", PASSES, ids=lambda x: str(x)[:24])
+def test_outputs_in_several_passes(hip, new, K, N, rank, kind):
+    spare = 3 if max(new) > 2 else 0  # (none where the form goes by a row, or four, a request)
+    for ranks in (None, "mixed"):
+        c = Case(new, K, [N, 9], kind, rank, adapters=2, ranks=ranks, seed=14, spare=spare, pad=(0, 1))
+        c.check_add(c.run(hip)[0])
+    c = Case(new, K, [N, N], kind, rank, adapters=2, ranks=None, seed=15, spare=spare)
+    for into_gate in (False, True):
+        ys, out = c.run(hip, "swiglu", into_gate=into_gate)
+        c.check_swiglu(out)
+        np.testing.assert_array_equal(ys[1], c.y[1])
+        np.testing.assert_array_equal(out[c.row0[-1]:], c.y[0][c.row0[-1]:] if into_gate else np.full_like(out[c.row0[-1]:], GUARD))
+
+
 @pytest.mark.parametrize("Ns", [[512, 96, 96], [40, 41]])
 @pytest.mark.parametrize("new", [[1, 1, 1], [50, 30]])
 @pytest.mark.parametrize("pad,shift", [((0, 0), 0), ((4, 3), 0), ((20, 4), 0), ((0, 0), 1), ((0, 4), 2)])
