@@ -782,6 +782,10 @@ int lora_few(const btf_lora& a, const Segs& segs, int nseg, hipStream_t st) {
   return launch_status("lora_expand_few_kernel");
 }
 
+// Which form: by the rows that a request has on average, as the sizes of the requests are device data. Where they are very
+// unlike, one form does for rows that the other would do better (K 5120, gate and up of 17408, ranks of 64: 199 single rows and
+// a prompt of 512 430 us, as two launches 101 + 66; 63 and 190 177 and 82, 63 and 200, above four rows on average, 107 and 82;
+// ranks of 16 57, 44; 64, 45. Q, K and V, ranks of 64: 171 and 85; 75, 47; 56, 48. 31 and 2048, ranks of 16, 52 and 56).
 template <bool BF>
 int lora_any(const btf_lora& a, const Segs& segs, int nseg, hipStream_t st) {
   if (a.T <= a.S) return lora_few<BF, 1>(a, segs, nseg, st);

@@ -773,6 +773,9 @@ int btf_hip_launch_shared_attention(const btf_shared_attention* a, const btf_kv_
  * rows' values. What the weights or the row's x have of infinities comes out as infinity
  * or as NaN, by the sizes of the launch; a row's x reaches no other row. Segments' y do not
  * overlap.
+ * The kernels' form follows T / S: one prompt piece among many single tokens, up to four
+ * rows a request on average, is done four rows at a time and is faster in a launch of its
+ * own (row0 and adapter from its request on, S the requests left).
  * Rows from row0[S] on are left as they were. ws: lora_ws_bytes of device scratch,
  * 16-byte aligned, one for each stream that launches; it need not be cleared, and the
  * bytes for the largest of each argument serve every launch. */
